@@ -46,7 +46,8 @@ enum rta_status {
  * reference, which streams GGUF rows as uploaded); every projection entry point
  * accepts RTA_Q4_K | RTA_TILED and RTA_Q6_K | RTA_TILED and then runs on the matrix
  * cores at every batch size. */
-enum rta_format { RTA_F32 = 0, RTA_F16 = 1, RTA_Q4_K = 12, RTA_Q6_K = 14, RTA_BF16 = 30, RTA_TILED = 0x100 };
+enum rta_format { RTA_F32 = 0, RTA_F16 = 1, RTA_Q4_K = 12, RTA_Q6_K = 14, RTA_BF16 = 30, RTA_TILED = 0x100,
+                  RTA_Q8_ROW = 0x200 /* pages only: int8 codes, one fp32 scale per position and kv head */ };
 
 /* Epilogue of a projection: y = W x, or y += W x (the residual add of the O and
  * down projections, resident_math.comp:70). */
@@ -58,6 +59,8 @@ enum rta_epilogue { RTA_EPI_STORE = 0, RTA_EPI_ACCUMULATE = 1 };
 #define RTA_DEVERR_VOCAB 2048u      /* vocabulary coverage != V                */
 #define RTA_DEVERR_DETECTOR 65536u  /* non-finite query / key / score          */
 #define RTA_DEVERR_TOKEN 4096u      /* token id >= vocabulary (rta_embed); no reference bit */
+#define RTA_DEVERR_PAGES 16384u     /* paged history: a bad sequence, row list or page, or no page left;
+                                       no reference bit */
 
 int rta_version(void);
 const char* rta_status_string(int status);
@@ -487,6 +490,114 @@ int rta_hybrid_decode_step_capture(const rta_hybrid_shape* shape, const rta_hybr
                                    void* state, uint32_t* tokens, float* logits_out,
                                    const rta_hybrid_capture* capture, void* workspace, size_t workspace_bytes,
                                    rta_stream_t stream);
+
+/* ---------------- paged history: the keys and values of many sequences in one pool of
+ * pages of `page` positions, handed out, shared, copied on write and closed up on the device.
+ * No counterpart in the reference, whose history is one preallocated ring per layer
+ * (optical_resident.cpp:455-481); a serving loop with sequences that come, fork and end needs
+ * it beside the rings of rta_decode_attention.
+ *
+ * Sequence s (0 <= s < max_seqs) holds positions 0 .. lengths[s] - 1; position p lies at offset
+ * p % page of page table[s * max_pages + p / page], in every layer alike (-1: no page).  refs
+ * counts the sequences that name a page; pages with refs 0 are free.  One page of one layer is
+ *   elements [key, value][kv_heads][page][head_dim]  (RTA_F16, RTA_BF16, or int8 codes)
+ *   RTA_Q8_ROW: then fp32 scales [key, value][kv_heads][page]; a value is code * scale
+ * padded to rta_page_bytes() bytes.  The caller owns the four arrays (device memory) and may
+ * fill or read them itself; the calls below keep them consistent.
+ *
+ * Every call is stream ordered, allocates nothing and may be captured in a HIP graph.  What
+ * cannot be known on the host is checked on the device: a sequence or page outside its range, a
+ * sequence listed twice, a length past max_pages * page, or a pool with too few free pages
+ * raises RTA_DEVERR_PAGES and that entry of the list is left undone. */
+typedef struct rta_pages {
+    int fmt;               /* RTA_F16, RTA_BF16 or RTA_Q8_ROW */
+    int kv_heads;          /* 1 .. 1024 */
+    int head_dim;          /* 64, 128 or 256 */
+    int page;              /* positions per page, 1 .. 65536 */
+    int layers, n_pages;   /* n_pages <= 2^20 */
+    int max_seqs, max_pages;
+    void* pool;            /* [layers][n_pages][rta_page_bytes()], 16-byte aligned */
+    int32_t* table;        /* [max_seqs][max_pages] */
+    int32_t* lengths;      /* [max_seqs] */
+    int32_t* refs;         /* [n_pages] */
+} rta_pages;
+
+/* Bytes of one page of one layer (a multiple of 128), -1 if invalid. */
+int64_t rta_page_bytes(int fmt, int kv_heads, int head_dim, int page);
+
+/* Empties the book: every table entry -1, lengths and refs 0.  The pool is not touched. */
+int rta_pages_init(const rta_pages* pages, rta_stream_t stream);
+
+/* The list arguments: n entries, seqs[i] (device; NULL: i) the sequence of entry i.
+ * Workspace of rta_pages_extend (n entries) and rta_pages_compact (any n), 16-byte aligned. */
+size_t rta_pages_workspace_bytes(const rta_pages* pages, int n);
+
+/* lengths[s] += add[i] (device; NULL: 1), with pages for the new positions, the lowest free
+ * pages first, in list order.  A last page that is partly filled and that other sequences name
+ * too is copied first (all layers; the last listed of its holders keeps it where all of them are
+ * listed).  When the free pages run out, that entry and those after it are left undone. */
+int rta_pages_extend(const rta_pages* pages, const int32_t* seqs, const int32_t* add, int n, void* workspace,
+                     size_t workspace_bytes, rta_stream_t stream);
+
+/* Sequence dst[i], which must be empty, becomes a copy of src[i] that names the same pages (no
+ * data moves; rta_pages_extend copies the last page when one of them grows).  A sequence is not
+ * both a source and a destination of one call. */
+int rta_pages_fork(const rta_pages* pages, const int32_t* src, const int32_t* dst, int n, rta_stream_t stream);
+
+/* Sequence seqs[i] gives up every page whose held positions all lie in [first[i], last[i])
+ * (device; NULL: 0 and the whole length); with last[i] >= its length it also ends at first[i].
+ * So the whole sequence is freed, its end is taken back, or (first = sinks, last = length -
+ * window) the pages that a window has left behind are freed; table entries become -1. */
+int rta_pages_free(const rta_pages* pages, const int32_t* seqs, const int32_t* first, const int32_t* last, int n,
+                   rta_stream_t stream);
+
+/* Closes the pool up: with U pages in use, the k-th used page at or past U moves (all layers)
+ * to the k-th free page below U, and the table follows.  used (device, may be NULL) gets U. */
+int rta_pages_compact(const rta_pages* pages, int32_t* used, void* workspace, size_t workspace_bytes,
+                      rta_stream_t stream);
+
+/* The row lists below: row r belongs to entry i with cu_rows[i] <= r < cu_rows[i + 1] (device,
+ * n + 1 nondecreasing values, the last at most rows); the c = cu_rows[i + 1] - cu_rows[i] rows
+ * of an entry are its sequence's newest c positions, oldest first.  cu_rows NULL: one row per
+ * entry (rows = n).  Rows outside every entry are left as they were. */
+
+/* The rows' keys and values k[r, :kv_heads * head_dim], v (fp32, row strides in floats) into
+ * the pages of layer `layer`: rounded to nearest even, or for RTA_Q8_ROW scale = max|x| * (1 / 127)
+ * over the head (fp32) and code = round(x / scale) (a head with a value that is not finite reads back
+ * as NaN).  A page named by several sequences is written for
+ * all of them (rta_pages_extend has made the last one the sequence's own).  Call it after
+ * rta_pages_extend. */
+int rta_paged_append(const rta_pages* pages, int layer, const float* k, int64_t k_stride, const float* v,
+                     int64_t v_stride, int rows, const int32_t* seqs, const int32_t* cu_rows, int n,
+                     rta_stream_t stream);
+
+/* The reverse: fp32 keys and values of those rows (either may be NULL).  A position without a
+ * page reads as zeros and raises RTA_DEVERR_PAGES. */
+int rta_paged_read(const rta_pages* pages, int layer, int rows, const int32_t* seqs, const int32_t* cu_rows, int n,
+                   float* k, int64_t k_stride, float* v, int64_t v_stride, rta_stream_t stream);
+
+/* Attention of the rows over their sequences' pages, causal:  row r at position t sees
+ * positions p <= t, and with window > 0 of those only p > t - window or p < sinks.
+ *   out[r, h, :] = sum_p e^(s_p - m) v_p / z,  s_p = q[r, h, :] . k_p / sqrt(head_dim),
+ *   m = max s_p, z = sum e^(s_p - m);  kv head h / (hq / kv_heads);  out *= sigmoid(gate).
+ *   q [rows, hq, head_dim] fp32 with row stride q_stride (floats), already rotated; gate and
+ *   out [rows, hq, head_dim] contiguous; m_out, z_out [rows, hq]; gate, m_out, z_out may be NULL.
+ *   max_rows  host upper bound of an entry's rows (one row per entry: 1)
+ *   max_len   host upper bound of the lengths (0: max_pages * page).  It sizes the grid and
+ *             the workspace: give the bound a captured loop will reach.
+ * A row that sees nothing (an empty sequence) gets out = 0, m = -inf, z = 0; so does a row of
+ * a bad entry, of a sequence longer than max_len and of a position before the sequence's start
+ * (all raise RTA_DEVERR_PAGES); rows past an entry's max_rows raise it and are left as they
+ * were; a visible position without a page raises it and is not seen.  A visible position whose
+ * score is not finite, or a result that is not, raises RTA_DEVERR_DETECTOR (that row's values
+ * then mean nothing).  What lies in a page past its sequence's length is never used.
+ * Workspace: rta_paged_attention_workspace_bytes() bytes, 16-byte aligned (0: none needed). */
+size_t rta_paged_attention_workspace_bytes(const rta_pages* pages, int hq, int rows, int n, int max_rows,
+                                           int max_len, int window, int sinks);
+int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64_t q_stride, int rows, int hq,
+                        const int32_t* seqs, const int32_t* cu_rows, int n, int max_rows, int max_len, int window,
+                        int sinks, const float* gate, float* out, float* m_out, float* z_out, void* workspace,
+                        size_t workspace_bytes, rta_stream_t stream);
 
 /* ---------------- on-disk assets (host only: no device work, no GPU needed).
  * Reads the exporter's optical_model.bin (RTRES004), geometry_weights.bin and

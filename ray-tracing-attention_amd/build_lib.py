@@ -10,7 +10,7 @@ from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 SOURCES = ["csrc/rta_gemv.hip", "csrc/rta_attention.hip", "csrc/rta_step.hip", "csrc/rta_model.hip",
-           "csrc/rta_asset.cpp"]
+           "csrc/rta_pages.hip", "csrc/rta_paged_attention.hip", "csrc/rta_asset.cpp"]
 LIB = HERE / "lib" / "librta.so"
 # the resident worker (stdin/stdout protocol of the reference's rt_optical_resident)
 WORKER_SRC = "worker/rt_optical_resident.cpp"

@@ -13,8 +13,9 @@ LIB_PATH = PKG_ROOT / "lib" / "librta.so"
 # GGUF type codes (resident_quant.glsl:6-20)
 F32, F16, Q4_K, Q6_K, BF16 = 0, 1, 12, 14, 30
 TILED = 0x100   # fmt | TILED: a K-quant matrix packed by rta_pack
+Q8_ROW = 0x200  # pages only: int8 codes, one fp32 scale per position and kv head
 EPI_STORE, EPI_ACCUMULATE = 0, 1
-DEVERR_HITS, DEVERR_VOCAB, DEVERR_DETECTOR = 8, 2048, 65536
+DEVERR_HITS, DEVERR_VOCAB, DEVERR_PAGES, DEVERR_DETECTOR = 8, 2048, 16384, 65536
 NOALLOC_SCRATCH_BYTES = 96 << 20   # RTA_NOALLOC_SCRATCH_BYTES
 ERR_SCRATCH = 9                    # RTA_ERR_SCRATCH
 
@@ -31,7 +32,14 @@ class Remap(ctypes.Structure):
                 ("key_rows", ctypes.c_int)]
 
 
-_remap_p = ctypes.POINTER(Remap)
+class Pages(ctypes.Structure):
+    """struct rta_pages: a paged history (device pointers)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("fmt", "kv_heads", "head_dim", "page", "layers", "n_pages", "max_seqs",
+                                            "max_pages")] + \
+               [(n, ctypes.c_void_p) for n in ("pool", "table", "lengths", "refs")]
+
+
+_remap_p, _pages_p = ctypes.POINTER(Remap), ctypes.POINTER(Pages)
 
 # name -> (restype, argtypes); must match include/rta.h
 SIGNATURES = {
@@ -80,6 +88,19 @@ SIGNATURES = {
     "rta_image_readout": (_i, [_i, _i, _p, _p, _i, _i, _p, _i, _p, _f, _p, _i, _p, _sz, ctypes.POINTER(_i), _p]),
     "rta_attention_receipt_records": (_i64, [_p, _i, _i, _i64, _i]),
     "rta_attention_receipts": (_i, [_p, _i, _i, _i, _i, _p, _i, _i, _p, _p, _i64, _i64, _i, _i, _p, _i64, _p]),
+    # paged history (rta.pages)
+    "rta_page_bytes": (_i64, [_i, _i, _i, _i]),
+    "rta_pages_init": (_i, [_pages_p, _p]),
+    "rta_pages_workspace_bytes": (_sz, [_pages_p, _i]),
+    "rta_pages_extend": (_i, [_pages_p, _p, _p, _i, _p, _sz, _p]),
+    "rta_pages_fork": (_i, [_pages_p, _p, _p, _i, _p]),
+    "rta_pages_free": (_i, [_pages_p, _p, _p, _p, _i, _p]),
+    "rta_pages_compact": (_i, [_pages_p, _p, _p, _sz, _p]),
+    "rta_paged_append": (_i, [_pages_p, _i, _p, _i64, _p, _i64, _i, _p, _p, _i, _p]),
+    "rta_paged_read": (_i, [_pages_p, _i, _i, _p, _p, _i, _p, _i64, _p, _i64, _p]),
+    "rta_paged_attention_workspace_bytes": (_sz, [_pages_p, _i, _i, _i, _i, _i, _i, _i]),
+    "rta_paged_attention": (_i, [_pages_p, _i, _p, _i64, _i, _i, _p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _sz,
+                                 _p]),
     # host-only asset reader (rta.asset binds the structs)
     "rta_asset_open": (_i, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_p), ctypes.c_char_p, _sz]),
     "rta_asset_close": (None, [_p]),
