@@ -1,0 +1,179 @@
+// rta_paged.hpp -- what the kernels of attention over the paged history share: the arguments,
+// what a row sees, and the matrix-core operands of its formats.
+//
+// The products run on v_mfma_f32_16x16x32 with the positions as rows:
+//   S^T = K Q^T   A = K (row: position), B = Q^T (column: a query), and
+//   O^T = V^T P^T A = V^T (row: dim),    B = P^T (column: the same query).
+// Lane (i = lane % 16, u = lane / 16) of the result of the first holds positions 4u .. 4u + 3 of
+// column i, which is where the second wants its B operand (k slots 8u ..) if its k axis is
+// ordered  slot 8u + s  <->  position 4u + s (s < 4), 16 + 4u + s - 4 (else) of 32 positions;
+// so weights never leave their lane, and V^T comes in that order from a transposing LDS read.
+//
+// fp32 queries and weights meet 16-bit values, so each is split into parts that are exact
+// 16-bit numbers and whose products are added in fp32:
+//   binary16 pages (and 8-bit codes, exact in binary16): two parts, 22 bits, of the value times a
+//   power of two that puts its row's largest in [2^13, 2^14);
+//   bfloat16 pages: three parts of 8 bits, 24 bits and no scale.
+// Two parts are neighbouring columns of one product (query g in columns 2g and 2g + 1), the
+// third a second product into the same accumulator.  One rounding to 16 bits instead would cost
+// 2^-12 (2^-9) of the result where fp32 results are wanted.
+#pragma once
+#include <math.h>
+
+#include "rta_pages.hpp"
+
+namespace rta {
+
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+struct PagedAttnArgs {
+    PageArgs p;
+    RowList l;
+    const float* q;
+    int64_t q_stride;
+    const float* gate;
+    float* out;
+    float* m_out;
+    float* z_out;
+    int hq, group;      // group: q heads per kv head
+    int max_rows, max_len, window, sinks;
+    // work split: chunks of `chunk` visible positions; with nchunk > 1 every (row, q head, chunk)
+    // leaves U[HD] in `part` and (m, z) in `mz`, both [row][hq][nchunk]
+    int chunk, nchunk;
+    float* part;
+    float2* mz;
+};
+
+// What a row at position t sees: the first `head` positions and then those from `lo` on, `count`
+// of them; the j-th is j for j < head, else j + lo - head.
+struct Visible {
+    int head, lo, count;
+    __device__ __forceinline__ int position(int j) const { return j < head ? j : j + lo - head; }
+};
+__device__ __forceinline__ Visible visible(int t, int window, int sinks) {
+    const int lo = window > 0 && t >= window ? t - window + 1 : 0;
+    const int head = min(lo, sinks);
+    return Visible{head, lo, head + t + 1 - lo};
+}
+
+// Row r's table row and what it sees (nothing for a bad one); false for a row that no entry
+// lists or that is past max_rows.  err collects the error bits.
+__device__ __forceinline__ bool resolve_row(const PagedAttnArgs& a, int r, const int32_t*& table, Visible& see,
+                                            uint32_t& err) {
+    int i, first, count;
+    see = Visible{0, 0, 0};
+    table = a.p.table;
+    if (!row_entry(a.l, r, i, first, count)) return false;
+    if (r - first >= a.max_rows) {
+        err |= RTA_DEVERR_PAGES;
+        return false;
+    }
+    const int s = list_seq(a.l.seqs, i);
+    if ((unsigned)s >= (unsigned)a.p.max_seqs) {
+        err |= RTA_DEVERR_PAGES;
+        return true;
+    }
+    const int len = a.p.lengths[s], t = len - count + (r - first);
+    table += (int64_t)s * a.p.max_pages;
+    if (len > a.max_len || len < 0 || (t < 0 && (len > 0 || count > 1))) err |= RTA_DEVERR_PAGES;
+    else if (t >= 0) see = visible(t, a.window, a.sinks);
+    return true;
+}
+
+// The final values of (row, q head) at dim c from U, M (natural units) and Z.
+__device__ __forceinline__ void write_result(const PagedAttnArgs& a, int64_t at, int hd, int c, float u, float m,
+                                             float z, uint32_t& err) {
+    float o = z > 0.0f || z != z ? u / z : 0.0f;   // nothing seen: zeros
+    if (a.gate) o *= detector_sigmoid(a.gate[at * hd + c]);
+    if (!isfinite(o)) err |= RTA_DEVERR_DETECTOR;
+    a.out[at * hd + c] = o;
+    if (c == 0) {
+        if (a.m_out) a.m_out[at] = m;
+        if (a.z_out) a.z_out[at] = z;
+    }
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// ---- operands by page format ----
+template <int FMT> struct PageFmt;
+template <> struct PageFmt<RTA_F16> {
+    static constexpr int kBytes = 2, kOps = 1;   // element bytes; products per operand pair
+    static constexpr bool kScaled = false;       // scales beside the elements
+};
+template <> struct PageFmt<RTA_BF16> {
+    static constexpr int kBytes = 2, kOps = 2;
+    static constexpr bool kScaled = false;
+};
+template <> struct PageFmt<RTA_Q8_ROW> {
+    static constexpr int kBytes = 1, kOps = 1;
+    static constexpr bool kScaled = true;
+};
+
+template <int FMT>
+__device__ __forceinline__ f4_t page_mfma(u4_t a, u4_t b, f4_t c) {
+    if constexpr (FMT == RTA_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0,
+                                                       0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0,
+                                                      0);
+}
+
+// Four int8 codes as four binary16 (1024 + (c + 128) has the code in its last bits; minus 1152).
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    const uint32_t x = w ^ 0x80808080u;
+    const h2v_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2v_t, __builtin_amdgcn_perm(x, 0x64646464u, 0x00050004u)) + off);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2v_t, __builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u)) + off);
+}
+
+// The upper halves of two floats as one dword: bfloat16 cut off, not rounded.
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+}
+__device__ __forceinline__ float cut(float v, uint32_t mask) {
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & mask);
+}
+
+// Part `part` (0, 1) of eight values as B operands (op 1, of bfloat16 only: the third part in
+// part 0's columns).  Parts are cut off, not rounded, so that each remainder is exact; a value
+// that is not finite stays so.
+template <int FMT>
+__device__ __forceinline__ void split_parts(const float v[8], int part, u4_t op[PageFmt<FMT>::kOps]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float x[2], y[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float w = v[2 * j + e], r = w - cut(w, FMT == RTA_BF16 ? 0xffff0000u : 0xffffe000u);
+            x[e] = part ? r : w;
+            if constexpr (FMT == RTA_BF16) y[e] = part ? 0.0f : r - cut(r, 0xffff0000u);
+        }
+        if constexpr (FMT == RTA_BF16) {
+            op[0][j] = upper_halves(x[0], x[1]);
+            op[1][j] = upper_halves(y[0], y[1]);
+        } else {
+            op[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
+        }
+    }
+}
+
+// Dims of element s of the 8 that lane segment u holds for product kb: 16-byte pieces of a row
+// follow the segments, one piece per product (2-byte elements) or two products (codes).
+template <int FMT>
+__device__ __forceinline__ int operand_dim(int kb, int u) {
+    if constexpr (FMT == RTA_Q8_ROW) return 64 * (kb >> 1) + 16 * u + 8 * (kb & 1);
+    else return 32 * kb + 8 * u;
+}
+
+// Power-of-two exponent that brings values up to mx below 2^14 (for binary16 operands);
+// zero or not finite: the lowest.
+__device__ __forceinline__ int part_exponent(float mx) {
+    int e = -110;
+    if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &e);
+    return e < -110 ? -110 : e;
+}
+
+}  // namespace rta

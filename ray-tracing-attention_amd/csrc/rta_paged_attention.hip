@@ -1,35 +1,8 @@
 // rta_paged_attention.hip -- causal attention of new rows over the paged history, with a sliding
 // window and first positions that stay visible (gfx950).
-#include <math.h>
-
-#include "rta_pages.hpp"
+#include "rta_paged_decode.hpp"
 
 namespace rta {
-
-struct PagedAttnArgs {
-    PageArgs p;
-    RowList l;
-    const float* q;
-    int64_t q_stride;
-    const float* gate;
-    float* out;
-    float* m_out;
-    float* z_out;
-    int hq, group;      // group: q heads per kv head
-    int max_rows, max_len, window, sinks;
-};
-
-// What a row at position t sees: the first `head` positions and then those from `lo` on, `count`
-// of them; the j-th is j for j < head, else j + lo - head.
-struct Visible {
-    int head, lo, count;
-    __device__ __forceinline__ int position(int j) const { return j < head ? j : j + lo - head; }
-};
-__device__ __forceinline__ Visible visible(int t, int window, int sinks) {
-    const int lo = window > 0 && t >= window ? t - window + 1 : 0;
-    const int head = min(lo, sinks);
-    return Visible{head, lo, head + t + 1 - lo};
-}
 
 template <int FMT>
 __device__ __forceinline__ float element(const uint8_t* page, int64_t i) {
@@ -132,6 +105,36 @@ __global__ void __launch_bounds__(256) paged_attention_kernel(const PagedAttnArg
     if (err) raise_error(err);
 }
 
+// How a call with one row per sequence is cut: chunks of a multiple of 128 positions (a tile for
+// each of 4 waves), so many that the chip has about kDecGroups workgroups to hand out if every
+// row sees the most it may.
+constexpr int kDecGroups = 4096;
+struct Cut {
+    int chunk, nchunk;
+};
+static Cut decode_cut(int rows, int heads, int64_t most) {
+    const int64_t want = (rows * (int64_t)heads * most / kDecGroups + 127) / 128 * 128;
+    const int64_t chunk = want < 128 ? 128 : want < 1 << 30 ? want : 1 << 30;
+    return Cut{(int)chunk, (int)((most + chunk - 1) / chunk)};
+}
+// Workgroups per row: kv heads times the groups of up to 8 (16) q heads that share one.
+static int decode_nc(int group, int hd) { return group > 8 && hd < 256 ? 2 : 1; }
+static int decode_heads(int kv_heads, int group, int hd) {
+    const int per = 8 * decode_nc(group, hd);
+    return kv_heads * ((group + per - 1) / per);
+}
+static int64_t most_visible(int64_t max_len, int window, int sinks) {
+    return window > 0 && max_len - window > sinks ? (int64_t)window + sinks : max_len;
+}
+static int64_t bound_len(const rta_pages* p, int max_len) {
+    const int64_t most = (int64_t)p->max_pages * p->page;
+    return max_len > 0 && max_len < most ? max_len : most;
+}
+static size_t split_bytes(int64_t rows, int hq, int hd, int nchunk) {
+    if (nchunk <= 1) return 0;
+    return ((size_t)rows * hq * nchunk * (hd + 2) * 4 + 15) / 16 * 16;
+}
+
 }  // namespace rta
 
 using namespace rta;
@@ -140,8 +143,16 @@ extern "C" {
 
 size_t rta_paged_attention_workspace_bytes(const rta_pages* pages, int hq, int rows, int n, int max_rows, int max_len,
                                            int window, int sinks) {
-    (void)pages, (void)hq, (void)rows, (void)n, (void)max_rows, (void)max_len, (void)window, (void)sinks;
-    return 0;
+    PageArgs p;
+    (void)n;
+    if (host::pages_args(pages, -1, &p) || hq <= 0 || hq % pages->kv_heads || rows <= 0 || max_rows <= 0 ||
+        max_len < 0 || window < 0 || sinks < 0)
+        return 0;
+    if (max_rows > 1) return 0;
+    const int group = hq / pages->kv_heads;
+    const Cut cut = decode_cut(rows, decode_heads(pages->kv_heads, group, pages->head_dim),
+                               most_visible(bound_len(pages, max_len), window, sinks));
+    return split_bytes(rows, hq, pages->head_dim, cut.nchunk);
 }
 
 int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64_t q_stride, int rows, int hq,
@@ -162,8 +173,9 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
     if (!host::aligned(q, 4) || !host::aligned(gate, 4) || !host::aligned(out, 4) || !host::aligned(m_out, 4) ||
         !host::aligned(z_out, 4))
         return RTA_ERR_ALIGN;
-    (void)workspace, (void)workspace_bytes;
-    const int most = pages->max_pages * pages->page;
+    const size_t need = rta_paged_attention_workspace_bytes(pages, hq, rows, n, max_rows, max_len, window, sinks);
+    if (need && (!workspace || workspace_bytes < need || !host::aligned(workspace, 16))) return RTA_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
     a.q = q;
     a.q_stride = q_stride;
     a.gate = gate;
@@ -173,13 +185,31 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
     a.hq = hq;
     a.group = hq / pages->kv_heads;
     a.max_rows = max_rows;
-    a.max_len = max_len && max_len < most ? max_len : most;
+    a.max_len = (int)bound_len(pages, max_len);
     a.window = window;
     a.sinks = sinks;
     auto launch = [&](auto fmt) {
-        auto go = [&](auto hd) {
-            hipLaunchKernelGGL((paged_attention_kernel<decltype(fmt)::value, decltype(hd)::value>), dim3(rows, hq),
-                               dim3(256), 0, (hipStream_t)stream, a);
+        constexpr int F = decltype(fmt)::value;
+        auto go = [&](auto hdim) {
+            constexpr int HD = decltype(hdim)::value;
+            if (max_rows > 1) {
+                hipLaunchKernelGGL((paged_attention_kernel<F, HD>), dim3(rows, hq), dim3(256), 0, s, a);
+                return;
+            }
+            const int heads = decode_heads(pages->kv_heads, a.group, HD);
+            const Cut cut = decode_cut(rows, heads, most_visible(a.max_len, window, sinks));
+            a.chunk = cut.chunk;
+            a.nchunk = cut.nchunk;
+            a.part = static_cast<float*>(workspace);
+            a.mz = reinterpret_cast<float2*>(a.part + (size_t)rows * hq * cut.nchunk * HD);
+            const dim3 grid(rows, heads, cut.nchunk), block(64 * kDecWaves);
+            if constexpr (HD < 256) {
+                if (decode_nc(a.group, HD) == 2) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2>), grid, block, 0, s, a);
+                else hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1>), grid, block, 0, s, a);
+            } else {
+                hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1>), grid, block, 0, s, a);
+            }
+            if (cut.nchunk > 1) hipLaunchKernelGGL((paged_merge_kernel<HD>), dim3(rows, hq), dim3(256), 0, s, a);
         };
         if (pages->head_dim == 64) go(std::integral_constant<int, 64>{});
         else if (pages->head_dim == 128) go(std::integral_constant<int, 128>{});

@@ -1,0 +1,408 @@
+// rta_paged_decode.hpp -- attention of one row per sequence over its pages.
+//
+// Bound by the history's bytes: every visible key and value is read once per kv head (for more
+// than 8 NC q heads per kv head once per group of those).  A workgroup of 4 waves takes one
+// (row, kv head, chunk of visible positions); a wave takes every fourth tile of 32 positions and
+// works alone until the end, so the waves of a compute unit (16 of them at 128 registers and 39 KB
+// of LDS per workgroup) drift apart and cover each other's waits:
+//   lane (i, u) loads piece u of the rows of positions i and 16 + i, keys straight as the A
+//   operand, values into LDS (32 rows, 16 bytes of padding each: the 16 rows that a transposing
+//   read touches then fall on every bank exactly twice) and back transposed;
+//   the next tile's keys go out as soon as the scores have been formed, its values as soon as
+//   these are in LDS, its pages' numbers a tile earlier.
+// The chunk's four (m, z, U) are joined in LDS, those of a row's chunks by paged_merge_kernel.
+#pragma once
+#include "rta_paged.hpp"
+
+namespace rta {
+
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4_t lds_s4_t;
+
+constexpr int kDecWaves = 4, kDecTile = 32;
+
+template <int FMT, int HD, int NC>
+struct DecLds {
+    static constexpr int kPitch = 2 * HD + 16;                                  // bytes of a V row
+    static constexpr int kQ = NC * PageFmt<FMT>::kOps * (HD / 32) * 64 * 16;    // Q^T operands, of all waves
+    static constexpr int kV = kDecTile * kPitch;                                // per wave: V, at the end U
+    static constexpr int kS = PageFmt<FMT>::kScaled ? 2 * kDecTile * 4 : 0;     // per wave: the tile's scales
+    static constexpr int kWave = kV + kS;
+    static constexpr int kHeads = 8 * NC;
+    static constexpr int kTotal = kQ + kDecWaves * kWave + kDecWaves * kHeads * 8;   // and (m, z) per wave and head
+    static_assert(kHeads * HD * 4 <= kV || NC > 1, "U of a wave fits its V rows");
+};
+
+template <int FMT, int HD, int NC>
+__global__ void __launch_bounds__(64 * kDecWaves) paged_decode_kernel(const PagedAttnArgs a) {
+    using L = DecLds<FMT, HD, NC>;
+    constexpr int kOps = PageFmt<FMT>::kOps, kB = PageFmt<FMT>::kBytes;
+    constexpr int kKb = HD / 32;                // products per 16 positions
+    constexpr int kLoads = HD * kB / 64;        // 16-byte pieces per lane and row
+    constexpr int kDt = HD / 16;                // dim tiles of O^T
+    constexpr bool kScaled = PageFmt<FMT>::kScaled;
+    __shared__ __align__(16) uint8_t lds[L::kTotal];
+    const int r = blockIdx.x, lane = threadIdx.x & 63, i = lane & 15, u = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int groups = (a.group + L::kHeads - 1) / L::kHeads;   // head groups of a kv head
+    const int kvh = blockIdx.y / groups, g0 = (blockIdx.y - kvh * groups) * L::kHeads;
+    const int heads = min(a.group - g0, L::kHeads);             // q heads of this workgroup
+    uint32_t err = 0;
+    Visible see;
+    const int32_t* table;
+    if (!resolve_row(a, r, table, see, err)) {
+        if (err && threadIdx.x == 0) raise_error(err);
+        return;
+    }
+    const int begin = blockIdx.z * a.chunk, end = see.count - begin > a.chunk ? begin + a.chunk : see.count;
+    if (begin >= end && blockIdx.z > 0) return;
+
+    // q as B operands, one wave per quarter of the products; column 2 g + part.  Every wave finds
+    // the heads' largest |q| (the power of two of binary16 operands).
+    const int part = i & 1;
+    float fac[NC];   // score = product * fac, in powers of two: 1 / s / sqrt(HD) * log2 e
+    int qe[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int g = 8 * c + (i >> 1);
+        const float* q = a.q + r * a.q_stride + ((int64_t)kvh * a.group + g0 + min(g, heads - 1)) * HD;
+        qe[c] = 14;
+        if constexpr (FMT != RTA_BF16) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int j = 0; j < HD / 4; ++j) mx = fmaxf(mx, fabsf(q[u * (HD / 4) + j]));
+            qe[c] = part_exponent(max_xor32(max_xor16(mx)));
+        }
+        fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe[c] - 14);
+        for (int kb = wave; kb < kKb; kb += kDecWaves) {
+            float v[8];
+            const float sg = ldexpf(1.0f, 14 - qe[c]);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) v[s] = q[operand_dim<FMT>(kb, u) + s] * sg;
+            u4_t op[kOps];
+            split_parts<FMT>(v, part, op);
+#pragma unroll
+            for (int o = 0; o < kOps; ++o)
+                *reinterpret_cast<u4_t*>(lds + (((c * kOps + o) * kKb + kb) * 64 + lane) * 16) = op[o];
+        }
+    }
+    __syncthreads();
+
+    uint8_t* vl = lds + L::kQ + wave * L::kWave;
+    float* sl = reinterpret_cast<float*>(vl + L::kV);
+    const int64_t plane = (int64_t)a.p.kv_heads * a.p.page;   // rows of a page's keys
+    const int64_t v_off = plane * HD * kB;
+    const int ntile = (end - begin + kDecTile - 1) / kDecTile;
+
+    f4_t o[NC][kDt];
+    float m[NC], z[NC];
+    int ve = -110;   // exponent of the largest value scale so far
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        m[c] = -INFINITY;
+        z[c] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDt; ++d) o[c][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float nonfinite = 0.0f;
+
+    // position i + 16 h of tile t: its page's number and place, clamped to the last visible one
+    struct Spot {
+        int page[2], off[2];
+    };
+    auto spot = [&](int t, Spot& s) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int j = min(begin + t * kDecTile + 16 * h + i, end - 1);
+            const uint32_t p = (uint32_t)see.position(j), e = a.p.by_page.div(p);
+            s.off[h] = (int)(p - e * a.p.page);
+            s.page[h] = table[e];
+        }
+    };
+    u4_t k[2][kLoads], v[2][kLoads];
+    float ks[2], vs[2];
+    uint32_t live = 0;   // positions of the tile in k that count
+    const uint8_t* row[2];
+    const float* srow[2];
+    auto aim = [&](int t, const Spot& s) {   // where tile t's rows are, and which count
+        uint32_t ok[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool have = (unsigned)s.page[h] < (unsigned)a.p.n_pages;
+            const bool in = begin + t * kDecTile + 16 * h + i < end;
+            if (in && !have) err |= RTA_DEVERR_PAGES;
+            const uint8_t* page = a.p.pool + (have ? s.page[h] : 0) * a.p.page_bytes;
+            const int64_t at = (int64_t)kvh * a.p.page + s.off[h];
+            row[h] = page + at * (HD * kB) + 16 * u;
+            srow[h] = reinterpret_cast<const float*>(page + 2 * v_off) + at;
+            ok[h] = (uint32_t)__builtin_amdgcn_ballot_w64(in && have) & 0xffffu;
+        }
+        live = ok[0] | ok[1] << 16;
+    };
+    auto load_k = [&] {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x) k[h][x] = *reinterpret_cast<const u4_t*>(row[h] + 64 * x);
+            if constexpr (kScaled) {
+                ks[h] = *srow[h];
+                vs[h] = srow[h][plane];
+            }
+        }
+    };
+    auto load_v = [&] {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x) v[h][x] = *reinterpret_cast<const u4_t*>(row[h] + v_off + 64 * x);
+    };
+
+    Spot next;
+    if (wave < ntile) {
+        spot(wave, next);
+        aim(wave, next);
+        load_k();
+        load_v();
+        spot(wave + kDecWaves, next);   // clamped past the end
+    }
+    for (int t = wave; t < ntile; t += kDecWaves) {
+        const uint32_t now = live;
+        const bool more = t + kDecWaves < ntile;
+        // scores of positions 4u + e (h = 0) and 16 + 4u + e (h = 1) in column i
+        f4_t s[NC][2];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kb = 0; kb < kKb; ++kb) {
+            u4_t ka[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (FMT == RTA_Q8_ROW) {
+                    const int x = kb >> 1, b = 2 * (kb & 1);
+                    uint32_t w[4];
+                    codes_to_half(k[h][x][b], w[0], w[1]);
+                    codes_to_half(k[h][x][b + 1], w[2], w[3]);
+                    ka[h] = u4_t{w[0], w[1], w[2], w[3]};
+                } else {
+                    ka[h] = k[h][kb];
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int op = 0; op < kOps; ++op) {
+                    const u4_t qb = *reinterpret_cast<const u4_t*>(lds + (((c * kOps + op) * kKb + kb) * 64 + lane) * 16);
+                    s[c][0] = page_mfma<FMT>(ka[0], qb, s[c][0]);
+                    s[c][1] = page_mfma<FMT>(ka[1], qb, s[c][1]);
+                }
+        }
+        // the tile's scales, from the lane of a position to the lanes that score it
+        f4_t kf[2], vf[2];
+        if constexpr (kScaled) {
+            if (u == 0) {
+                sl[i] = ks[0];
+                sl[16 + i] = ks[1];
+                sl[32 + i] = vs[0];
+                sl[48 + i] = vs[1];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                kf[h] = *reinterpret_cast<const f4_t*>(sl + 16 * h + 4 * u);
+                vf[h] = *reinterpret_cast<const f4_t*>(sl + 32 + 16 * h + 4 * u);
+            }
+        }
+        // V into LDS (rows that do not count as zeros), then the next tile's rows
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (now != 0xffffffffu) {   // uniform: the last tile, or one with a page missing
+                const bool on = (now >> (16 * h + i)) & 1u;
+#pragma unroll
+                for (int x = 0; x < kLoads; ++x) v[h][x] = on ? v[h][x] : u4_t{0, 0, 0, 0};
+                if constexpr (kScaled) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) vf[h][e] = (now >> (16 * h + 4 * u + e)) & 1u ? vf[h][e] : 0.0f;
+                }
+            }
+            uint8_t* dst = vl + (16 * h + i) * L::kPitch;
+#pragma unroll
+            for (int x = 0; x < kLoads; ++x) {
+                if constexpr (FMT == RTA_Q8_ROW) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) codes_to_half(v[h][x][y], w[2 * y], w[2 * y + 1]);
+                    *reinterpret_cast<u4_t*>(dst + 128 * x + 32 * u) = u4_t{w[0], w[1], w[2], w[3]};
+                    *reinterpret_cast<u4_t*>(dst + 128 * x + 32 * u + 16) = u4_t{w[4], w[5], w[6], w[7]};
+                } else {
+                    *reinterpret_cast<u4_t*>(dst + 64 * x + 16 * u) = v[h][x];
+                }
+            }
+        }
+        if (more) {
+            aim(t + kDecWaves, next);
+            load_k();
+            load_v();
+            spot(t + 2 * kDecWaves, next);
+        }
+        // value scales: w = p * scale / 2^ve below 2^14
+        float wscale = 16384.0f;
+        int ve_new = ve;
+        if constexpr (kScaled) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(vf[h][e]));
+            ve_new = max(ve, part_exponent(max_xor32(max_xor16(mx))));
+            wscale = ldexpf(1.0f, 14 - ve_new);
+        }
+        // softmax in the lane's column
+        u4_t pb[NC][kOps];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float x[8];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = s[c][j >> 2][j & 3];
+                x[j] = (d + dpp_mov<0xB1>(d)) * fac[c];   // both parts
+                if constexpr (kScaled) x[j] *= kf[j >> 2][j & 3];
+            }
+            if (now != 0xffffffffu) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool on = (now >> (16 * (j >> 2) + 4 * u + (j & 3))) & 1u;
+                    if (on) nonfinite = fmaf(x[j], 0.0f, nonfinite);
+                    x[j] = on ? x[j] : -INFINITY;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) nonfinite = fmaf(x[j], 0.0f, nonfinite);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, x[j]);
+            const float mn = fmaxf(m[c], max_xor32(max_xor16(mx)));
+            const float base = mn == -INFINITY ? 0.0f : mn;   // (all of the tile missing)
+            if (__builtin_amdgcn_ballot_w64(mn > m[c]) || ve_new != ve) {
+                const float al = __builtin_amdgcn_exp2f(m[c] - base), f = kScaled ? ldexpf(al, ve - ve_new) : al;
+                z[c] *= al;
+#pragma unroll
+                for (int d = 0; d < kDt; ++d) o[c][d] *= f;
+            }
+            m[c] = mn;
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(x[j] - base);
+                z[c] += w[j];
+                w[j] *= kScaled ? vf[j >> 2][j & 3] * wscale : wscale;
+            }
+            split_parts<FMT>(w, part, pb[c]);
+        }
+        ve = ve_new;
+#pragma unroll
+        for (int d = 0; d < kDt; ++d) {
+            const uint8_t* src = vl + (4 * u + (i >> 2)) * L::kPitch + 32 * d + 8 * (i & 3);
+            const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)src);
+            const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(src + 16 * L::kPitch));
+            const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+            const u4_t va = {l2.x, l2.y, h2.x, h2.y};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int op = 0; op < kOps; ++op) o[c][d] = page_mfma<FMT>(va, pb[c][op], o[c][d]);
+        }
+    }
+    if (nonfinite != nonfinite) err |= RTA_DEVERR_DETECTOR;
+
+    // join: U of both parts per head and dim in the wave's own LDS, then over the waves
+    float2* mzl = reinterpret_cast<float2*>(lds + L::kQ + kDecWaves * L::kWave);
+    const float unscale = ldexpf(1.0f, (kScaled ? ve : 0) - 14);
+    const int64_t h0 = (int64_t)r * a.hq + (int64_t)kvh * a.group + g0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int g = i >> 1;
+        float zz = add_xor32(add_xor16(z[c]));
+        if (lane < 16 && part == 0) mzl[wave * 8 + g] = float2{m[c], zz};
+        float* ul = reinterpret_cast<float*>(vl) + g * HD;
+#pragma unroll
+        for (int d = 0; d < kDt; ++d) {
+            f4_t x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (o[c][d][e] + dpp_mov<0xB1>(o[c][d][e])) * unscale;
+            if (part == 0) *reinterpret_cast<f4_t*>(ul + 16 * d + 4 * u) = x;
+        }
+        __syncthreads();
+        for (int at = threadIdx.x; at < min(8, heads - 8 * c) * HD; at += 64 * kDecWaves) {
+            const int hd = at / HD, dim = at - hd * HD;
+            float M = -INFINITY, Z = 0.0f, U = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, mzl[w * 8 + hd].x);
+            const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < kDecWaves; ++w) {
+                const float2 t = mzl[w * 8 + hd];
+                const float f = __builtin_amdgcn_exp2f(t.x - base);
+                Z += t.y * f;
+                U += reinterpret_cast<const float*>(lds + L::kQ + w * L::kWave)[at] * f;
+            }
+            const int64_t row_head = h0 + 8 * c + hd;
+            if (a.nchunk == 1) {
+                write_result(a, row_head, HD, dim, U, M * kLn2, Z, err);
+            } else {
+                const int64_t rec = row_head * a.nchunk + blockIdx.z;
+                a.part[rec * HD + dim] = U;
+                if (dim == 0) a.mz[rec] = float2{M, Z};
+            }
+        }
+        if (c + 1 < NC) __syncthreads();
+    }
+    if (err) raise_error(err);
+}
+
+// Joins the chunks of a (row, q head): M = max m, o = sum U e^(m - M) / sum z e^(m - M).  HD / 4
+// lanes of 4 dims by the rest of 256 threads over the chunks.  Bound by latency: the lengths, the
+// (m, z) of the chunks and their U, each one trip.
+template <int HD>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a) {
+    constexpr int kLanes = HD / 4, kRows = 256 / kLanes;
+    __shared__ f4_t us[kRows][kLanes];
+    __shared__ float red[4], zred[4];
+    const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+    uint32_t err = 0;
+    Visible see;
+    const int32_t* table;
+    if (!resolve_row(a, r, table, see, err)) return;   // the chunks have reported what is wrong
+    err = 0;
+    const int64_t at = (int64_t)r * a.hq + h;
+    const int n = (see.count + a.chunk - 1) / a.chunk;
+    const float2* mz = a.mz + at * a.nchunk;
+    float m = -INFINITY;
+    for (int c = tid; c < n; c += 256) m = fmaxf(m, mz[c].x);
+    m = wave_max_dpp(m);
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = M == -INFINITY ? 0.0f : M;
+    const int d = tid % kLanes, k = tid / kLanes;
+    f4_t u = {0.0f, 0.0f, 0.0f, 0.0f};
+    float z = 0.0f;
+    for (int c = k; c < n; c += kRows) {
+        const float2 t = mz[c];
+        const float f = __builtin_amdgcn_exp2f(t.x - base);
+        z += t.y * f;
+        u += *reinterpret_cast<const f4_t*>(a.part + (at * a.nchunk + c) * HD + 4 * d) * f;
+    }
+    us[k][d] = u;
+    // lanes of one row hold the same z: one of them counts
+    const float zw = wave_sum_dpp(d == 0 ? z : 0.0f);
+    if ((tid & 63) == 0) zred[tid >> 6] = zw;
+    __syncthreads();
+    if (tid >= HD) return;
+    const float Z = (zred[0] + zred[1]) + (zred[2] + zred[3]);
+    float U = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) U += us[j][tid >> 2][tid & 3];
+    write_result(a, at, HD, tid, U, M * kLn2, Z, err);
+    if (err) raise_error(err);
+}
+
+}  // namespace rta
