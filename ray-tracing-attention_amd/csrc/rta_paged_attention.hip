@@ -202,7 +202,7 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
             a.nchunk = cut.nchunk;
             a.part = static_cast<float*>(workspace);
             a.mz = reinterpret_cast<float2*>(a.part + (size_t)rows * hq * cut.nchunk * HD);
-            const dim3 grid(rows, heads, cut.nchunk), block(64 * kDecWaves);
+            const dim3 grid(rows * heads, 1, cut.nchunk), block(64 * kDecWaves);
             if constexpr (HD < 256) {
                 if (decode_nc(a.group, HD) == 2) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2>), grid, block, 0, s, a);
                 else hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1>), grid, block, 0, s, a);

@@ -30,11 +30,13 @@ struct DecLds {
     static constexpr int kWave = kV + kS;
     static constexpr int kHeads = 8 * NC;
     static constexpr int kTotal = kQ + kDecWaves * kWave + kDecWaves * kHeads * 8;   // and (m, z) per wave and head
-    static_assert(kHeads * HD * 4 <= kV || NC > 1, "U of a wave fits its V rows");
+    static_assert(8 * HD * 4 <= kV, "U of a wave's 8 heads fits its V rows");
+    // waves per SIMD, by registers: 168 hold keys, values and sums of 128-wide heads
+    static constexpr int kPerSimd = HD == 64 ? (NC == 1 ? 4 : 2) : HD == 128 && NC == 1 ? 3 : HD == 128 ? 2 : 1;
 };
 
 template <int FMT, int HD, int NC>
-__global__ void __launch_bounds__(64 * kDecWaves) paged_decode_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd)) paged_decode_kernel(const PagedAttnArgs a) {
     using L = DecLds<FMT, HD, NC>;
     constexpr int kOps = PageFmt<FMT>::kOps, kB = PageFmt<FMT>::kBytes;
     constexpr int kKb = HD / 32;                // products per 16 positions
@@ -42,10 +44,14 @@ __global__ void __launch_bounds__(64 * kDecWaves) paged_decode_kernel(const Page
     constexpr int kDt = HD / 16;                // dim tiles of O^T
     constexpr bool kScaled = PageFmt<FMT>::kScaled;
     __shared__ __align__(16) uint8_t lds[L::kTotal];
-    const int r = blockIdx.x, lane = threadIdx.x & 63, i = lane & 15, u = lane >> 4;
+    const int lane = threadIdx.x & 63, i = lane & 15, u = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int groups = (a.group + L::kHeads - 1) / L::kHeads;   // head groups of a kv head
-    const int kvh = blockIdx.y / groups, g0 = (blockIdx.y - kvh * groups) * L::kHeads;
+    // Workgroups go round the 8 XCDs in order.  Heads first and rows turned by the chunk keep a long
+    // row's chunks on all of them (rows first: 32 rows of 256 to 8192 bf16 positions 124 us, so 65)
+    const int per_row = a.p.kv_heads * groups, y = blockIdx.x % per_row;
+    const int r = (int)((blockIdx.x / per_row + blockIdx.z) % a.l.rows);
+    const int kvh = y / groups, g0 = (y - kvh * groups) * L::kHeads;
     const int heads = min(a.group - g0, L::kHeads);             // q heads of this workgroup
     uint32_t err = 0;
     Visible see;
@@ -56,37 +62,6 @@ __global__ void __launch_bounds__(64 * kDecWaves) paged_decode_kernel(const Page
     }
     const int begin = blockIdx.z * a.chunk, end = see.count - begin > a.chunk ? begin + a.chunk : see.count;
     if (begin >= end && blockIdx.z > 0) return;
-
-    // q as B operands, one wave per quarter of the products; column 2 g + part.  Every wave finds
-    // the heads' largest |q| (the power of two of binary16 operands).
-    const int part = i & 1;
-    float fac[NC];   // score = product * fac, in powers of two: 1 / s / sqrt(HD) * log2 e
-    int qe[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int g = 8 * c + (i >> 1);
-        const float* q = a.q + r * a.q_stride + ((int64_t)kvh * a.group + g0 + min(g, heads - 1)) * HD;
-        qe[c] = 14;
-        if constexpr (FMT != RTA_BF16) {
-            float mx = 0.0f;
-#pragma unroll
-            for (int j = 0; j < HD / 4; ++j) mx = fmaxf(mx, fabsf(q[u * (HD / 4) + j]));
-            qe[c] = part_exponent(max_xor32(max_xor16(mx)));
-        }
-        fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe[c] - 14);
-        for (int kb = wave; kb < kKb; kb += kDecWaves) {
-            float v[8];
-            const float sg = ldexpf(1.0f, 14 - qe[c]);
-#pragma unroll
-            for (int s = 0; s < 8; ++s) v[s] = q[operand_dim<FMT>(kb, u) + s] * sg;
-            u4_t op[kOps];
-            split_parts<FMT>(v, part, op);
-#pragma unroll
-            for (int o = 0; o < kOps; ++o)
-                *reinterpret_cast<u4_t*>(lds + (((c * kOps + o) * kKb + kb) * 64 + lane) * 16) = op[o];
-        }
-    }
-    __syncthreads();
 
     uint8_t* vl = lds + L::kQ + wave * L::kWave;
     float* sl = reinterpret_cast<float*>(vl + L::kV);
@@ -157,6 +132,7 @@ __global__ void __launch_bounds__(64 * kDecWaves) paged_decode_kernel(const Page
             for (int x = 0; x < kLoads; ++x) v[h][x] = *reinterpret_cast<const u4_t*>(row[h] + v_off + 64 * x);
     };
 
+    // the first tile's rows are on their way while q is prepared
     Spot next;
     if (wave < ntile) {
         spot(wave, next);
@@ -165,6 +141,38 @@ __global__ void __launch_bounds__(64 * kDecWaves) paged_decode_kernel(const Page
         load_v();
         spot(wave + kDecWaves, next);   // clamped past the end
     }
+
+    // q as B operands, one wave per quarter of the products; column 2 g + part.  Every wave finds
+    // the heads' largest |q| (the power of two of binary16 operands).
+    const int part = i & 1;
+    float fac[NC];   // score = product * fac, in powers of two: 1 / s / sqrt(HD) * log2 e
+    int qe[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int g = 8 * c + (i >> 1);
+        const float* q = a.q + r * a.q_stride + ((int64_t)kvh * a.group + g0 + min(g, heads - 1)) * HD;
+        qe[c] = 14;
+        if constexpr (FMT != RTA_BF16) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int j = 0; j < HD / 4; ++j) mx = fmaxf(mx, fabsf(q[u * (HD / 4) + j]));
+            qe[c] = part_exponent(max_xor32(max_xor16(mx)));
+        }
+        fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe[c] - 14);
+        for (int kb = wave; kb < kKb; kb += kDecWaves) {
+            float v[8];
+            const float sg = ldexpf(1.0f, 14 - qe[c]);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) v[s] = q[operand_dim<FMT>(kb, u) + s] * sg;
+            u4_t op[kOps];
+            split_parts<FMT>(v, part, op);
+#pragma unroll
+            for (int o = 0; o < kOps; ++o)
+                *reinterpret_cast<u4_t*>(lds + (((c * kOps + o) * kKb + kb) * 64 + lane) * 16) = op[o];
+        }
+    }
+    __syncthreads();
+
     for (int t = wave; t < ntile; t += kDecWaves) {
         const uint32_t now = live;
         const bool more = t + kDecWaves < ntile;
