@@ -41,6 +41,9 @@ struct PagedAttnArgs {
     // work split: chunks of `chunk` visible positions; with nchunk > 1 every (row, q head, chunk)
     // leaves U[HD] in `part` and (m, z) in `mz`, both [row][hq][nchunk]
     int chunk, nchunk;
+    // several rows per entry: tiles of `cols` (row, q head) columns, `ntile` of them at most (0:
+    // one row per entry, a chunk counts along that row's own visible positions)
+    int cols, ntile;
     float* part;
     float2* mz;
 };

@@ -367,50 +367,4 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
     if (err) raise_error(err);
 }
 
-// Joins the chunks of a (row, q head): M = max m, o = sum U e^(m - M) / sum z e^(m - M).  HD / 4
-// lanes of 4 dims by the rest of 256 threads over the chunks.  Bound by latency: the lengths, the
-// (m, z) of the chunks and their U, each one trip.
-template <int HD>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a) {
-    constexpr int kLanes = HD / 4, kRows = 256 / kLanes;
-    __shared__ f4_t us[kRows][kLanes];
-    __shared__ float red[4], zred[4];
-    const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-    uint32_t err = 0;
-    Visible see;
-    const int32_t* table;
-    if (!resolve_row(a, r, table, see, err)) return;   // the chunks have reported what is wrong
-    err = 0;
-    const int64_t at = (int64_t)r * a.hq + h;
-    const int n = (see.count + a.chunk - 1) / a.chunk;
-    const float2* mz = a.mz + at * a.nchunk;
-    float m = -INFINITY;
-    for (int c = tid; c < n; c += 256) m = fmaxf(m, mz[c].x);
-    m = wave_max_dpp(m);
-    if ((tid & 63) == 0) red[tid >> 6] = m;
-    __syncthreads();
-    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = M == -INFINITY ? 0.0f : M;
-    const int d = tid % kLanes, k = tid / kLanes;
-    f4_t u = {0.0f, 0.0f, 0.0f, 0.0f};
-    float z = 0.0f;
-    for (int c = k; c < n; c += kRows) {
-        const float2 t = mz[c];
-        const float f = __builtin_amdgcn_exp2f(t.x - base);
-        z += t.y * f;
-        u += *reinterpret_cast<const f4_t*>(a.part + (at * a.nchunk + c) * HD + 4 * d) * f;
-    }
-    us[k][d] = u;
-    // lanes of one row hold the same z: one of them counts
-    const float zw = wave_sum_dpp(d == 0 ? z : 0.0f);
-    if ((tid & 63) == 0) zred[tid >> 6] = zw;
-    __syncthreads();
-    if (tid >= HD) return;
-    const float Z = (zred[0] + zred[1]) + (zred[2] + zred[3]);
-    float U = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kRows; ++j) U += us[j][tid >> 2][tid & 3];
-    write_result(a, at, HD, tid, U, M * kLn2, Z, err);
-    if (err) raise_error(err);
-}
-
 }  // namespace rta

@@ -1,0 +1,437 @@
+// rta_paged_prompt.hpp -- causal attention of several rows per sequence over its pages.
+//
+// Bound by the matrix cores: 4 hq HD operations per (row, position), twice that with q and the
+// weights in two binary16 parts, three times in three bfloat16 parts (rta_paged.hpp).  The columns
+// of a kv head's products are its (row, q head) pairs, so the heads that share keys share their
+// loads and no group size leaves columns empty.  A workgroup of 4 waves takes 4 x 16 NQ columns
+// and the positions that any of them sees, in tiles staged in LDS by all of it (two buffers, one
+// barrier per tile; a row's 16 bytes of padding keep the operand reads off each other's banks);
+// each wave keeps its q operands, running maxima and sums, and O^T in registers.  A tile that
+// every column of a wave sees whole takes no masks, one that no column sees is skipped.
+// The last rows, which see most, come first; kv heads go over the XCDs, so that one L2 serves
+// all rows of a head.  With few workgroups the positions are cut into chunks as well, joined by
+// paged_merge_kernel.
+#pragma once
+#include "rta_paged_decode.hpp"
+
+namespace rta {
+
+template <int FMT, int HD>
+struct PromptLds {
+    static constexpr int kNQ = HD == 256 ? 1 : 2;      // column tiles of a wave
+    static constexpr int kTile = HD == 256 ? 32 : 64;  // positions per tile
+    static constexpr int kCols = 64 * kNQ;             // columns of a workgroup
+    static constexpr int kPitch = 2 * HD + 16;
+    static constexpr int kRows = 2 * kTile * kPitch;   // keys, then values
+    static constexpr int kScales = PageFmt<FMT>::kScaled ? 2 * kTile * 4 : 0;
+    static constexpr int kBuf = kRows + kScales + kTile * 4;   // and which rows count
+    static constexpr int kTotal = 2 * kBuf;
+};
+
+typedef f4_t f4u_t __attribute__((aligned(4)));   // at an address of a multiple of 4
+
+// What the columns [tile kCols, ..) of an entry of `count` rows and a sequence of `len` positions
+// see, any of them; t0: the first one's position.
+__device__ __forceinline__ Visible prompt_span(const PagedAttnArgs& a, int len, int count, int tile, int cols) {
+    const int tok0 = (int)((int64_t)tile * cols / a.group);
+    const int tok1 = min((int)(((int64_t)(tile + 1) * cols - 1) / a.group), count - 1);
+    const int t0 = max(len - count + tok0, 0), t1 = len - count + tok1;
+    if (t1 < 0) return Visible{0, 0, 0};
+    const int lo = a.window > 0 && t0 >= a.window ? t0 - a.window + 1 : 0;
+    const int head = min(lo, a.sinks);
+    return Visible{head, lo, head + t1 + 1 - lo};
+}
+
+// All parts of eight values as operands.
+template <int FMT>
+__device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float a = v[2 * j], b = v[2 * j + 1];
+        if constexpr (FMT == RTA_BF16) {
+            const float ra = a - cut(a, 0xffff0000u), rb = b - cut(b, 0xffff0000u);
+            op[0][j] = upper_halves(a, b);
+            op[1][j] = upper_halves(ra, rb);
+            op[2][j] = upper_halves(ra - cut(ra, 0xffff0000u), rb - cut(rb, 0xffff0000u));
+        } else {
+            op[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+            op[1][j] = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_pkrtz(a - cut(a, 0xffffe000u), b - cut(b, 0xffffe000u)));
+        }
+    }
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArgs a) {
+    using L = PromptLds<FMT, HD>;
+    constexpr int kParts = FMT == RTA_BF16 ? 3 : 2, kB = PageFmt<FMT>::kBytes, NQ = L::kNQ;
+    constexpr int kKb = HD / 32, kDt = HD / 16;
+    constexpr int kPieces = HD * kB / 16, kStep = 256 / kPieces, kPass = L::kTile / kStep;
+    constexpr bool kScaled = PageFmt<FMT>::kScaled;
+    __shared__ __align__(16) uint8_t lds[L::kTotal];
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, u = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hkv = a.p.kv_heads;
+    const int kvh = blockIdx.x % hkv, rest = blockIdx.x / hkv;
+    const int entry = rest % a.l.n, tile = a.ntile - 1 - rest / a.l.n;
+    uint32_t err = 0;
+    const int base = a.l.cu[entry];
+    int count = a.l.cu[entry + 1] - base;
+    if (base < 0 || base >= a.l.rows || count <= 0) return;
+    int live_rows = min(count, min(a.max_rows, a.l.rows - base));   // rows that are written
+    if (count > a.max_rows && tile == 0) err |= RTA_DEVERR_PAGES;
+    if ((int64_t)tile * L::kCols >= (int64_t)live_rows * a.group) return;
+    const int s = list_seq(a.l.seqs, entry);
+    int len = 0;
+    const int32_t* table = a.p.table;
+    if ((unsigned)s < (unsigned)a.p.max_seqs) {
+        len = a.p.lengths[s];
+        table += (int64_t)s * a.p.max_pages;
+        if (len < 0 || len > a.max_len) {
+            err |= RTA_DEVERR_PAGES;
+            len = 0;
+        } else if (len < count && (len > 0 || count > 1)) {
+            err |= RTA_DEVERR_PAGES;
+        }
+    } else {
+        err |= RTA_DEVERR_PAGES;
+    }
+    const Visible see = len ? prompt_span(a, len, count, tile, L::kCols) : Visible{0, 0, 0};
+    const int begin = blockIdx.z * a.chunk, end = see.count - begin > a.chunk ? begin + a.chunk : see.count;
+    if (begin >= end && blockIdx.z > 0) return;
+    const int nt = (end - begin + L::kTile - 1) / L::kTile;
+
+    // staging: thread -> piece of a row; its rows of a tile are kStep apart
+    const int64_t plane = (int64_t)hkv * a.p.page, v_off = plane * HD * kB;
+    const int piece = tid % kPieces, row0 = tid / kPieces;
+    struct Spot {
+        int page[kPass], off[kPass];
+    };
+    auto spot = [&](int t, Spot& sp) {
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) {
+            const int j = min(begin + t * L::kTile + row0 + k * kStep, end - 1);
+            const uint32_t p = (uint32_t)see.position(j), e = a.p.by_page.div(p);
+            sp.off[k] = (int)(p - e * a.p.page);
+            sp.page[k] = table[e];
+        }
+    };
+    u4_t kr[kPass], vr[kPass];
+    float ksr[kPass], vsr[kPass];
+    uint32_t okr = 0;
+    auto load = [&](int t, const Spot& sp) {
+        okr = 0;
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) {
+            const bool have = (unsigned)sp.page[k] < (unsigned)a.p.n_pages;
+            const bool in = begin + t * L::kTile + row0 + k * kStep < end;
+            if (in && !have) err |= RTA_DEVERR_PAGES;
+            if (in && have) okr |= 1u << k;
+            const uint8_t* page = a.p.pool + (have ? sp.page[k] : 0) * a.p.page_bytes;
+            const int64_t at = (int64_t)kvh * a.p.page + sp.off[k];
+            const uint8_t* src = page + at * (HD * kB) + 16 * piece;
+            kr[k] = *reinterpret_cast<const u4_t*>(src);
+            vr[k] = *reinterpret_cast<const u4_t*>(src + v_off);
+            if constexpr (kScaled) {
+                const float* f = reinterpret_cast<const float*>(page + 2 * v_off) + at;
+                ksr[k] = f[0];
+                vsr[k] = f[plane];
+            }
+        }
+    };
+    auto put = [&](uint8_t* dst, u4_t x) {   // one piece as 2-byte elements
+        if constexpr (FMT == RTA_Q8_ROW) {
+            uint32_t w[8];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) codes_to_half(x[y], w[2 * y], w[2 * y + 1]);
+            *reinterpret_cast<u4_t*>(dst + 32 * piece) = u4_t{w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<u4_t*>(dst + 32 * piece + 16) = u4_t{w[4], w[5], w[6], w[7]};
+        } else {
+            *reinterpret_cast<u4_t*>(dst + 16 * piece) = x;
+        }
+    };
+    auto store = [&](uint8_t* buf) {
+#pragma unroll
+        for (int k = 0; k < kPass; ++k) {
+            const int row = row0 + k * kStep;
+            const bool ok = (okr >> k) & 1u;
+            // rows that do not count are zeros: a weight of 0 times what lies there must be 0
+            const u4_t zero = {0, 0, 0, 0};
+            put(buf + row * L::kPitch, ok ? kr[k] : zero);
+            put(buf + (L::kTile + row) * L::kPitch, ok ? vr[k] : zero);
+            if constexpr (!kScaled) {   // a key with every exponent bit set: inf or NaN
+                constexpr uint32_t kE = FMT == RTA_BF16 ? 0x7f807f80u : 0x7c007c00u;
+                uint32_t hit = 0;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const uint32_t n = ~kr[k][y] & kE;   // a half of zeros: all set
+                    hit |= (uint32_t)((n & 0xffffu) == 0u) | (uint32_t)((n & 0xffff0000u) == 0u);
+                }
+                if (ok && hit) err |= RTA_DEVERR_DETECTOR;
+            } else if (ok && !(fabsf(ksr[k]) < INFINITY)) {
+                err |= RTA_DEVERR_DETECTOR;
+            }
+            if (piece == 0) {
+                if constexpr (kScaled) {
+                    float* f = reinterpret_cast<float*>(buf + L::kRows);
+                    f[row] = ok ? ksr[k] : 0.0f;
+                    f[L::kTile + row] = ok ? vsr[k] : 0.0f;
+                }
+                reinterpret_cast<uint32_t*>(buf + L::kRows + L::kScales)[row] = ok;
+            }
+        }
+    };
+    Spot next;
+    if (nt > 0) {
+        spot(0, next);
+        load(0, next);
+        spot(1, next);
+    }
+
+    // the lane's columns: (row, head) pairs, their positions and q operands
+    const int col0 = tile * L::kCols + wave * 16 * NQ, cols = live_rows * a.group;
+    const bool on = col0 < cols;   // uniform: this wave has columns
+    int t_col[NQ];
+    u4_t qb[NQ][kKb][kParts];
+    float fac[NQ];
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        const int col = min(col0 + 16 * c + i, cols - 1), tok = col / a.group, g = col - tok * a.group;
+        t_col[c] = len - count + tok;
+        const float* q = a.q + (int64_t)(base + tok) * a.q_stride + ((int64_t)kvh * a.group + g) * HD;
+        float v[kKb][8], mx = 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[kb][e] = q[32 * kb + 8 * u + e];
+                mx = fmaxf(mx, fabsf(v[kb][e]));
+            }
+        int qe = 14;
+        if constexpr (FMT != RTA_BF16) qe = part_exponent(max_xor32(max_xor16(mx)));
+        const float sg = ldexpf(1.0f, 14 - qe);
+        fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe - 14);
+#pragma unroll
+        for (int kb = 0; kb < kKb; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[kb][e] *= sg;
+            split_all<FMT>(v[kb], qb[c][kb]);
+        }
+    }
+    // the wave's first and last positions
+    const int t_lo = len - count + col0 / a.group;
+    const int t_hi = len - count + min(col0 + 16 * NQ - 1, cols - 1) / a.group;
+
+    f4_t o[NQ][kDt];
+    // weights are 2^(score - low): low is the largest score less 14, in log2 units
+    float low[NQ], z[NQ];
+    int ve = -110;
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        low[c] = -INFINITY;
+        z[c] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDt; ++d) o[c][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if (nt > 0) store(lds);
+    __syncthreads();
+
+    for (int t = 0; t < nt; ++t) {
+        const uint8_t* buf = lds + (t & 1) * L::kBuf;
+        if (t + 1 < nt) {
+            load(t + 1, next);
+            spot(t + 2, next);
+        }
+        const int j0 = begin + t * L::kTile, j1 = min(j0 + L::kTile, end) - 1;
+        const int p0 = see.position(j0), p1 = see.position(j1);
+        if (on && p0 <= t_hi) {
+            const uint64_t okm = __builtin_amdgcn_ballot_w64(
+                lane < L::kTile && reinterpret_cast<const uint32_t*>(buf + L::kRows + L::kScales)[lane & (L::kTile - 1)]);
+            const bool whole = okm == (L::kTile == 64 ? ~0ull : 0xffffffffull) && p1 <= t_lo &&
+                               (a.window == 0 || p0 > t_hi - a.window);
+            const float* sc = reinterpret_cast<const float*>(buf + L::kRows);
+            float wscale = 1.0f;
+            int ve_new = ve;
+            if constexpr (kScaled) {   // value scales below 2^0 (weights carry 2^14)
+                const float mx = lane < L::kTile ? fabsf(sc[L::kTile + lane]) : 0.0f;
+                ve_new = max(ve, part_exponent(wave_max_dpp(mx)));
+                wscale = ldexpf(1.0f, -ve_new);
+            }
+#pragma unroll
+            for (int sub = 0; sub < L::kTile / 32; ++sub) {
+                // S^T of 32 positions
+                f4_t x[NQ][2];
+#pragma unroll
+                for (int c = 0; c < NQ; ++c) x[c][0] = x[c][1] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const u4_t ka = *reinterpret_cast<const u4_t*>(buf + (32 * sub + 16 * h + i) * L::kPitch +
+                                                                       64 * kb + 16 * u);
+#pragma unroll
+                        for (int c = 0; c < NQ; ++c)
+#pragma unroll
+                            for (int p = 0; p < kParts; ++p) x[c][h] = page_mfma<FMT>(ka, qb[c][kb][p], x[c][h]);
+                    }
+                f4_t vf[2];
+                if constexpr (kScaled) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const f4_t kf = *reinterpret_cast<const f4_t*>(sc + 32 * sub + 16 * h + 4 * u);
+                        vf[h] = *reinterpret_cast<const f4_t*>(sc + L::kTile + 32 * sub + 16 * h + 4 * u) * wscale;
+#pragma unroll
+                        for (int c = 0; c < NQ; ++c) x[c][h] *= kf;
+                    }
+                }
+                u4_t pb[NQ][kParts];
+#pragma unroll
+                for (int c = 0; c < NQ; ++c) {
+                    if (!whole) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int k = 32 * sub + 16 * h + 4 * u + e, p = see.position(j0 + k);
+                                const bool vis = ((okm >> k) & 1u) && p <= t_col[c] &&
+                                                 (a.window == 0 || p > t_col[c] - a.window || p < a.sinks);
+                                x[c][h][e] = vis ? x[c][h][e] : -INFINITY;
+                            }
+                    }
+                    float mx = x[c][0][0];
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[c][j >> 2][j & 3]);
+                    const float top = fmaxf(low[c], fmaf(max_xor32(max_xor16(mx)), fac[c], -14.0f));
+                    const float base = top == -INFINITY ? 0.0f : top;   // (nothing seen yet: weights 0)
+                    if (__builtin_amdgcn_ballot_w64(top > low[c]) || (kScaled && ve_new != ve)) {
+                        const float al = __builtin_amdgcn_exp2f(low[c] - base);
+                        const float f = kScaled ? ldexpf(al, ve - ve_new) : al;
+                        z[c] *= al;
+#pragma unroll
+                        for (int d = 0; d < kDt; ++d) o[c][d] *= f;
+                        low[c] = top;
+                    }
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        w[j] = __builtin_amdgcn_exp2f(fmaf(x[c][j >> 2][j & 3], fac[c], -base));
+                        z[c] += w[j];
+                        if constexpr (kScaled) w[j] *= vf[j >> 2][j & 3];
+                    }
+                    split_all<FMT>(w, pb[c]);
+                }
+                ve = ve_new;
+                // O^T += V^T P^T
+                const uint8_t* vb = buf + (L::kTile + 32 * sub + 4 * u + (i >> 2)) * L::kPitch + 8 * (i & 3);
+#pragma unroll
+                for (int d = 0; d < kDt; ++d) {
+                    const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(vb + 32 * d));
+                    const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(vb + 16 * L::kPitch + 32 * d));
+                    const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+                    const u4_t va = {l2.x, l2.y, h2.x, h2.y};
+#pragma unroll
+                    for (int c = 0; c < NQ; ++c)
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p) o[c][d] = page_mfma<FMT>(va, pb[c][p], o[c][d]);
+                }
+            }
+        }
+        if (t + 1 < nt) store(lds + ((t + 1) & 1) * L::kBuf);
+        __syncthreads();
+    }
+
+    const float unscale = ldexpf(1.0f, (kScaled ? ve : 0) - 14);
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        const float Z = add_xor32(add_xor16(z[c])) * 0x1p-14f;
+        const int col = col0 + 16 * c + i;
+        if (col >= cols) continue;
+        const int tok = col / a.group, g = col - tok * a.group;
+        const int64_t at = (int64_t)(base + tok) * a.hq + (int64_t)kvh * a.group + g;
+        if (a.nchunk > 1) {
+            const int64_t rec = at * a.nchunk + blockIdx.z;
+#pragma unroll
+            for (int d = 0; d < kDt; ++d)
+                *reinterpret_cast<f4_t*>(a.part + rec * HD + 16 * d + 4 * u) = o[c][d] * unscale;
+            if (u == 0) a.mz[rec] = float2{low[c] + 14.0f, Z};
+            continue;
+        }
+        const float scale = Z > 0.0f || Z != Z ? unscale / Z : 0.0f;   // nothing seen: zeros
+#pragma unroll
+        for (int d = 0; d < kDt; ++d) {
+            const int64_t to = at * HD + 16 * d + 4 * u;
+            f4_t x = o[c][d] * scale;
+            if (a.gate) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] *= detector_sigmoid(a.gate[to + e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!isfinite(x[e])) err |= RTA_DEVERR_DETECTOR;
+            *reinterpret_cast<f4u_t*>(a.out + to) = x;
+        }
+        if (u == 0) {
+            if (a.m_out) a.m_out[at] = (low[c] + 14.0f) * kLn2;
+            if (a.z_out) a.z_out[at] = Z;
+        }
+    }
+    if (err) raise_error(err);
+}
+
+// Joins the chunks of a (row, q head): M = max m, o = sum U e^(m - M) / sum z e^(m - M).  HD / 4
+// lanes of 4 dims by the rest of 256 threads over the chunks.  Bound by latency: the lengths, the
+// (m, z) of the chunks and their U, each one trip.
+template <int HD>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a) {
+    constexpr int kLanes = HD / 4, kRows = 256 / kLanes;
+    __shared__ f4_t us[kRows][kLanes];
+    __shared__ float red[4], zred[4];
+    const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
+    uint32_t err = 0;
+    Visible see;
+    const int32_t* table;
+    if (!resolve_row(a, r, table, see, err)) return;   // the chunks have reported what is wrong
+    err = 0;
+    const int64_t at = (int64_t)r * a.hq + h;
+    int span = see.count;
+    if (a.cols) {   // the chunks of the row's column tile
+        int i, first, count;
+        row_entry(a.l, r, i, first, count);
+        const int s = list_seq(a.l.seqs, i);   // bad ones see nothing
+        if (span) {
+            const int tile = (int)(((int64_t)(r - first) * a.group + h % a.group) / a.cols);
+            span = prompt_span(a, a.p.lengths[s], count, tile, a.cols).count;
+        }
+    }
+    const int n = (int)(((int64_t)span + a.chunk - 1) / a.chunk);
+    const float2* mz = a.mz + at * a.nchunk;
+    float m = -INFINITY;
+    for (int c = tid; c < n; c += 256) m = fmaxf(m, mz[c].x);
+    m = wave_max_dpp(m);
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), base = M == -INFINITY ? 0.0f : M;
+    const int d = tid % kLanes, k = tid / kLanes;
+    f4_t u = {0.0f, 0.0f, 0.0f, 0.0f};
+    float z = 0.0f;
+    for (int c = k; c < n; c += kRows) {
+        const float2 t = mz[c];
+        const float f = __builtin_amdgcn_exp2f(t.x - base);
+        z += t.y * f;
+        u += *reinterpret_cast<const f4_t*>(a.part + (at * a.nchunk + c) * HD + 4 * d) * f;
+    }
+    us[k][d] = u;
+    // lanes of one row hold the same z: one of them counts
+    const float zw = wave_sum_dpp(d == 0 ? z : 0.0f);
+    if ((tid & 63) == 0) zred[tid >> 6] = zw;
+    __syncthreads();
+    if (tid >= HD) return;
+    const float Z = (zred[0] + zred[1]) + (zred[2] + zred[3]);
+    float U = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) U += us[j][tid >> 2][tid & 3];
+    write_result(a, at, HD, tid, U, M * kLn2, Z, err);
+    if (err) raise_error(err);
+}
+
+}  // namespace rta
