@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
     uint8_t* vl = lds + L::kQ + wave * L::kWave;
     float* sl = reinterpret_cast<float*>(vl + L::kV);
     const int64_t plane = (int64_t)a.p.kv_heads * a.p.page;   // rows of a page's keys
-    const int64_t v_off = plane * HD * kB;
+    const int64_t v_off = plane * HD * kB, head_row = (int64_t)kvh * a.p.page, head_off = head_row * HD * kB;
     const int ntile = (end - begin + kDecTile - 1) / kDecTile;
 
     f4_t o[NC][kDt];
@@ -106,10 +106,9 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
             const bool have = (unsigned)s.page[h] < (unsigned)a.p.n_pages;
             const bool in = begin + t * kDecTile + 16 * h + i < end;
             if (in && !have) err |= RTA_DEVERR_PAGES;
-            const uint8_t* page = a.p.pool + (have ? s.page[h] : 0) * a.p.page_bytes;
-            const int64_t at = (int64_t)kvh * a.p.page + s.off[h];
-            row[h] = page + at * (HD * kB) + 16 * u;
-            srow[h] = reinterpret_cast<const float*>(page + 2 * v_off) + at;
+            const uint8_t* page = a.p.pool + page_offset(a.p, have ? s.page[h] : 0);
+            row[h] = page + head_off + (uint32_t)(s.off[h] * (HD * kB) + 16 * u);
+            srow[h] = reinterpret_cast<const float*>(page + 2 * v_off) + head_row + s.off[h];
             ok[h] = (uint32_t)__builtin_amdgcn_ballot_w64(in && have) & 0xffffu;
         }
         live = ok[0] | ok[1] << 16;

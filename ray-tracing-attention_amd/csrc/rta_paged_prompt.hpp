@@ -19,7 +19,7 @@ namespace rta {
 template <int FMT, int HD>
 struct PromptLds {
     static constexpr int kNQ = HD == 256 ? 1 : 2;      // column tiles of a wave
-    static constexpr int kTile = HD == 256 ? 32 : 64;  // positions per tile
+    static constexpr int kTile = HD > 64 ? 32 : 64;    // positions per tile
     static constexpr int kCols = 64 * kNQ;             // columns of a workgroup
     static constexpr int kPitch = 2 * HD + 16;
     static constexpr int kRows = 2 * kTile * kPitch;   // keys, then values
@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
 
     // staging: thread -> piece of a row; its rows of a tile are kStep apart
     const int64_t plane = (int64_t)hkv * a.p.page, v_off = plane * HD * kB;
+    const int64_t head_row = (int64_t)kvh * a.p.page, head_off = head_row * HD * kB;
     const int piece = tid % kPieces, row0 = tid / kPieces;
     struct Spot {
         int page[kPass], off[kPass];
@@ -127,13 +128,12 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
             const bool in = begin + t * L::kTile + row0 + k * kStep < end;
             if (in && !have) err |= RTA_DEVERR_PAGES;
             if (in && have) okr |= 1u << k;
-            const uint8_t* page = a.p.pool + (have ? sp.page[k] : 0) * a.p.page_bytes;
-            const int64_t at = (int64_t)kvh * a.p.page + sp.off[k];
-            const uint8_t* src = page + at * (HD * kB) + 16 * piece;
+            const uint8_t* page = a.p.pool + page_offset(a.p, have ? sp.page[k] : 0);
+            const uint8_t* src = page + head_off + (uint32_t)(sp.off[k] * (HD * kB) + 16 * piece);
             kr[k] = *reinterpret_cast<const u4_t*>(src);
             vr[k] = *reinterpret_cast<const u4_t*>(src + v_off);
             if constexpr (kScaled) {
-                const float* f = reinterpret_cast<const float*>(page + 2 * v_off) + at;
+                const float* f = reinterpret_cast<const float*>(page + 2 * v_off) + head_row + sp.off[k];
                 ksr[k] = f[0];
                 vsr[k] = f[plane];
             }
@@ -151,33 +151,27 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
         }
     };
     auto store = [&](uint8_t* buf) {
+        // rows that do not count are zeros: a weight of 0 times what lies there must be 0
+        if (__builtin_amdgcn_ballot_w64(okr != (1u << kPass) - 1)) {   // the last tile, or a page missing
+#pragma unroll
+            for (int k = 0; k < kPass; ++k)
+                if (!((okr >> k) & 1u)) {
+                    kr[k] = vr[k] = u4_t{0, 0, 0, 0};
+                    if constexpr (kScaled) ksr[k] = vsr[k] = 0.0f;
+                }
+        }
 #pragma unroll
         for (int k = 0; k < kPass; ++k) {
             const int row = row0 + k * kStep;
-            const bool ok = (okr >> k) & 1u;
-            // rows that do not count are zeros: a weight of 0 times what lies there must be 0
-            const u4_t zero = {0, 0, 0, 0};
-            put(buf + row * L::kPitch, ok ? kr[k] : zero);
-            put(buf + (L::kTile + row) * L::kPitch, ok ? vr[k] : zero);
-            if constexpr (!kScaled) {   // a key with every exponent bit set: inf or NaN
-                constexpr uint32_t kE = FMT == RTA_BF16 ? 0x7f807f80u : 0x7c007c00u;
-                uint32_t hit = 0;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const uint32_t n = ~kr[k][y] & kE;   // a half of zeros: all set
-                    hit |= (uint32_t)((n & 0xffffu) == 0u) | (uint32_t)((n & 0xffff0000u) == 0u);
-                }
-                if (ok && hit) err |= RTA_DEVERR_DETECTOR;
-            } else if (ok && !(fabsf(ksr[k]) < INFINITY)) {
-                err |= RTA_DEVERR_DETECTOR;
-            }
+            put(buf + row * L::kPitch, kr[k]);
+            put(buf + (L::kTile + row) * L::kPitch, vr[k]);
             if (piece == 0) {
                 if constexpr (kScaled) {
                     float* f = reinterpret_cast<float*>(buf + L::kRows);
-                    f[row] = ok ? ksr[k] : 0.0f;
-                    f[L::kTile + row] = ok ? vsr[k] : 0.0f;
+                    f[row] = ksr[k];
+                    f[L::kTile + row] = vsr[k];
                 }
-                reinterpret_cast<uint32_t*>(buf + L::kRows + L::kScales)[row] = ok;
+                reinterpret_cast<uint32_t*>(buf + L::kRows + L::kScales)[row] = (okr >> k) & 1u;
             }
         }
     };
@@ -223,12 +217,14 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     const int t_hi = len - count + min(col0 + 16 * NQ - 1, cols - 1) / a.group;
 
     f4_t o[NQ][kDt];
-    // weights are 2^(score - low): low is the largest score less 14, in log2 units
-    float low[NQ], z[NQ];
+    // weights are 2^(score - low) in log2 units, 2^kTop for the largest score when low was set and
+    // below 2^(kTop + kSlack) <= 2^15 until it is set again
+    constexpr float kTop = 8.0f, kSlack = 7.0f;
+    float m[NQ], low[NQ], z[NQ], lowest = INFINITY;   // m, lowest: of the products
     int ve = -110;
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-        low[c] = -INFINITY;
+        m[c] = low[c] = -INFINITY;
         z[c] = 0.0f;
 #pragma unroll
         for (int d = 0; d < kDt; ++d) o[c][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -252,7 +248,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
             const float* sc = reinterpret_cast<const float*>(buf + L::kRows);
             float wscale = 1.0f;
             int ve_new = ve;
-            if constexpr (kScaled) {   // value scales below 2^0 (weights carry 2^14)
+            if constexpr (kScaled) {   // value scales below 2^0
                 const float mx = lane < L::kTile ? fabsf(sc[L::kTile + lane]) : 0.0f;
                 ve_new = max(ve, part_exponent(wave_max_dpp(mx)));
                 wscale = ldexpf(1.0f, -ve_new);
@@ -284,33 +280,55 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                         for (int c = 0; c < NQ; ++c) x[c][h] *= kf;
                     }
                 }
-                u4_t pb[NQ][kParts];
+                float mx[NQ];
 #pragma unroll
                 for (int c = 0; c < NQ; ++c) {
-                    if (!whole) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
+                    for (int j = 0; j < 8; ++j) lowest = fminf(lowest, x[c][j >> 2][j & 3]);
+                }
+                if (!whole) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int k = 32 * sub + 16 * h + 4 * u + e, p = see.position(j0 + k);
-                                const bool vis = ((okm >> k) & 1u) && p <= t_col[c] &&
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int k = 32 * sub + 16 * h + 4 * u + e, p = see.position(j0 + k);
+                            const bool ok = (okm >> k) & 1u;
+#pragma unroll
+                            for (int c = 0; c < NQ; ++c) {
+                                const bool vis = ok && p <= t_col[c] &&
                                                  (a.window == 0 || p > t_col[c] - a.window || p < a.sinks);
                                 x[c][h][e] = vis ? x[c][h][e] : -INFINITY;
                             }
-                    }
-                    float mx = x[c][0][0];
+                        }
+                }
+                // the running maximum, and the weights' base behind it: it follows only when weights
+                // would pass 2^15, so that sums are seldom rescaled
+                bool lift = kScaled && ve_new != ve;
 #pragma unroll
-                    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[c][j >> 2][j & 3]);
-                    const float top = fmaxf(low[c], fmaf(max_xor32(max_xor16(mx)), fac[c], -14.0f));
-                    const float base = top == -INFINITY ? 0.0f : top;   // (nothing seen yet: weights 0)
-                    if (__builtin_amdgcn_ballot_w64(top > low[c]) || (kScaled && ve_new != ve)) {
-                        const float al = __builtin_amdgcn_exp2f(low[c] - base);
+                for (int c = 0; c < NQ; ++c) {
+                    mx[c] = x[c][0][0];
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) mx[c] = fmaxf(mx[c], x[c][j >> 2][j & 3]);
+                    m[c] = fmaxf(m[c], max_xor32(max_xor16(mx[c])));
+                    mx[c] = fmaf(m[c], fac[c], -kTop);   // the base that the maximum asks for
+                    lift = lift || mx[c] > low[c] + kSlack;
+                }
+                if (__builtin_amdgcn_ballot_w64(lift)) {
+#pragma unroll
+                    for (int c = 0; c < NQ; ++c) {
+                        const float base = mx[c] > low[c] ? mx[c] : low[c];
+                        const float al = __builtin_amdgcn_exp2f(low[c] - (base == -INFINITY ? 0.0f : base));
                         const float f = kScaled ? ldexpf(al, ve - ve_new) : al;
                         z[c] *= al;
 #pragma unroll
                         for (int d = 0; d < kDt; ++d) o[c][d] *= f;
-                        low[c] = top;
+                        low[c] = base;
                     }
+                }
+                u4_t pb[NQ][kParts];
+#pragma unroll
+                for (int c = 0; c < NQ; ++c) {
+                    const float base = low[c] == -INFINITY ? 0.0f : low[c];   // (nothing seen yet: weights 0)
                     float w[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
@@ -340,10 +358,12 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
         __syncthreads();
     }
 
-    const float unscale = ldexpf(1.0f, (kScaled ? ve : 0) - 14);
+    if (lowest == -INFINITY) err |= RTA_DEVERR_DETECTOR;   // (larger ones and NaN reach the results)
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-        const float Z = add_xor32(add_xor16(z[c])) * 0x1p-14f;
+        // back to the maximum as the base
+        const float M = m[c] * fac[c], back = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(low[c] - M);
+        const float Z = add_xor32(add_xor16(z[c])) * back, unscale = kScaled ? ldexpf(back, ve) : back;
         const int col = col0 + 16 * c + i;
         if (col >= cols) continue;
         const int tok = col / a.group, g = col - tok * a.group;
@@ -353,7 +373,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
 #pragma unroll
             for (int d = 0; d < kDt; ++d)
                 *reinterpret_cast<f4_t*>(a.part + rec * HD + 16 * d + 4 * u) = o[c][d] * unscale;
-            if (u == 0) a.mz[rec] = float2{low[c] + 14.0f, Z};
+            if (u == 0) a.mz[rec] = float2{M, Z};
             continue;
         }
         const float scale = Z > 0.0f || Z != Z ? unscale / Z : 0.0f;   // nothing seen: zeros
@@ -371,7 +391,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
             *reinterpret_cast<f4u_t*>(a.out + to) = x;
         }
         if (u == 0) {
-            if (a.m_out) a.m_out[at] = (low[c] + 14.0f) * kLn2;
+            if (a.m_out) a.m_out[at] = M * kLn2;
             if (a.z_out) a.z_out[at] = Z;
         }
     }

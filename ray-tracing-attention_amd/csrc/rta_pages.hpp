@@ -8,18 +8,17 @@
 
 namespace rta {
 
-// p / d for 0 <= p < 2^31 as (p m) >> sh, m = floor(2^sh / d) + 1, sh = 31 + ceil(log2 d): the
-// error p (m d - 2^sh) / (d 2^sh) stays below 1 / d because m d - 2^sh <= d <= 2^(sh - 31).
+// p / d for 0 <= p < 2^31 and 1 <= d <= 65536 as (p m) >> (31 + l), m = floor(2^(31 + l) / d) + 1,
+// l = ceil(log2 d): the error p (m d - 2^(31 + l)) / (d 2^(31 + l)) stays below 1 / d because
+// m d - 2^(31 + l) <= d <= 2^l.  (2 p m) >> 32 >> l: one multiplication and two shifts.
 struct FastDiv {
-    uint32_t d = 1, m = 0, sh = 31;
+    uint32_t d = 1, m = 0, l = 0;
     FastDiv() = default;
     explicit FastDiv(uint32_t v) : d(v) {
-        uint32_t l = 0;
         while ((1ull << l) < v) ++l;
-        sh = 31 + l;
-        m = (uint32_t)((1ull << sh) / v + 1);
+        m = (uint32_t)((1ull << (31 + l)) / v + 1);
     }
-    __device__ __forceinline__ uint32_t div(uint32_t p) const { return (uint32_t)(((uint64_t)p * m) >> sh); }
+    __device__ __forceinline__ uint32_t div(uint32_t p) const { return __umulhi(2 * p, m) >> l; }
 };
 
 struct PageArgs {
@@ -60,6 +59,11 @@ __device__ __forceinline__ bool row_entry(const RowList& l, int r, int& i, int& 
     first = l.cu[lo];
     count = l.cu[lo + 1] - first;
     return r >= first && r - first < count;
+}
+
+// Byte offset of page pg of a layer: page sizes are multiples of 128 below 2^38.
+__device__ __forceinline__ uint64_t page_offset(const PageArgs& a, int pg) {
+    return ((uint64_t)(uint32_t)pg * (uint32_t)(a.page_bytes >> 7)) << 7;
 }
 
 // Page of position p of a sequence's table row, -1 where there is none.
