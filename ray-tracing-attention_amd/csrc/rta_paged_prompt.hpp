@@ -260,16 +260,19 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
 #pragma unroll
                 for (int c = 0; c < NQ; ++c) x[c][0] = x[c][1] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int kb = 0; kb < kKb; ++kb)
+                for (int kb = 0; kb < kKb; ++kb) {
+                    u4_t ka[2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const u4_t ka = *reinterpret_cast<const u4_t*>(buf + (32 * sub + 16 * h + i) * L::kPitch +
-                                                                       64 * kb + 16 * u);
+                    for (int h = 0; h < 2; ++h)
+                        ka[h] = *reinterpret_cast<const u4_t*>(buf + (32 * sub + 16 * h + i) * L::kPitch + 64 * kb +
+                                                               16 * u);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)   // neighbours go into different accumulators
 #pragma unroll
                         for (int c = 0; c < NQ; ++c)
 #pragma unroll
-                            for (int p = 0; p < kParts; ++p) x[c][h] = page_mfma<FMT>(ka, qb[c][kb][p], x[c][h]);
-                    }
+                            for (int h = 0; h < 2; ++h) x[c][h] = page_mfma<FMT>(ka[h], qb[c][kb][p], x[c][h]);
+                }
                 f4_t vf[2];
                 if constexpr (kScaled) {
 #pragma unroll
@@ -342,15 +345,22 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                 // O^T += V^T P^T
                 const uint8_t* vb = buf + (L::kTile + 32 * sub + 4 * u + (i >> 2)) * L::kPitch + 8 * (i & 3);
 #pragma unroll
-                for (int d = 0; d < kDt; ++d) {
-                    const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(vb + 32 * d));
-                    const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(vb + 16 * L::kPitch + 32 * d));
-                    const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-                    const u4_t va = {l2.x, l2.y, h2.x, h2.y};
+                for (int d = 0; d < kDt; d += 2) {
+                    u4_t va[2];
 #pragma unroll
-                    for (int c = 0; c < NQ; ++c)
+                    for (int y = 0; y < 2; ++y) {
+                        const uint8_t* src = vb + 32 * (d + y);
+                        const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)src);
+                        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(src + 16 * L::kPitch));
+                        const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+                        va[y] = u4_t{l2.x, l2.y, h2.x, h2.y};
+                    }
 #pragma unroll
-                        for (int p = 0; p < kParts; ++p) o[c][d] = page_mfma<FMT>(va, pb[c][p], o[c][d]);
+                    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+#pragma unroll
+                            for (int c = 0; c < NQ; ++c) o[c][d + y] = page_mfma<FMT>(va[y], pb[c][p], o[c][d + y]);
                 }
             }
         }
