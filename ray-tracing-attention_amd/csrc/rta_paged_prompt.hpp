@@ -25,7 +25,8 @@ struct PromptLds {
     static constexpr int kRows = 2 * kTile * kPitch;   // keys, then values
     static constexpr int kScales = PageFmt<FMT>::kScaled ? 2 * kTile * 4 : 0;
     static constexpr int kBuf = kRows + kScales + kTile * 4;   // and which rows count
-    static constexpr int kTotal = 2 * kBuf;
+    static constexpr int kThird = FMT == RTA_BF16 ? kNQ * (HD / 32) * 1024 : 0;   // per wave: q's third part
+    static constexpr int kTotal = 2 * kBuf + 4 * kThird;
 };
 
 typedef f4_t f4u_t __attribute__((aligned(4)));   // at an address of a multiple of 4
@@ -66,6 +67,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     using L = PromptLds<FMT, HD>;
     constexpr int kParts = FMT == RTA_BF16 ? 3 : 2, kB = PageFmt<FMT>::kBytes, NQ = L::kNQ;
     constexpr int kKb = HD / 32, kDt = HD / 16;
+    constexpr int kKg = kKb < 4 ? kKb : 4, kDg = 4;   // operands read ahead
     constexpr int kPieces = HD * kB / 16, kStep = 256 / kPieces, kPass = L::kTile / kStep;
     constexpr bool kScaled = PageFmt<FMT>::kScaled;
     __shared__ __align__(16) uint8_t lds[L::kTotal];
@@ -186,7 +188,8 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     const int col0 = tile * L::kCols + wave * 16 * NQ, cols = live_rows * a.group;
     const bool on = col0 < cols;   // uniform: this wave has columns
     int t_col[NQ];
-    u4_t qb[NQ][kKb][kParts];
+    u4_t qb[NQ][kKb][2];   // (the third part of bfloat16 lies in LDS: 96 registers would leave none for operands)
+    u4_t* third = reinterpret_cast<u4_t*>(lds + 2 * L::kBuf + wave * L::kThird) + lane;
     float fac[NQ];
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
@@ -209,7 +212,11 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
         for (int kb = 0; kb < kKb; ++kb) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[kb][e] *= sg;
-            split_all<FMT>(v[kb], qb[c][kb]);
+            u4_t part[kParts];
+            split_all<FMT>(v[kb], part);
+            qb[c][kb][0] = part[0];
+            qb[c][kb][1] = part[1];
+            if constexpr (kParts == 3) third[(c * kKb + kb) * 64] = part[2];
         }
     }
     // the wave's first and last positions
@@ -260,19 +267,41 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
 #pragma unroll
                 for (int c = 0; c < NQ; ++c) x[c][0] = x[c][1] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int kb = 0; kb < kKb; ++kb) {
-                    u4_t ka[2];
+                for (int k0 = 0; k0 < kKb; k0 += kKg) {
+                    u4_t ka[kKg][2];   // all on their way before the first product
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        ka[h] = *reinterpret_cast<const u4_t*>(buf + (32 * sub + 16 * h + i) * L::kPitch + 64 * kb +
-                                                               16 * u);
+                    for (int k = 0; k < kKg; ++k)
 #pragma unroll
-                    for (int p = 0; p < kParts; ++p)   // neighbours go into different accumulators
+                        for (int h = 0; h < 2; ++h)
+                            ka[k][h] = *reinterpret_cast<const u4_t*>(buf + (32 * sub + 16 * h + i) * L::kPitch +
+                                                                      64 * (k0 + k) + 16 * u);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int c = 0; c < NQ; ++c)
+                    for (int k = 0; k < kKg; ++k)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) x[c][h] = page_mfma<FMT>(ka[h], qb[c][kb][p], x[c][h]);
+                        for (int p = 0; p < kParts; ++p)   // neighbours go into different accumulators
+#pragma unroll
+                            for (int c = 0; c < NQ; ++c) {
+                                const u4_t q = p < 2 ? qb[c][k0 + k][p & 1] : third[(c * kKb + k0 + k) * 64];
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) x[c][h] = page_mfma<FMT>(ka[k][h], q, x[c][h]);
+                            }
                 }
+                // the first of V^T's operands, ready when the weights are
+                const uint8_t* vb = buf + (L::kTile + 32 * sub + 4 * u + (i >> 2)) * L::kPitch + 8 * (i & 3);
+                u4_t va[2][kDg];
+                auto load_va = [&](int d0) {
+#pragma unroll
+                    for (int d = 0; d < kDg; ++d) {
+                        const uint8_t* src = vb + 32 * (d0 + d);
+                        const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)src);
+                        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(src + 16 * L::kPitch));
+                        const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+                        va[(d0 / kDg) & 1][d] = u4_t{l2.x, l2.y, h2.x, h2.y};
+                    }
+                };
+                load_va(0);
+                __builtin_amdgcn_sched_barrier(0);
                 f4_t vf[2];
                 if constexpr (kScaled) {
 #pragma unroll
@@ -343,24 +372,18 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                 }
                 ve = ve_new;
                 // O^T += V^T P^T
-                const uint8_t* vb = buf + (L::kTile + 32 * sub + 4 * u + (i >> 2)) * L::kPitch + 8 * (i & 3);
 #pragma unroll
-                for (int d = 0; d < kDt; d += 2) {
-                    u4_t va[2];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const uint8_t* src = vb + 32 * (d + y);
-                        const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)src);
-                        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(src + 16 * L::kPitch));
-                        const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-                        va[y] = u4_t{l2.x, l2.y, h2.x, h2.y};
+                for (int d0 = 0; d0 < kDt; d0 += kDg) {
+                    if (d0 + kDg < kDt) {
+                        load_va(d0 + kDg);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
 #pragma unroll
                     for (int p = 0; p < kParts; ++p)
 #pragma unroll
-                        for (int y = 0; y < 2; ++y)
+                        for (int d = 0; d < kDg; ++d)
 #pragma unroll
-                            for (int c = 0; c < NQ; ++c) o[c][d + y] = page_mfma<FMT>(va[y], pb[c][p], o[c][d + y]);
+                            for (int c = 0; c < NQ; ++c) o[c][d0 + d] = page_mfma<FMT>(va[(d0 / kDg) & 1][d], pb[c][p], o[c][d0 + d]);
                 }
             }
         }
