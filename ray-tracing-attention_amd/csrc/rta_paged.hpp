@@ -14,8 +14,9 @@
 //   binary16 pages (and 8-bit codes, exact in binary16): two parts, 22 bits, of the value times a
 //   power of two that puts its row's largest in [2^13, 2^14);
 //   bfloat16 pages: three parts of 8 bits, 24 bits and no scale.
-// Two parts are neighbouring columns of one product (query g in columns 2g and 2g + 1), the
-// third a second product into the same accumulator.  One rounding to 16 bits instead would cost
+// Where few of a product's 16 columns are needed, two parts are neighbouring columns (query g in
+// 2g and 2g + 1) and the third a second product into the same accumulator; else every part is a
+// product of its own.  One rounding to 16 bits instead would cost
 // 2^-12 (2^-9) of the result where fp32 results are wanted.
 #pragma once
 #include <math.h>
@@ -102,15 +103,16 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // ---- operands by page format ----
 template <int FMT> struct PageFmt;
 template <> struct PageFmt<RTA_F16> {
-    static constexpr int kBytes = 2, kOps = 1;   // element bytes; products per operand pair
+    // element bytes; parts of a query or weight; products of a pair of operands with parts in columns
+    static constexpr int kBytes = 2, kParts = 2, kOps = 1;
     static constexpr bool kScaled = false;       // scales beside the elements
 };
 template <> struct PageFmt<RTA_BF16> {
-    static constexpr int kBytes = 2, kOps = 2;
+    static constexpr int kBytes = 2, kParts = 3, kOps = 2;
     static constexpr bool kScaled = false;
 };
 template <> struct PageFmt<RTA_Q8_ROW> {
-    static constexpr int kBytes = 1, kOps = 1;
+    static constexpr int kBytes = 1, kParts = 2, kOps = 1;
     static constexpr bool kScaled = true;
 };
 
@@ -177,6 +179,69 @@ __device__ __forceinline__ int part_exponent(float mx) {
     int e = -110;
     if (mx > 0.0f && mx < INFINITY) (void)frexpf(mx, &e);
     return e < -110 ? -110 : e;
+}
+
+// An entry's rows as columns (row, q head of one kv head): column c is row c / group.
+struct Entry {
+    int base, count;    // its first row and how many it has
+    int rows;           // of which this many are written
+    int len;            // its sequence's positions, 0 for a bad one
+    const int32_t* table;
+};
+// False for an entry without rows.  err collects the error bits.
+__device__ __forceinline__ bool resolve_entry(const PagedAttnArgs& a, int entry, Entry& e, uint32_t& err) {
+    e.base = a.l.cu[entry];
+    e.count = a.l.cu[entry + 1] - e.base;
+    if (e.base < 0 || e.base >= a.l.rows || e.count <= 0) return false;
+    e.rows = min(e.count, min(a.max_rows, a.l.rows - e.base));
+    if (e.count > a.max_rows) err |= RTA_DEVERR_PAGES;
+    const int s = list_seq(a.l.seqs, entry);
+    e.len = 0;
+    e.table = a.p.table;
+    if ((unsigned)s >= (unsigned)a.p.max_seqs) {
+        err |= RTA_DEVERR_PAGES;
+        return true;
+    }
+    const int len = a.p.lengths[s];
+    e.table += (int64_t)s * a.p.max_pages;
+    if (len < 0 || len > a.max_len) {
+        err |= RTA_DEVERR_PAGES;
+        return true;
+    }
+    e.len = len;
+    if (len < e.count && (len > 0 || e.count > 1)) err |= RTA_DEVERR_PAGES;
+    return true;
+}
+
+// What the columns [tile cols, (tile + 1) cols) of an entry of `count` rows and a sequence of `len` positions
+// see, any of them; t0: the first one's position.
+__device__ __forceinline__ Visible prompt_span(const PagedAttnArgs& a, int len, int count, int tile, int cols) {
+    const int tok0 = (int)((int64_t)tile * cols / a.group);
+    const int tok1 = min((int)(((int64_t)(tile + 1) * cols - 1) / a.group), count - 1);
+    const int t0 = max(len - count + tok0, 0), t1 = len - count + tok1;
+    if (t1 < 0) return Visible{0, 0, 0};
+    const int lo = a.window > 0 && t0 >= a.window ? t0 - a.window + 1 : 0;
+    const int head = min(lo, a.sinks);
+    return Visible{head, lo, head + t1 + 1 - lo};
+}
+
+// All parts of eight values as operands.
+template <int FMT>
+__device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float a = v[2 * j], b = v[2 * j + 1];
+        if constexpr (FMT == RTA_BF16) {
+            const float ra = a - cut(a, 0xffff0000u), rb = b - cut(b, 0xffff0000u);
+            op[0][j] = upper_halves(a, b);
+            op[1][j] = upper_halves(ra, rb);
+            op[2][j] = upper_halves(ra - cut(ra, 0xffff0000u), rb - cut(rb, 0xffff0000u));
+        } else {
+            op[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+            op[1][j] = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_pkrtz(a - cut(a, 0xffffe000u), b - cut(b, 0xffffe000u)));
+        }
+    }
 }
 
 }  // namespace rta

@@ -16,9 +16,14 @@ static Cut decode_cut(int rows, int heads, int64_t most) {
     const int64_t chunk = want < 128 ? 128 : want < 1 << 30 ? want : 1 << 30;
     return Cut{(int)chunk, (int)((most + chunk - 1) / chunk)};
 }
+// Up to kFewCols (row, q head) columns of a kv head are few: the kernel of single rows takes them
+// in groups of 16 or 32, each reading the history once (bound by its bytes; the tiles of 128
+// columns of the other kernel would stay mostly empty).
+constexpr int kFewCols = 64;
 // With several rows: column tiles enough for two workgroups per compute unit stand alone, fewer
 // are cut into chunks of positions (a multiple of 64, 256 at least).
 constexpr int kPromptGroups = 1024;
+static int few_cols(int cols) { return cols <= 16 ? 16 : 32; }
 static int prompt_cols(int hd) { return hd == 256 ? 64 : 128; }
 static Cut prompt_cut(int64_t tiles, int64_t most) {
     if (2 * tiles >= kPromptGroups) return Cut{INT_MAX, 1};
@@ -47,15 +52,21 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
     *ntile = 0;
     if (!several)
         return decode_cut(rows, decode_heads(p->kv_heads, group, p->head_dim), most_visible(len, window, sinks));
-    const int cols = prompt_cols(p->head_dim);
+    const bool few = (int64_t)max_rows * group <= kFewCols;
+    const int cols = few ? few_cols(max_rows * group) : prompt_cols(p->head_dim);
     *ntile = (int)(((int64_t)max_rows * group + cols - 1) / cols);
     // (a column tile sees from its first row's window on)
-    const int64_t span = window > 0 ? window + cols / group + 1 : 0;
-    return prompt_cut((int64_t)*ntile * n * p->kv_heads, span ? most_visible(len, (int)(span < INT_MAX ? span : INT_MAX), sinks) : len);
+    int64_t most = len;
+    if (window > 0) {
+        const int64_t span = (int64_t)window + cols / group + 1;
+        most = most_visible(len, (int)(span < INT_MAX ? span : INT_MAX), sinks);
+    }
+    if (few) return decode_cut(n, *ntile * p->kv_heads, most);
+    return prompt_cut((int64_t)*ntile * n * p->kv_heads, most);
 }
 // Workgroups of 256 threads in one grid dimension: below 2^32 threads.
 static bool grid_fits(const rta_pages* p, int hq, int rows, int n, int max_rows) {
-    const int64_t group = hq / p->kv_heads, most = (1 << 24) - 1, tiles = (max_rows * group + 63) / 64;
+    const int64_t group = hq / p->kv_heads, most = (1 << 24) - 1, tiles = (max_rows * group + 15) / 16;
     return rows <= most && (int64_t)rows * p->kv_heads * group <= INT_MAX &&
            rows * (int64_t)decode_heads(p->kv_heads, (int)group, p->head_dim) <= most &&
            (max_rows == 1 || tiles <= most / ((int64_t)n * p->kv_heads));
@@ -125,16 +136,21 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
             a.nchunk = cut.nchunk;
             a.part = static_cast<float*>(workspace);
             a.mz = reinterpret_cast<float2*>(a.part + (size_t)rows * hq * cut.nchunk * HD);
-            if (ntile) {
+            a.ntile = ntile;
+            if (ntile && (int64_t)max_rows * a.group <= kFewCols) {
+                a.cols = few_cols(max_rows * a.group);
+                const dim3 grid(ntile * n * pages->kv_heads, 1, cut.nchunk), block(64 * kDecWaves);
+                if (a.cols == 16) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1, true>), grid, block, 0, s, a);
+                else hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2, true>), grid, block, 0, s, a);
+            } else if (ntile) {
                 a.cols = PromptLds<F, HD>::kCols;
-                a.ntile = ntile;
                 hipLaunchKernelGGL((paged_prompt_kernel<F, HD>), dim3(ntile * n * pages->kv_heads, 1, cut.nchunk),
                                    dim3(256), 0, s, a);
             } else {
                 const dim3 grid(rows * decode_heads(pages->kv_heads, a.group, HD), 1, cut.nchunk), block(64 * kDecWaves);
                 if (decode_nc(a.group, HD) == 1)
-                    hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1>), grid, block, 0, s, a);
-                else if constexpr (HD < 256) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2>), grid, block, 0, s, a);
+                    hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1, false>), grid, block, 0, s, a);
+                else if constexpr (HD < 256) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2, false>), grid, block, 0, s, a);
             }
             if (cut.nchunk > 1) hipLaunchKernelGGL((paged_merge_kernel<HD>), dim3(rows, hq), dim3(256), 0, s, a);
         };

@@ -21,24 +21,27 @@ typedef __attribute__((address_space(3))) s4_t lds_s4_t;
 
 constexpr int kDecWaves = 4, kDecTile = 32;
 
-template <int FMT, int HD, int NC>
+template <int FMT, int HD, int NC, bool MULTI>
 struct DecLds {
     static constexpr int kPitch = 2 * HD + 16;                                  // bytes of a V row
-    static constexpr int kQ = NC * PageFmt<FMT>::kOps * (HD / 32) * 64 * 16;    // Q^T operands, of all waves
+    static constexpr int kOps = MULTI ? PageFmt<FMT>::kParts : PageFmt<FMT>::kOps;
+    static constexpr int kQ = NC * kOps * (HD / 32) * 64 * 16;                  // Q^T operands, of all waves
     static constexpr int kV = kDecTile * kPitch;                                // per wave: V, at the end U
     static constexpr int kS = PageFmt<FMT>::kScaled ? 2 * kDecTile * 4 : 0;     // per wave: the tile's scales
     static constexpr int kWave = kV + kS;
-    static constexpr int kHeads = 8 * NC;
-    static constexpr int kTotal = kQ + kDecWaves * kWave + kDecWaves * kHeads * 8;   // and (m, z) per wave and head
-    static_assert(8 * HD * 4 <= kV, "U of a wave's 8 heads fits its V rows");
+    static constexpr int kPer = MULTI ? 16 : 8;                                 // queries of a column tile
+    static constexpr int kHeads = kPer * NC;
+    static constexpr int kTotal = kQ + kDecWaves * kWave + kDecWaves * kPer * 8;   // and (m, z) per wave and head
+    static_assert(kPer * HD * 4 <= kV, "U of a wave's queries fits its V rows");
     // waves per SIMD, by registers: 168 hold keys, values and sums of 128-wide heads
-    static constexpr int kPerSimd = HD == 64 ? (NC == 1 ? 4 : 2) : HD == 128 && NC == 1 ? 3 : HD == 128 ? 2 : 1;
+    static constexpr int kPerSimd =
+        HD == 64 ? (NC == 1 && !MULTI ? 4 : NC == 1 ? 3 : 2) : HD == 128 ? (NC == 1 && !MULTI ? 3 : 2) : 1;
 };
 
-template <int FMT, int HD, int NC>
-__global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd)) paged_decode_kernel(const PagedAttnArgs a) {
-    using L = DecLds<FMT, HD, NC>;
-    constexpr int kOps = PageFmt<FMT>::kOps, kB = PageFmt<FMT>::kBytes;
+template <int FMT, int HD, int NC, bool MULTI>
+__global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::kPerSimd)) paged_decode_kernel(const PagedAttnArgs a) {
+    using L = DecLds<FMT, HD, NC, MULTI>;
+    constexpr int kOps = L::kOps, kB = PageFmt<FMT>::kBytes, kPer = L::kPer;
     constexpr int kKb = HD / 32;                // products per 16 positions
     constexpr int kLoads = HD * kB / 64;        // 16-byte pieces per lane and row
     constexpr int kDt = HD / 16;                // dim tiles of O^T
@@ -46,22 +49,42 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
     __shared__ __align__(16) uint8_t lds[L::kTotal];
     const int lane = threadIdx.x & 63, i = lane & 15, u = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int groups = (a.group + L::kHeads - 1) / L::kHeads;   // head groups of a kv head
     // Workgroups go round the 8 XCDs in order.  Heads first and rows turned by the chunk keep a long
     // row's chunks on all of them (rows first: 32 rows of 256 to 8192 bf16 positions 124 us, so 65)
+    const int groups = MULTI ? a.ntile : (a.group + L::kHeads - 1) / L::kHeads;   // column groups of a kv head
     const int per_row = a.p.kv_heads * groups, y = blockIdx.x % per_row;
-    const int r = (int)((blockIdx.x / per_row + blockIdx.z) % a.l.rows);
+    const int turned = (int)((blockIdx.x / per_row + blockIdx.z) % (MULTI ? a.l.n : a.l.rows));
     const int kvh = y / groups, g0 = (y - kvh * groups) * L::kHeads;
-    const int heads = min(a.group - g0, L::kHeads);             // q heads of this workgroup
     uint32_t err = 0;
     Visible see;
     const int32_t* table;
-    if (!resolve_row(a, r, table, see, err)) {
-        if (err && threadIdx.x == 0) raise_error(err);
-        return;
+    // columns g0 .. g0 + cols - 1 of the entry: (row, head) pairs (MULTI), or the row's heads
+    int row0 = turned, cols, t0 = 0;   // t0: the position of the entry's first row
+    if constexpr (MULTI) {
+        Entry en;
+        if (!resolve_entry(a, turned, en, err)) return;
+        if (g0 > 0 || kvh > 0) err &= ~RTA_DEVERR_PAGES;   // told once
+        cols = min(en.rows * a.group - g0, L::kHeads);
+        if (cols <= 0) return;
+        row0 = en.base;
+        table = en.table;
+        t0 = en.len - en.count;
+        see = en.len ? prompt_span(a, en.len, en.count, g0 / L::kHeads, L::kHeads) : Visible{0, 0, 0};
+    } else {
+        if (!resolve_row(a, turned, table, see, err)) {
+            if (err && threadIdx.x == 0) raise_error(err);
+            return;
+        }
+        cols = min(a.group - g0, L::kHeads);
     }
     const int begin = blockIdx.z * a.chunk, end = see.count - begin > a.chunk ? begin + a.chunk : see.count;
     if (begin >= end && blockIdx.z > 0) return;
+    // row and q head of column c (< cols)
+    auto column = [&](int c, int& row, int& head) {
+        const int at = g0 + c, tok = MULTI ? at / a.group : 0;
+        row = row0 + tok;
+        head = kvh * a.group + at - tok * a.group;
+    };
 
     uint8_t* vl = lds + L::kQ + wave * L::kWave;
     float* sl = reinterpret_cast<float*>(vl + L::kV);
@@ -141,15 +164,18 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
         spot(wave + kDecWaves, next);   // clamped past the end
     }
 
-    // q as B operands, one wave per quarter of the products; column 2 g + part.  Every wave finds
-    // the heads' largest |q| (the power of two of binary16 operands).
-    const int part = i & 1;
+    // q as B operands, one wave per quarter of the products.  Every wave finds the queries' largest
+    // |q| (the power of two of binary16 operands).
+    const int part = MULTI ? 0 : i & 1, query = MULTI ? i : i >> 1;   // lane's column of a column tile
+    int t_col[NC];
     float fac[NC];   // score = product * fac, in powers of two: 1 / s / sqrt(HD) * log2 e
     int qe[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int g = 8 * c + (i >> 1);
-        const float* q = a.q + r * a.q_stride + ((int64_t)kvh * a.group + g0 + min(g, heads - 1)) * HD;
+        int row, head;
+        column(min(kPer * c + query, cols - 1), row, head);
+        t_col[c] = t0 + row - row0;
+        const float* q = a.q + row * a.q_stride + (int64_t)head * HD;
         qe[c] = 14;
         if constexpr (FMT != RTA_BF16) {
             float mx = 0.0f;
@@ -164,17 +190,28 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
 #pragma unroll
             for (int s = 0; s < 8; ++s) v[s] = q[operand_dim<FMT>(kb, u) + s] * sg;
             u4_t op[kOps];
-            split_parts<FMT>(v, part, op);
+            if constexpr (MULTI) split_all<FMT>(v, op);
+            else split_parts<FMT>(v, part, op);
 #pragma unroll
             for (int o = 0; o < kOps; ++o)
                 *reinterpret_cast<u4_t*>(lds + (((c * kOps + o) * kKb + kb) * 64 + lane) * 16) = op[o];
         }
+    }
+    int t_first = 0, t_last = 0;   // the columns' first and last positions
+    if constexpr (MULTI) {
+        t_first = t0 + g0 / a.group;
+        t_last = t0 + (g0 + cols - 1) / a.group;
     }
     __syncthreads();
 
     for (int t = wave; t < ntile; t += kDecWaves) {
         const uint32_t now = live;
         const bool more = t + kDecWaves < ntile;
+        // every column sees the whole tile
+        bool whole = now == 0xffffffffu;
+        if constexpr (MULTI)
+            whole = whole && see.position(begin + t * kDecTile + kDecTile - 1) <= t_first &&
+                    (a.window == 0 || see.position(begin + t * kDecTile) > t_last - a.window);
         // scores of positions 4u + e (h = 0) and 16 + 4u + e (h = 1) in column i
         f4_t s[NC][2];
 #pragma unroll
@@ -271,14 +308,19 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float d = s[c][j >> 2][j & 3];
-                x[j] = (d + dpp_mov<0xB1>(d)) * fac[c];   // both parts
+                x[j] = (MULTI ? d : d + dpp_mov<0xB1>(d)) * fac[c];   // (both parts)
                 if constexpr (kScaled) x[j] *= kf[j >> 2][j & 3];
             }
-            if (now != 0xffffffffu) {
+            if (!whole) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const bool on = (now >> (16 * (j >> 2) + 4 * u + (j & 3))) & 1u;
+                    const int k = 16 * (j >> 2) + 4 * u + (j & 3);
+                    bool on = (now >> k) & 1u;
                     if (on) nonfinite = fmaf(x[j], 0.0f, nonfinite);
+                    if constexpr (MULTI) {
+                        const int p = see.position(begin + t * kDecTile + k);
+                        on = on && p <= t_col[c] && (a.window == 0 || p > t_col[c] - a.window || p < a.sinks);
+                    }
                     x[j] = on ? x[j] : -INFINITY;
                 }
             } else {
@@ -303,7 +345,8 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
                 z[c] += w[j];
                 w[j] *= kScaled ? vf[j >> 2][j & 3] * wscale : wscale;
             }
-            split_parts<FMT>(w, part, pb[c]);
+            if constexpr (MULTI) split_all<FMT>(w, pb[c]);
+            else split_parts<FMT>(w, part, pb[c]);
         }
         ve = ve_new;
 #pragma unroll
@@ -324,35 +367,35 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC>::kPerSimd
     // join: U of both parts per head and dim in the wave's own LDS, then over the waves
     float2* mzl = reinterpret_cast<float2*>(lds + L::kQ + kDecWaves * L::kWave);
     const float unscale = ldexpf(1.0f, (kScaled ? ve : 0) - 14);
-    const int64_t h0 = (int64_t)r * a.hq + (int64_t)kvh * a.group + g0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int g = i >> 1;
-        float zz = add_xor32(add_xor16(z[c]));
-        if (lane < 16 && part == 0) mzl[wave * 8 + g] = float2{m[c], zz};
-        float* ul = reinterpret_cast<float*>(vl) + g * HD;
+        const float zz = add_xor32(add_xor16(z[c]));
+        if (lane < 16 && part == 0) mzl[wave * kPer + query] = float2{m[c], zz};
+        float* ul = reinterpret_cast<float*>(vl) + query * HD;
 #pragma unroll
         for (int d = 0; d < kDt; ++d) {
             f4_t x;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (o[c][d][e] + dpp_mov<0xB1>(o[c][d][e])) * unscale;
+            for (int e = 0; e < 4; ++e) x[e] = (MULTI ? o[c][d][e] : o[c][d][e] + dpp_mov<0xB1>(o[c][d][e])) * unscale;
             if (part == 0) *reinterpret_cast<f4_t*>(ul + 16 * d + 4 * u) = x;
         }
         __syncthreads();
-        for (int at = threadIdx.x; at < min(8, heads - 8 * c) * HD; at += 64 * kDecWaves) {
-            const int hd = at / HD, dim = at - hd * HD;
+        for (int at = threadIdx.x; at < min(kPer, cols - kPer * c) * HD; at += 64 * kDecWaves) {
+            const int j = at / HD, dim = at - j * HD;
             float M = -INFINITY, Z = 0.0f, U = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, mzl[w * 8 + hd].x);
+            for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, mzl[w * kPer + j].x);
             const float base = M == -INFINITY ? 0.0f : M;
 #pragma unroll
             for (int w = 0; w < kDecWaves; ++w) {
-                const float2 t = mzl[w * 8 + hd];
+                const float2 t = mzl[w * kPer + j];
                 const float f = __builtin_amdgcn_exp2f(t.x - base);
                 Z += t.y * f;
                 U += reinterpret_cast<const float*>(lds + L::kQ + w * L::kWave)[at] * f;
             }
-            const int64_t row_head = h0 + 8 * c + hd;
+            int row, head;
+            column(kPer * c + j, row, head);
+            const int64_t row_head = (int64_t)row * a.hq + head;
             if (a.nchunk == 1) {
                 write_result(a, row_head, HD, dim, U, M * kLn2, Z, err);
             } else {

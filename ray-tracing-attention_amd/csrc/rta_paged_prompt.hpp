@@ -31,41 +31,10 @@ struct PromptLds {
 
 typedef f4_t f4u_t __attribute__((aligned(4)));   // at an address of a multiple of 4
 
-// What the columns [tile kCols, ..) of an entry of `count` rows and a sequence of `len` positions
-// see, any of them; t0: the first one's position.
-__device__ __forceinline__ Visible prompt_span(const PagedAttnArgs& a, int len, int count, int tile, int cols) {
-    const int tok0 = (int)((int64_t)tile * cols / a.group);
-    const int tok1 = min((int)(((int64_t)(tile + 1) * cols - 1) / a.group), count - 1);
-    const int t0 = max(len - count + tok0, 0), t1 = len - count + tok1;
-    if (t1 < 0) return Visible{0, 0, 0};
-    const int lo = a.window > 0 && t0 >= a.window ? t0 - a.window + 1 : 0;
-    const int head = min(lo, a.sinks);
-    return Visible{head, lo, head + t1 + 1 - lo};
-}
-
-// All parts of eight values as operands.
-template <int FMT>
-__device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float a = v[2 * j], b = v[2 * j + 1];
-        if constexpr (FMT == RTA_BF16) {
-            const float ra = a - cut(a, 0xffff0000u), rb = b - cut(b, 0xffff0000u);
-            op[0][j] = upper_halves(a, b);
-            op[1][j] = upper_halves(ra, rb);
-            op[2][j] = upper_halves(ra - cut(ra, 0xffff0000u), rb - cut(rb, 0xffff0000u));
-        } else {
-            op[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-            op[1][j] = __builtin_bit_cast(
-                uint32_t, __builtin_amdgcn_cvt_pkrtz(a - cut(a, 0xffffe000u), b - cut(b, 0xffffe000u)));
-        }
-    }
-}
-
 template <int FMT, int HD>
 __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArgs a) {
     using L = PromptLds<FMT, HD>;
-    constexpr int kParts = FMT == RTA_BF16 ? 3 : 2, kB = PageFmt<FMT>::kBytes, NQ = L::kNQ;
+    constexpr int kParts = PageFmt<FMT>::kParts, kB = PageFmt<FMT>::kBytes, NQ = L::kNQ;
     constexpr int kKb = HD / 32, kDt = HD / 16;
     constexpr int kKg = kKb < 4 ? kKb : 4, kDg = 4;   // operands read ahead
     constexpr int kPieces = HD * kB / 16, kStep = 256 / kPieces, kPass = L::kTile / kStep;
@@ -77,27 +46,12 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     const int kvh = blockIdx.x % hkv, rest = blockIdx.x / hkv;
     const int entry = rest % a.l.n, tile = a.ntile - 1 - rest / a.l.n;
     uint32_t err = 0;
-    const int base = a.l.cu[entry];
-    int count = a.l.cu[entry + 1] - base;
-    if (base < 0 || base >= a.l.rows || count <= 0) return;
-    int live_rows = min(count, min(a.max_rows, a.l.rows - base));   // rows that are written
-    if (count > a.max_rows && tile == 0) err |= RTA_DEVERR_PAGES;
-    if ((int64_t)tile * L::kCols >= (int64_t)live_rows * a.group) return;
-    const int s = list_seq(a.l.seqs, entry);
-    int len = 0;
-    const int32_t* table = a.p.table;
-    if ((unsigned)s < (unsigned)a.p.max_seqs) {
-        len = a.p.lengths[s];
-        table += (int64_t)s * a.p.max_pages;
-        if (len < 0 || len > a.max_len) {
-            err |= RTA_DEVERR_PAGES;
-            len = 0;
-        } else if (len < count && (len > 0 || count > 1)) {
-            err |= RTA_DEVERR_PAGES;
-        }
-    } else {
-        err |= RTA_DEVERR_PAGES;
-    }
+    Entry en;
+    if (!resolve_entry(a, entry, en, err)) return;
+    if (tile > 0) err &= ~RTA_DEVERR_PAGES;   // the first tile tells
+    if ((int64_t)tile * L::kCols >= (int64_t)en.rows * a.group) return;
+    const int base = en.base, count = en.count, live_rows = en.rows, len = en.len;
+    const int32_t* table = en.table;
     const Visible see = len ? prompt_span(a, len, count, tile, L::kCols) : Visible{0, 0, 0};
     const int begin = blockIdx.z * a.chunk, end = see.count - begin > a.chunk ? begin + a.chunk : see.count;
     if (begin >= end && blockIdx.z > 0) return;

@@ -172,12 +172,12 @@ class PagedCache:
 
     def read(self, rows, layer=0, seqs=None, cu_rows=None, k=None, v=None):
         """The keys and values of those rows as fp32: (k, v), each [rows, kv_heads * head_dim].
-        Without k and v given, new tensors (zero where no entry lists the row)."""
+        Rows that no entry lists are left as they were in k and v, and mean nothing in tensors
+        made here."""
         sp, cu, n = self._list(rows, seqs, cu_rows)
-        make = torch.empty if cu_rows is None else torch.zeros
         shape = (rows, self.kv_heads * self.head_dim)
-        k = make(shape, dtype=torch.float32, device=self.device) if k is None else k
-        v = make(shape, dtype=torch.float32, device=self.device) if v is None else v
+        k = torch.empty(shape, dtype=torch.float32, device=self.device) if k is None else k
+        v = torch.empty(shape, dtype=torch.float32, device=self.device) if v is None else v
         self._call("rta_paged_read", layer, rows, sp, cu, n, *self._strided(k, "k", rows), *self._strided(v, "v", rows))
         return k, v
 
@@ -193,8 +193,8 @@ class PagedCache:
         first `sinks`.  Returns (out [rows, hq, head_dim], m [rows, hq], z [rows, hq]).
 
         max_rows: the most rows of an entry (None: one without cu_rows, else all of them);
-        max_len: the longest sequence (0: max_pages * page).  Rows that no entry lists are zero
-        in tensors made here and left as they were in given ones."""
+        max_len: the longest sequence (0: max_pages * page).  Rows that no entry lists are left as
+        they were in out, m and z, and mean nothing in tensors made here."""
         if not isinstance(q, torch.Tensor) or q.device != self.device or q.dtype != torch.float32:
             raise TypeError(f"q must be a float32 tensor on {self.device}")
         if q.dim() != 3 or q.shape[2] != self.head_dim or q.stride(2) != 1 or q.stride(1) != self.head_dim:
@@ -203,13 +203,12 @@ class PagedCache:
         sp, cu, n = self._list(rows, seqs, cu_rows)
         if max_rows is None:
             max_rows = 1 if cu_rows is None else rows
-        make = torch.empty if cu_rows is None else torch.zeros
         if out is None:
-            out = make(rows, hq, hd, dtype=torch.float32, device=self.device)
+            out = torch.empty(rows, hq, hd, dtype=torch.float32, device=self.device)
         if m is None:
-            m = make(rows, hq, dtype=torch.float32, device=self.device)
+            m = torch.empty(rows, hq, dtype=torch.float32, device=self.device)
         if z is None:
-            z = make(rows, hq, dtype=torch.float32, device=self.device)
+            z = torch.empty(rows, hq, dtype=torch.float32, device=self.device)
         need = self.attention_workspace_bytes(hq, rows, n, max_rows, max_len, window, sinks)
         ws = _workspace(need, self.device, workspace)
         stride = q.stride(0) if rows > 1 else max(q.stride(0), hq * hd)

@@ -105,6 +105,25 @@ def test_several_rows_per_sequence(env, fmt, hq, hkv, hd, page, window, sinks):
     assert ops.device_error() == 0 and len(order) == 7
 
 
+@pytest.mark.parametrize("fmt", [ref.F16, ref.BF16, ref.Q8_ROW])
+@pytest.mark.parametrize("hq,hkv,hd,page,window,sinks", [(8, 2, 128, 16, 0, 0), (32, 4, 128, 64, 40, 4),
+                                                         (12, 2, 64, 5, 0, 0), (6, 3, 256, 33, 64, 70),
+                                                         (40, 2, 256, 64, 0, 0), (20, 1, 64, 8, 3, 1)])
+def test_a_few_rows_per_sequence(env, fmt, hq, hkv, hd, page, window, sinks):
+    torch, _, dev = env
+    lens, counts = [3, 300, 64, 0, 129, 1, 1200], [3, 2, 3, 0, 1, 1, 3]
+    c = filled(env, fmt, hkv, hd, page, lens)
+    fill(env, c, lens, 31)
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    q = rows_of(torch, dev, int(cu[-1]), hq, hd, 32)
+    gate = rows_of(torch, dev, int(cu[-1]), hq, hd, 33).contiguous()
+    for g, most in ((None, 3), (gate, 5)):   # the bound may be above the most there are
+        got = c.attention(q, cu_rows=ints(torch, cu, dev), max_rows=most, max_len=1200, window=window, sinks=sinks, gate=g)
+        want = want_rows(c, q, [(s, int(cu[s]), counts[s]) for s in range(7)], window=window, sinks=sinks, gate=g)
+        ref.check_rows(got, want, (fmt, hq, hkv, hd, page))
+    assert ops.device_error() == 0
+
+
 @pytest.mark.parametrize("rows,length", [(2, 4000), (9, 2500), (200, 1500), (513, 513)])
 def test_rows_split_over_long_histories(env, rows, length):
     torch, _, dev = env
