@@ -85,13 +85,21 @@ __device__ __forceinline__ bool resolve_row(const PagedAttnArgs& a, int r, const
     return true;
 }
 
-// The final values of (row, q head) at dim c from U, M (natural units) and Z.
-__device__ __forceinline__ void write_result(const PagedAttnArgs& a, int64_t at, int hd, int c, float u, float m,
+typedef f4_t f4u_t __attribute__((aligned(4)));   // at an address of a multiple of 4
+
+// The final values of (row, q head) at dims c .. c + 3 from U, M (natural units) and Z.
+__device__ __forceinline__ void write_result(const PagedAttnArgs& a, int64_t at, int hd, int c, f4_t u, float m,
                                              float z, uint32_t& err) {
-    float o = z > 0.0f || z != z ? u / z : 0.0f;   // nothing seen: zeros
-    if (a.gate) o *= detector_sigmoid(a.gate[at * hd + c]);
-    if (!isfinite(o)) err |= RTA_DEVERR_DETECTOR;
-    a.out[at * hd + c] = o;
+    f4_t o = u * (z > 0.0f || z != z ? 1.0f / z : 0.0f);   // nothing seen: zeros
+    const int64_t to = at * hd + c;
+    if (a.gate) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= detector_sigmoid(a.gate[to + e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (!isfinite(o[e])) err |= RTA_DEVERR_DETECTOR;
+    *reinterpret_cast<f4u_t*>(a.out + to) = o;
     if (c == 0) {
         if (a.m_out) a.m_out[at] = m;
         if (a.z_out) a.z_out[at] = z;
@@ -243,5 +251,94 @@ __device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
         }
     }
 }
+
+// Masks the products of 32 positions j0 .. of a list that the columns see between them: bit k of
+// ok says whether position k counts, t_col is the lane's column's position, -1 at least.  What a
+// column sees is one unsigned comparison of its distance (the first positions' window is all):
+// booleans of their own would each take a pair of scalar registers.
+template <int NC>
+__device__ __forceinline__ void mask_columns(f4_t (*x)[2], uint32_t ok, const Visible& see, int j0, int u,
+                                             const int* t_col, int window, int sinks) {
+    const uint32_t mine = ok >> (4 * u);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int p = see.position(j0 + 16 * h + 4 * u + e);
+            const uint32_t reach = window == 0 || p < sinks ? 0x80000000u : (uint32_t)window;
+            const int at = (mine >> (16 * h + e)) & 1u ? p : INT_MAX;   // no distance reaches it
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                x[c][h][e] = (uint32_t)(t_col[c] - at) < reach ? x[c][h][e] : -INFINITY;
+        }
+}
+
+// The online softmax of NC column tiles, a lane holding 8 positions of its column of each
+// (products x; score = x fac in log2 units).  Weights are 2^(score - low), 2^kTop for the largest
+// score when low was set; low follows the maximum only when weights would pass 2^(kTop + kSlack)
+// = 2^15, so the sums are seldom rescaled, and binary16 parts neither overflow nor lose more than
+// 2^-32 of the largest weight.
+template <int NC>
+struct Softmax {
+    static constexpr float kTop = 8.0f, kSlack = 7.0f;
+    float m[NC], low[NC], z[NC];   // m: the largest product; z: of the lane's positions
+    float lowest;                  // of all products: a visible -inf shows nowhere else
+    float ask[NC];
+
+    __device__ __forceinline__ void start() {
+        lowest = INFINITY;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            m[c] = low[c] = -INFINITY;
+            z[c] = 0.0f;
+        }
+    }
+    __device__ __forceinline__ void watch(const f4_t (*x)[2]) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) lowest = fminf(lowest, x[c][j >> 2][j & 3]);
+    }
+    // Takes in the maxima of x (masked positions -inf) and brings z and o to the new base; vshift:
+    // the power of two by which o has to follow a value scale.
+    template <int DT>
+    __device__ __forceinline__ void raise(const f4_t (*x)[2], const float* fac, int vshift, f4_t (*o)[DT]) {
+        bool lift = vshift != 0;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float t = x[c][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) t = fmaxf(t, x[c][j >> 2][j & 3]);
+            m[c] = fmaxf(m[c], max_xor32(max_xor16(t)));
+            ask[c] = fmaf(m[c], fac[c], -kTop);
+            lift = lift || ask[c] > low[c] + kSlack;
+        }
+        if (__builtin_amdgcn_ballot_w64(lift)) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float base = ask[c] > low[c] ? ask[c] : low[c];
+                const float al = __builtin_amdgcn_exp2f(low[c] - (base == -INFINITY ? 0.0f : base));
+                const float f = ldexpf(al, vshift);
+                z[c] *= al;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[c][d] *= f;
+                low[c] = base;
+            }
+        }
+    }
+    __device__ __forceinline__ void weights(int c, const f4_t* x, float fac, float w[8]) {
+        const float base = low[c] == -INFINITY ? 0.0f : low[c];   // (nothing seen yet: weights 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = __builtin_amdgcn_exp2f(fmaf(x[j >> 2][j & 3], fac, -base));
+            z[c] += w[j];
+        }
+    }
+    // The maximum in log2 units, and what brings sums over weights to it as the base.
+    __device__ __forceinline__ void finish(int c, float fac, float& M, float& back) const {
+        M = m[c] * fac;
+        back = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(low[c] - M);
+    }
+};
 
 }  // namespace rta

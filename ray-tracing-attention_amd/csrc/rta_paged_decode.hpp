@@ -93,17 +93,13 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     const int ntile = (end - begin + kDecTile - 1) / kDecTile;
 
     f4_t o[NC][kDt];
-    float m[NC], z[NC];
+    Softmax<NC> sm;
+    sm.start();
     int ve = -110;   // exponent of the largest value scale so far
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        m[c] = -INFINITY;
-        z[c] = 0.0f;
-#pragma unroll
         for (int d = 0; d < kDt; ++d) o[c][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    float nonfinite = 0.0f;
-
     // position i + 16 h of tile t: its page's number and place, clamped to the last visible one
     struct Spot {
         int page[2], off[2];
@@ -174,7 +170,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     for (int c = 0; c < NC; ++c) {
         int row, head;
         column(min(kPer * c + query, cols - 1), row, head);
-        t_col[c] = t0 + row - row0;
+        t_col[c] = max(t0 + row - row0, -1);
         const float* q = a.q + row * a.q_stride + (int64_t)head * HD;
         qe[c] = 14;
         if constexpr (FMT != RTA_BF16) {
@@ -287,68 +283,56 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             load_v();
             spot(t + 2 * kDecWaves, next);
         }
-        // value scales: w = p * scale / 2^ve below 2^14
-        float wscale = 16384.0f;
         int ve_new = ve;
-        if constexpr (kScaled) {
+        if constexpr (kScaled) {   // value scales below 2^0
             float mx = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(vf[h][e]));
             ve_new = max(ve, part_exponent(max_xor32(max_xor16(mx))));
-            wscale = ldexpf(1.0f, 14 - ve_new);
+            const float down = ldexpf(1.0f, -ve_new);
+            vf[0] *= down;
+            vf[1] *= down;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s[c][0] *= kf[0];
+                s[c][1] *= kf[1];
+            }
         }
-        // softmax in the lane's column
+        if constexpr (!MULTI) {   // both parts
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[c][j >> 2][j & 3] += dpp_mov<0xB1>(s[c][j >> 2][j & 3]);
+        }
+        sm.watch(s);
+        if (!whole) {
+            if constexpr (MULTI) {
+                mask_columns<NC>(s, now, see, begin + t * kDecTile, u, t_col, a.window, a.sinks);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool on = (now >> (16 * (j >> 2) + 4 * u + (j & 3))) & 1u;
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) s[c][j >> 2][j & 3] = on ? s[c][j >> 2][j & 3] : -INFINITY;
+                }
+            }
+        }
+        sm.template raise<kDt>(s, fac, kScaled ? ve - ve_new : 0, o);
+        ve = ve_new;
         u4_t pb[NC][kOps];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            float x[8];
-            float mx = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = s[c][j >> 2][j & 3];
-                x[j] = (MULTI ? d : d + dpp_mov<0xB1>(d)) * fac[c];   // (both parts)
-                if constexpr (kScaled) x[j] *= kf[j >> 2][j & 3];
-            }
-            if (!whole) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int k = 16 * (j >> 2) + 4 * u + (j & 3);
-                    bool on = (now >> k) & 1u;
-                    if (on) nonfinite = fmaf(x[j], 0.0f, nonfinite);
-                    if constexpr (MULTI) {
-                        const int p = see.position(begin + t * kDecTile + k);
-                        on = on && p <= t_col[c] && (a.window == 0 || p > t_col[c] - a.window || p < a.sinks);
-                    }
-                    x[j] = on ? x[j] : -INFINITY;
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) nonfinite = fmaf(x[j], 0.0f, nonfinite);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, x[j]);
-            const float mn = fmaxf(m[c], max_xor32(max_xor16(mx)));
-            const float base = mn == -INFINITY ? 0.0f : mn;   // (all of the tile missing)
-            if (__builtin_amdgcn_ballot_w64(mn > m[c]) || ve_new != ve) {
-                const float al = __builtin_amdgcn_exp2f(m[c] - base), f = kScaled ? ldexpf(al, ve - ve_new) : al;
-                z[c] *= al;
-#pragma unroll
-                for (int d = 0; d < kDt; ++d) o[c][d] *= f;
-            }
-            m[c] = mn;
             float w[8];
+            sm.weights(c, s[c], fac[c], w);
+            if constexpr (kScaled) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] = __builtin_amdgcn_exp2f(x[j] - base);
-                z[c] += w[j];
-                w[j] *= kScaled ? vf[j >> 2][j & 3] * wscale : wscale;
+                for (int j = 0; j < 8; ++j) w[j] *= vf[j >> 2][j & 3];
             }
             if constexpr (MULTI) split_all<FMT>(w, pb[c]);
             else split_parts<FMT>(w, part, pb[c]);
         }
-        ve = ve_new;
 #pragma unroll
         for (int d = 0; d < kDt; ++d) {
             const uint8_t* src = vl + (4 * u + (i >> 2)) * L::kPitch + 32 * d + 8 * (i & 3);
@@ -362,15 +346,16 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 for (int op = 0; op < kOps; ++op) o[c][d] = page_mfma<FMT>(va, pb[c][op], o[c][d]);
         }
     }
-    if (nonfinite != nonfinite) err |= RTA_DEVERR_DETECTOR;
+    if (sm.lowest == -INFINITY) err |= RTA_DEVERR_DETECTOR;   // (larger ones and NaN reach the results)
 
-    // join: U of both parts per head and dim in the wave's own LDS, then over the waves
+    // join: U per query and dim in the wave's own LDS, then over the waves
     float2* mzl = reinterpret_cast<float2*>(lds + L::kQ + kDecWaves * L::kWave);
-    const float unscale = ldexpf(1.0f, (kScaled ? ve : 0) - 14);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const float zz = add_xor32(add_xor16(z[c]));
-        if (lane < 16 && part == 0) mzl[wave * kPer + query] = float2{m[c], zz};
+        float M, back;
+        sm.finish(c, fac[c], M, back);
+        const float zz = add_xor32(add_xor16(sm.z[c])) * back, unscale = kScaled ? ldexpf(back, ve) : back;
+        if (lane < 16 && part == 0) mzl[wave * kPer + query] = float2{M, zz};
         float* ul = reinterpret_cast<float*>(vl) + query * HD;
 #pragma unroll
         for (int d = 0; d < kDt; ++d) {
@@ -380,18 +365,22 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             if (part == 0) *reinterpret_cast<f4_t*>(ul + 16 * d + 4 * u) = x;
         }
         __syncthreads();
-        for (int at = threadIdx.x; at < min(kPer, cols - kPer * c) * HD; at += 64 * kDecWaves) {
-            const int j = at / HD, dim = at - j * HD;
-            float M = -INFINITY, Z = 0.0f, U = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, mzl[w * kPer + j].x);
-            const float base = M == -INFINITY ? 0.0f : M;
+        for (int at = threadIdx.x; at < min(kPer, cols - kPer * c) * (HD / 4); at += 64 * kDecWaves) {
+            const int j = at / (HD / 4), dim = 4 * (at - j * (HD / 4));
+            float2 mz[kDecWaves];
+            float M = -INFINITY, Z = 0.0f;
 #pragma unroll
             for (int w = 0; w < kDecWaves; ++w) {
-                const float2 t = mzl[w * kPer + j];
-                const float f = __builtin_amdgcn_exp2f(t.x - base);
-                Z += t.y * f;
-                U += reinterpret_cast<const float*>(lds + L::kQ + w * L::kWave)[at] * f;
+                mz[w] = mzl[w * kPer + j];
+                M = fmaxf(M, mz[w].x);
+            }
+            const float base = M == -INFINITY ? 0.0f : M;
+            f4_t U = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kDecWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(mz[w].x - base);
+                Z += mz[w].y * f;
+                U += reinterpret_cast<const f4_t*>(lds + L::kQ + w * L::kWave)[at] * f;
             }
             int row, head;
             column(kPer * c + j, row, head);
@@ -400,7 +389,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 write_result(a, row_head, HD, dim, U, M * kLn2, Z, err);
             } else {
                 const int64_t rec = row_head * a.nchunk + blockIdx.z;
-                a.part[rec * HD + dim] = U;
+                *reinterpret_cast<f4_t*>(a.part + rec * HD + dim) = U;
                 if (dim == 0) a.mz[rec] = float2{M, Z};
             }
         }

@@ -29,8 +29,6 @@ struct PromptLds {
     static constexpr int kTotal = 2 * kBuf + 4 * kThird;
 };
 
-typedef f4_t f4u_t __attribute__((aligned(4)));   // at an address of a multiple of 4
-
 template <int FMT, int HD>
 __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArgs a) {
     using L = PromptLds<FMT, HD>;
@@ -148,7 +146,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
         const int col = min(col0 + 16 * c + i, cols - 1), tok = col / a.group, g = col - tok * a.group;
-        t_col[c] = len - count + tok;
+        t_col[c] = max(len - count + tok, -1);
         const float* q = a.q + (int64_t)(base + tok) * a.q_stride + ((int64_t)kvh * a.group + g) * HD;
         float v[kKb][8], mx = 0.0f;
 #pragma unroll
@@ -178,16 +176,11 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     const int t_hi = len - count + min(col0 + 16 * NQ - 1, cols - 1) / a.group;
 
     f4_t o[NQ][kDt];
-    // weights are 2^(score - low) in log2 units, 2^kTop for the largest score when low was set and
-    // below 2^(kTop + kSlack) <= 2^15 until it is set again
-    constexpr float kTop = 8.0f, kSlack = 7.0f;
-    float m[NQ], low[NQ], z[NQ], lowest = INFINITY;   // m, lowest: of the products
+    Softmax<NQ> sm;
+    sm.start();
     int ve = -110;
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-        m[c] = low[c] = -INFINITY;
-        z[c] = 0.0f;
-#pragma unroll
         for (int d = 0; d < kDt; ++d) o[c][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if (nt > 0) store(lds);
@@ -266,61 +259,18 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                         for (int c = 0; c < NQ; ++c) x[c][h] *= kf;
                     }
                 }
-                float mx[NQ];
-#pragma unroll
-                for (int c = 0; c < NQ; ++c) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) lowest = fminf(lowest, x[c][j >> 2][j & 3]);
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int k = 32 * sub + 16 * h + 4 * u + e, p = see.position(j0 + k);
-                            const bool ok = (okm >> k) & 1u;
-#pragma unroll
-                            for (int c = 0; c < NQ; ++c) {
-                                const bool vis = ok && p <= t_col[c] &&
-                                                 (a.window == 0 || p > t_col[c] - a.window || p < a.sinks);
-                                x[c][h][e] = vis ? x[c][h][e] : -INFINITY;
-                            }
-                        }
-                }
-                // the running maximum, and the weights' base behind it: it follows only when weights
-                // would pass 2^15, so that sums are seldom rescaled
-                bool lift = kScaled && ve_new != ve;
-#pragma unroll
-                for (int c = 0; c < NQ; ++c) {
-                    mx[c] = x[c][0][0];
-#pragma unroll
-                    for (int j = 1; j < 8; ++j) mx[c] = fmaxf(mx[c], x[c][j >> 2][j & 3]);
-                    m[c] = fmaxf(m[c], max_xor32(max_xor16(mx[c])));
-                    mx[c] = fmaf(m[c], fac[c], -kTop);   // the base that the maximum asks for
-                    lift = lift || mx[c] > low[c] + kSlack;
-                }
-                if (__builtin_amdgcn_ballot_w64(lift)) {
-#pragma unroll
-                    for (int c = 0; c < NQ; ++c) {
-                        const float base = mx[c] > low[c] ? mx[c] : low[c];
-                        const float al = __builtin_amdgcn_exp2f(low[c] - (base == -INFINITY ? 0.0f : base));
-                        const float f = kScaled ? ldexpf(al, ve - ve_new) : al;
-                        z[c] *= al;
-#pragma unroll
-                        for (int d = 0; d < kDt; ++d) o[c][d] *= f;
-                        low[c] = base;
-                    }
-                }
+                sm.watch(x);
+                if (!whole)
+                    mask_columns<NQ>(x, (uint32_t)(okm >> (32 * sub)), see, j0 + 32 * sub, u, t_col, a.window, a.sinks);
+                sm.template raise<kDt>(x, fac, kScaled ? ve - ve_new : 0, o);
                 u4_t pb[NQ][kParts];
 #pragma unroll
                 for (int c = 0; c < NQ; ++c) {
-                    const float base = low[c] == -INFINITY ? 0.0f : low[c];   // (nothing seen yet: weights 0)
                     float w[8];
+                    sm.weights(c, x[c], fac[c], w);
+                    if constexpr (kScaled) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        w[j] = __builtin_amdgcn_exp2f(fmaf(x[c][j >> 2][j & 3], fac[c], -base));
-                        z[c] += w[j];
-                        if constexpr (kScaled) w[j] *= vf[j >> 2][j & 3];
+                        for (int j = 0; j < 8; ++j) w[j] *= vf[j >> 2][j & 3];
                     }
                     split_all<FMT>(w, pb[c]);
                 }
@@ -345,12 +295,12 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
         __syncthreads();
     }
 
-    if (lowest == -INFINITY) err |= RTA_DEVERR_DETECTOR;   // (larger ones and NaN reach the results)
+    if (sm.lowest == -INFINITY) err |= RTA_DEVERR_DETECTOR;   // (larger ones and NaN reach the results)
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-        // back to the maximum as the base
-        const float M = m[c] * fac[c], back = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(low[c] - M);
-        const float Z = add_xor32(add_xor16(z[c])) * back, unscale = kScaled ? ldexpf(back, ve) : back;
+        float M, back;
+        sm.finish(c, fac[c], M, back);
+        const float Z = add_xor32(add_xor16(sm.z[c])) * back, unscale = kScaled ? ldexpf(back, ve) : back;
         const int col = col0 + 16 * c + i;
         if (col >= cols) continue;
         const int tok = col / a.group, g = col - tok * a.group;
@@ -363,24 +313,8 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
             if (u == 0) a.mz[rec] = float2{M, Z};
             continue;
         }
-        const float scale = Z > 0.0f || Z != Z ? unscale / Z : 0.0f;   // nothing seen: zeros
 #pragma unroll
-        for (int d = 0; d < kDt; ++d) {
-            const int64_t to = at * HD + 16 * d + 4 * u;
-            f4_t x = o[c][d] * scale;
-            if (a.gate) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] *= detector_sigmoid(a.gate[to + e]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (!isfinite(x[e])) err |= RTA_DEVERR_DETECTOR;
-            *reinterpret_cast<f4u_t*>(a.out + to) = x;
-        }
-        if (u == 0) {
-            if (a.m_out) a.m_out[at] = M * kLn2;
-            if (a.z_out) a.z_out[at] = Z;
-        }
+        for (int d = 0; d < kDt; ++d) write_result(a, at, HD, 16 * d + 4 * u, o[c][d] * unscale, M * kLn2, Z, err);
     }
     if (err) raise_error(err);
 }
@@ -432,12 +366,12 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnArgs a)
     const float zw = wave_sum_dpp(d == 0 ? z : 0.0f);
     if ((tid & 63) == 0) zred[tid >> 6] = zw;
     __syncthreads();
-    if (tid >= HD) return;
+    if (tid >= kLanes) return;
     const float Z = (zred[0] + zred[1]) + (zred[2] + zred[3]);
-    float U = 0.0f;
+    f4_t U = us[0][tid];
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) U += us[j][tid >> 2][tid & 3];
-    write_result(a, at, HD, tid, U, M * kLn2, Z, err);
+    for (int j = 1; j < kRows; ++j) U += us[j][tid];
+    write_result(a, at, HD, 4 * tid, U, M * kLn2, Z, err);
     if (err) raise_error(err);
 }
 
