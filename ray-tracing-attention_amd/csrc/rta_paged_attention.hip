@@ -6,14 +6,19 @@ namespace rta {
 
 // How a call with one row per sequence is cut: chunks of a multiple of 128 positions (a tile for
 // each of 4 waves), so many that the chip has about kDecGroups workgroups to hand out if every
-// row sees the most it may.
+// row sees the most it may.  Chunks of 128 are for calls that run in one go on the chip's two
+// workgroups per compute unit (wide heads: one), where every further tile of a wave adds its
+// latency (us, chunks of 128 / 256 / 512: one sequence of 1000 positions 9.4 / 11.9 / 17.0); past
+// that a workgroup's start costs more (one of 16000: 25.2 / 22.1 / 21.6; 32 of 1000, 8-bit: 27.3 /
+// 23.4 / 22.4), and larger ones yet balance ragged rows worse (32 of 256 to 8192: 512 70, 1024 75).
 constexpr int kDecGroups = 4096;
 struct Cut {
     int chunk, nchunk;
 };
-static Cut decode_cut(int rows, int heads, int64_t most) {
+static Cut decode_cut(int rows, int heads, int hd, int64_t most) {
     const int64_t want = (rows * (int64_t)heads * most / kDecGroups + 127) / 128 * 128;
-    const int64_t chunk = want < 128 ? 128 : want < 1 << 30 ? want : 1 << 30;
+    const int64_t least = rows * (int64_t)heads * ((most + 127) / 128) <= (hd == 256 ? 256 : 512) ? 128 : 256;
+    const int64_t chunk = want < least ? least : want < 1 << 30 ? want : 1 << 30;
     return Cut{(int)chunk, (int)((most + chunk - 1) / chunk)};
 }
 // Up to kFewCols (row, q head) columns of a kv head are few: the kernel of single rows takes them
@@ -51,7 +56,8 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
     const int64_t len = bound_len(p, max_len);
     *ntile = 0;
     if (!several)
-        return decode_cut(rows, decode_heads(p->kv_heads, group, p->head_dim), most_visible(len, window, sinks));
+        return decode_cut(rows, decode_heads(p->kv_heads, group, p->head_dim), p->head_dim,
+                          most_visible(len, window, sinks));
     const bool few = (int64_t)max_rows * group <= kFewCols;
     const int cols = few ? few_cols(max_rows * group) : prompt_cols(p->head_dim);
     *ntile = (int)(((int64_t)max_rows * group + cols - 1) / cols);
@@ -61,7 +67,7 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
         const int64_t span = (int64_t)window + cols / group + 1;
         most = most_visible(len, (int)(span < INT_MAX ? span : INT_MAX), sinks);
     }
-    if (few) return decode_cut(n, *ntile * p->kv_heads, most);
+    if (few) return decode_cut(n, *ntile * p->kv_heads, p->head_dim, most);
     return prompt_cut((int64_t)*ntile * n * p->kv_heads, most);
 }
 // Workgroups of 256 threads in one grid dimension: below 2^32 threads.

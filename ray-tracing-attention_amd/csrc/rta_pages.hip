@@ -86,13 +86,14 @@ struct Want {
 __device__ __forceinline__ bool want_of(const PageArgs& a, const int32_t* seqs, const int32_t* add, int i, Want& w) {
     w.seq = list_seq(seqs, i);
     w.add = add ? add[i] : 1;
+    w.len = w.fresh = 0;
+    w.tail = -2;
     if ((unsigned)w.seq >= (unsigned)a.max_seqs || w.add < 0) return false;
     w.len = a.lengths[w.seq];
     if (w.len < 0 || (int64_t)w.len + w.add > (int64_t)a.max_pages * a.page) return false;
     const int last = w.len + w.add;   // <= max_pages page <= INT_MAX
     auto pages = [&](int n) { return n ? (int)a.by_page.div((uint32_t)n - 1) + 1 : 0; };
     w.fresh = pages(last) - pages(w.len);
-    w.tail = -2;
     const int e = (int)a.by_page.div((uint32_t)w.len);
     if (w.add > 0 && w.len - e * a.page > 0) w.tail = page_of(a, a.table + (int64_t)w.seq * a.max_pages, e);
     return true;
@@ -100,35 +101,50 @@ __device__ __forceinline__ bool want_of(const PageArgs& a, const int32_t* seqs, 
 
 // One workgroup plans an extend: claims (a sequence listed twice keeps its first entry), the
 // shared last pages, how many pages each entry needs, the free pages, and who gets which.
-// Bound by latency: a few dependent trips through L2 and a read of refs up to the last page handed out.
+// Bound by latency: a few dependent trips through L2 and a read of refs up to the last page handed
+// out.  What an entry wants is found once and kept in LDS (the first 1024 of them: the rest is
+// found again where it is needed; 16 entries and 4096 pages 10.0 us so, 5 times each).
 __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const PageArgs a, const int32_t* __restrict__ seqs,
                                                                    const int32_t* __restrict__ add, int n, PlanWs ws) {
     __shared__ int red[kPlanWaves];
     __shared__ int s_pairs;
+    __shared__ Want kept[kPlanThreads];
+    __shared__ uint8_t kept_ok[kPlanThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     bool bad = false;
     if (tid == 0) s_pairs = 0;
     for (int i = tid; i < n; i += kPlanThreads) {
-        const int s = list_seq(seqs, i);
-        if ((unsigned)s < (unsigned)a.max_seqs) store_agent(ws.owner + s, INT_MAX);
+        Want w;
+        const bool ok = want_of(a, seqs, add, i, w);
+        if ((unsigned)w.seq < (unsigned)a.max_seqs) store_agent(ws.owner + w.seq, INT_MAX);
+        if (i < kPlanThreads) {
+            kept[i] = w;
+            kept_ok[i] = ok;
+        }
     }
+    auto entry = [&](int i, Want& w) {
+        if (i >= kPlanThreads) return want_of(a, seqs, add, i, w);
+        w = kept[i];
+        return kept_ok[i] != 0;
+    };
     __syncthreads();
     for (int i = tid; i < n; i += kPlanThreads) {
-        const int s = list_seq(seqs, i);
-        if ((unsigned)s < (unsigned)a.max_seqs) atomicMin(ws.owner + s, i);
         Want w;
-        if (want_of(a, seqs, add, i, w) && w.tail >= 0) {
+        const bool ok = entry(i, w);
+        if ((unsigned)w.seq < (unsigned)a.max_seqs) atomicMin(ws.owner + w.seq, i);
+        if (ok && w.tail >= 0) {
             store_agent(ws.holders + w.tail, 0);
             store_agent(ws.keeper + w.tail, -1);
         }
     }
     __syncthreads();
-    auto mine = [&](int i, Want& w) {   // entry i wants something and is its sequence's first
-        return want_of(a, seqs, add, i, w) && load_agent(ws.owner + w.seq) == i;
-    };
+    // entry i wants something and is its sequence's first
+    auto mine = [&](int i, Want& w) { return entry(i, w) && load_agent(ws.owner + w.seq) == i; };
     for (int i = tid; i < n; i += kPlanThreads) {
         Want w;
-        if (mine(i, w) && w.tail >= 0 && a.refs[w.tail] > 1) {
+        const bool ok = mine(i, w);
+        if (i < kPlanThreads) kept_ok[i] = ok;   // (settled: mine() finds the same below)
+        if (ok && w.tail >= 0 && a.refs[w.tail] > 1) {
             atomicAdd(ws.holders + w.tail, 1);
             atomicMax(ws.keeper + w.tail, i);
         }
@@ -140,13 +156,15 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const PageArg
         const int i = base + tid;
         int need = 0, kind = 0;
         Want w;
-        bool ok = i < n && mine(i, w);
+        bool ok = i < n && (i < kPlanThreads ? entry(i, w) : mine(i, w));
         if (i < n && !ok) bad = true;
         if (ok) {
-            if (w.tail == -1) kind = 2;
-            else if (w.tail >= 0 && a.refs[w.tail] > 1 &&
-                     !(load_agent(ws.holders + w.tail) == a.refs[w.tail] && load_agent(ws.keeper + w.tail) == i))
-                kind = 1;
+            if (w.tail == -1) {
+                kind = 2;
+            } else if (w.tail >= 0) {
+                const int refs = a.refs[w.tail];
+                if (refs > 1 && !(load_agent(ws.holders + w.tail) == refs && load_agent(ws.keeper + w.tail) == i)) kind = 1;
+            }
             need = w.fresh + (kind ? 1 : 0);
         }
         int total;
@@ -163,21 +181,22 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const PageArg
         upto += total;
     }
     const int wanted = upto < a.n_pages ? (int)upto : a.n_pages;
-    // the lowest free pages, as many as wanted
+    // the lowest free pages, as many as wanted: 16 a thread and turn
+    constexpr int kPer = 16;
     int found = 0;
-    for (int base = 0; base < a.n_pages && found < wanted; base += 4 * kPlanThreads) {
-        int p[4], k = 0;
+    for (int base = 0; base < a.n_pages && found < wanted; base += kPer * kPlanThreads) {
+        uint32_t mask = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int at = base + 4 * tid + j;
-            p[j] = at < a.n_pages && a.refs[at] == 0;
-            k += p[j];
+        for (int j = 0; j < kPer; ++j) {
+            const int at = base + kPer * tid + j;
+            mask |= (at < a.n_pages && a.refs[min(at, a.n_pages - 1)] == 0 ? 1u : 0u) << j;
         }
         int total;
-        int at = found + block_scan(k, red, total);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (p[j]) ws.list[at++] = base + 4 * tid + j;
+        int at = found + block_scan(__popc(mask), red, total);
+        for (; mask; mask &= mask - 1) {
+            if (at < wanted) ws.list[at] = base + kPer * tid + __ffs(mask) - 1;
+            ++at;
+        }
         found += total;
     }
     __syncthreads();   // list, begin, kind are the workgroup's to read
@@ -186,7 +205,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan_kernel(const PageArg
         const int begin = ws.begin[i];
         if (begin < 0) continue;
         Want w;
-        want_of(a, seqs, add, i, w);
+        entry(i, w);
         const int kind = ws.kind[i], need = w.fresh + (kind ? 1 : 0);
         if (begin + need > found) {
             bad = true;

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import BF16, F16, Q8_ROW, check
-from .ops import _rows, _rs, _workspace
+from .ops import _rows, _rs
 
 WHOLE = 2**31 - 1   # a `last` past every length
 
@@ -73,12 +73,24 @@ class PagedCache:
     # ------------------------------------------------------------------ helpers ----
     def _call(self, name, *args):
         """One entry point on the current stream of the pool's device."""
-        fn = getattr(self.lib, name)
-        if torch.cuda.current_device() == self.device.index:
-            check(fn(self._at, *args, torch.cuda.current_stream().cuda_stream), name)
-            return
-        with torch.cuda.device(self.device):
-            check(fn(self._at, *args, torch.cuda.current_stream().cuda_stream), name)
+        fn, index = getattr(self.lib, name), self.device.index
+        # (the raw handle: building a Stream object takes 3 us, as long as a launch)
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        if torch.cuda.current_device() == index:
+            status = fn(self._at, *args, stream)
+        else:
+            with torch.cuda.device(index):
+                status = fn(self._at, *args, stream)
+        if status:
+            check(status, name)
+
+    def _scratch(self, need, given):
+        """(pointer, bytes) of a call's workspace; the tensor comes third, to outlive the launch."""
+        if given is None:
+            if not need:
+                return None, 0, None
+            given = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return given.data_ptr(), given.numel() * given.element_size(), given
 
     def _ints(self, t, name, n=None):
         if t is None:
@@ -89,14 +101,11 @@ class PagedCache:
             raise ValueError(f"{name} must be contiguous and 1-D" + (f" of {n} values" if n is not None else ""))
         return t.data_ptr()
 
-    def _floats(self, t, name, shape):
-        if t is None:
-            return None
+    def _check_floats(self, t, name, shape):
         if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.float32:
             raise TypeError(f"{name} must be a float32 tensor on {self.device}")
-        if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous of shape {tuple(shape)}")
-        return t.data_ptr()
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous of shape {shape}")
 
     def _list(self, rows, seqs, cu_rows):
         """(seqs pointer, cu_rows pointer, entries) of a row list over `rows` rows."""
@@ -127,8 +136,8 @@ class PagedCache:
         page shared with another sequence is copied first.  seqs None: the first n sequences."""
         n = self._entries(seqs, n)
         sp, ap = self._ints(seqs, "seqs", n), self._ints(add, "add", n)
-        ws = _workspace(self.workspace_bytes(n), self.device, workspace)
-        self._call("rta_pages_extend", sp, ap, n, ws.data_ptr(), ws.numel())
+        ws, size, _keep = self._scratch(self.workspace_bytes(n), workspace)
+        self._call("rta_pages_extend", sp, ap, n, ws, size)
 
     def fork(self, src, dst):
         """The empty sequences dst become copies of src that share their pages."""
@@ -149,8 +158,8 @@ class PagedCache:
         if used is None:
             used = torch.empty(1, dtype=torch.int32, device=self.device)
         up = self._ints(used, "used", 1)
-        ws = _workspace(self.workspace_bytes(), self.device, workspace)
-        self._call("rta_pages_compact", up, ws.data_ptr(), ws.numel())
+        ws, size, _keep = self._scratch(self.workspace_bytes(), workspace)
+        self._call("rta_pages_compact", up, ws, size)
         return used
 
     # ------------------------------------------------------------------ rows ----
@@ -203,18 +212,23 @@ class PagedCache:
         sp, cu, n = self._list(rows, seqs, cu_rows)
         if max_rows is None:
             max_rows = 1 if cu_rows is None else rows
+        for t, name, shape in ((gate, "gate", (rows, hq, hd)), (out, "out", (rows, hq, hd)), (m, "m", (rows, hq)),
+                               (z, "z", (rows, hq))):
+            if t is not None:
+                self._check_floats(t, name, shape)
         if out is None:
             out = torch.empty(rows, hq, hd, dtype=torch.float32, device=self.device)
         if m is None:
             m = torch.empty(rows, hq, dtype=torch.float32, device=self.device)
         if z is None:
             z = torch.empty(rows, hq, dtype=torch.float32, device=self.device)
-        need = self.attention_workspace_bytes(hq, rows, n, max_rows, max_len, window, sinks)
-        ws = _workspace(need, self.device, workspace)
+        max_len = max_len or 0
+        need = self.lib.rta_paged_attention_workspace_bytes(self._at, hq, rows, n, max_rows, max_len, window, sinks)
+        ws, size, _keep = self._scratch(need, workspace)
         stride = q.stride(0) if rows > 1 else max(q.stride(0), hq * hd)
         self._call("rta_paged_attention", layer, q.data_ptr(), stride, rows, hq, sp, cu, n, max_rows, max_len, window,
-                   sinks, self._floats(gate, "gate", (rows, hq, hd)), self._floats(out, "out", (rows, hq, hd)),
-                   self._floats(m, "m", (rows, hq)), self._floats(z, "z", (rows, hq)), ws.data_ptr(), ws.numel())
+                   sinks, None if gate is None else gate.data_ptr(), out.data_ptr(), m.data_ptr(), z.data_ptr(), ws,
+                   size)
         return out, m, z
 
 
