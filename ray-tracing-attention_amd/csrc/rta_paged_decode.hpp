@@ -283,6 +283,15 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             load_v();
             spot(t + 2 * kDecWaves, next);
         }
+        // Both parts of a score.  The two columns have to come to the same weights bit by bit, since
+        // one takes its upper part and the other the rest: so their sum comes first (behind a
+        // product it could be contracted, to one rounding here and another there).
+        if constexpr (!MULTI) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[c][j >> 2][j & 3] += dpp_mov<0xB1>(s[c][j >> 2][j & 3]);
+        }
         int ve_new = ve;
         if constexpr (kScaled) {   // value scales below 2^0
             float mx = 0.0f;
@@ -299,12 +308,6 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 s[c][0] *= kf[0];
                 s[c][1] *= kf[1];
             }
-        }
-        if constexpr (!MULTI) {   // both parts
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) s[c][j >> 2][j & 3] += dpp_mov<0xB1>(s[c][j >> 2][j & 3]);
         }
         sm.watch(s);
         if (!whole) {

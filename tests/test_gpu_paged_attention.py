@@ -242,24 +242,27 @@ def test_pools_past_four_gigabytes(env):
 
 
 @pytest.mark.parametrize("fmt", [ref.F16, ref.BF16, ref.Q8_ROW])
-def test_long_histories_keep_fp32_precision(env, fmt):
-    """Over 60000 positions nearly all of the sum lies in weights far below the largest.  Bound:
-    every weight carries the roundings of its score (up to 16 in log2 units: half a step 2^-21) and
-    of its parts (2^-22), all of them independent: 2^-20 of the result as a whole, doubled."""
+@pytest.mark.parametrize("length", [2048, 60000])
+def test_long_histories_keep_fp32_precision(env, fmt, length):
+    """Over a long history nearly all of the sum lies in weights far below the largest, and values
+    around zero leave nothing of it but the weights' own errors.  Bound: every weight carries the
+    roundings of its score (up to 16 in log2 units: half a step 2^-21) and of its parts (2^-22),
+    all of them independent: 2^-20 of a head's result, doubled."""
     torch, _, dev = env
-    lens = [60000]
-    c = filled(env, fmt, 1, 64, 256, lens)
-    fill(env, c, lens, 34)
-    q = rows_of(torch, dev, 3, 8, 64, 35, 2.0)
+    c = filled(env, fmt, 1, 128, 256, [length])
+    gen = torch.Generator(device=dev).manual_seed(34)
+    k, v = (torch.randn(length, 128, generator=gen, device=dev) for _ in range(2))
+    c.append(k, v, cu_rows=ints(torch, [0, length], dev))
+    q = rows_of(torch, dev, 5, 8, 128, 35, 1.5)
     k, v, _ = ref.dense(c, 0, 0)
-    p = np.exp(q.cpu().double().numpy() @ k[:, 0].T / 8.0)   # [3, 8, 60000]
-    for n in (1, 3):   # one row, and three in the kernel of several
-        got = c.attention(q[:n], seqs=ints(torch, [0], dev), cu_rows=ints(torch, [0, n], dev), max_rows=n)[0]
+    p = np.exp(q.cpu().double().numpy() @ k[:, 0].T / np.sqrt(128))   # [5, 8, length]
+    for n in (1, 2, 5):   # one row, and two and five in 16 and 32 columns of the kernel of a few
+        got = c.attention(q[:n], cu_rows=ints(torch, [0, n], dev), max_rows=n)[0]
         for r in range(n):
-            w = p[r][:, : lens[0] - n + 1 + r]
+            w = p[r][:, : length - n + 1 + r]
             want = w @ v[: w.shape[1], 0] / w.sum(1, keepdims=True)
-            err = got[r].cpu().double().numpy() - want
-            assert np.linalg.norm(err) <= 2 * 2.0**-20 * np.linalg.norm(want), (n, r)
+            err = np.linalg.norm(got[r].cpu().double().numpy() - want, axis=1)
+            assert np.all(err <= 2 * 2.0**-20 * np.linalg.norm(want, axis=1)), (n, r, err / np.linalg.norm(want, axis=1))
 
 
 def test_tensors_on_another_stream(env):
