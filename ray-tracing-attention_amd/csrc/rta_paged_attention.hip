@@ -15,16 +15,19 @@ constexpr int kDecGroups = 4096;
 struct Cut {
     int chunk, nchunk;
 };
-static Cut decode_cut(int rows, int heads, int hd, int64_t most) {
-    const int64_t want = (rows * (int64_t)heads * most / kDecGroups + 127) / 128 * 128;
-    const int64_t least = rows * (int64_t)heads * ((most + 127) / 128) <= (hd == 256 ? 256 : 512) ? 128 : 256;
+static Cut decode_cut(int64_t rows, int heads, int hd, int64_t most) {
+    const int64_t want = (rows * heads * most / kDecGroups + 127) / 128 * 128;
+    const int64_t least = rows * heads * ((most + 127) / 128) <= (hd == 256 ? 256 : 512) ? 128 : 256;
     const int64_t chunk = want < least ? least : want < 1 << 30 ? want : 1 << 30;
     return Cut{(int)chunk, (int)((most + chunk - 1) / chunk)};
 }
-// Up to kFewCols (row, q head) columns of a kv head are few: the kernel of single rows takes them
-// in groups of 16 or 32, each reading the history once (bound by its bytes; the tiles of 128
-// columns of the other kernel would stay mostly empty).
-constexpr int kFewCols = 64;
+// Up to 32 (row, q head) columns of a kv head (wide heads: 16) are few: the kernel of single rows
+// takes them in one group, bound by the history's bytes, where the other kernel's 128 columns would
+// stay mostly empty (us, this / the other: 16 sequences of 4 rows over 4000 bf16 positions, 4 q
+// heads per kv head 60 / 91, 8 rows 76 / 97; one of 12 rows over 8000, in two groups 31 / 27).
+// Their workgroups start and end with more work, so a quarter as many are asked for (5 rows of 16
+// sequences over 8000 8-bit positions 136 -> 86).
+static bool few_rows(int64_t max_rows, int group, int hd) { return max_rows * group <= (hd == 256 ? 16 : 32); }
 // With several rows: column tiles enough for two workgroups per compute unit stand alone, fewer
 // are cut into chunks of positions (a multiple of 64, 256 at least).
 constexpr int kPromptGroups = 1024;
@@ -58,7 +61,7 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
     if (!several)
         return decode_cut(rows, decode_heads(p->kv_heads, group, p->head_dim), p->head_dim,
                           most_visible(len, window, sinks));
-    const bool few = (int64_t)max_rows * group <= kFewCols;
+    const bool few = few_rows(max_rows, group, p->head_dim);
     const int cols = few ? few_cols(max_rows * group) : prompt_cols(p->head_dim);
     *ntile = (int)(((int64_t)max_rows * group + cols - 1) / cols);
     // (a column tile sees from its first row's window on)
@@ -67,12 +70,12 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
         const int64_t span = (int64_t)window + cols / group + 1;
         most = most_visible(len, (int)(span < INT_MAX ? span : INT_MAX), sinks);
     }
-    if (few) return decode_cut(n, *ntile * p->kv_heads, p->head_dim, most);
+    if (few) return decode_cut(4 * (int64_t)n, p->kv_heads, p->head_dim, most);
     return prompt_cut((int64_t)*ntile * n * p->kv_heads, most);
 }
 // Workgroups of 256 threads in one grid dimension: below 2^32 threads.
 static bool grid_fits(const rta_pages* p, int hq, int rows, int n, int max_rows) {
-    const int64_t group = hq / p->kv_heads, most = (1 << 24) - 1, tiles = (max_rows * group + 15) / 16;
+    const int64_t group = hq / p->kv_heads, most = (1 << 24) - 1, tiles = (max_rows * group + 63) / 64;
     return rows <= most && (int64_t)rows * p->kv_heads * group <= INT_MAX &&
            rows * (int64_t)decode_heads(p->kv_heads, (int)group, p->head_dim) <= most &&
            (max_rows == 1 || tiles <= most / ((int64_t)n * p->kv_heads));
@@ -143,11 +146,11 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
             a.part = static_cast<float*>(workspace);
             a.mz = reinterpret_cast<float2*>(a.part + (size_t)rows * hq * cut.nchunk * HD);
             a.ntile = ntile;
-            if (ntile && (int64_t)max_rows * a.group <= kFewCols) {
+            if (ntile && few_rows(max_rows, a.group, HD)) {   // one group of columns
                 a.cols = few_cols(max_rows * a.group);
-                const dim3 grid(ntile * n * pages->kv_heads, 1, cut.nchunk), block(64 * kDecWaves);
+                const dim3 grid(n * pages->kv_heads, 1, cut.nchunk), block(64 * kDecWaves);
                 if (a.cols == 16) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1, true>), grid, block, 0, s, a);
-                else hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2, true>), grid, block, 0, s, a);
+                else if constexpr (HD < 256) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2, true>), grid, block, 0, s, a);
             } else if (ntile) {
                 a.cols = PromptLds<F, HD>::kCols;
                 hipLaunchKernelGGL((paged_prompt_kernel<F, HD>), dim3(ntile * n * pages->kv_heads, 1, cut.nchunk),

@@ -51,10 +51,10 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Workgroups go round the 8 XCDs in order.  Heads first and rows turned by the chunk keep a long
     // row's chunks on all of them (rows first: 32 rows of 256 to 8192 bf16 positions 124 us, so 65)
-    const int groups = MULTI ? a.ntile : (a.group + L::kHeads - 1) / L::kHeads;   // column groups of a kv head
+    const int groups = MULTI ? 1 : (a.group + L::kHeads - 1) / L::kHeads;   // column groups of a kv head
     const int per_row = a.p.kv_heads * groups, y = blockIdx.x % per_row;
     const int turned = (int)((blockIdx.x / per_row + blockIdx.z) % (MULTI ? a.l.n : a.l.rows));
-    const int kvh = y / groups, g0 = (y - kvh * groups) * L::kHeads;
+    const int kvh = MULTI ? y : y / groups, g0 = (y - kvh * groups) * L::kHeads;
     uint32_t err = 0;
     Visible see;
     const int32_t* table;
@@ -63,13 +63,12 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     if constexpr (MULTI) {
         Entry en;
         if (!resolve_entry(a, turned, en, err)) return;
-        if (g0 > 0 || kvh > 0) err &= ~RTA_DEVERR_PAGES;   // told once
-        cols = min(en.rows * a.group - g0, L::kHeads);
-        if (cols <= 0) return;
+        if (kvh > 0) err &= ~RTA_DEVERR_PAGES;   // told once
+        cols = en.rows * a.group;                // <= kHeads: max_rows bounds them
         row0 = en.base;
         table = en.table;
         t0 = en.len - en.count;
-        see = en.len ? prompt_span(a, en.len, en.count, g0 / L::kHeads, L::kHeads) : Visible{0, 0, 0};
+        see = en.len ? prompt_span(a, en.len, en.count, 0, L::kHeads) : Visible{0, 0, 0};
     } else {
         if (!resolve_row(a, turned, table, see, err)) {
             if (err && threadIdx.x == 0) raise_error(err);
@@ -195,8 +194,8 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     }
     int t_first = 0, t_last = 0;   // the columns' first and last positions
     if constexpr (MULTI) {
-        t_first = t0 + g0 / a.group;
-        t_last = t0 + (g0 + cols - 1) / a.group;
+        t_first = t0;
+        t_last = t0 + (cols - 1) / a.group;
     }
     __syncthreads();
 
