@@ -590,7 +590,8 @@ int rta_paged_read(const rta_pages* pages, int layer, int rows, const int32_t* s
  * (all raise RTA_DEVERR_PAGES); rows past an entry's max_rows raise it and are left as they
  * were; a visible position without a page raises it and is not seen.  A visible position whose
  * score is not finite, or a result that is not, raises RTA_DEVERR_DETECTOR (that row's values
- * then mean nothing).  What lies in a page past its sequence's length is never used.
+ * then mean nothing; rows that do not see the position keep theirs).  What lies in a page past its
+ * sequence's length is never used.
  * Workspace: rta_paged_attention_workspace_bytes() bytes, 16-byte aligned (0: none needed). */
 size_t rta_paged_attention_workspace_bytes(const rta_pages* pages, int hq, int rows, int n, int max_rows,
                                            int max_len, int window, int sinks);

@@ -173,6 +173,17 @@ __device__ __forceinline__ void split_parts(const float v[8], int part, u4_t op[
     }
 }
 
+// Whether a piece of 2-byte elements holds an inf or a NaN: an exponent of ones carries into the
+// half's top bit.
+template <int FMT>
+__device__ __forceinline__ bool piece_not_finite(u4_t x) {
+    constexpr uint32_t kE = FMT == RTA_BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = FMT == RTA_BF16 ? 0x00800080u : 0x04000400u;
+    uint32_t hit = 0;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) hit |= (x[y] & kE) + kOne;
+    return (hit & 0x80008000u) != 0;
+}
+
 // Dims of element s of the 8 that lane segment u holds for product kb: 16-byte pieces of a row
 // follow the segments, one piece per product (2-byte elements) or two products (codes).
 template <int FMT>
@@ -334,6 +345,17 @@ struct Softmax {
             w[j] = __builtin_amdgcn_exp2f(fmaf(x[j >> 2][j & 3], fac, -base));
             z[c] += w[j];
         }
+    }
+    // A weight of 0 times a value that is not finite is not 0.  Where the columns do not all see a
+    // tile whole, rows with such values (bad, bit 16 h + 4 u + e of a lane's position) are zeros in
+    // the product, and the sums of the columns that do see one become NaN.
+    __device__ __forceinline__ void poison(const f4_t (*s)[2], uint32_t bad, int u) {
+        const uint32_t mine = bad >> (4 * u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (((mine >> (16 * (j >> 2) + (j & 3))) & 1u) && s[c][j >> 2][j & 3] != -INFINITY) z[c] = NAN;
     }
     // The maximum in log2 units, and what brings sums over weights to it as the base.
     __device__ __forceinline__ void finish(int c, float fac, float& M, float& back) const {

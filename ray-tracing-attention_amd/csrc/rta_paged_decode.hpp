@@ -3,8 +3,8 @@
 // Bound by the history's bytes: every visible key and value is read once per kv head (for more
 // than 8 NC q heads per kv head once per group of those).  A workgroup of 4 waves takes one
 // (row, kv head, chunk of visible positions); a wave takes every fourth tile of 32 positions and
-// works alone until the end, so the waves of a compute unit (16 of them at 128 registers and 39 KB
-// of LDS per workgroup) drift apart and cover each other's waits:
+// works alone until the end, so the waves of a compute unit (12 of them for 128-wide heads) drift apart
+// and cover each other's waits:
 //   lane (i, u) loads piece u of the rows of positions i and 16 + i, keys straight as the A
 //   operand, values into LDS (32 rows, 16 bytes of padding each: the 16 rows that a transposing
 //   read touches then fall on every bank exactly twice) and back transposed;
@@ -250,6 +250,29 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 vf[h] = *reinterpret_cast<const f4_t*>(sl + 32 + 16 * h + 4 * u);
             }
         }
+        uint32_t bad = 0;
+        if (MULTI && !whole) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                bool hit = false;
+                if constexpr (kScaled) {   // (the scale as its position's lanes hold it)
+                    hit = !(fabsf(sl[32 + 16 * h + i]) < INFINITY);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) vf[h][e] = fabsf(vf[h][e]) < INFINITY ? vf[h][e] : 0.0f;
+                } else {
+#pragma unroll
+                    for (int x = 0; x < kLoads; ++x)
+                        if (piece_not_finite<FMT>(v[h][x])) {
+                            v[h][x] = u4_t{0, 0, 0, 0};
+                            hit = true;
+                        }
+                }
+                uint64_t rows = __builtin_amdgcn_ballot_w64(hit);   // bit 16 u + i: a piece of row i
+                rows |= rows >> 32;
+                bad |= (uint32_t)((rows | rows >> 16) & 0xffffu) << (16 * h);
+            }
+            bad &= now;
+        }
         // V into LDS (rows that do not count as zeros), then the next tile's rows
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -312,6 +335,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
         if (!whole) {
             if constexpr (MULTI) {
                 mask_columns<NC>(s, now, see, begin + t * kDecTile, u, t_col, a.window, a.sinks);
+                if (bad) sm.poison(s, bad, u);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {

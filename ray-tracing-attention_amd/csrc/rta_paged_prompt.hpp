@@ -30,7 +30,7 @@ struct PromptLds {
 };
 
 template <int FMT, int HD>
-__global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 1 : 2)) paged_prompt_kernel(const PagedAttnArgs a) {
     using L = PromptLds<FMT, HD>;
     constexpr int kParts = PageFmt<FMT>::kParts, kB = PageFmt<FMT>::kBytes, NQ = L::kNQ;
     constexpr int kKb = HD / 32, kDt = HD / 16;
@@ -104,7 +104,11 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
             *reinterpret_cast<u4_t*>(dst + 16 * piece) = x;
         }
     };
-    auto store = [&](uint8_t* buf) {
+    // the rows' first and last positions: tiles that all of them see whole need no care for values
+    // that are not finite
+    const int lo = len - count + tile * L::kCols / a.group;
+    const int hi = len - count + min((tile + 1) * L::kCols - 1, live_rows * a.group - 1) / a.group;
+    auto store = [&](int t, uint8_t* buf) {
         // rows that do not count are zeros: a weight of 0 times what lies there must be 0
         if (__builtin_amdgcn_ballot_w64(okr != (1u << kPass) - 1)) {   // the last tile, or a page missing
 #pragma unroll
@@ -113,6 +117,24 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                     kr[k] = vr[k] = u4_t{0, 0, 0, 0};
                     if constexpr (kScaled) ksr[k] = vsr[k] = 0.0f;
                 }
+        }
+        uint32_t bad = 0;
+        const int j0 = begin + t * L::kTile;
+        if (see.position(min(j0 + L::kTile, end) - 1) > lo || (a.window && see.position(j0) <= hi - a.window)) {
+#pragma unroll
+            for (int k = 0; k < kPass; ++k) {
+                if constexpr (kScaled) {
+                    if (!(fabsf(vsr[k]) < INFINITY)) {
+                        vsr[k] = 0.0f;
+                        bad |= 1u << k;
+                    }
+                } else {   // a row's threads are of one wave
+                    constexpr uint64_t kRow = kPieces == 32 ? 0xffffffffull : (1ull << kPieces) - 1;
+                    const bool hit = piece_not_finite<FMT>(vr[k]);
+                    if (hit) vr[k] = u4_t{0, 0, 0, 0};
+                    if (__builtin_amdgcn_ballot_w64(hit) & (kRow << (lane & ~(kPieces - 1)))) bad |= 1u << k;
+                }
+            }
         }
 #pragma unroll
         for (int k = 0; k < kPass; ++k) {
@@ -125,7 +147,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                     f[row] = ksr[k];
                     f[L::kTile + row] = vsr[k];
                 }
-                reinterpret_cast<uint32_t*>(buf + L::kRows + L::kScales)[row] = (okr >> k) & 1u;
+                reinterpret_cast<uint32_t*>(buf + L::kRows + L::kScales)[row] = ((okr >> k) & 1u) | ((bad >> k) & 1u) << 1;
             }
         }
     };
@@ -183,7 +205,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
     for (int c = 0; c < NQ; ++c) {
         for (int d = 0; d < kDt; ++d) o[c][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    if (nt > 0) store(lds);
+    if (nt > 0) store(0, lds);
     __syncthreads();
 
     for (int t = 0; t < nt; ++t) {
@@ -195,9 +217,10 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
         const int j0 = begin + t * L::kTile, j1 = min(j0 + L::kTile, end) - 1;
         const int p0 = see.position(j0), p1 = see.position(j1);
         if (on && p0 <= t_hi) {
-            const uint64_t okm = __builtin_amdgcn_ballot_w64(
-                lane < L::kTile && reinterpret_cast<const uint32_t*>(buf + L::kRows + L::kScales)[lane & (L::kTile - 1)]);
-            const bool whole = okm == (L::kTile == 64 ? ~0ull : 0xffffffffull) && p1 <= t_lo &&
+            uint32_t row_state = reinterpret_cast<const uint32_t*>(buf + L::kRows + L::kScales)[lane & (L::kTile - 1)];
+            if (L::kTile < 64 && lane >= L::kTile) row_state = 0;
+            const uint64_t okm = __builtin_amdgcn_ballot_w64(row_state != 0), badm = __builtin_amdgcn_ballot_w64(row_state > 1);
+            const bool whole = okm == (L::kTile == 64 ? ~0ull : 0xffffffffull) && badm == 0 && p1 <= t_lo &&
                                (a.window == 0 || p0 > t_hi - a.window);
             const float* sc = reinterpret_cast<const float*>(buf + L::kRows);
             float wscale = 1.0f;
@@ -260,8 +283,10 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                     }
                 }
                 sm.watch(x);
-                if (!whole)
+                if (!whole) {
                     mask_columns<NQ>(x, (uint32_t)(okm >> (32 * sub)), see, j0 + 32 * sub, u, t_col, a.window, a.sinks);
+                    if (badm) sm.poison(x, (uint32_t)(badm >> (32 * sub)), u);
+                }
                 sm.template raise<kDt>(x, fac, kScaled ? ve - ve_new : 0, o);
                 u4_t pb[NQ][kParts];
 #pragma unroll
@@ -291,7 +316,7 @@ __global__ void __launch_bounds__(256, 2) paged_prompt_kernel(const PagedAttnArg
                 }
             }
         }
-        if (t + 1 < nt) store(lds + ((t + 1) & 1) * L::kBuf);
+        if (t + 1 < nt) store(t + 1, lds + ((t + 1) & 1) * L::kBuf);
         __syncthreads();
     }
 

@@ -201,6 +201,52 @@ def test_a_visible_value_that_is_not_finite_is_reported(env):
     assert ops.device_error() == 0
 
 
+@pytest.mark.parametrize("fmt", [ref.F16, ref.BF16, ref.Q8_ROW])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,hq,hkv,window", [(4, 4, 1, 0), (8, 4, 1, 5), (90, 8, 2, 0), (90, 8, 2, 24)])
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(env, fmt, hd, rows, hq, hkv, window):
+    """Keys and values of two positions are inf and NaN: rows before them, and rows whose window has
+    passed them, come out as if those positions held anything else."""
+    torch, _, dev = env
+    length = 130
+    c = filled(env, fmt, hkv, hd, 16, [length])
+    fill(env, c, [length], 36)
+    q = rows_of(torch, dev, rows, hq, hd, 37)
+    cu = ints(torch, [0, rows], dev)
+    p0 = length - rows
+    odd = sorted({p0 + 2, p0 + rows // 2})
+    for p in odd:
+        for which in (0, 1):
+            page = int(c.table[0, p // 16])
+            if fmt == ref.Q8_ROW:
+                at = (which * hkv * 16 + p % 16) * 4 + 2 * hkv * 16 * hd
+                c.pool[0, page, at : at + 4] = torch.tensor([float("inf")], device=dev).view(torch.uint8)
+            else:
+                e = c.pool[0, page].view(torch.float16 if fmt == ref.F16 else torch.bfloat16)
+                at = (which * hkv * 16 + p % 16) * hd
+                e[at + 3], e[at + 5] = float("nan"), float("-inf")
+    out, m, z = c.attention(q, cu_rows=cu, max_rows=rows, window=window)
+    assert ops.device_error() & _lib.DEVERR_DETECTOR
+    # the oracle sees finite numbers there: rows that may not look at them do not change
+    k, v, held = ref.dense(c, 0, 0)
+    k, v = np.nan_to_num(k, nan=1.0, posinf=1.0, neginf=1.0), np.nan_to_num(v, nan=1.0, posinf=1.0, neginf=1.0)
+    per = hq // hkv
+    clean = seen = 0
+    for r in range(rows):
+        t = p0 + r
+        sees = any(p <= t and (not window or p > t - window) for p in odd)
+        if sees:
+            seen += 1
+            heads = slice(per, hq)   # kv head 0 holds them: its values mean nothing
+        else:
+            clean += 1
+            heads = slice(0, hq)
+        want = ref.attend(q[r].cpu().double().numpy(), k, v, held, t, window)
+        if heads.start < hq:
+            ref.check_rows([x[r : r + 1, heads] for x in (out, m, z)], [tuple(w[heads] for w in want)], r)
+    assert clean >= 2 and seen >= 2
+
+
 def test_large_scores_and_tiny_queries(env):
     torch, _, dev = env
     lens = [300, 300, 300]
