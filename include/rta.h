@@ -507,8 +507,9 @@ int rta_hybrid_decode_step_capture(const rta_hybrid_shape* shape, const rta_hybr
  *
  * Every call is stream ordered, allocates nothing and may be captured in a HIP graph.  What
  * cannot be known on the host is checked on the device: a sequence or page outside its range, a
- * sequence listed twice, a length past max_pages * page, or a pool with too few free pages
- * raises RTA_DEVERR_PAGES and that entry of the list is left undone. */
+ * sequence listed twice (to be extended, forked into or freed), a length past max_pages * page,
+ * or a pool with too few free pages raises RTA_DEVERR_PAGES and that entry of the list is left
+ * undone. */
 typedef struct rta_pages {
     int fmt;               /* RTA_F16, RTA_BF16 or RTA_Q8_ROW */
     int kv_heads;          /* 1 .. 1024 */
@@ -564,9 +565,9 @@ int rta_pages_compact(const rta_pages* pages, int32_t* used, void* workspace, si
 /* The rows' keys and values k[r, :kv_heads * head_dim], v (fp32, row strides in floats) into
  * the pages of layer `layer`: rounded to nearest even, or for RTA_Q8_ROW scale = max|x| * (1 / 127)
  * over the head (fp32) and code = round(x / scale) (a head with a value that is not finite reads back
- * as NaN).  A page named by several sequences is written for
- * all of them (rta_pages_extend has made the last one the sequence's own).  Call it after
- * rta_pages_extend. */
+ * as NaN).  A page named by several sequences is written for all of them (rta_pages_extend has
+ * made the last one the sequence's own), and of a sequence listed twice either entry's values
+ * may stay.  Call it after rta_pages_extend. */
 int rta_paged_append(const rta_pages* pages, int layer, const float* k, int64_t k_stride, const float* v,
                      int64_t v_stride, int rows, const int32_t* seqs, const int32_t* cu_rows, int n,
                      rta_stream_t stream);

@@ -90,6 +90,10 @@ class PagedCache:
             if not need:
                 return None, 0, None
             given = torch.empty(need, dtype=torch.uint8, device=self.device)
+        elif not isinstance(given, torch.Tensor) or given.device != self.device:
+            raise TypeError(f"workspace must be a tensor on {self.device}")
+        elif not given.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         return given.data_ptr(), given.numel() * given.element_size(), given
 
     def _ints(self, t, name, n=None):

@@ -311,6 +311,40 @@ def test_long_histories_keep_fp32_precision(env, fmt, length):
             assert np.all(err <= 2 * 2.0**-20 * np.linalg.norm(want, axis=1)), (n, r, err / np.linalg.norm(want, axis=1))
 
 
+@pytest.mark.parametrize("fmt", [ref.F16, ref.BF16, ref.Q8_ROW])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("counts", [[1, 1], [5, 3], [80, 41]])
+def test_tensors_at_any_multiple_of_four_bytes(env, fmt, hd, counts):
+    """Queries of an odd row stride, and out, gate, m and z at addresses that are no multiple of 16."""
+    torch, _, dev = env
+    lens, hq = [600, 41], 4
+    c = filled(env, fmt, 2, hd, 16, lens)
+    fill(env, c, lens, 38)
+    rows = sum(counts)
+    q, gate = rows_of(torch, dev, rows, hq, hd, 39), rows_of(torch, dev, rows, hq, hd, 40)
+    cu = None if max(counts) == 1 else ints(torch, np.concatenate([[0], np.cumsum(counts)]), dev)
+    how = dict(cu_rows=cu, max_rows=max(counts), max_len=600, window=300, sinks=2)
+    want = c.attention(q, gate=gate, **how)
+
+    def odd(t, shift, pitch):
+        flat = torch.full((shift + rows * pitch + 8,), 7.0, device=dev)
+        x = flat[shift : shift + rows * pitch].view(rows, pitch)[:, : t[0].numel()].view(t.shape)
+        x.copy_(t)
+        return flat, x
+
+    n = hq * hd
+    for shift in (1, 2, 3):
+        _, q2 = odd(q, shift, n + shift)
+        _, g2 = odd(gate, 4 - shift, n)
+        flat, out = odd(torch.zeros_like(q), shift, n)
+        _, m = odd(torch.zeros(rows, hq, device=dev), shift, hq)
+        _, z = odd(torch.zeros(rows, hq, device=dev), 4 - shift, hq)
+        c.attention(q2, gate=g2, out=out, m=m, z=z, **how)
+        assert all(torch.equal(x, y) for x, y in zip((out, m, z), want)), shift
+        assert torch.all(flat[:shift] == 7.0) and torch.all(flat[shift + rows * n :] == 7.0)
+    assert ops.device_error() == 0
+
+
 def test_tensors_on_another_stream(env):
     torch, _, dev = env
     lens = [200, 3]

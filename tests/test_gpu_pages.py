@@ -323,6 +323,51 @@ def test_rows_of_bad_entries(env):
     assert ops.device_error() == _lib.DEVERR_PAGES
 
 
+def test_a_workspace_elsewhere_is_refused(env):
+    torch, pages, dev = env
+    c, _ = make(env)
+    need = c.workspace_bytes(1)
+    with pytest.raises(TypeError):
+        c.extend(n=1, workspace=torch.empty(need, dtype=torch.uint8))
+    with pytest.raises(TypeError):
+        c.compact(workspace=np.empty(need, np.uint8))
+    with pytest.raises(ValueError):
+        c.extend(n=1, workspace=torch.empty(need, 2, dtype=torch.uint8, device=dev)[:, 0])
+    with pytest.raises(_lib.RtaError):
+        c.extend(n=1, workspace=torch.empty(need - 1, dtype=torch.uint8, device=dev))
+    c.extend(n=1, workspace=torch.empty(need, dtype=torch.uint8, device=dev))
+    assert c.lengths.tolist()[0] == 1 and ops.device_error() == 0
+
+
+@pytest.mark.parametrize("fmt", [ref.F16, ref.BF16, ref.Q8_ROW])
+def test_rows_at_any_multiple_of_four_bytes(env, fmt):
+    """append and read at strides and addresses that are no multiple of 16 bytes."""
+    torch, pages, dev = env
+    gen = torch.Generator(device=dev).manual_seed(5)
+    got = []
+    for shift, pitch in ((0, 128), (1, 131), (3, 129)):
+        c = filled(env, fmt, 2, 64, 5, [7, 3])
+        gen.manual_seed(5)
+        rows = torch.randn(10, 2, 128, generator=gen, device=dev)
+        flat = torch.zeros(2, 10 * pitch + 4, device=dev)
+        k, v = (flat[i, shift : shift + 10 * pitch].view(10, pitch)[:, :128] for i in (0, 1))
+        k.copy_(rows[:, 0])
+        v.copy_(rows[:, 1])
+        cu = ints(torch, [0, 7, 10], dev)
+        c.append(k, v, cu_rows=cu)
+        back = torch.full((2, 10 * pitch + 4), 7.0, device=dev)
+        kb, vb = (back[i, shift : shift + 10 * pitch].view(10, pitch)[:, :128] for i in (0, 1))
+        c.read(10, cu_rows=cu, k=kb, v=vb)
+        outside = torch.ones_like(back, dtype=torch.bool)
+        for i in (0, 1):
+            outside[i, shift : shift + 10 * pitch].view(10, pitch)[:, :128] = False
+        assert torch.all(back[outside] == 7.0)
+        got.append((kb.clone(), vb.clone()))
+    for kb, vb in got[1:]:
+        assert torch.equal(kb, got[0][0]) and torch.equal(vb, got[0][1])
+    assert ops.device_error() == 0
+
+
 def test_python_refusals(env):
     torch, pages, dev = env
     with pytest.raises(ValueError):
