@@ -8,6 +8,8 @@
 // column i, which is where the second wants its B operand (k slots 8u ..) if its k axis is
 // ordered  slot 8u + s  <->  position 4u + s (s < 4), 16 + 4u + s - 4 (else) of 32 positions;
 // so weights never leave their lane, and V^T comes in that order from a transposing LDS read.
+// On v_mfma_f32_32x32x16 (prompts) lane (i = lane % 32, u = lane / 32) holds positions 8h + 4u + e
+// of 32, h = 0 .. 3, and the two products of 16 positions have their k axis in that order.
 //
 // fp32 queries and weights meet 16-bit values, so each is split into parts that are exact
 // 16-bit numbers and whose products are added in fp32:
@@ -27,6 +29,7 @@ namespace rta {
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef float acc16_t __attribute__((ext_vector_type(16)));
 
 struct PagedAttnArgs {
     PageArgs p;
@@ -133,6 +136,19 @@ __device__ __forceinline__ f4_t page_mfma(u4_t a, u4_t b, f4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0,
                                                       0);
 }
+template <int FMT>
+__device__ __forceinline__ acc16_t page_mfma(u4_t a, u4_t b, acc16_t c) {
+    if constexpr (FMT == RTA_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0,
+                                                       0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0,
+                                                      0);
+}
+
+// Registers 4h .. 4h + 3 of a product: four rows that follow each other.
+__device__ __forceinline__ f4_t quad_of(f4_t c, int) { return c; }
+__device__ __forceinline__ f4_t quad_of(acc16_t c, int h) { return f4_t{c[4 * h], c[4 * h + 1], c[4 * h + 2], c[4 * h + 3]}; }
 
 // Four int8 codes as four binary16 (1024 + (c + 128) has the code in its last bits; minus 1152).
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -256,41 +272,46 @@ __device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
             op[1][j] = upper_halves(ra, rb);
             op[2][j] = upper_halves(ra - cut(ra, 0xffff0000u), rb - cut(rb, 0xffff0000u));
         } else {
-            op[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-            op[1][j] = __builtin_bit_cast(
-                uint32_t, __builtin_amdgcn_cvt_pkrtz(a - cut(a, 0xffffe000u), b - cut(b, 0xffffe000u)));
+            // (one mixed fma per remainder; a multiplication by 1 in sight would become two instructions)
+            float minus = -1.0f;
+            asm("" : "+s"(minus));
+            const h2v_t hi = __builtin_bit_cast(h2v_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+            op[0][j] = __builtin_bit_cast(uint32_t, hi);
+            op[1][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus, a),
+                                                                               fmaf((float)hi[1], minus, b)));
         }
     }
 }
 
-// Masks the products of 32 positions j0 .. of a list that the columns see between them: bit k of
+// Masks the products of 32 positions j0 .. of a list that the columns see between them (a lane
+// holds positions 32 / N h + 4u + e of each column tile, h < N, e < 4): bit k of
 // ok says whether position k counts, t_col is the lane's column's position, -1 at least.  What a
 // column sees is one unsigned comparison of its distance (the first positions' window is all):
 // booleans of their own would each take a pair of scalar registers.
-template <int NC>
-__device__ __forceinline__ void mask_columns(f4_t (*x)[2], uint32_t ok, const Visible& see, int j0, int u,
+template <int NC, int N>
+__device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Visible& see, int j0, int u,
                                              const int* t_col, int window, int sinks) {
     const uint32_t mine = ok >> (4 * u);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < N; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int p = see.position(j0 + 16 * h + 4 * u + e);
+            const int p = see.position(j0 + 32 / N * h + 4 * u + e);
             const uint32_t reach = window == 0 || p < sinks ? 0x80000000u : (uint32_t)window;
-            const int at = (mine >> (16 * h + e)) & 1u ? p : INT_MAX;   // no distance reaches it
+            const int at = (mine >> (32 / N * h + e)) & 1u ? p : INT_MAX;   // no distance reaches it
 #pragma unroll
             for (int c = 0; c < NC; ++c)
                 x[c][h][e] = (uint32_t)(t_col[c] - at) < reach ? x[c][h][e] : -INFINITY;
         }
 }
 
-// The online softmax of NC column tiles, a lane holding 8 positions of its column of each
-// (products x; score = x fac in log2 units).  Weights are 2^(score - low), 2^kTop for the largest
+// The online softmax of NC column tiles, a lane holding 4N positions of its column of each, N = 2
+// (16 columns) or 4 (32 columns) (products x; score = x fac in log2 units).  Weights are 2^(score - low), 2^kTop for the largest
 // score when low was set; low follows the maximum only when weights would pass 2^(kTop + kSlack)
 // = 2^15, so the sums are not rescaled for every small step, and binary16 parts do not overflow.
 // kTop is as high as that allows: the second part ends at 2^-24, and over a long history most of
 // the sum lies in weights far below the largest.
-template <int NC>
+template <int NC, int N>
 struct Softmax {
     static constexpr float kTop = 14.0f, kSlack = 1.0f;
     float m[NC], low[NC], z[NC];   // m: the largest product; z: of the lane's positions
@@ -305,23 +326,32 @@ struct Softmax {
             z[c] = 0.0f;
         }
     }
-    __device__ __forceinline__ void watch(const f4_t (*x)[2]) {
+    // Over the lanes that hold a column.
+    static __device__ __forceinline__ float column_max(float v) {
+        if constexpr (N == 2) v = max_xor16(v);
+        return max_xor32(v);
+    }
+    static __device__ __forceinline__ float column_sum(float v) {
+        if constexpr (N == 2) v = add_xor16(v);
+        return add_xor32(v);
+    }
+    __device__ __forceinline__ void watch(const f4_t (*x)[N]) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) lowest = fminf(lowest, x[c][j >> 2][j & 3]);
+            for (int j = 0; j < 4 * N; ++j) lowest = fminf(lowest, x[c][j >> 2][j & 3]);
     }
     // Takes in the maxima of x (masked positions -inf) and brings z and o to the new base; vshift:
     // the power of two by which o has to follow a value scale.
-    template <int DT>
-    __device__ __forceinline__ void raise(const f4_t (*x)[2], const float* fac, int vshift, f4_t (*o)[DT]) {
+    template <class O, int DT>
+    __device__ __forceinline__ void raise(const f4_t (*x)[N], const float* fac, int vshift, O (*o)[DT]) {
         bool lift = vshift != 0;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float t = x[c][0][0];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) t = fmaxf(t, x[c][j >> 2][j & 3]);
-            m[c] = fmaxf(m[c], max_xor32(max_xor16(t)));
+            for (int j = 1; j < 4 * N; ++j) t = fmaxf(t, x[c][j >> 2][j & 3]);
+            m[c] = fmaxf(m[c], column_max(t));
             ask[c] = fmaf(m[c], fac[c], -kTop);
             lift = lift || ask[c] > low[c] + kSlack;
         }
@@ -347,15 +377,15 @@ struct Softmax {
         }
     }
     // A weight of 0 times a value that is not finite is not 0.  Where the columns do not all see a
-    // tile whole, rows with such values (bad, bit 16 h + 4 u + e of a lane's position) are zeros in
+    // tile whole, rows with such values (bad, bit 32 / N h + 4 u + e of a lane's position) are zeros in
     // the product, and the sums of the columns that do see one become NaN.
-    __device__ __forceinline__ void poison(const f4_t (*s)[2], uint32_t bad, int u) {
+    __device__ __forceinline__ void poison(const f4_t (*s)[N], uint32_t bad, int u) {
         const uint32_t mine = bad >> (4 * u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 4 * N; ++j)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
-                if (((mine >> (16 * (j >> 2) + (j & 3))) & 1u) && s[c][j >> 2][j & 3] != -INFINITY) z[c] = NAN;
+                if (((mine >> (32 / N * (j >> 2) + (j & 3))) & 1u) && s[c][j >> 2][j & 3] != -INFINITY) z[c] = NAN;
     }
     // The maximum in log2 units, and what brings sums over weights to it as the base.
     __device__ __forceinline__ void finish(int c, float fac, float& M, float& back) const {

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     const int ntile = (end - begin + kDecTile - 1) / kDecTile;
 
     f4_t o[NC][kDt];
-    Softmax<NC> sm;
+    Softmax<NC, 2> sm;
     sm.start();
     int ve = -110;   // exponent of the largest value scale so far
 #pragma unroll
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 }
             }
         }
-        sm.template raise<kDt>(s, fac, kScaled ? ve - ve_new : 0, o);
+        sm.raise(s, fac, kScaled ? ve - ve_new : 0, o);
         ve = ve_new;
         u4_t pb[NC][kOps];
 #pragma unroll
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     for (int c = 0; c < NC; ++c) {
         float M, back;
         sm.finish(c, fac[c], M, back);
-        const float zz = add_xor32(add_xor16(sm.z[c])) * back, unscale = kScaled ? ldexpf(back, ve) : back;
+        const float zz = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve) : back;
         if (lane < 16 && part == 0) mzl[wave * kPer + query] = float2{M, zz};
         float* ul = reinterpret_cast<float*>(vl) + query * HD;
 #pragma unroll

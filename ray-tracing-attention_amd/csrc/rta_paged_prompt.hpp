@@ -1,16 +1,19 @@
 // rta_paged_prompt.hpp -- causal attention of several rows per sequence over its pages.
 //
-// Bound by the matrix cores: 4 hq HD operations per (row, position), twice that with q and the
-// weights in two binary16 parts, three times in three bfloat16 parts (rta_paged.hpp).  The columns
-// of a kv head's products are its (row, q head) pairs, so the heads that share keys share their
-// loads and no group size leaves columns empty.  A workgroup of 4 waves takes 4 x 16 NQ columns
-// and the positions that any of them sees, in tiles staged in LDS by all of it (two buffers, one
-// barrier per tile; a row's 16 bytes of padding keep the operand reads off each other's banks);
-// each wave keeps its q operands, running maxima and sums, and O^T in registers.  A tile that
-// every column of a wave sees whole takes no masks, one that no column sees is skipped.
-// The last rows, which see most, come first; kv heads go over the XCDs, so that one L2 serves
-// all rows of a head.  With few workgroups the positions are cut into chunks as well, joined by
-// paged_merge_kernel.
+// Bound by the matrix cores and, beside them, by vector instructions: 4 hq HD operations per
+// (row, position), twice that with q and the weights in two binary16 parts, three times in three
+// bfloat16 parts (rta_paged.hpp), and about 200 vector instructions per 32 x 32 scores, of which
+// two waves of a SIMD hide some.  4096 rows of 32 heads over 4096 bf16 positions: 348 us, three
+// parts at the rate of a large library product 350; the matrix cores are busy 45% of it (two
+// binary16 parts: 37%).
+// The columns of a kv head's products are its (row, q head) pairs, so the heads that share keys
+// share their loads and no group size leaves columns empty.  A workgroup of 4 waves takes 128 (wide
+// heads: 64) columns and the positions that any of them sees, in tiles staged in LDS by all of it
+// (two buffers, one barrier per tile); each wave keeps its q operands, running maxima and sums, and
+// O^T in registers.  A tile that every column of a wave sees whole takes no masks, one that no
+// column sees is skipped.  The last rows, which see most, come first; kv heads go over the XCDs, so
+// that one L2 serves all rows of a head.  With few workgroups the positions are cut into chunks as
+// well, joined by paged_merge_kernel.
 #pragma once
 #include "rta_paged_decode.hpp"
 
@@ -18,27 +21,38 @@ namespace rta {
 
 template <int FMT, int HD>
 struct PromptLds {
-    static constexpr int kNQ = HD == 256 ? 1 : 2;      // column tiles of a wave
     static constexpr int kTile = HD > 64 ? 32 : 64;    // positions per tile
-    static constexpr int kCols = 64 * kNQ;             // columns of a workgroup
-    static constexpr int kPitch = 2 * HD + 16;
-    static constexpr int kRows = 2 * kTile * kPitch;   // keys, then values
+    // a wave's columns are NQ tiles of kWide (32: half the matrix instructions and one column per lane,
+    // 64-wide heads 111 -> 97 us, 128-wide 163 -> 153; with bfloat16's third part, which comes from
+    // LDS between them, 348 -> 378 us)
+    static constexpr int kWide = HD == 256 || FMT == RTA_BF16 ? 16 : 32;
+    static constexpr int kNQ = HD == 256 ? 1 : 32 / kWide;
+    static constexpr int kCols = 4 * kWide * kNQ;      // columns of a workgroup
+    // Bytes of a row: 16 of padding spread the rows of a key operand over the banks, and the 16 rows
+    // that a transposing read of values touches, 32 bytes each; 8 rows of 64 bytes need 64.
+    static constexpr int kPitch = 2 * HD + 16, kPitchV = 2 * HD + (kWide == 32 ? 64 : 16);
+    static constexpr int kKeys = kTile * kPitch, kRows = kKeys + kTile * kPitchV;
     static constexpr int kScales = PageFmt<FMT>::kScaled ? 2 * kTile * 4 : 0;
     static constexpr int kBuf = kRows + kScales + kTile * 4;   // and which rows count
-    static constexpr int kThird = FMT == RTA_BF16 ? kNQ * (HD / 32) * 1024 : 0;   // per wave: q's third part
+    static constexpr int kThird = FMT == RTA_BF16 ? kNQ * kWide * HD * 2 : 0;   // per wave: q's third part
     static constexpr int kTotal = 2 * kBuf + 4 * kThird;
 };
 
 template <int FMT, int HD>
 __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 1 : 2)) paged_prompt_kernel(const PagedAttnArgs a) {
     using L = PromptLds<FMT, HD>;
-    constexpr int kParts = PageFmt<FMT>::kParts, kB = PageFmt<FMT>::kBytes, NQ = L::kNQ;
-    constexpr int kKb = HD / 32, kDt = HD / 16;
-    constexpr int kKg = kKb < 4 ? kKb : 4, kDg = 4;   // operands read ahead
+    constexpr int kParts = PageFmt<FMT>::kParts, kB = PageFmt<FMT>::kBytes;
+    // products: kDims dims of kWide positions, kH of them for 32 positions, then kWide dims of
+    // 32 / kP positions; kKg and kDg of them have their operands read ahead
+    constexpr int W = L::kWide, NQ = L::kNQ, kDims = 512 / W, kH = 32 / W, kP = W / 16, N = W / 8;
+    constexpr int kKb = HD / kDims, kDt = HD / W, kKg = kKb * kH < 8 ? kKb : 8 / kH;
+    constexpr int kDg = kDt < 4 ? kDt : 4, kDn = kP * kDt / kDg;   // V^T: kDn groups of kDg operands
+    using Acc = std::conditional_t<W == 32, acc16_t, f4_t>;
+    constexpr int kQuads = sizeof(Acc) / 16;
     constexpr int kPieces = HD * kB / 16, kStep = 256 / kPieces, kPass = L::kTile / kStep;
     constexpr bool kScaled = PageFmt<FMT>::kScaled;
     __shared__ __align__(16) uint8_t lds[L::kTotal];
-    const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, u = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, i = lane & (W - 1), u = lane / W;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hkv = a.p.kv_heads;
     const int kvh = blockIdx.x % hkv, rest = blockIdx.x / hkv;
@@ -140,7 +154,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
         for (int k = 0; k < kPass; ++k) {
             const int row = row0 + k * kStep;
             put(buf + row * L::kPitch, kr[k]);
-            put(buf + (L::kTile + row) * L::kPitch, vr[k]);
+            put(buf + L::kKeys + row * L::kPitchV, vr[k]);
             if (piece == 0) {
                 if constexpr (kScaled) {
                     float* f = reinterpret_cast<float*>(buf + L::kRows);
@@ -159,27 +173,33 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     }
 
     // the lane's columns: (row, head) pairs, their positions and q operands
-    const int col0 = tile * L::kCols + wave * 16 * NQ, cols = live_rows * a.group;
+    const int col0 = tile * L::kCols + wave * W * NQ, cols = live_rows * a.group;
     const bool on = col0 < cols;   // uniform: this wave has columns
     int t_col[NQ];
-    u4_t qb[NQ][kKb][2];   // (the third part of bfloat16 lies in LDS: 96 registers would leave none for operands)
+    u4_t qb[NQ][kKb][2];   // (the third part of bfloat16 lies in LDS: its registers would leave none for operands)
     u4_t* third = reinterpret_cast<u4_t*>(lds + 2 * L::kBuf + wave * L::kThird) + lane;
     float fac[NQ];
+    auto column = [&](int c, int& tok, int& head) {   // past the last one: the last
+        const int col = min(col0 + W * c + i, cols - 1);
+        tok = col / a.group;
+        head = kvh * a.group + col - tok * a.group;
+    };
 #pragma unroll
     for (int c = 0; c < NQ; ++c) {
-        const int col = min(col0 + 16 * c + i, cols - 1), tok = col / a.group, g = col - tok * a.group;
+        int tok, head;
+        column(c, tok, head);
         t_col[c] = max(len - count + tok, -1);
-        const float* q = a.q + (int64_t)(base + tok) * a.q_stride + ((int64_t)kvh * a.group + g) * HD;
+        const float* q = a.q + (int64_t)(base + tok) * a.q_stride + (int64_t)head * HD;
         float v[kKb][8], mx = 0.0f;
 #pragma unroll
         for (int kb = 0; kb < kKb; ++kb)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[kb][e] = q[32 * kb + 8 * u + e];
+                v[kb][e] = q[kDims * kb + 8 * u + e];
                 mx = fmaxf(mx, fabsf(v[kb][e]));
             }
         int qe = 14;
-        if constexpr (FMT != RTA_BF16) qe = part_exponent(max_xor32(max_xor16(mx)));
+        if constexpr (FMT != RTA_BF16) qe = part_exponent(Softmax<NQ, N>::column_max(mx));
         const float sg = ldexpf(1.0f, 14 - qe);
         fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe - 14);
 #pragma unroll
@@ -195,16 +215,18 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     }
     // the wave's first and last positions
     const int t_lo = len - count + col0 / a.group;
-    const int t_hi = len - count + min(col0 + 16 * NQ - 1, cols - 1) / a.group;
+    const int t_hi = len - count + min(col0 + W * NQ - 1, cols - 1) / a.group;
 
-    f4_t o[NQ][kDt];
-    Softmax<NQ> sm;
+    Acc o[NQ][kDt];
+    Softmax<NQ, N> sm;
     sm.start();
     int ve = -110;
 #pragma unroll
-    for (int c = 0; c < NQ; ++c) {
-        for (int d = 0; d < kDt; ++d) o[c][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int c = 0; c < NQ; ++c)
+#pragma unroll
+        for (int d = 0; d < kDt; ++d)
+#pragma unroll
+            for (int e = 0; e < 4 * kQuads; ++e) o[c][d][e] = 0.0f;
     if (nt > 0) store(0, lds);
     __syncthreads();
 
@@ -233,18 +255,22 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
 #pragma unroll
             for (int sub = 0; sub < L::kTile / 32; ++sub) {
                 // S^T of 32 positions
-                f4_t x[NQ][2];
+                Acc st[NQ][kH];
 #pragma unroll
-                for (int c = 0; c < NQ; ++c) x[c][0] = x[c][1] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int c = 0; c < NQ; ++c)
+#pragma unroll
+                    for (int h = 0; h < kH; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4 * kQuads; ++e) st[c][h][e] = 0.0f;
 #pragma unroll
                 for (int k0 = 0; k0 < kKb; k0 += kKg) {
-                    u4_t ka[kKg][2];   // all on their way before the first product
+                    u4_t ka[kKg][kH];   // all on their way before the first product
 #pragma unroll
                     for (int k = 0; k < kKg; ++k)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            ka[k][h] = *reinterpret_cast<const u4_t*>(buf + (32 * sub + 16 * h + i) * L::kPitch +
-                                                                      64 * (k0 + k) + 16 * u);
+                        for (int h = 0; h < kH; ++h)
+                            ka[k][h] = *reinterpret_cast<const u4_t*>(buf + (32 * sub + W * h + i) * L::kPitch +
+                                                                      2 * kDims * (k0 + k) + 16 * u);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int k = 0; k < kKg; ++k)
@@ -254,30 +280,37 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                             for (int c = 0; c < NQ; ++c) {
                                 const u4_t q = p < 2 ? qb[c][k0 + k][p & 1] : third[(c * kKb + k0 + k) * 64];
 #pragma unroll
-                                for (int h = 0; h < 2; ++h) x[c][h] = page_mfma<FMT>(ka[k][h], q, x[c][h]);
+                                for (int h = 0; h < kH; ++h) st[c][h] = page_mfma<FMT>(ka[k][h], q, st[c][h]);
                             }
                 }
                 // the first of V^T's operands, ready when the weights are
-                const uint8_t* vb = buf + (L::kTile + 32 * sub + 4 * u + (i >> 2)) * L::kPitch + 8 * (i & 3);
+                const uint8_t* vb = buf + L::kKeys + (32 * sub + 4 * u + ((lane & 15) >> 2)) * L::kPitchV +
+                                    32 * (i >> 4) + 8 * (lane & 3);
                 u4_t va[2][kDg];
-                auto load_va = [&](int d0) {
+                auto load_va = [&](int n) {   // group n: dim tiles d0 .. of positions 32 / kP h ..
+                    const int h = n * kDg / kDt, d0 = n * kDg % kDt;
 #pragma unroll
                     for (int d = 0; d < kDg; ++d) {
-                        const uint8_t* src = vb + 32 * (d0 + d);
+                        const uint8_t* src = vb + 2 * W * (d0 + d) + 16 * h * L::kPitchV;
                         const s4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)src);
-                        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(src + 16 * L::kPitch));
+                        const s4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_t*)(src + 16 / kP * L::kPitchV));
                         const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-                        va[(d0 / kDg) & 1][d] = u4_t{l2.x, l2.y, h2.x, h2.y};
+                        va[n & 1][d] = u4_t{l2.x, l2.y, h2.x, h2.y};
                     }
                 };
                 load_va(0);
                 __builtin_amdgcn_sched_barrier(0);
-                f4_t vf[2];
+                f4_t x[NQ][N], vf[N];   // positions 32 / N h + 4 u + e
+#pragma unroll
+                for (int c = 0; c < NQ; ++c)
+#pragma unroll
+                    for (int h = 0; h < N; ++h) x[c][h] = quad_of(st[c][h / kQuads], h % kQuads);
                 if constexpr (kScaled) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const f4_t kf = *reinterpret_cast<const f4_t*>(sc + 32 * sub + 16 * h + 4 * u);
-                        vf[h] = *reinterpret_cast<const f4_t*>(sc + L::kTile + 32 * sub + 16 * h + 4 * u) * wscale;
+                    for (int h = 0; h < N; ++h) {
+                        const float* at = sc + 32 * sub + 32 / N * h + 4 * u;
+                        const f4_t kf = *reinterpret_cast<const f4_t*>(at);
+                        vf[h] = *reinterpret_cast<const f4_t*>(at + L::kTile) * wscale;
 #pragma unroll
                         for (int c = 0; c < NQ; ++c) x[c][h] *= kf;
                     }
@@ -287,32 +320,34 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                     mask_columns<NQ>(x, (uint32_t)(okm >> (32 * sub)), see, j0 + 32 * sub, u, t_col, a.window, a.sinks);
                     if (badm) sm.poison(x, (uint32_t)(badm >> (32 * sub)), u);
                 }
-                sm.template raise<kDt>(x, fac, kScaled ? ve - ve_new : 0, o);
-                u4_t pb[NQ][kParts];
-#pragma unroll
-                for (int c = 0; c < NQ; ++c) {
-                    float w[8];
-                    sm.weights(c, x[c], fac[c], w);
-                    if constexpr (kScaled) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] *= vf[j >> 2][j & 3];
-                    }
-                    split_all<FMT>(w, pb[c]);
-                }
+                sm.raise(x, fac, kScaled ? ve - ve_new : 0, o);
                 ve = ve_new;
                 // O^T += V^T P^T
+                u4_t pb[NQ][kP][kParts];
 #pragma unroll
-                for (int d0 = 0; d0 < kDt; d0 += kDg) {
-                    if (d0 + kDg < kDt) {
-                        load_va(d0 + kDg);
-                        __builtin_amdgcn_sched_barrier(0);
+                for (int n = 0; n < kDn; ++n) {
+                    const int h = n * kDg / kDt, d0 = n * kDg % kDt;
+#pragma unroll
+                    for (int c = 0; c < NQ && d0 == 0; ++c) {
+                        float w[8];
+                        sm.weights(c, x[c] + 2 * h, fac[c], w);
+                        if constexpr (kScaled) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) w[e] *= vf[2 * h + (e >> 2)][e & 3];
+                        }
+                        split_all<FMT>(w, pb[c][h]);
+                    }
+                    if (n + 1 < kDn) {
+                        load_va(n + 1);
+                        if constexpr (kP == 1) __builtin_amdgcn_sched_barrier(0);
                     }
 #pragma unroll
                     for (int p = 0; p < kParts; ++p)
 #pragma unroll
                         for (int d = 0; d < kDg; ++d)
 #pragma unroll
-                            for (int c = 0; c < NQ; ++c) o[c][d0 + d] = page_mfma<FMT>(va[(d0 / kDg) & 1][d], pb[c][p], o[c][d0 + d]);
+                            for (int c = 0; c < NQ; ++c)
+                                o[c][d0 + d] = page_mfma<FMT>(va[n & 1][d], pb[c][h][p], o[c][d0 + d]);
                 }
             }
         }
@@ -325,21 +360,21 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     for (int c = 0; c < NQ; ++c) {
         float M, back;
         sm.finish(c, fac[c], M, back);
-        const float Z = add_xor32(add_xor16(sm.z[c])) * back, unscale = kScaled ? ldexpf(back, ve) : back;
-        const int col = col0 + 16 * c + i;
-        if (col >= cols) continue;
-        const int tok = col / a.group, g = col - tok * a.group;
-        const int64_t at = (int64_t)(base + tok) * a.hq + (int64_t)kvh * a.group + g;
-        if (a.nchunk > 1) {
-            const int64_t rec = at * a.nchunk + blockIdx.z;
+        const float Z = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve) : back;
+        if (col0 + W * c + i >= cols) continue;
+        int tok, head;
+        column(c, tok, head);
+        const int64_t at = (int64_t)(base + tok) * a.hq + head, rec = at * a.nchunk + blockIdx.z;
+        if (a.nchunk > 1 && u == 0) a.mz[rec] = float2{M, Z};
 #pragma unroll
-            for (int d = 0; d < kDt; ++d)
-                *reinterpret_cast<f4_t*>(a.part + rec * HD + 16 * d + 4 * u) = o[c][d] * unscale;
-            if (u == 0) a.mz[rec] = float2{M, Z};
-            continue;
-        }
+        for (int d = 0; d < kDt; ++d)
 #pragma unroll
-        for (int d = 0; d < kDt; ++d) write_result(a, at, HD, 16 * d + 4 * u, o[c][d] * unscale, M * kLn2, Z, err);
+            for (int h = 0; h < kQuads; ++h) {
+                const int dim = W * d + 8 * h + 4 * u;
+                const f4_t U = quad_of(o[c][d], h) * unscale;
+                if (a.nchunk > 1) *reinterpret_cast<f4_t*>(a.part + rec * HD + dim) = U;
+                else write_result(a, at, HD, dim, U, M * kLn2, Z, err);
+            }
     }
     if (err) raise_error(err);
 }
