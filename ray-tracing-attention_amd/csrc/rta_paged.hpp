@@ -45,9 +45,8 @@ struct PagedAttnArgs {
     // work split: chunks of `chunk` visible positions; with nchunk > 1 every (row, q head, chunk)
     // leaves U[HD] in `part` and (m, z) in `mz`, both [row][hq][nchunk]
     int chunk, nchunk;
-    // several rows per entry: tiles of `cols` (row, q head) columns, `ntile` of them at most (0:
-    // one row per entry, a chunk counts along that row's own visible positions)
-    int cols, ntile;
+    int ntile;          // several rows per entry: tiles of (row, q head) columns, at most (0: one row
+                        // per entry, a chunk counts along that row's own visible positions)
     float* part;
     float2* mz;
 };

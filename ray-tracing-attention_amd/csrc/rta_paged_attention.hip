@@ -147,12 +147,10 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
             a.mz = reinterpret_cast<float2*>(a.part + (size_t)rows * hq * cut.nchunk * HD);
             a.ntile = ntile;
             if (ntile && few_rows(max_rows, a.group, HD)) {   // one group of columns
-                a.cols = few_cols(max_rows * a.group);
-                const dim3 grid(n * pages->kv_heads, 1, cut.nchunk), block(64 * kDecWaves);
-                if (a.cols == 16) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1, true>), grid, block, 0, s, a);
+                                const dim3 grid(n * pages->kv_heads, 1, cut.nchunk), block(64 * kDecWaves);
+                if (few_cols(max_rows * a.group) == 16) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1, true>), grid, block, 0, s, a);
                 else if constexpr (HD < 256) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2, true>), grid, block, 0, s, a);
             } else if (ntile) {
-                a.cols = PromptLds<F, HD>::kCols;
                 hipLaunchKernelGGL((paged_prompt_kernel<F, HD>), dim3(ntile * n * pages->kv_heads, 1, cut.nchunk),
                                    dim3(256), 0, s, a);
             } else {

@@ -77,13 +77,22 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
         cols = min(a.group - g0, L::kHeads);
     }
     const int begin = blockIdx.z * a.chunk, end = see.count - begin > a.chunk ? begin + a.chunk : see.count;
-    if (begin >= end && blockIdx.z > 0) return;
     // row and q head of column c (< cols)
     auto column = [&](int c, int& row, int& head) {
         const int at = g0 + c, tok = MULTI ? at / a.group : 0;
         row = row0 + tok;
         head = kvh * a.group + at - tok * a.group;
     };
+    if (begin >= end && blockIdx.z > 0) {
+        // (m, z) for paged_merge_kernel, which takes the chunks of a single row from its length instead
+        // (ragged batches leave many empty: 72 us with them written for 32 of 256 to 8192, without 67.5)
+        for (int c = threadIdx.x; MULTI && c < cols; c += 64 * kDecWaves) {
+            int row, head;
+            column(c, row, head);
+            a.mz[((int64_t)row * a.hq + head) * a.nchunk + blockIdx.z] = float2{-INFINITY, 0.0f};
+        }
+        return;
+    }
 
     uint8_t* vl = lds + L::kQ + wave * L::kWave;
     float* sl = reinterpret_cast<float*>(vl + L::kV);
