@@ -25,8 +25,8 @@ static Cut decode_cut(int64_t rows, int heads, int hd, int64_t most) {
 // takes them in one group, bound by the history's bytes, where the other kernel's 128 columns would
 // stay mostly empty (us, this / the other: 16 sequences of 4 rows over 4000 bf16 positions, 4 q
 // heads per kv head 60 / 91, 8 rows 76 / 97; one of 12 rows over 8000, in two groups 31 / 27).
-// Their workgroups start and end with more work, so a quarter as many are asked for (5 rows of 16
-// sequences over 8000 8-bit positions 136 -> 86).
+// Their workgroups start and end with more work, so fewer are asked for, as for 4 rows an entry (5
+// rows of 16 sequences over 500 to 16384 8-bit positions 73.5; as for 2, 3, 6 and 8: 81, 76, 97, 123).
 static bool few_rows(int64_t max_rows, int group, int hd) { return max_rows * group <= (hd == 256 ? 16 : 32); }
 // With several rows: column tiles enough for two workgroups per compute unit stand alone, fewer
 // are cut into chunks of positions (a multiple of 64, 256 at least).
