@@ -259,6 +259,20 @@ __device__ __forceinline__ Visible prompt_span(const PagedAttnArgs& a, int len, 
     return Visible{head, lo, head + t1 + 1 - lo};
 }
 
+// Over 8-bit pages an operand of the second product is a weight times a value scale, the scales brought
+// below 1 by the largest met so far (2^ve): one multiplication for all columns.  The parts end at
+// 2^-24, so what a scale is below the largest is lost at that end, and the largest may have no
+// weight, or be at a position that the column cannot see.  So in a tile with a scale below
+// 2^(ve - kSpread) every column's operands and sums have a power of two of their own (Softmax::up).
+// Relative error of a sum over 65536 positions whose scales are 2^-6, 2^-8 and 2^-12 of the largest: 1.4e-7
+// (as at 2^0), 1.7e-7, 1.9e-6.  Scales of normal values differ by less than 2^3, ve's rounding
+// included: their tiles pay for the comparison only (1 to 2.5% of a call); where every tile is spread, single
+// rows of 32 sequences over 4000 positions take 74.8 us, else 72.9, a prompt of 4096 rows 406, else 339.
+constexpr int kSpread = 6;
+__device__ __forceinline__ bool far_below(float scale, int ve) {
+    return scale != 0.0f && fabsf(scale) < ldexpf(1.0f, ve - kSpread);
+}
+
 // All parts of eight values as operands.
 template <int FMT>
 __device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
@@ -309,20 +323,24 @@ __device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Vi
 // score when low was set; low follows the maximum only when weights would pass 2^(kTop + kSlack)
 // = 2^15, so the sums are not rescaled for every small step, and binary16 parts do not overflow.
 // kTop is as high as that allows: the second part ends at 2^-24, and over a long history most of
-// the sum lies in weights far below the largest.
-template <int NC, int N>
+// the sum lies in weights far below the largest.  SCALED: 8-bit pages.
+template <int NC, int N, bool SCALED>
 struct Softmax {
     static constexpr float kTop = 14.0f, kSlack = 1.0f;
     float m[NC], low[NC], z[NC];   // m: the largest product; z: of the lane's positions
     float lowest;                  // of all products: a visible -inf shows nowhere else
     float ask[NC];
+    int up[NC];                    // SCALED: the sums o and the tile's operands are 2^up times what they are else
+    bool lifted;                   // some of them are not 0
 
     __device__ __forceinline__ void start() {
         lowest = INFINITY;
+        lifted = false;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             m[c] = low[c] = -INFINITY;
             z[c] = 0.0f;
+            up[c] = 0;
         }
     }
     // Over the lanes that hold a column.
@@ -341,10 +359,12 @@ struct Softmax {
             for (int j = 0; j < 4 * N; ++j) lowest = fminf(lowest, x[c][j >> 2][j & 3]);
     }
     // Takes in the maxima of x (masked positions -inf) and brings z and o to the new base; vshift:
-    // the power of two by which o has to follow a value scale.
+    // the power of two by which o has to follow a value scale; spread (all lanes alike): the scales vf are
+    // far apart, so each column's largest operand is brought to 2^14, but no sum past 2^100.
     template <class O, int DT>
-    __device__ __forceinline__ void raise(const f4_t (*x)[N], const float* fac, int vshift, O (*o)[DT]) {
-        bool lift = vshift != 0;
+    __device__ __forceinline__ void raise(const f4_t (*x)[N], const float* fac, int vshift, O (*o)[DT], bool spread,
+                                          const f4_t* vf) {
+        bool lift = vshift != 0 || spread || lifted;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float t = x[c][0][0];
@@ -355,23 +375,45 @@ struct Softmax {
             lift = lift || ask[c] > low[c] + kSlack;
         }
         if (__builtin_amdgcn_ballot_w64(lift)) {
+            lifted = spread;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const float base = ask[c] > low[c] ? ask[c] : low[c];
                 const float al = __builtin_amdgcn_exp2f(low[c] - (base == -INFINITY ? 0.0f : base));
-                const float f = ldexpf(al, vshift);
+                int by = vshift;
                 z[c] *= al;
+                low[c] = base;
+                if constexpr (SCALED) {
+                    by -= up[c];
+                    up[c] = 0;
+                    if (spread) {
+                        float most = 0.0f, sum = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 4 * N; ++j)
+                            most = fmaxf(most, fabsf(weight(c, x[c][j >> 2][j & 3], fac[c]) * vf[j >> 2][j & 3]));
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int e = 0; e < (int)(sizeof(O) / 4); ++e) sum = fmaxf(sum, fabsf(o[c][d][e]));
+                        up[c] = min(14 - part_exponent(column_max(most)),
+                                    100 - by - part_exponent(column_max(sum) * al));
+                        by += up[c];
+                    }
+                }
+                const float f = ldexpf(al, by);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[c][d] *= f;
-                low[c] = base;
             }
         }
     }
-    __device__ __forceinline__ void weights(int c, const f4_t* x, float fac, float w[8]) {
+    __device__ __forceinline__ float weight(int c, float x, float fac) const {
         const float base = low[c] == -INFINITY ? 0.0f : low[c];   // (nothing seen yet: weights 0)
+        return __builtin_amdgcn_exp2f(fmaf(x, fac, -base));
+    }
+    __device__ __forceinline__ void weights(int c, const f4_t* x, float fac, float w[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            w[j] = __builtin_amdgcn_exp2f(fmaf(x[j >> 2][j & 3], fac, -base));
+            w[j] = weight(c, x[j >> 2][j & 3], fac);
             z[c] += w[j];
         }
     }

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     const int ntile = (end - begin + kDecTile - 1) / kDecTile;
 
     f4_t o[NC][kDt];
-    Softmax<NC, 2> sm;
+    Softmax<NC, 2, kScaled> sm;
     sm.start();
     int ve = -110;   // exponent of the largest value scale so far
 #pragma unroll
@@ -246,7 +246,13 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
         }
         // the tile's scales, from the lane of a position to the lanes that score it
         f4_t kf[2], vf[2];
+        float mine[2];      // the value scales of the lane's positions that count, as far as they are finite
+        int largest = 0;    // and the exponent of the tile's largest
         if constexpr (kScaled) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mine[h] = ((now >> (16 * h + i)) & 1u) && fabsf(vs[h]) < INFINITY ? vs[h] : 0.0f;
+            // (the four rows of 16 lanes hold the same positions)
+            largest = __builtin_amdgcn_readfirstlane(part_exponent(group_max(fmaxf(fabsf(mine[0]), fabsf(mine[1])), 16)));
             if (u == 0) {
                 sl[i] = ks[0];
                 sl[16 + i] = ks[1];
@@ -324,13 +330,10 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 for (int j = 0; j < 8; ++j) s[c][j >> 2][j & 3] += dpp_mov<0xB1>(s[c][j >> 2][j & 3]);
         }
         int ve_new = ve;
+        bool spread = false;
         if constexpr (kScaled) {   // value scales below 2^0
-            float mx = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(vf[h][e]));
-            ve_new = max(ve, part_exponent(max_xor32(max_xor16(mx))));
+            ve_new = max(ve, largest);
+            spread = __builtin_amdgcn_ballot_w64(far_below(mine[0], ve_new) || far_below(mine[1], ve_new)) != 0;
             const float down = ldexpf(1.0f, -ve_new);
             vf[0] *= down;
             vf[1] *= down;
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 }
             }
         }
-        sm.raise(s, fac, kScaled ? ve - ve_new : 0, o);
+        sm.raise(s, fac, kScaled ? ve - ve_new : 0, o, spread, vf);
         ve = ve_new;
         u4_t pb[NC][kOps];
 #pragma unroll
@@ -364,6 +367,10 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             if constexpr (kScaled) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) w[j] *= vf[j >> 2][j & 3];
+                if (spread) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = ldexpf(w[j], sm.up[c]);
+                }
             }
             if constexpr (MULTI) split_all<FMT>(w, pb[c]);
             else split_parts<FMT>(w, part, pb[c]);
@@ -389,7 +396,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     for (int c = 0; c < NC; ++c) {
         float M, back;
         sm.finish(c, fac[c], M, back);
-        const float zz = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve) : back;
+        const float zz = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve - sm.up[c]) : back;
         if (lane < 16 && part == 0) mzl[wave * kPer + query] = float2{M, zz};
         float* ul = reinterpret_cast<float*>(vl) + query * HD;
 #pragma unroll

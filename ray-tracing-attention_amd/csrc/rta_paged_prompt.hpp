@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                 mx = fmaxf(mx, fabsf(v[kb][e]));
             }
         int qe = 14;
-        if constexpr (FMT != RTA_BF16) qe = part_exponent(Softmax<NQ, N>::column_max(mx));
+        if constexpr (FMT != RTA_BF16) qe = part_exponent(Softmax<NQ, N, kScaled>::column_max(mx));
         const float sg = ldexpf(1.0f, 14 - qe);
         fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe - 14);
 #pragma unroll
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     const int t_hi = len - count + min(col0 + W * NQ - 1, cols - 1) / a.group;
 
     Acc o[NQ][kDt];
-    Softmax<NQ, N> sm;
+    Softmax<NQ, N, kScaled> sm;
     sm.start();
     int ve = -110;
 #pragma unroll
@@ -254,9 +254,11 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
             const float* sc = reinterpret_cast<const float*>(buf + L::kRows);
             float wscale = 1.0f;
             int ve_new = ve;
+            bool spread = false;
             if constexpr (kScaled) {   // value scales below 2^0
                 const float mx = lane < L::kTile ? fabsf(sc[L::kTile + lane]) : 0.0f;
-                ve_new = max(ve, part_exponent(wave_max_dpp(mx)));
+                ve_new = max(ve, __builtin_amdgcn_readfirstlane(part_exponent(wave_max_dpp(mx))));
+                spread = __builtin_amdgcn_ballot_w64(far_below(mx, ve_new)) != 0;
                 wscale = ldexpf(1.0f, -ve_new);
             }
 #pragma unroll
@@ -327,8 +329,16 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                     mask_columns<NQ>(x, (uint32_t)(okm >> (32 * sub)), see, j0 + 32 * sub, u, t_col, a.window, a.sinks);
                     if (badm) sm.poison(x, (uint32_t)(badm >> (32 * sub)), u);
                 }
-                sm.raise(x, fac, kScaled ? ve - ve_new : 0, o);
+                sm.raise(x, fac, kScaled ? ve - ve_new : 0, o, spread, vf);
                 ve = ve_new;
+                if constexpr (kScaled) {
+                    static_assert(NQ == 1, "the value scales take on one column's power of two");
+                    if (spread) {
+                        const float by = ldexpf(1.0f, sm.up[0]);
+#pragma unroll
+                        for (int h = 0; h < N; ++h) vf[h] *= by;
+                    }
+                }
                 // O^T += V^T P^T
                 u4_t pb[NQ][kP][kParts];
 #pragma unroll
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     for (int c = 0; c < NQ; ++c) {
         float M, back;
         sm.finish(c, fac[c], M, back);
-        const float Z = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve) : back;
+        const float Z = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve - sm.up[c]) : back;
         if (col0 + W * c + i >= cols) continue;
         int tok, head;
         column(c, tok, head);

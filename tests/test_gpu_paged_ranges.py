@@ -1,0 +1,99 @@
+"""Attention over the paged history at the ends of its ranges: value scales, values and scores far
+apart or near the end of fp32, and what rows may not see, against 64-bit results.
+
+The tolerance of a head is `bound` of paged_reference.attend (the relative error of every weight)
+times sum p |v| of the head's worst dim, doubled: errors of the terms add up to no more."""
+import numpy as np
+import pytest
+
+import paged_reference as ref
+from rta import _lib, ops
+from test_gpu_paged_attention import rows_of
+from test_gpu_pages import env, ints  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+ALL = [ref.F16, ref.BF16, ref.Q8_ROW]
+
+
+def holding(env, fmt, hkv, hd, page, k, v):
+    """A cache whose only sequence holds k and v [length, hkv * hd]."""
+    torch, pages, dev = env
+    n = -(-len(k) // page)
+    c = pages.PagedCache(fmt, hkv, hd, page, n_pages=n + 2, max_seqs=2, max_pages=n + 1)
+    c.pool.fill_(255)
+    c.extend(ints(torch, [0], dev), ints(torch, [len(k)], dev))
+    c.append(k.to(dev), v.to(dev), seqs=ints(torch, [0], dev), cu_rows=ints(torch, [0, len(k)], dev))
+    return c
+
+
+def newest(env, c, q, **how):
+    """Attention of the rows q as the newest positions of sequence 0."""
+    torch, _, dev = env
+    return c.attention(q, seqs=ints(torch, [0], dev), cu_rows=ints(torch, [0, len(q)], dev), max_rows=len(q), **how)
+
+
+def check_terms(c, q, got, rows=None, window=0, sinks=0):
+    out, m, z = (t.cpu().double().numpy() for t in got)
+    k, v, held = ref.dense(c, 0, 0)
+    x = q.cpu().double().numpy()
+    for r in range(len(q)) if rows is None else rows:
+        t = len(k) - len(q) + r
+        wo, wm, wz, bound, _ = ref.attend(x[r], k, v, held, t, window, sinks)
+        terms = ref.attend(x[r], k, np.abs(v), held, t, window, sinks)[0]
+        err = np.abs(out[r] - wo).max(1)
+        assert np.all(err <= 2 * bound * terms.max(1)), (r, float((err / terms.max(1)).max()), float(bound.max()))
+        assert np.all(np.abs(m[r] - wm) <= bound) and np.all(np.abs(z[r] - wz) <= (bound + 2.0**-21) * wz), r
+
+
+def normal(env, seed, *shape):
+    torch = env[0]
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+# ------------------------------------------------------------------ value scales far apart ----
+@pytest.mark.parametrize("spread", [12, 30, 45, 100])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,hq,hkv,window", [(4, 4, 1, 0), (8, 4, 1, 5), (90, 8, 2, 0), (90, 8, 2, 24)])
+def test_a_large_value_scale_out_of_sight(env, spread, hd, rows, hq, hkv, window):
+    """A value 2^spread times the others at a position in the middle of the new rows: rows before it,
+    and rows whose window has passed it, keep their precision; the others get it as it is."""
+    length = 130
+    k, v = normal(env, 1, length, hkv * hd), normal(env, 2, length, hkv * hd)
+    v[length - rows + rows // 2] *= 2.0**spread
+    c = holding(env, ref.Q8_ROW, hkv, hd, 16, k, v)
+    q = rows_of(env[0], env[2], rows, hq, hd, 3)
+    check_terms(c, q, newest(env, c, q, window=window), window=window)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("spread", [8, 16, 24, 40, 90])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 2, 5, 40])
+def test_a_large_value_scale_of_no_weight(env, spread, hd, rows):
+    """The largest value scale at a visible position whose weight is e^-90 of the largest, early and
+    late in a history of several tiles and chunks: the other positions' sum stays whole."""
+    torch, _, dev = env
+    length = 700
+    q = rows_of(torch, dev, rows, 4, hd, 4, 0.01) + 0.5
+    k, v = 0.1 * normal(env, 5, length, hd), normal(env, 6, length, hd)
+    for p in (9, 400):
+        k[p] = -90 * hd**0.5 / (0.5 * hd)   # q . k / sqrt(hd) = -90 for q = 0.5 in every dim
+        v[p] *= 2.0**spread
+    c = holding(env, ref.Q8_ROW, 1, hd, 16, k, v)
+    check_terms(c, q, newest(env, c, q))
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 5, 40])
+def test_value_scales_of_every_size(env, hd, rows):
+    """Scales spread log-normally over some 2^+-30, and some heads' values zero."""
+    length = 500
+    k, v = normal(env, 7, length, hd), normal(env, 8, length, hd)
+    v *= (8 * normal(env, 9, length, 1)).exp()
+    v[::7] = 0.0
+    c = holding(env, ref.Q8_ROW, 1, hd, 8, k, v)
+    q = rows_of(env[0], env[2], rows, 4, hd, 10, 4.0)
+    check_terms(c, q, newest(env, c, q))
+    assert ops.device_error() == 0
