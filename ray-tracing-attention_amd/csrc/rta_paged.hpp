@@ -89,7 +89,10 @@ __device__ __forceinline__ bool resolve_row(const PagedAttnArgs& a, int r, const
 
 typedef f4_t f4u_t __attribute__((aligned(4)));   // at an address of a multiple of 4
 
-// The final values of (row, q head) at dims c .. c + 3 from U, M (natural units) and Z.
+// Sums of weights leave the kernels' loops 2^-kRoom times what they are against the maximum (weight 2^-kRoom
+// for the largest score): a mean of finite values is finite, and their plain sum need not be.
+constexpr int kRoom = 24;
+// The final values of (row, q head) at dims c .. c + 3 from U and Z (both 2^-kRoom times) and M (natural units).
 __device__ __forceinline__ void write_result(const PagedAttnArgs& a, int64_t at, int hd, int c, f4_t u, float m,
                                              float z, uint32_t& err) {
     f4_t o = u * (z > 0.0f || z != z ? 1.0f / z : 0.0f);   // nothing seen: zeros
@@ -104,7 +107,7 @@ __device__ __forceinline__ void write_result(const PagedAttnArgs& a, int64_t at,
     *reinterpret_cast<f4u_t*>(a.out + to) = o;
     if (c == 0) {
         if (a.m_out) a.m_out[at] = m;
-        if (a.z_out) a.z_out[at] = z;
+        if (a.z_out) a.z_out[at] = ldexpf(z, kRoom);
     }
 }
 
@@ -320,13 +323,15 @@ __device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Vi
 
 // The online softmax of NC column tiles, a lane holding 4N positions of its column of each, N = 2
 // (16 columns) or 4 (32 columns) (products x; score = x fac in log2 units).  Weights are 2^(score - low), 2^kTop for the largest
-// score when low was set; low follows the maximum only when weights would pass 2^(kTop + kSlack)
-// = 2^15, so the sums are not rescaled for every small step, and binary16 parts do not overflow.
+// score when low was set; low follows the maximum only when weights would pass 2^(kTop + kSlack),
+// 2^15 for binary16 parts, so the sums are not rescaled for every small step, and binary16 parts do not overflow.
 // kTop is as high as that allows: the second part ends at 2^-24, and over a long history most of
-// the sum lies in weights far below the largest.  SCALED: 8-bit pages.
-template <int NC, int N, bool SCALED>
+// the sum lies in weights far below the largest.  bfloat16 parts have fp32's exponents, and values may too:
+// there the largest weight is 2^-kRoom from the start; sums of values down to 2^-100 stay normal numbers.
+template <int NC, int N, int FMT>
 struct Softmax {
-    static constexpr float kTop = 14.0f, kSlack = 1.0f;
+    static constexpr float kTop = FMT == RTA_BF16 ? -kRoom : 14, kSlack = 1.0f;
+    static constexpr bool SCALED = PageFmt<FMT>::kScaled;
     float m[NC], low[NC], z[NC];   // m: the largest product; z: of the lane's positions
     float lowest;                  // of all products: a visible -inf shows nowhere else
     float ask[NC];
@@ -428,10 +433,15 @@ struct Softmax {
             for (int c = 0; c < NC; ++c)
                 if (((mine >> (32 / N * (j >> 2) + (j & 3))) & 1u) && s[c][j >> 2][j & 3] != -INFINITY) z[c] = NAN;
     }
-    // The maximum in log2 units, and what brings sums over weights to it as the base.
+    // The maximum in log2 units, and what brings sums over weights to 2^-kRoom against it: back 2^kBack.
+    static constexpr int kBack = -(int)kTop - kRoom;
     __device__ __forceinline__ void finish(int c, float fac, float& M, float& back) const {
         M = m[c] * fac;
-        back = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(low[c] - M);
+        back = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(low[c] - M + kTop);
+    }
+    // A sum of o so, the value scales below 2^ve (one power of two at the end: parts of it may have none).
+    __device__ __forceinline__ float settled(int c, float o, float back, int ve) const {
+        return SCALED ? ldexpf(o * back, ve - up[c] + kBack) : o * ldexpf(back, kBack);
     }
 };
 

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     const int ntile = (end - begin + kDecTile - 1) / kDecTile;
 
     f4_t o[NC][kDt];
-    Softmax<NC, 2, kScaled> sm;
+    Softmax<NC, 2, FMT> sm;
     sm.start();
     int ve = -110;   // exponent of the largest value scale so far
 #pragma unroll
@@ -396,14 +396,15 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     for (int c = 0; c < NC; ++c) {
         float M, back;
         sm.finish(c, fac[c], M, back);
-        const float zz = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve - sm.up[c]) : back;
+        const float zz = sm.column_sum(sm.z[c]) * ldexpf(back, sm.kBack);
         if (lane < 16 && part == 0) mzl[wave * kPer + query] = float2{M, zz};
         float* ul = reinterpret_cast<float*>(vl) + query * HD;
 #pragma unroll
         for (int d = 0; d < kDt; ++d) {
             f4_t x;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = (MULTI ? o[c][d][e] : o[c][d][e] + dpp_mov<0xB1>(o[c][d][e])) * unscale;
+            for (int e = 0; e < 4; ++e)
+                x[e] = sm.settled(c, MULTI ? o[c][d][e] : o[c][d][e] + dpp_mov<0xB1>(o[c][d][e]), back, ve);
             if (part == 0) *reinterpret_cast<f4_t*>(ul + 16 * d + 4 * u) = x;
         }
         __syncthreads();

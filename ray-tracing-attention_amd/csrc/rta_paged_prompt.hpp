@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                 mx = fmaxf(mx, fabsf(v[kb][e]));
             }
         int qe = 14;
-        if constexpr (FMT != RTA_BF16) qe = part_exponent(Softmax<NQ, N, kScaled>::column_max(mx));
+        if constexpr (FMT != RTA_BF16) qe = part_exponent(Softmax<NQ, N, FMT>::column_max(mx));
         const float sg = ldexpf(1.0f, 14 - qe);
         fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe - 14);
 #pragma unroll
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     const int t_hi = len - count + min(col0 + W * NQ - 1, cols - 1) / a.group;
 
     Acc o[NQ][kDt];
-    Softmax<NQ, N, kScaled> sm;
+    Softmax<NQ, N, FMT> sm;
     sm.start();
     int ve = -110;
 #pragma unroll
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     for (int c = 0; c < NQ; ++c) {
         float M, back;
         sm.finish(c, fac[c], M, back);
-        const float Z = sm.column_sum(sm.z[c]) * back, unscale = kScaled ? ldexpf(back, ve - sm.up[c]) : back;
+        const float Z = sm.column_sum(sm.z[c]) * ldexpf(back, sm.kBack);
         if (col0 + W * c + i >= cols) continue;
         int tok, head;
         column(c, tok, head);
@@ -388,7 +388,9 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
 #pragma unroll
             for (int h = 0; h < kQuads; ++h) {
                 const int dim = W * d + 8 * h + 4 * u;
-                const f4_t U = quad_of(o[c][d], h) * unscale;
+                f4_t U = quad_of(o[c][d], h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) U[e] = sm.settled(c, U[e], back, ve);
                 if (a.nchunk > 1) *reinterpret_cast<f4_t*>(a.part + rec * HD + dim) = U;
                 else write_result(a, at, HD, dim, U, M * kLn2, Z, err);
             }

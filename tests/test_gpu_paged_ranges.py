@@ -97,3 +97,20 @@ def test_value_scales_of_every_size(env, hd, rows):
     q = rows_of(env[0], env[2], rows, 4, hd, 10, 4.0)
     check_terms(c, q, newest(env, c, q))
     assert ops.device_error() == 0
+
+
+# ------------------------------------------------------------------ values near the end ----
+@pytest.mark.parametrize("fmt", [ref.BF16, ref.Q8_ROW])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 5, 40])
+@pytest.mark.parametrize("size", [1e30, 1e36, 3e38])
+def test_values_near_the_end_of_fp32(env, fmt, hd, rows, size):
+    """A mean of finite values is finite: 1500 positions of about the same weight, all of one sign,
+    whose plain sum would overflow."""
+    length = 1500
+    k = normal(env, 11, length, hd)
+    v = size * (1 - 0.5 * normal(env, 12, length, hd).abs().clamp(max=1))
+    c = holding(env, fmt, 1, hd, 64, k, v)
+    q = rows_of(env[0], env[2], rows, 4, hd, 13, 0.1)
+    check_terms(c, q, newest(env, c, q))
+    assert ops.device_error() == 0
