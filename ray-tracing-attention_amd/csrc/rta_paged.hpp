@@ -299,6 +299,10 @@ __device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
     }
 }
 
+// A product under its mask: -inf is a masked one's from here on, so one that is seen becomes NaN (as does
+// inf), which reaches the result.
+__device__ __forceinline__ float seen_or_masked(float x, bool sees) { return sees ? fmaf(x, 0.0f, x) : -INFINITY; }
+
 // Masks the products of 32 positions j0 .. of a list that the columns see between them (a lane
 // holds positions 32 / N h + 4u + e of each column tile, h < N, e < 4): bit k of
 // ok says whether position k counts, t_col is the lane's column's position, -1 at least.  What a
@@ -317,7 +321,7 @@ __device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Vi
             const int at = (mine >> (32 / N * h + e)) & 1u ? p : INT_MAX;   // no distance reaches it
 #pragma unroll
             for (int c = 0; c < NC; ++c)
-                x[c][h][e] = (uint32_t)(t_col[c] - at) < reach ? x[c][h][e] : -INFINITY;
+                x[c][h][e] = seen_or_masked(x[c][h][e], (uint32_t)(t_col[c] - at) < reach);
         }
 }
 
@@ -333,7 +337,7 @@ struct Softmax {
     static constexpr float kTop = FMT == RTA_BF16 ? -kRoom : 14, kSlack = 1.0f;
     static constexpr bool SCALED = PageFmt<FMT>::kScaled;
     float m[NC], low[NC], z[NC];   // m: the largest product; z: of the lane's positions
-    float lowest;                  // of all products: a visible -inf shows nowhere else
+    float lowest;                  // of the products in tiles that are seen whole: a -inf shows nowhere else
     float ask[NC];
     int up[NC];                    // SCALED: the sums o and the tile's operands are 2^up times what they are else
     bool lifted;                   // some of them are not 0
@@ -357,11 +361,13 @@ struct Softmax {
         if constexpr (N == 2) v = add_xor16(v);
         return add_xor32(v);
     }
-    __device__ __forceinline__ void watch(const f4_t (*x)[N]) {
+    __device__ __forceinline__ void watch(const f4_t (*x)[N], bool whole) {
+        float t = lowest;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int j = 0; j < 4 * N; ++j) lowest = fminf(lowest, x[c][j >> 2][j & 3]);
+            for (int j = 0; j < 4 * N; ++j) t = fminf(t, x[c][j >> 2][j & 3]);
+        lowest = whole ? t : lowest;
     }
     // Takes in the maxima of x (masked positions -inf) and brings z and o to the new base; vshift:
     // the power of two by which o has to follow a value scale; spread (all lanes alike): the scales vf are

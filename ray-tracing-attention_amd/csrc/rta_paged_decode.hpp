@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 s[c][1] *= kf[1];
             }
         }
-        sm.watch(s);
+        sm.watch(s, whole);
         if (!whole) {
             if constexpr (MULTI) {
                 mask_columns<NC>(s, now, see, begin + t * kDecTile, u, t_col, a.window, a.sinks);
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                 for (int j = 0; j < 8; ++j) {
                     const bool on = (now >> (16 * (j >> 2) + 4 * u + (j & 3))) & 1u;
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) s[c][j >> 2][j & 3] = on ? s[c][j >> 2][j & 3] : -INFINITY;
+                    for (int c = 0; c < NC; ++c) s[c][j >> 2][j & 3] = seen_or_masked(s[c][j >> 2][j & 3], on);
                 }
             }
         }

@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                         for (int c = 0; c < NQ; ++c) x[c][h] *= kf;
                     }
                 }
-                sm.watch(x);
+                sm.watch(x, whole);
                 if (!whole) {
                     mask_columns<NQ>(x, (uint32_t)(okm >> (32 * sub)), see, j0 + 32 * sub, u, t_col, a.window, a.sinks);
                     if (badm) sm.poison(x, (uint32_t)(badm >> (32 * sub)), u);

@@ -114,3 +114,76 @@ def test_values_near_the_end_of_fp32(env, fmt, hd, rows, size):
     q = rows_of(env[0], env[2], rows, 4, hd, 13, 0.1)
     check_terms(c, q, newest(env, c, q))
     assert ops.device_error() == 0
+
+
+# ------------------------------------------------------------------ what a row may not see ----
+@pytest.mark.parametrize("fmt", ALL)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_a_missing_page_is_not_scored(env, fmt, hd, rows):
+    """Where a page is missing nothing is read for it: infinite keys in page 0 (another sequence's)
+    report nothing."""
+    torch, pages, dev = env
+    length = 100
+    c = pages.PagedCache(fmt, 1, hd, 16, n_pages=20, max_seqs=2, max_pages=8)
+    c.extend(ints(torch, [1, 0], dev), ints(torch, [16, length], dev))
+    assert c.table[1, 0].item() == 0
+    k, v = normal(env, 14, length + 16, hd), normal(env, 15, length + 16, hd)
+    c.append(k.to(dev), v.to(dev), seqs=ints(torch, [1, 0], dev), cu_rows=ints(torch, [0, 16, 16 + length], dev))
+    if fmt == ref.Q8_ROW:
+        c.pool[0, 0, : 16 * hd] = 0
+        c.pool[0, 0, : 16 * hd].view(16, hd)[:, 0] = 1
+        c.pool[0, 0, 2 * 16 * hd :][: 16 * 4] = torch.full((16,), 3e38, device=dev).view(torch.uint8)
+    else:
+        kv = c.pool[0, 0].view(torch.float16 if fmt == ref.F16 else torch.bfloat16)
+        kv[: 16 * hd] = 0
+        kv[: 16 * hd].view(16, hd)[:, 0] = float("inf")
+    c.table[0, 2] = -1
+    q = rows_of(torch, dev, rows, 4, hd, 16)
+    q[:, :, 0] = -8.0    # a score of -inf wherever page 0 is looked at
+    got = newest(env, c, q)
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    k, v, held = ref.dense(c, 0, 0, missing_ok=True)
+    want = [ref.attend(q[r].cpu().double().numpy(), np.where(held[:, None, None], k, 0), v, held, length - rows + r)
+            for r in range(rows)]
+    ref.check_rows(got, want)
+
+
+@pytest.mark.parametrize("fmt", [ref.BF16, ref.Q8_ROW])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [4, 40])
+def test_a_score_out_of_sight_reports_nothing(env, fmt, hd, rows):
+    """A later position's key would overflow the scores of rows before it (and only theirs)."""
+    length = 90
+    k, v = normal(env, 17, length, hd), normal(env, 18, length, hd)
+    p = length - rows // 2
+    k[p] = 0.0
+    k[p, 0] = 3e38
+    c = holding(env, fmt, 1, hd, 16, k, v)
+    q = rows_of(env[0], env[2], rows, 4, hd, 19)
+    q[: rows - rows // 2, :, 0] = -100.0
+    q[rows - rows // 2 :, :, 0] = 0.0
+    got = newest(env, c, q)
+    assert ops.device_error() == 0
+    check_terms(c, q, got, rows=range(rows - rows // 2))
+    assert all(bool(t.isfinite().all()) for t in got)
+
+
+@pytest.mark.parametrize("fmt", [ref.BF16, ref.Q8_ROW])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows,length", [(1, 64), (1, 70), (4, 70), (40, 70), (40, 300)])
+def test_a_score_of_minus_infinity_in_sight_is_reported(env, fmt, hd, rows, length):
+    """In the newest position (seen by the last row alone) and in the oldest (seen by all).  (A binary16
+    key is below 2^16 and a query is taken by its head's power of two, so there is no such product.)"""
+    torch = env[0]
+    q = rows_of(torch, env[2], rows, 4, hd, 24)
+    q[:, :, 0] = -1e10
+    for p in (length - 1, 0):
+        k, v = normal(env, 25, length, hd), normal(env, 26, length, hd)
+        k[:, 0] = 0.0
+        k[p, 0] = 3e38
+        c = holding(env, fmt, 1, hd, 16, k, v)
+        out = newest(env, c, q)[0]
+        assert ops.device_error() == _lib.DEVERR_DETECTOR
+        if p:   # rows that do not see it keep theirs
+            assert bool(out[: rows - 1].isfinite().all())
