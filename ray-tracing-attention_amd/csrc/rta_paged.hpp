@@ -328,7 +328,8 @@ __device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Vi
 // The online softmax of NC column tiles, a lane holding 4N positions of its column of each, N = 2
 // (16 columns) or 4 (32 columns) (products x; score = x fac in log2 units).  Weights are 2^(score - low), 2^kTop for the largest
 // score when low was set; low follows the maximum only when weights would pass 2^(kTop + kSlack),
-// 2^15 for binary16 parts, so the sums are not rescaled for every small step, and binary16 parts do not overflow.
+// 2^15 for binary16 parts (fac is a power of two: a score is its product exactly, and its distance from low
+// is rounded once, however large both are), so the sums are not rescaled for every small step, and binary16 parts do not overflow.
 // kTop is as high as that allows: the second part ends at 2^-24, and over a long history most of
 // the sum lies in weights far below the largest.  bfloat16 parts have fp32's exponents, and values may too:
 // there the largest weight is 2^-kRoom from the start; sums of values down to 2^-100 stay normal numbers.
@@ -338,7 +339,6 @@ struct Softmax {
     static constexpr bool SCALED = PageFmt<FMT>::kScaled;
     float m[NC], low[NC], z[NC];   // m: the largest product; z: of the lane's positions
     float lowest;                  // of the products in tiles that are seen whole: a -inf shows nowhere else
-    float ask[NC];
     int up[NC];                    // SCALED: the sums o and the tile's operands are 2^up times what they are else
     bool lifted;                   // some of them are not 0
 
@@ -382,14 +382,15 @@ struct Softmax {
 #pragma unroll
             for (int j = 1; j < 4 * N; ++j) t = fmaxf(t, x[c][j >> 2][j & 3]);
             m[c] = fmaxf(m[c], column_max(t));
-            ask[c] = fmaf(m[c], fac[c], -kTop);
-            lift = lift || ask[c] > low[c] + kSlack;
+            lift = lift || fmaf(m[c], fac[c], -low[c]) > kTop + kSlack;
         }
         if (__builtin_amdgcn_ballot_w64(lift)) {
             lifted = spread;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const float base = ask[c] > low[c] ? ask[c] : low[c];
+                const float top = m[c] * fac[c];
+                float base = fmaxf(low[c], top - kTop);
+                if (top - base > kTop + kSlack) base = top;   // (past 2^25, where floats are 4 apart)
                 const float al = __builtin_amdgcn_exp2f(low[c] - (base == -INFINITY ? 0.0f : base));
                 int by = vshift;
                 z[c] *= al;

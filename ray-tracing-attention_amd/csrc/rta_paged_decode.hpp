@@ -172,8 +172,9 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     // |q| (the power of two of binary16 operands).
     const int part = MULTI ? 0 : i & 1, query = MULTI ? i : i >> 1;   // lane's column of a column tile
     int t_col[NC];
-    float fac[NC];   // score = product * fac, in powers of two: 1 / s / sqrt(HD) * log2 e
+    float fac[NC];   // score in log2 units = product * fac, a power of two; q takes log2 e / sqrt(HD) with it
     int qe[NC];
+    const float kScale = kLog2e / sqrtf((float)HD);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         int row, head;
@@ -185,12 +186,12 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             float mx = 0.0f;
 #pragma unroll
             for (int j = 0; j < HD / 4; ++j) mx = fmaxf(mx, fabsf(q[u * (HD / 4) + j]));
-            qe[c] = part_exponent(max_xor32(max_xor16(mx)));
+            qe[c] = part_exponent(max_xor32(max_xor16(mx)) * kScale);
         }
-        fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe[c] - 14);
+        fac[c] = ldexpf(1.0f, qe[c] - 14);
         for (int kb = wave; kb < kKb; kb += kDecWaves) {
             float v[8];
-            const float sg = ldexpf(1.0f, 14 - qe[c]);
+            const float sg = ldexpf(kScale, 14 - qe[c]);
 #pragma unroll
             for (int s = 0; s < 8; ++s) v[s] = q[operand_dim<FMT>(kb, u) + s] * sg;
             u4_t op[kOps];

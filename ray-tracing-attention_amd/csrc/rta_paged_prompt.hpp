@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     u4_t qb[NQ][kKb][2];   // (the third part of bfloat16 lies in LDS: its registers would leave none for operands)
     u4_t* third = reinterpret_cast<u4_t*>(lds + 2 * L::kBuf + wave * L::kThird) + lane;
     float fac[NQ];
+    const float kScale = kLog2e / sqrtf((float)HD);   // (into q: then a score is its product times a power of two)
     auto column = [&](int c, int& tok, int& head) {   // past the last one: the last
         const int col = min(col0 + W * c + i, cols - 1);
         tok = col / a.group;
@@ -206,9 +207,9 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                 mx = fmaxf(mx, fabsf(v[kb][e]));
             }
         int qe = 14;
-        if constexpr (FMT != RTA_BF16) qe = part_exponent(Softmax<NQ, N, FMT>::column_max(mx));
-        const float sg = ldexpf(1.0f, 14 - qe);
-        fac[c] = ldexpf(kLog2e / sqrtf((float)HD), qe - 14);
+        if constexpr (FMT != RTA_BF16) qe = part_exponent(Softmax<NQ, N, FMT>::column_max(mx) * kScale);
+        const float sg = ldexpf(kScale, 14 - qe);
+        fac[c] = ldexpf(1.0f, qe - 14);
 #pragma unroll
         for (int kb = 0; kb < kKb; ++kb) {
 #pragma unroll

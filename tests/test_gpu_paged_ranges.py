@@ -187,3 +187,35 @@ def test_a_score_of_minus_infinity_in_sight_is_reported(env, fmt, hd, rows, leng
         assert ops.device_error() == _lib.DEVERR_DETECTOR
         if p:   # rows that do not see it keep theirs
             assert bool(out[: rows - 1].isfinite().all())
+
+
+# ------------------------------------------------------------------ large scores ----
+@pytest.mark.parametrize("fmt", ALL)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e8, 1e9, 1e12, 1e20])
+def test_scores_of_any_finite_size(env, fmt, hd, rows, size):
+    """Far apart as they are, one position takes all: out is its value, z is 1.  A score's error is
+    below sqrt(hd) roundings of 2^-22 of sum |q k|, so heads whose two largest are further apart than
+    2^-14 of that are told apart."""
+    length = 400
+    k, v = normal(env, 20, length, hd), normal(env, 21, length, hd)
+    c = holding(env, fmt, 1, hd, 16, k, v)
+    q = rows_of(env[0], env[2], rows, 4, hd, 22, size)
+    out, m, z = (t.cpu().double().numpy() for t in newest(env, c, q))
+    assert ops.device_error() == 0
+    k, v, _ = ref.dense(c, 0, 0)
+    told = 0
+    for r in range(rows):
+        n = length - rows + r + 1
+        for h in range(4):
+            x = q[r, h].cpu().double().numpy()
+            s = k[:n, 0] @ x / hd**0.5
+            a, b = np.argsort(s)[-2:][::-1]
+            most = (np.abs(k[:n, 0]) @ np.abs(x)).max() / hd**0.5
+            if s[a] - s[b] <= 2.0**-14 * most + 30:
+                continue
+            told += 1
+            assert np.abs(out[r, h] - v[a, 0]).max() <= 2.0**-20 * np.abs(v[a, 0]).max(), (r, h)
+            assert abs(m[r, h] - s[a]) <= hd**0.5 * 2.0**-22 * most and abs(z[r, h] - 1) <= 2.0**-20, (r, h, z[r, h])
+    assert told >= rows
