@@ -558,9 +558,11 @@ int rta_pages_compact(const rta_pages* pages, int32_t* used, void* workspace, si
                       rta_stream_t stream);
 
 /* The row lists below: row r belongs to entry i with cu_rows[i] <= r < cu_rows[i + 1] (device,
- * n + 1 nondecreasing values, the last at most rows); the c = cu_rows[i + 1] - cu_rows[i] rows
+ * n + 1 nondecreasing values from 0 to at most rows); the c = cu_rows[i + 1] - cu_rows[i] rows
  * of an entry are its sequence's newest c positions, oldest first.  cu_rows NULL: one row per
- * entry (rows = n).  Rows outside every entry are left as they were. */
+ * entry (rows = n).  Rows outside every entry are left as they were.  An entry whose rows do not lie
+ * in [0, rows), and a list that falls, raise RTA_DEVERR_PAGES: that entry's rows are left as they
+ * were, and where a list falls any of its rows may be; a row of two entries means nothing. */
 
 /* The rows' keys and values k[r, :kv_heads * head_dim], v (fp32, row strides in floats) into
  * the pages of layer `layer`: rounded to nearest even, or for RTA_Q8_ROW scale = max|x| * (1 / 127)

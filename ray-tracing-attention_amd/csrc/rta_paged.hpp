@@ -225,12 +225,14 @@ struct Entry {
     int len;            // its sequence's positions, 0 for a bad one
     const int32_t* table;
 };
-// False for an entry without rows.  err collects the error bits.
+// False for an entry without rows or with bad ones.  err collects the error bits.
 __device__ __forceinline__ bool resolve_entry(const PagedAttnArgs& a, int entry, Entry& e, uint32_t& err) {
-    e.base = a.l.cu[entry];
-    e.count = a.l.cu[entry + 1] - e.base;
-    if (e.base < 0 || e.base >= a.l.rows || e.count <= 0) return false;
-    e.rows = min(e.count, min(a.max_rows, a.l.rows - e.base));
+    if (!entry_rows(a.l, entry, e.base, e.count)) {
+        err |= RTA_DEVERR_PAGES;
+        return false;
+    }
+    if (!e.count) return false;
+    e.rows = min(e.count, a.max_rows);
     if (e.count > a.max_rows) err |= RTA_DEVERR_PAGES;
     const int s = list_seq(a.l.seqs, entry);
     e.len = 0;

@@ -59,8 +59,12 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     const int entry = rest % a.l.n, tile = a.ntile - 1 - rest / a.l.n;
     uint32_t err = 0;
     Entry en;
-    if (!resolve_entry(a, entry, en, err)) return;
+    const bool ok = resolve_entry(a, entry, en, err);
     if (tile > 0) err &= ~RTA_DEVERR_PAGES;   // the first tile tells
+    if (!ok) {
+        if (err && tid == 0) raise_error(err);
+        return;
+    }
     if ((int64_t)tile * L::kCols >= (int64_t)en.rows * a.group) return;
     const int base = en.base, count = en.count, live_rows = en.rows, len = en.len;
     const int32_t* table = en.table;

@@ -412,6 +412,7 @@ __global__ void __launch_bounds__(256) append_kernel(const PageArgs a, const Row
     const int r = blockIdx.x;
     int off = 0;
     bool listed;
+    if (r == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
     uint8_t* page = row_page(a, l, r, off, listed);
     if (!page) {
         if (listed && threadIdx.x == 0 && blockIdx.y == 0) raise_error(RTA_DEVERR_PAGES);
@@ -466,6 +467,7 @@ __global__ void __launch_bounds__(256) page_read_kernel(const PageArgs a, const 
     const int r = blockIdx.x;
     int off = 0;
     bool listed;
+    if (r == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
     const uint8_t* page = row_page(a, l, r, off, listed);
     if (!listed) return;
     if (!page && threadIdx.x == 0 && blockIdx.y == 0) raise_error(RTA_DEVERR_PAGES);

@@ -41,8 +41,16 @@ struct RowList {
 
 __device__ __forceinline__ int list_seq(const int32_t* seqs, int i) { return seqs ? seqs[i] : i; }
 
+// Entry i's first row and its row count; false unless they lie in order within the rows.
+__device__ __forceinline__ bool entry_rows(const RowList& l, int i, int& first, int& count) {
+    first = l.cu[i];
+    const int last = l.cu[i + 1];
+    count = last - first;
+    return first >= 0 && first <= last && last <= l.rows;
+}
+
 // Entry i with cu[i] <= r < cu[i + 1], its first row and its row count; false for a row outside
-// every entry.  Every lane of a wave may ask for another row.
+// every entry or of one that entry_rows refuses.  Every lane of a wave may ask for another row.
 __device__ __forceinline__ bool row_entry(const RowList& l, int r, int& i, int& first, int& count) {
     if (!l.cu) {
         i = first = r;
@@ -56,9 +64,16 @@ __device__ __forceinline__ bool row_entry(const RowList& l, int r, int& i, int& 
         else hi = mid;
     }
     i = lo;
-    first = l.cu[lo];
-    count = l.cu[lo + 1] - first;
-    return r >= first && r - first < count;
+    return entry_rows(l, lo, first, count) && r >= first && r - first < count;
+}
+
+// Whether an entry's rows are refused, over a whole list: for one workgroup of a kernel that goes by rows,
+// where an entry may have none to find it by.
+__device__ __forceinline__ bool bad_rows(const RowList& l) {
+    bool bad = false;
+    int first, count;
+    for (int i = threadIdx.x; l.cu && i < l.n; i += blockDim.x) bad = bad || !entry_rows(l, i, first, count);
+    return bad;
 }
 
 // Byte offset of page pg of a layer: page sizes are multiples of 128 below 2^38.

@@ -1,0 +1,115 @@
+"""Lists and books that the paged history's calls refuse on the device: the entry is left undone,
+RTA_DEVERR_PAGES is raised, and the others come out as they should."""
+import numpy as np
+import pytest
+
+import paged_reference as ref
+from rta import _lib, ops
+from test_gpu_paged_attention import fill, rows_of, want_rows
+from test_gpu_pages import env, filled, ints  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+LENS = [1500, 40, 700]
+# row offsets over nine rows and three entries, and the entries that are good
+LISTS = [([-3, 2, 5, 9], [1, 2]), ([0, 2, 5, 12], [0, 1]), ([0, 2, 5, 2**31 - 1], [0, 1]), ([4, 9, 12, 20], [0]),
+         ([12, 13, 14, 15], []), ([-9, -5, -2, 0], []), ([-2**31, 0, 4, 9], [1, 2])]
+# where a list falls, a row has two entries (whose parts of it may mix) or is not found by the offsets around it:
+# a row of one entry comes out as that has it, or stays as it was
+FALLING = [([0, 4, 3, 9], [0, 2]), ([3, 3, 1, 6], [0, 2])]
+
+
+def rows_left(cu, good):
+    """(entries with rows as (entry, first row, count), rows that no good entry has)."""
+    held = np.zeros(9, int)
+    for i in good:
+        held[cu[i] : cu[i + 1]] += 1
+    return [(i, cu[i], cu[i + 1] - cu[i]) for i in good], np.flatnonzero(held == 0)
+
+
+# ------------------------------------------------------------------ row lists ----
+@pytest.mark.parametrize("fmt", [ref.F16, ref.Q8_ROW])
+@pytest.mark.parametrize("hq", [4, 16])   # few columns, and more
+@pytest.mark.parametrize("cu,good", LISTS + FALLING, ids=str)
+def test_attention_leaves_bad_rows(env, fmt, hq, cu, good):
+    torch, _, dev = env
+    c = filled(env, fmt, 1, 64, 16, LENS)
+    fill(env, c, LENS, 3)
+    q = rows_of(torch, dev, 9, hq, 64, 4)
+    out = torch.full((9, hq, 64), 7.0, device=dev)
+    m, z = torch.full((9, hq), 7.0, device=dev), torch.full((9, hq), 7.0, device=dev)
+    how = dict(cu_rows=ints(torch, cu, dev), max_rows=6, max_len=1500)
+    assert c.attention_workspace_bytes(hq, 9, 3, 6, 1500) > 0   # cut into chunks, so there is a merge
+    # what an earlier call left in the workspace must not come out
+    ws = torch.full((c.attention_workspace_bytes(hq, 9, 3, 6, 1500),), 63, dtype=torch.uint8, device=dev)
+    c.attention(q, out=out, m=m, z=z, workspace=ws, **how)
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    entries, left = rows_left(cu, good)
+    for t in (out, m, z):
+        assert all((t[r] == 7.0).all() for r in left)
+    if (cu, good) not in FALLING:
+        for i, first, count in entries:
+            ref.check_rows([t[first : first + count] for t in (out, m, z)], want_rows(c, q, [(i, first, count)]), (cu, i))
+        return
+    for r in set(range(9)) - set(left.tolist()):
+        of = [(i, first, count) for i, first, count in entries if first <= r < first + count]
+        if len(of) == 1 and not (out[r] == 7.0).all():
+            ref.check_rows([t[r : r + 1] for t in (out, m, z)], [want_rows(c, q, of)[r - of[0][1]]], r)
+
+
+@pytest.mark.parametrize("cu,good", [([-1, 1, 2, 3], [1, 2]), ([0, 1, 2, 4], [0, 1]), ([3, 4, 5, 6], [])], ids=str)
+@pytest.mark.parametrize("max_len", [1500, 100])
+def test_single_rows_of_bad_lists(env, cu, good, max_len):
+    torch, _, dev = env
+    lens = [min(n, max_len) for n in LENS]
+    c = filled(env, ref.F16, 1, 64, 16, lens)
+    fill(env, c, lens, 5)
+    q = rows_of(torch, dev, 3, 4, 64, 6)
+    out = torch.full((3, 4, 64), 7.0, device=dev)
+    _, m, z = c.attention(q, cu_rows=ints(torch, cu, dev), max_rows=1, max_len=max_len, out=out)
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    for r in range(3):
+        i = [i for i in good if cu[i] == r]
+        if i:
+            ref.check_rows([t[r : r + 1] for t in (out, m, z)], want_rows(c, q, [(i[0], r, 1)]))
+        else:
+            assert (out[r] == 7.0).all()
+
+
+@pytest.mark.parametrize("cu,good", LISTS, ids=str)
+def test_rows_in_and_out_of_bad_lists(env, cu, good):
+    torch, _, dev = env
+    c, d = (filled(env, ref.BF16, 2, 64, 16, LENS) for _ in range(2))
+    d.pool.copy_(c.pool)
+    entries, left = rows_left(cu, good)
+    x = torch.randn(9, 2, 128, generator=torch.Generator().manual_seed(7)).to(dev)
+    c.append(x[:, 0], x[:, 1], cu_rows=ints(torch, cu, dev))
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    for i, first, count in entries:   # the same rows by lists of their own
+        rows = x[first : first + count]
+        d.append(rows[:, 0], rows[:, 1], seqs=ints(torch, [i], dev), cu_rows=ints(torch, [0, count], dev))
+    assert ops.device_error() == 0
+    assert torch.equal(c.pool, d.pool)
+    back = [torch.full((9, 128), 7.0, device=dev) for _ in range(2)]
+    d.read(9, cu_rows=ints(torch, cu, dev), k=back[0], v=back[1])
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    want = x.bfloat16().float()
+    want[left.tolist()] = 7.0
+    assert torch.equal(back[0], want[:, 0]) and torch.equal(back[1], want[:, 1])
+
+
+@pytest.mark.parametrize("cu,good", FALLING, ids=str)
+def test_rows_in_and_out_of_falling_lists(env, cu, good):
+    torch, _, dev = env
+    c = filled(env, ref.BF16, 2, 64, 16, LENS)
+    before = c.pool.clone()
+    _, left = rows_left(cu, good)
+    x = torch.ones(9, 128, device=dev)
+    c.append(x, x, cu_rows=ints(torch, cu, dev))
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    changed = c.pool.view(torch.bfloat16)[c.pool.view(torch.bfloat16).view(torch.int16) != before.view(torch.int16)]
+    assert bool((changed == 1.0).all())
+    back = torch.full((9, 128), 7.0, device=dev)
+    c.read(9, cu_rows=ints(torch, cu, dev), k=back, v=back.clone())
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    assert all((back[r] == 7.0).all() for r in left)
