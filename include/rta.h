@@ -553,7 +553,9 @@ int rta_pages_free(const rta_pages* pages, const int32_t* seqs, const int32_t* f
                    rta_stream_t stream);
 
 /* Closes the pool up: with U pages in use, the k-th used page at or past U moves (all layers)
- * to the k-th free page below U, and the table follows.  used (device, may be NULL) gets U. */
+ * to the k-th free page below U, and the table follows.  used (device, may be NULL) gets U.  Where
+ * pages move, a table entry that names none of the pages in use (and is not -1) raises
+ * RTA_DEVERR_PAGES and stays as it is. */
 int rta_pages_compact(const rta_pages* pages, int32_t* used, void* workspace, size_t workspace_bytes,
                       rta_stream_t stream);
 

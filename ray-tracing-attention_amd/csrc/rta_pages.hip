@@ -53,7 +53,7 @@ struct PlanWs {
     int32_t* list;      // [n_pages] free pages in order
     int32_t* holders;   // [n_pages] listed sequences that share a page
     int32_t* keeper;    // [n_pages] the last of them
-    int32_t* map;       // [n_pages] where a page moves
+    int32_t* map;       // [n_pages] where a page goes (itself, if it stays), -1: it is free
     int32_t* count;     // pairs in src / dst
 };
 
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256) pages_init_kernel(const PageArgs a) {
 
 // ------------------------------------------------------------------ compact ----
 // One workgroup: the number U of used pages, the holes below it and the used pages past it, both
-// in order (they are equally many), and the map from the latter to the former.
+// in order (they are equally many), and where every page goes.
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PageArgs a, PlanWs ws, int32_t* used_out) {
     __shared__ int red[kPlanWaves];
     const int tid = threadIdx.x;
@@ -350,18 +350,18 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PageAr
         at = movers + block_scan(mover, red, k);
         if (mover) ws.src[at] = i;
         movers += k;
+        if (in && !mover) ws.map[i] = use ? i : -1;
     }
     __syncthreads();
     for (int k = tid; k < movers; k += kPlanThreads) ws.map[ws.src[k]] = ws.dst[k];
     if (tid == 0) {
         *ws.count = movers;
         if (used_out) *used_out = U;
-        ws.count[1] = U;
     }
 }
 
 __global__ void __launch_bounds__(256) compact_kernel(const PageArgs a, PlanWs ws) {
-    const int pairs = ws.count[0], U = ws.count[1];
+    const int pairs = ws.count[0];
     if (!pairs) return;
     const int64_t step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     for (int64_t k = at; k < pairs; k += step) {
@@ -369,10 +369,15 @@ __global__ void __launch_bounds__(256) compact_kernel(const PageArgs a, PlanWs w
         a.refs[ws.src[k]] = 0;
     }
     const int64_t entries = (int64_t)a.max_seqs * a.max_pages;
+    bool bad = false;
     for (int64_t e = at; e < entries; e += step) {
         const int p = a.table[e];
-        if (p >= U && p < a.n_pages) a.table[e] = ws.map[p];
+        if (p == -1) continue;
+        const int to = (unsigned)p < (unsigned)a.n_pages ? ws.map[p] : -1;
+        if (to < 0) bad = true;   // (left as it is: a page that the counts call free)
+        else if (to != p) a.table[e] = to;
     }
+    if (bad) raise_error(RTA_DEVERR_PAGES);
     copy_pages(a, ws.src, ws.dst, pairs);
 }
 

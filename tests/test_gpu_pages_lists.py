@@ -113,3 +113,28 @@ def test_rows_in_and_out_of_falling_lists(env, cu, good):
     c.read(9, cu_rows=ints(torch, cu, dev), k=back, v=back.clone())
     assert ops.device_error() == _lib.DEVERR_PAGES
     assert all((back[r] == 7.0).all() for r in left)
+
+
+# ------------------------------------------------------------------ compaction ----
+@pytest.mark.parametrize("page", [1, 4])
+def test_compact_leaves_entries_of_free_pages(env, page):
+    """Table entries that name pages outside the pool or that the counts call free, below and past the
+    pages in use, stay as they are; the others follow their pages."""
+    torch, pages, dev = env
+    c = pages.PagedCache(ref.F16, 1, 64, page, n_pages=600, max_seqs=6, max_pages=200)
+    b = ref.Book(page, 600, 6, 200)
+    add = [100 * page, 60 * page, 120 * page]
+    c.extend(ints(torch, range(3), dev), ints(torch, add, dev))
+    b.extend([0, 1, 2], add)
+    c.free(ints(torch, [1], dev))
+    b.free([1])
+    # sequences 4 and 5 (empty in the book): a hole below the pages in use, free ones past them, a page in use, outside
+    odd = {(4, 0): 130, (4, 1): 590, (4, 7): 279 + 1, (5, 0): 600, (5, 3): -2, (5, 4): 2**31 - 1, (5, 5): 270}
+    for (s, e), p in odd.items():
+        c.table[s, e] = b.table[s][e] = p
+    ws = torch.full((c.workspace_bytes(),), 1, dtype=torch.uint8, device=dev)   # (numbers that are no answer)
+    used = c.compact(workspace=ws)
+    n, pairs = b.compact()
+    assert pairs and used.tolist() == [n] and b.table[5][5] != 270
+    b.check(c)
+    assert ops.device_error() == _lib.DEVERR_PAGES
