@@ -95,7 +95,10 @@ __device__ __forceinline__ bool want_of(const PageArgs& a, const int32_t* seqs, 
     auto pages = [&](int n) { return n ? (int)a.by_page.div((uint32_t)n - 1) + 1 : 0; };
     w.fresh = pages(last) - pages(w.len);
     const int e = (int)a.by_page.div((uint32_t)w.len);
-    if (w.add > 0 && w.len - e * a.page > 0) w.tail = page_of(a, a.table + (int64_t)w.seq * a.max_pages, e);
+    if (w.add > 0 && w.len - e * a.page > 0) {
+        w.tail = a.table[(int64_t)w.seq * a.max_pages + e];
+        if (bad_page(a, w.tail)) return false;
+    }
     return true;
 }
 
@@ -276,19 +279,21 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(const PageArgs a, const
     ok = !listed_before(dst, i, d) && ok;
     ok = !listed_before(src, n, d) && ok;
     const int len = ok ? a.lengths[s] : 0;
-    if (!ok || a.lengths[d] != 0 || len < 0) {
+    ok = ok && !bad_length(a, len) && a.lengths[d] == 0;
+    const int pages = ok && len ? (int)a.by_page.div((uint32_t)len - 1) + 1 : 0;
+    const int32_t* from = a.table + (int64_t)s * a.max_pages;
+    int32_t* to = a.table + (int64_t)d * a.max_pages;
+    bool bad = false;
+    for (int e = threadIdx.x; e < pages; e += 256) bad = bad || bad_page(a, from[e]);
+    if (__syncthreads_or(bad) || !ok) {   // (and every thread has read lengths[d])
         if (threadIdx.x == 0) raise_error(RTA_DEVERR_PAGES);
         return;
     }
-    const int pages = len ? (int)a.by_page.div((uint32_t)len - 1) + 1 : 0;
-    const int32_t* from = a.table + (int64_t)s * a.max_pages;
-    int32_t* to = a.table + (int64_t)d * a.max_pages;
-    for (int e = threadIdx.x; e < pages && e < a.max_pages; e += 256) {
-        const int p = page_of(a, from, e);
+    for (int e = threadIdx.x; e < pages; e += 256) {
+        const int p = from[e];
         to[e] = p;
         if (p >= 0) atomicAdd(a.refs + p, 1);
     }
-    __syncthreads();   // every thread has read lengths[d]
     if (threadIdx.x == 0) a.lengths[d] = len;
 }
 
@@ -298,24 +303,24 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const PageArgs a, const
     const int i = blockIdx.x, s = list_seq(seqs, i);
     bool ok = (unsigned)s < (unsigned)a.max_seqs;
     if (seqs) ok = !listed_before(seqs, i, s) && ok;
-    const int lo = first ? first[i] : 0;
-    if (!ok || lo < 0) {
+    const int lo = first ? first[i] : 0, len = ok ? a.lengths[s] : 0, hi = last ? last[i] : len;
+    ok = ok && lo >= 0 && !bad_length(a, len);
+    const int pages = ok && len ? (int)a.by_page.div((uint32_t)len - 1) + 1 : 0;
+    int32_t* row = a.table + (int64_t)s * a.max_pages;
+    // the first page that begins at or past lo, and how many from there end at hi
+    const int e0 = ok ? (int)a.by_page.div((uint32_t)lo) + (lo % a.page ? 1 : 0) : 0;
+    const int e1 = !ok ? 0 : hi >= len ? pages : hi > 0 ? (int)a.by_page.div((uint32_t)hi) : 0;
+    bool bad = false;
+    for (int e = e0 + (int)threadIdx.x; e < e1; e += 256) bad = bad || bad_page(a, row[e]);
+    if (__syncthreads_or(bad) || !ok) {   // (and every thread has read lengths[s])
         if (threadIdx.x == 0) raise_error(RTA_DEVERR_PAGES);
         return;
     }
-    const int len = min(a.lengths[s], (int)((int64_t)a.max_pages * a.page)), hi = last ? last[i] : len;
-    const int pages = len > 0 ? (int)a.by_page.div((uint32_t)len - 1) + 1 : 0;
-    int32_t* row = a.table + (int64_t)s * a.max_pages;
-    // the first page that begins at or past lo
-    const int e0 = (int)a.by_page.div((uint32_t)lo) + (lo % a.page ? 1 : 0);
-    for (int e = e0 + (int)threadIdx.x; e < pages; e += 256) {
-        const int end = e + 1 < pages ? (e + 1) * a.page : len;   // past its last held position
-        if (end > hi) break;
-        const int p = page_of(a, row, e);
+    for (int e = e0 + (int)threadIdx.x; e < e1; e += 256) {
+        const int p = row[e];
         row[e] = -1;
         if (p >= 0) atomicSub(a.refs + p, 1);
     }
-    __syncthreads();   // every thread has read lengths[s]
     if (threadIdx.x == 0 && hi >= len && lo < len) a.lengths[s] = lo;
 }
 

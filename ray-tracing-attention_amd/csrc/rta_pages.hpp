@@ -87,6 +87,13 @@ __device__ __forceinline__ int page_of(const PageArgs& a, const int32_t* __restr
     return (unsigned)p < (unsigned)a.n_pages ? p : -1;
 }
 
+// A table entry that is neither a page of the pool nor -1.
+__device__ __forceinline__ bool bad_page(const PageArgs& a, int p) { return p < -1 || p >= a.n_pages; }
+// A length that the table cannot hold.
+__device__ __forceinline__ bool bad_length(const PageArgs& a, int len) {
+    return len < 0 || len > (int)((int64_t)a.max_pages * a.page);   // (<= INT_MAX)
+}
+
 namespace host {
 
 inline int page_element(int fmt) { return fmt == RTA_F16 || fmt == RTA_BF16 ? 2 : fmt == RTA_Q8_ROW ? 1 : 0; }

@@ -138,3 +138,75 @@ def test_compact_leaves_entries_of_free_pages(env, page):
     assert pairs and used.tolist() == [n] and b.table[5][5] != 270
     b.check(c)
     assert ops.device_error() == _lib.DEVERR_PAGES
+
+
+# ------------------------------------------------------------------ lengths and pages outside ----
+def grown(env):
+    """Four sequences of 20, 33, 64 and 16 positions, pages of 16, at most 4 each; the book beside it."""
+    torch, pages, dev = env
+    c = pages.PagedCache(ref.F16, 1, 64, 16, n_pages=40, max_seqs=8, max_pages=4)
+    b = ref.Book(16, 40, 8, 4)
+    c.extend(ints(torch, range(4), dev), ints(torch, [20, 33, 64, 16], dev))
+    b.extend([0, 1, 2, 3], [20, 33, 64, 16])
+    return c, b
+
+
+@pytest.mark.parametrize("length", [65, 2**31 - 1, -1, -2**31])
+def test_lengths_that_the_table_cannot_hold(env, length):
+    """A caller's length of sequence 2: forks of it, frees (whole, its end, its middle) and extends are
+    left undone, the other entries are done."""
+    torch, _, dev = env
+    for what in ("fork", "whole", "end", "middle", "extend"):
+        c, b = grown(env)
+        c.lengths[2] = b.lengths[2] = length
+        if what == "fork":
+            c.fork(ints(torch, [2, 1], dev), ints(torch, [5, 6], dev))
+            b.fork([1], [6])
+        elif what == "extend":
+            c.extend(ints(torch, [2, 1], dev))
+            b.extend([1], [1])
+        else:
+            first, last = {"whole": (None, None), "end": ([16, 16], None), "middle": ([16, 16], [32, 32])}[what]
+            c.free(ints(torch, [2, 1], dev), None if first is None else ints(torch, first, dev),
+                   None if last is None else ints(torch, last, dev))
+            b.free([1], first and first[:1], last and last[:1])
+        b.check(c)
+        assert ops.device_error() == _lib.DEVERR_PAGES, what
+
+
+@pytest.mark.parametrize("page", [40, 2**31 - 1, -2, -2**31])
+def test_pages_outside_the_pool(env, page):
+    """A caller's table entry that is neither a page nor -1: what would copy, free or replace it is left
+    undone; what does not touch it is done."""
+    torch, _, dev = env
+    for what in ("fork", "free", "before", "extend"):
+        c, b = grown(env)
+        c.table[1, 2] = b.table[1][2] = page   # the third, partly filled page of sequence 1
+        if what == "fork":
+            c.fork(ints(torch, [1, 0], dev), ints(torch, [5, 6], dev))
+            b.fork([0], [6])
+        elif what == "free":
+            c.free(ints(torch, [1, 0], dev))
+            b.free([0])
+        elif what == "extend":
+            c.extend(ints(torch, [1, 0], dev))
+            b.extend([0], [1])
+        else:   # the first two pages of it
+            c.free(ints(torch, [1], dev), None, ints(torch, [32], dev))
+            b.free([1], None, [32])
+        b.check(c)
+        assert ops.device_error() == (0 if what == "before" else _lib.DEVERR_PAGES), what
+
+
+def test_holes_are_forked_and_freed(env):
+    """-1 is no bad page: a sequence whose window has passed its first pages goes on like any other."""
+    torch, _, dev = env
+    c, b = grown(env)
+    c.free(ints(torch, [2], dev), None, ints(torch, [40], dev))
+    b.free([2], None, [40])
+    c.fork(ints(torch, [2], dev), ints(torch, [7], dev))
+    b.fork([2], [7])
+    c.free(ints(torch, [2], dev))
+    b.free([2])
+    b.check(c)
+    assert b.table[7] == [-1, -1] + b.table[7][2:] and ops.device_error() == 0
