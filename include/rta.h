@@ -505,7 +505,8 @@ int rta_hybrid_decode_step_capture(const rta_hybrid_shape* shape, const rta_hybr
  * padded to rta_page_bytes() bytes.  The caller owns the four arrays (device memory) and may
  * fill or read them itself; the calls below keep them consistent.
  *
- * Every call is stream ordered, allocates nothing and may be captured in a HIP graph.  What
+ * Every call is stream ordered, allocates nothing and may be captured in a HIP graph; rows, and the
+ * entries of fork and free, are fewer than 2^24 a call (RTA_ERR_RANGE).  What
  * cannot be known on the host is checked on the device: a sequence or page outside its range, a
  * sequence listed twice (to be extended, forked into or freed), a length past max_pages * page,
  * or a pool with too few free pages raises RTA_DEVERR_PAGES and that entry of the list is left

@@ -73,10 +73,9 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
     if (few) return decode_cut(4 * (int64_t)n, p->kv_heads, p->head_dim, most);
     return prompt_cut((int64_t)*ntile * n * p->kv_heads, most);
 }
-// Workgroups of 256 threads in one grid dimension: below 2^32 threads.
 static bool grid_fits(const rta_pages* p, int hq, int rows, int n, int max_rows) {
-    const int64_t group = hq / p->kv_heads, most = (1 << 24) - 1, tiles = (max_rows * group + 63) / 64;
-    return rows <= most && (int64_t)rows * p->kv_heads * group <= INT_MAX &&
+    const int64_t group = hq / p->kv_heads, most = host::kMostGroups, tiles = (max_rows * group + 63) / 64;
+    return (int64_t)rows * p->kv_heads * group <= INT_MAX &&
            rows * (int64_t)decode_heads(p->kv_heads, (int)group, p->head_dim) <= most &&
            (max_rows == 1 || tiles <= most / ((int64_t)n * p->kv_heads));
 }

@@ -577,6 +577,7 @@ int rta_pages_fork(const rta_pages* pages, const int32_t* src, const int32_t* ds
     if (rc) return rc;
     if (!src || !dst) return RTA_ERR_NULL;
     if (n <= 0) return RTA_ERR_SHAPE;
+    if (n > host::kMostGroups) return RTA_ERR_RANGE;
     if (!host::aligned(src, 4) || !host::aligned(dst, 4)) return RTA_ERR_ALIGN;
     hipLaunchKernelGGL(pages_fork_kernel, dim3(n), dim3(256), 0, (hipStream_t)stream, a, src, dst, n);
     return launched();
@@ -588,6 +589,7 @@ int rta_pages_free(const rta_pages* pages, const int32_t* seqs, const int32_t* f
     const int rc = host::pages_args(pages, -1, &a);
     if (rc) return rc;
     if (n <= 0) return RTA_ERR_SHAPE;
+    if (n > host::kMostGroups) return RTA_ERR_RANGE;
     if (!host::aligned(seqs, 4) || !host::aligned(first, 4) || !host::aligned(last, 4)) return RTA_ERR_ALIGN;
     hipLaunchKernelGGL(pages_free_kernel, dim3(n), dim3(256), 0, (hipStream_t)stream, a, seqs, first, last);
     return launched();

@@ -135,8 +135,12 @@ inline int pages_args(const rta_pages* p, int layer, PageArgs* a) {
     return RTA_OK;
 }
 
+// Workgroups of 256 threads in one grid dimension: below 2^32 threads.
+constexpr int kMostGroups = (1 << 24) - 1;
+
 inline int rows_args(int rows, const int32_t* seqs, const int32_t* cu, int n, RowList* l) {
     if (rows <= 0 || n <= 0 || (!cu && rows != n)) return RTA_ERR_SHAPE;
+    if (rows > kMostGroups) return RTA_ERR_RANGE;
     if (!aligned(seqs, 4) || !aligned(cu, 4)) return RTA_ERR_ALIGN;
     *l = RowList{seqs, cu, rows, n};
     return RTA_OK;
