@@ -124,6 +124,7 @@ class PagedCache:
 
     def _entries(self, seqs, n):
         if seqs is not None:
+            self._ints(seqs, "seqs")
             return seqs.shape[0]
         return self.table.shape[0] if n is None else n
 
@@ -147,8 +148,9 @@ class PagedCache:
         """The empty sequences dst become copies of src that share their pages."""
         if src is None or dst is None:
             raise TypeError("src and dst must be tensors")
+        sp = self._ints(src, "src")
         n = src.shape[0]
-        self._call("rta_pages_fork", self._ints(src, "src", n), self._ints(dst, "dst", n), n)
+        self._call("rta_pages_fork", sp, self._ints(dst, "dst", n), n)
 
     def free(self, seqs=None, first=None, last=None, n=None):
         """Gives up the pages of seqs whose positions lie in [first, last) (None: all of them); with
@@ -178,7 +180,7 @@ class PagedCache:
     def append(self, k, v, layer=0, seqs=None, cu_rows=None):
         """Keys and values [rows, kv_heads * head_dim] fp32 (rows may be strided) of the sequences'
         newest positions into the pages of `layer`.  Call it after extend."""
-        rows = k.shape[0]
+        rows = _rows(k, "k").shape[0]
         sp, cu, n = self._list(rows, seqs, cu_rows)
         self._call("rta_paged_append", layer, *self._strided(k, "k", rows), *self._strided(v, "v", rows), rows, sp, cu,
                    n)
@@ -210,7 +212,8 @@ class PagedCache:
         they were in out, m and z, and mean nothing in tensors made here."""
         if not isinstance(q, torch.Tensor) or q.device != self.device or q.dtype != torch.float32:
             raise TypeError(f"q must be a float32 tensor on {self.device}")
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.stride(2) != 1 or q.stride(1) != self.head_dim:
+        if q.dim() != 3 or q.shape[2] != self.head_dim or q.stride(2) != 1 or \
+                (q.shape[1] > 1 and q.stride(1) != self.head_dim):
             raise ValueError(f"q must be [rows, heads, {self.head_dim}] with contiguous rows")
         rows, hq, hd = q.shape
         sp, cu, n = self._list(rows, seqs, cu_rows)

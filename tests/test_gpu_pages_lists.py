@@ -210,3 +210,30 @@ def test_holes_are_forked_and_freed(env):
     b.free([2])
     b.check(c)
     assert b.table[7] == [-1, -1] + b.table[7][2:] and ops.device_error() == 0
+
+
+# ------------------------------------------------------------------ arguments ----
+def test_queries_of_one_head_at_any_stride(env):
+    """A head's stride says nothing where there is one head."""
+    torch, _, dev = env
+    lens = [30, 70, 5]
+    c = filled(env, ref.F16, 1, 64, 16, lens)
+    fill(env, c, lens, 8)
+    q = rows_of(torch, dev, 3, 1, 64, 9)
+    turned = torch.empty(1, 3, 64, device=dev).transpose(0, 1).copy_(q)
+    assert turned.stride(1) != 64
+    got, want = c.attention(turned, max_len=70), c.attention(q, max_len=70)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and ops.device_error() == 0
+
+
+def test_lists_that_are_no_tensors(env):
+    torch, _, dev = env
+    c, _ = grown(env)
+    for call in (lambda: c.extend([1, 2]), lambda: c.free([1]), lambda: c.fork([0], ints(torch, [5], dev)),
+                 lambda: c.fork(ints(torch, [0], dev), [5]), lambda: c.attention(torch.zeros(1, 1, 64, device=dev), seqs=[0])):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: c.extend(ints(torch, [[1, 2]], dev)), lambda: c.append([1.0], [2.0])):
+        with pytest.raises(ValueError):
+            call()
+    assert c.lengths.tolist()[:4] == [20, 33, 64, 16] and ops.device_error() == 0
