@@ -14,7 +14,10 @@
 // fp32 queries and weights meet 16-bit values, so each is split into parts that are exact
 // 16-bit numbers and whose products are added in fp32:
 //   binary16 pages (and 8-bit codes, exact in binary16): two parts, 22 bits, of the value times a
-//   power of two that puts its row's largest in [2^13, 2^14);
+//   power of two that puts its row's largest at 2^13 to 2^14.  They are cut off, not rounded: the instruction
+//   that packs two of them cuts.  The second part ends at 2^-24, so values below 2^-16 of the
+//   largest have fewer bits and those below 2^-38 none: weights of N positions lose N 2^-38 of
+//   their sum at most;
 //   bfloat16 pages: three parts of 8 bits, 24 bits and no scale.
 // Where few of a product's 16 columns are needed, two parts are neighbouring columns (query g in
 // 2g and 2g + 1) and the third a second product into the same accumulator; else every part is a
@@ -271,7 +274,7 @@ __device__ __forceinline__ Visible prompt_span(const PagedAttnArgs& a, int len, 
 // 2^(ve - kSpread) every column's operands and sums have a power of two of their own (Softmax::up).
 // Relative error of a sum over 65536 positions whose scales are 2^-6, 2^-8 and 2^-12 of the largest: 1.4e-7
 // (as at 2^0), 1.7e-7, 1.9e-6.  Scales of normal values differ by less than 2^3, ve's rounding
-// included: their tiles pay for the comparison only (1 to 2.5% of a call); where every tile is spread, single
+// included: their tiles pay for the comparison only (1 to 3.5% of a call); where every tile is spread, single
 // rows of 32 sequences over 4000 positions take 74.8 us, else 72.9, a prompt of 4096 rows 406, else 339.
 constexpr int kSpread = 6;
 __device__ __forceinline__ bool far_below(float scale, int ve) {

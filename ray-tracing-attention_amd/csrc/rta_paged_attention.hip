@@ -26,7 +26,8 @@ static Cut decode_cut(int64_t rows, int heads, int hd, int64_t most) {
 // stay mostly empty (us, this / the other: 16 sequences of 4 rows over 4000 bf16 positions, 4 q
 // heads per kv head 60 / 91, 8 rows 76 / 97; one of 12 rows over 8000, in two groups 31 / 27).
 // Their workgroups start and end with more work, so fewer are asked for, as for 4 rows an entry (5
-// rows of 16 sequences over 500 to 16384 8-bit positions 73.5; as for 2, 3, 6 and 8: 81, 76, 97, 123).
+// rows of 16 sequences over 500 to 16384 8-bit positions 73.5; as for 2, 3, 6 and 8: 81, 76, 97, 123;
+// the one set of lengths and rows that this was measured on).
 static bool few_rows(int64_t max_rows, int group, int hd) { return max_rows * group <= (hd == 256 ? 16 : 32); }
 // With several rows: column tiles enough for two workgroups per compute unit stand alone, fewer
 // are cut into chunks of positions (a multiple of 64, 256 at least).
@@ -146,7 +147,7 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
             a.mz = reinterpret_cast<float2*>(a.part + (size_t)rows * hq * cut.nchunk * HD);
             a.ntile = ntile;
             if (ntile && few_rows(max_rows, a.group, HD)) {   // one group of columns
-                                const dim3 grid(n * pages->kv_heads, 1, cut.nchunk), block(64 * kDecWaves);
+                const dim3 grid(n * pages->kv_heads, 1, cut.nchunk), block(64 * kDecWaves);
                 if (few_cols(max_rows * a.group) == 16) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1, true>), grid, block, 0, s, a);
                 else if constexpr (HD < 256) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2, true>), grid, block, 0, s, a);
             } else if (ntile) {

@@ -207,7 +207,8 @@ class PagedCache:
         their sequences' pages; with window > 0 a row sees its last `window` positions and the
         first `sinks`.  Returns (out [rows, hq, head_dim], m [rows, hq], z [rows, hq]).
 
-        max_rows: the most rows of an entry (None: one without cu_rows, else all of them);
+        max_rows: the most rows of an entry (None: one without cu_rows, else all of them), which
+        decides the kernel for all entries: prompts and single rows are faster in calls of their own;
         max_len: the longest sequence (0: max_pages * page).  Rows that no entry lists are left as
         they were in out, m and z, and mean nothing in tensors made here."""
         if not isinstance(q, torch.Tensor) or q.device != self.device or q.dtype != torch.float32:
