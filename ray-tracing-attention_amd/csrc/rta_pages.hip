@@ -416,13 +416,11 @@ __device__ __forceinline__ uint8_t* row_page(const PageArgs& a, const RowList& l
 
 // A workgroup per row and 2048 of its 2 kv_heads hd values: 8 values a thread.
 template <int FMT, int HD>
-__global__ void __launch_bounds__(256) append_kernel(const PageArgs a, const RowList l, const float* __restrict__ k,
-                                                     int64_t k_stride, const float* __restrict__ v,
-                                                     int64_t v_stride) {
+__device__ __forceinline__ void append_row(const PageArgs& a, const RowList& l, const float* __restrict__ k,
+                                           int64_t k_stride, const float* __restrict__ v, int64_t v_stride) {
     const int r = blockIdx.x;
     int off = 0;
     bool listed;
-    if (r == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
     uint8_t* page = row_page(a, l, r, off, listed);
     if (!page) {
         if (listed && threadIdx.x == 0 && blockIdx.y == 0) raise_error(RTA_DEVERR_PAGES);
@@ -472,12 +470,19 @@ __global__ void __launch_bounds__(256) append_kernel(const PageArgs a, const Row
 }
 
 template <int FMT, int HD>
-__global__ void __launch_bounds__(256) page_read_kernel(const PageArgs a, const RowList l, float* __restrict__ k,
-                                                        int64_t k_stride, float* __restrict__ v, int64_t v_stride) {
+__global__ void __launch_bounds__(256) append_kernel(const PageArgs a, const RowList l, const float* __restrict__ k,
+                                                     int64_t k_stride, const float* __restrict__ v,
+                                                     int64_t v_stride) {
+    append_row<FMT, HD>(a, l, k, k_stride, v, v_stride);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
+}
+
+template <int FMT, int HD>
+__device__ __forceinline__ void read_row(const PageArgs& a, const RowList& l, float* __restrict__ k, int64_t k_stride,
+                                         float* __restrict__ v, int64_t v_stride) {
     const int r = blockIdx.x;
     int off = 0;
     bool listed;
-    if (r == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
     const uint8_t* page = row_page(a, l, r, off, listed);
     if (!listed) return;
     if (!page && threadIdx.x == 0 && blockIdx.y == 0) raise_error(RTA_DEVERR_PAGES);
@@ -508,6 +513,13 @@ __global__ void __launch_bounds__(256) page_read_kernel(const PageArgs a, const 
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = f[j];
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(256) page_read_kernel(const PageArgs a, const RowList l, float* __restrict__ k,
+                                                        int64_t k_stride, float* __restrict__ v, int64_t v_stride) {
+    read_row<FMT, HD>(a, l, k, k_stride, v, v_stride);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
 }
 
 // f(std::integral_constant<int, FMT>, std::integral_constant<int, HD>) of a checked descriptor.
