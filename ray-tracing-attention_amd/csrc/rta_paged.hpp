@@ -14,8 +14,8 @@
 // fp32 queries and weights meet 16-bit values, so each is split into parts that are exact
 // 16-bit numbers and whose products are added in fp32:
 //   binary16 pages (and 8-bit codes, exact in binary16): two parts, 22 bits, of the value times a
-//   power of two that puts its row's largest at 2^13 to 2^14.  They are cut off, not rounded: the instruction
-//   that packs two of them cuts.  The second part ends at 2^-24, so values below 2^-16 of the
+//   power of two that puts its row's largest at 2^13 to 2^14.  Weights are cut off, not rounded: the instruction
+//   that packs two of them cuts (queries, outside the loops, have their second part rounded).  The second part ends at 2^-24, so values below 2^-16 of the
 //   largest have fewer bits and those below 2^-38 none: weights of N positions lose N 2^-38 of
 //   their sum at most;
 //   bfloat16 pages: three parts of 8 bits, 24 bits and no scale.
@@ -171,25 +171,32 @@ __device__ __forceinline__ float cut(float v, uint32_t mask) {
     return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & mask);
 }
 
+// Two floats as binary16, cut off or rounded to the nearest.
+template <bool NEAREST>
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    if constexpr (NEAREST) return __builtin_bit_cast(uint32_t, h2v_t{(_Float16)lo, (_Float16)hi});
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+}
+
 // Part `part` (0, 1) of eight values as B operands (op 1, of bfloat16 only: the third part in
 // part 0's columns).  Parts are cut off, not rounded, so that each remainder is exact; a value
 // that is not finite stays so.
-template <int FMT>
+template <int FMT, bool NEAREST = false>
 __device__ __forceinline__ void split_parts(const float v[8], int part, u4_t op[PageFmt<FMT>::kOps]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float x[2], y[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float w = v[2 * j + e], r = w - cut(w, FMT == RTA_BF16 ? 0xffff0000u : 0xffffe000u);
-            x[e] = part ? r : w;
+            const float w = v[2 * j + e], top = cut(w, FMT == RTA_BF16 ? 0xffff0000u : 0xffffe000u), r = w - top;
+            x[e] = part ? r : NEAREST ? top : w;
             if constexpr (FMT == RTA_BF16) y[e] = part ? 0.0f : r - cut(r, 0xffff0000u);
         }
         if constexpr (FMT == RTA_BF16) {
             op[0][j] = upper_halves(x[0], x[1]);
             op[1][j] = upper_halves(y[0], y[1]);
         } else {
-            op[0][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
+            op[0][j] = pack_half<NEAREST>(x[0], x[1]);
         }
     }
 }
@@ -282,7 +289,7 @@ __device__ __forceinline__ bool far_below(float scale, int ve) {
 }
 
 // All parts of eight values as operands.
-template <int FMT>
+template <int FMT, bool NEAREST = false>
 __device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -298,8 +305,7 @@ __device__ __forceinline__ void split_all(const float v[8], u4_t* op) {
             asm("" : "+s"(minus));
             const h2v_t hi = __builtin_bit_cast(h2v_t, __builtin_amdgcn_cvt_pkrtz(a, b));
             op[0][j] = __builtin_bit_cast(uint32_t, hi);
-            op[1][j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], minus, a),
-                                                                               fmaf((float)hi[1], minus, b)));
+            op[1][j] = pack_half<NEAREST>(fmaf((float)hi[0], minus, a), fmaf((float)hi[1], minus, b));
         }
     }
 }

@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
 #pragma unroll
             for (int s = 0; s < 8; ++s) v[s] = q[operand_dim<FMT>(kb, u) + s] * sg;
             u4_t op[kOps];
-            if constexpr (MULTI) split_all<FMT>(v, op);
-            else split_parts<FMT>(v, part, op);
+            if constexpr (MULTI) split_all<FMT, true>(v, op);
+            else split_parts<FMT, true>(v, part, op);
 #pragma unroll
             for (int o = 0; o < kOps; ++o)
                 *reinterpret_cast<u4_t*>(lds + (((c * kOps + o) * kKb + kb) * 64 + lane) * 16) = op[o];

@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[kb][e] *= sg;
             u4_t part[kParts];
-            split_all<FMT>(v[kb], part);
+            split_all<FMT, true>(v[kb], part);
             qb[c][kb][0] = part[0];
             qb[c][kb][1] = part[1];
             if constexpr (kParts == 3) third[(c * kKb + kb) * 64] = part[2];
