@@ -3,9 +3,9 @@
 // Bound by the matrix cores and, beside them, by vector instructions: 4 hq HD operations per
 // (row, position), twice that with q and the weights in two binary16 parts, three times in three
 // bfloat16 parts (rta_paged.hpp), and about 200 vector instructions per 32 x 32 scores, of which
-// two waves of a SIMD hide some.  4096 rows of 32 heads over 4096 bf16 positions: 348 us, three
-// parts at the rate of a large library product 350; the matrix cores are busy 45% of it (two
-// binary16 parts: 37%).
+// two waves of a SIMD hide some.  4096 rows of 32 heads over 4096 bf16 positions: 348 to 360 us, three
+// parts at the rate of a large library product 350; the matrix cores are busy 45% of it (binary16
+// pages 311 to 320 us, 38%; 8-bit ones 345 to 351, 32%).
 // The columns of a kv head's products are its (row, q head) pairs, so the heads that share keys
 // share their loads and no group size leaves columns empty.  A workgroup of 4 waves takes 128 (wide
 // heads: 64) columns and the positions that any of them sees, in tiles staged in LDS by all of it
