@@ -600,7 +600,8 @@ int rta_paged_read(const rta_pages* pages, int layer, int rows, const int32_t* s
  * sequence's length is never used.
  * Sums are fp32.  Queries and weights meet the pages' values in parts: over RTA_F16 and RTA_Q8_ROW
  * they count to 2^-38 of the largest of their row and head (22 bits of those above 2^-16), over
- * RTA_BF16 24 bits each.
+ * RTA_BF16 24 bits each.  Finite values give finite results up to 2^20 positions of about the same
+ * weight at the end of fp32; values below 2^-100 lose bits.
  * Workspace: rta_paged_attention_workspace_bytes() bytes, 16-byte aligned (0: none needed). */
 size_t rta_paged_attention_workspace_bytes(const rta_pages* pages, int hq, int rows, int n, int max_rows,
                                            int max_len, int window, int sinks);

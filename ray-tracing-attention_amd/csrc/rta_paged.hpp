@@ -14,10 +14,10 @@
 // fp32 queries and weights meet 16-bit values, so each is split into parts that are exact
 // 16-bit numbers and whose products are added in fp32:
 //   binary16 pages (and 8-bit codes, exact in binary16): two parts, 22 bits, of the value times a
-//   power of two that puts its row's largest at 2^13 to 2^14.  Weights are cut off, not rounded: the instruction
-//   that packs two of them cuts (queries, outside the loops, have their second part rounded).  The second part ends at 2^-24, so values below 2^-16 of the
-//   largest have fewer bits and those below 2^-38 none: weights of N positions lose N 2^-38 of
-//   their sum at most;
+//   power of two that puts its row's largest at 2^13 to 2^14.  Weights are cut off, not rounded:
+//   the instruction that packs two of them cuts (queries, outside the loops, have their second part
+//   rounded).  The second part ends at 2^-24, so values below 2^-16 of the largest have fewer
+//   bits and those below 2^-38 none: weights of N positions lose N 2^-38 of their sum at most;
 //   bfloat16 pages: three parts of 8 bits, 24 bits and no scale.
 // Where few of a product's 16 columns are needed, two parts are neighbouring columns (query g in
 // 2g and 2g + 1) and the third a second product into the same accumulator; else every part is a
@@ -93,8 +93,9 @@ __device__ __forceinline__ bool resolve_row(const PagedAttnArgs& a, int r, const
 typedef f4_t f4u_t __attribute__((aligned(4)));   // at an address of a multiple of 4
 
 // Sums of weights leave the kernels' loops 2^-kRoom times what they are against the maximum (weight 2^-kRoom
-// for the largest score): a mean of finite values is finite, and their plain sum need not be.
-constexpr int kRoom = 24;
+// for the largest score): a mean of finite values is finite, and their plain sum need not be.  20: 2^20 positions of
+// the same weight with values at fp32's end, and values down to 2^-100 whose sums are normal numbers.
+constexpr int kRoom = 20;
 // The final values of (row, q head) at dims c .. c + 3 from U and Z (both 2^-kRoom times) and M (natural units).
 __device__ __forceinline__ void write_result(const PagedAttnArgs& a, int64_t at, int hd, int c, f4_t u, float m,
                                              float z, uint32_t& err) {
@@ -343,7 +344,7 @@ __device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Vi
 // is rounded once, however large both are), so the sums are not rescaled for every small step, and binary16 parts do not overflow.
 // kTop is as high as that allows: the second part ends at 2^-24, and over a long history most of
 // the sum lies in weights far below the largest.  bfloat16 parts have fp32's exponents, and values may too:
-// there the largest weight is 2^-kRoom from the start; sums of values down to 2^-100 stay normal numbers.
+// there the largest weight is 2^-kRoom from the start.
 template <int NC, int N, int FMT>
 struct Softmax {
     static constexpr float kTop = FMT == RTA_BF16 ? -kRoom : 14, kSlack = 1.0f;

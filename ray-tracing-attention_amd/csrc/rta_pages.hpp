@@ -72,7 +72,8 @@ __device__ __forceinline__ bool row_entry(const RowList& l, int r, int& i, int& 
 __device__ __forceinline__ bool bad_rows(const RowList& l) {
     bool bad = false;
     int first, count;
-    for (int i = threadIdx.x; l.cu && i < l.n; i += blockDim.x) bad = bad || !entry_rows(l, i, first, count);
+#pragma unroll 4
+    for (int i = threadIdx.x; l.cu && i < l.n; i += blockDim.x) bad |= !entry_rows(l, i, first, count);
     return bad;
 }
 

@@ -219,3 +219,17 @@ def test_scores_of_any_finite_size(env, fmt, hd, rows, size):
             assert np.abs(out[r, h] - v[a, 0]).max() <= 2.0**-20 * np.abs(v[a, 0]).max(), (r, h)
             assert abs(m[r, h] - s[a]) <= hd**0.5 * 2.0**-22 * most and abs(z[r, h] - 1) <= 2.0**-20, (r, h, z[r, h])
     assert told >= rows
+
+
+# ------------------------------------------------------------------ small values ----
+@pytest.mark.parametrize("fmt", [ref.BF16, ref.Q8_ROW])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 5, 40])
+@pytest.mark.parametrize("size", [1e-20, 2.0**-98])
+def test_values_near_zero(env, fmt, hd, rows, size):
+    length = 700
+    k, v = normal(env, 27, length, hd), size * normal(env, 28, length, hd)
+    c = holding(env, fmt, 1, hd, 64, k, v)
+    q = rows_of(env[0], env[2], rows, 4, hd, 29)
+    check_terms(c, q, newest(env, c, q))
+    assert ops.device_error() == 0
