@@ -338,13 +338,14 @@ __device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Vi
 }
 
 // The online softmax of NC column tiles, a lane holding 4N positions of its column of each, N = 2
-// (16 columns) or 4 (32 columns) (products x; score = x fac in log2 units).  Weights are 2^(score - low), 2^kTop for the largest
-// score when low was set; low follows the maximum only when weights would pass 2^(kTop + kSlack),
-// 2^15 for binary16 parts (fac is a power of two: a score is its product exactly, and its distance from low
-// is rounded once, however large both are), so the sums are not rescaled for every small step, and binary16 parts do not overflow.
-// kTop is as high as that allows: the second part ends at 2^-24, and over a long history most of
-// the sum lies in weights far below the largest.  bfloat16 parts have fp32's exponents, and values may too:
-// there the largest weight is 2^-kRoom from the start.
+// (16 columns) or 4 (32 columns) (products x; score = x fac in log2 units, fac a power of two: so a
+// score is its product exactly, and its distance from low is rounded once, however large both are).
+// Weights are 2^(score - low), 2^kTop for the largest score when low was set; low follows the
+// maximum only when weights would pass 2^(kTop + kSlack), 2^15 for binary16 parts, so the sums are
+// not rescaled for every small step, and binary16 parts do not overflow.  kTop is as high as that
+// allows: the second part ends at 2^-24, and over a long history most of the sum lies in weights far
+// below the largest.  bfloat16 parts have fp32's exponents, and values may too: there the largest
+// weight is 2^-kRoom from the start.
 template <int NC, int N, int FMT>
 struct Softmax {
     static constexpr float kTop = FMT == RTA_BF16 ? -kRoom : 14, kSlack = 1.0f;
