@@ -47,7 +47,8 @@ enum rta_status {
  * accepts RTA_Q4_K | RTA_TILED and RTA_Q6_K | RTA_TILED and then runs on the matrix
  * cores at every batch size. */
 enum rta_format { RTA_F32 = 0, RTA_F16 = 1, RTA_Q4_K = 12, RTA_Q6_K = 14, RTA_BF16 = 30, RTA_TILED = 0x100,
-                  RTA_Q8_ROW = 0x200 /* pages only: int8 codes, one fp32 scale per position and kv head */ };
+                  RTA_Q8_ROW = 0x200, /* pages only: int8 codes, one fp32 scale per position and kv head */
+                  RTA_Q4_GROUP = 0x400 /* pages only: 4-bit codes, a scale and a zero point per 32 dims */ };
 
 /* Epilogue of a projection: y = W x, or y += W x (the residual add of the O and
  * down projections, resident_math.comp:70). */
@@ -502,6 +503,11 @@ int rta_hybrid_decode_step_capture(const rta_hybrid_shape* shape, const rta_hybr
  * counts the sequences that name a page; pages with refs 0 are free.  One page of one layer is
  *   elements [key, value][kv_heads][page][head_dim]  (RTA_F16, RTA_BF16, or int8 codes)
  *   RTA_Q8_ROW: then fp32 scales [key, value][kv_heads][page]; a value is code * scale
+ *   RTA_Q4_GROUP: [key, value][kv_heads][page] rows of head_dim / 2 bytes of codes, then as many rows of
+ *     head_dim / 32 16-bit words, one per 32 dims: its upper 11 bits are a binary16 scale (sign, exponent, five
+ *     bits of fraction; the other bits 0), its last four the zero point; a value is scale * (code - zero), exactly.
+ *     A row's blocks of 128 dims (head_dim 64: one of 64) have G = 4 (2) groups of 32; dword u G + g of a
+ *     block holds dims 32 g + 8 u .. + 7 of it, dim 2 j + b of these in bits 16 b + 4 j .. + 3
  * padded to rta_page_bytes() bytes.  The caller owns the four arrays (device memory) and may
  * fill or read them itself; the calls below keep them consistent.
  *
@@ -512,7 +518,7 @@ int rta_hybrid_decode_step_capture(const rta_hybrid_shape* shape, const rta_hybr
  * or a pool with too few free pages raises RTA_DEVERR_PAGES and that entry of the list is left
  * undone. */
 typedef struct rta_pages {
-    int fmt;               /* RTA_F16, RTA_BF16 or RTA_Q8_ROW */
+    int fmt;               /* RTA_F16, RTA_BF16, RTA_Q8_ROW or RTA_Q4_GROUP */
     int kv_heads;          /* 1 .. 1024 */
     int head_dim;          /* 64, 128 or 256 */
     int page;              /* positions per page, 1 .. 65536 */
@@ -570,7 +576,10 @@ int rta_pages_compact(const rta_pages* pages, int32_t* used, void* workspace, si
 /* The rows' keys and values k[r, :kv_heads * head_dim], v (fp32, row strides in floats) into
  * the pages of layer `layer`: rounded to nearest even, or for RTA_Q8_ROW scale = max|x| * (1 / 127)
  * over the head (fp32) and code = round(x / scale) (a head with a value that is not finite reads back
- * as NaN).  A page named by several sequences is written for all of them (rta_pages_extend has
+ * as NaN).  For RTA_Q4_GROUP, in fp32 over the group's 32 dims with lo = min(0, min x), hi = max(0, max x):
+ * scale = (hi - lo) * (1 / 15) rounded up to six significant bits and to a multiple of 2^-19, zero =
+ * round(-lo / scale), code = round(x / scale) + zero held to 0 .. 15 (a group with a value that is not finite,
+ * or with a range (hi - lo) * (1 / 15) above 2112, reads back as NaN).  A page named by several sequences is written for all of them (rta_pages_extend has
  * made the last one the sequence's own), and of a sequence listed twice either entry's values
  * may stay.  Call it after rta_pages_extend. */
 int rta_paged_append(const rta_pages* pages, int layer, const float* k, int64_t k_stride, const float* v,
@@ -598,8 +607,8 @@ int rta_paged_read(const rta_pages* pages, int layer, int rows, const int32_t* s
  * score is not finite, or a result that is not, raises RTA_DEVERR_DETECTOR (that row's values
  * then mean nothing; rows that do not see the position keep theirs).  What lies in a page past its
  * sequence's length is never used.
- * Sums are fp32.  Queries and weights meet the pages' values in parts: over RTA_F16 and RTA_Q8_ROW
- * they count to 2^-38 of the largest of their row and head (22 bits of those above 2^-16), over
+ * Sums are fp32.  Queries and weights meet the pages' values in parts: over RTA_F16, RTA_Q8_ROW and
+ * RTA_Q4_GROUP (whose scales a caller that fills pages keeps to 2112) they count to 2^-38 of the largest of their row and head (22 bits of those above 2^-16), over
  * RTA_BF16 24 bits each.  Finite values give finite results up to 2^20 positions of about the same
  * weight at the end of fp32; values below 2^-100 lose bits.
  * Workspace: rta_paged_attention_workspace_bytes() bytes, 16-byte aligned (0: none needed). */

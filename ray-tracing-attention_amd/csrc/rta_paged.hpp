@@ -31,6 +31,7 @@
 namespace rta {
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef float acc16_t __attribute__((ext_vector_type(16)));
 
@@ -120,17 +121,21 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // ---- operands by page format ----
 template <int FMT> struct PageFmt;
 template <> struct PageFmt<RTA_F16> {
-    // element bytes; parts of a query or weight; products of a pair of operands with parts in columns
-    static constexpr int kBytes = 2, kParts = 2, kOps = 1;
+    // parts of a query or weight; products of a pair of operands with parts in columns
+    static constexpr int kParts = 2, kOps = 1;
     static constexpr bool kScaled = false;       // scales beside the elements
 };
 template <> struct PageFmt<RTA_BF16> {
-    static constexpr int kBytes = 2, kParts = 3, kOps = 2;
+    static constexpr int kParts = 3, kOps = 2;
     static constexpr bool kScaled = false;
 };
 template <> struct PageFmt<RTA_Q8_ROW> {
-    static constexpr int kBytes = 1, kParts = 2, kOps = 1;
+    static constexpr int kParts = 2, kOps = 1;
     static constexpr bool kScaled = true;
+};
+template <> struct PageFmt<RTA_Q4_GROUP> {
+    static constexpr int kParts = 2, kOps = 1;
+    static constexpr bool kScaled = false;       // the values are binary16 numbers (q4_to_half)
 };
 
 template <int FMT>
@@ -162,6 +167,32 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
     const h2v_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
     lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2v_t, __builtin_amdgcn_perm(x, 0x64646464u, 0x00050004u)) + off);
     hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2v_t, __builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u)) + off);
+}
+
+// The eight values of a dword of RTA_Q4_GROUP from its group's word (in the lower half), as binary16 in
+// order of their dims: the codes as the upper bits of a fraction under 16's exponent are 16 + c, and
+// scale (16 + c) - scale (16 + zero), one fma, is exact.
+struct Q4Word {
+    h2v_t scale, off;
+    __device__ __forceinline__ explicit Q4Word(uint32_t word) {
+        const uint32_t s = word & kQ4Scale, z = (word & 15u) << 6 | 0x4c00u;
+        scale = __builtin_bit_cast(h2v_t, s | s << 16);
+        off = -scale * __builtin_bit_cast(h2v_t, z | z << 16);
+    }
+};
+__device__ __forceinline__ u4_t q4_to_half(uint32_t w, const Q4Word& g) {
+    u4_t r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t x = j == 0 ? w << 6 : j == 1 ? w << 2 : j == 2 ? w >> 2 : w >> 6;
+        r[j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(h2v_t, (x & 0x03c003c0u) | 0x4c004c00u),
+                                                                      g.scale, g.off));
+    }
+    return r;
+}
+// Whether either of two words stands for values that are not finite.
+__device__ __forceinline__ bool q4_not_finite(uint32_t words) {
+    return (((words & 0x7c007c00u) + 0x04000400u) & 0x80008000u) != 0;
 }
 
 // The upper halves of two floats as one dword: bfloat16 cut off, not rounded.

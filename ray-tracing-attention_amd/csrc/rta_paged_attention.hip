@@ -167,7 +167,8 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
     };
     if (pages->fmt == RTA_F16) launch(std::integral_constant<int, RTA_F16>{});
     else if (pages->fmt == RTA_BF16) launch(std::integral_constant<int, RTA_BF16>{});
-    else launch(std::integral_constant<int, RTA_Q8_ROW>{});
+    else if (pages->fmt == RTA_Q8_ROW) launch(std::integral_constant<int, RTA_Q8_ROW>{});
+    else launch(std::integral_constant<int, RTA_Q4_GROUP>{});
     return hipGetLastError() == hipSuccess ? RTA_OK : RTA_ERR_LAUNCH;
 }
 

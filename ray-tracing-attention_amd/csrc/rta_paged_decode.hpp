@@ -41,9 +41,13 @@ struct DecLds {
 template <int FMT, int HD, int NC, bool MULTI>
 __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::kPerSimd)) paged_decode_kernel(const PagedAttnArgs a) {
     using L = DecLds<FMT, HD, NC, MULTI>;
-    constexpr int kOps = L::kOps, kB = PageFmt<FMT>::kBytes, kPer = L::kPer;
+    constexpr int kOps = L::kOps, kPer = L::kPer;
+    constexpr int kRow = page_row_bytes(FMT, HD), kScaleRow = page_scale_bytes(FMT, HD);
+    constexpr bool kQ4 = FMT == RTA_Q4_GROUP;
     constexpr int kKb = HD / 32;                // products per 16 positions
-    constexpr int kLoads = HD * kB / 64;        // 16-byte pieces per lane and row
+    constexpr int kPiece = kRow < 64 ? kRow / 4 : 16;    // bytes that a lane loads at once
+    constexpr int kLoads = kRow / (4 * kPiece);          // pieces per lane and row
+    constexpr int kWords = HD / 64;             // pairs of RTA_Q4_GROUP's words of a row
     constexpr int kDt = HD / 16;                // dim tiles of O^T
     constexpr bool kScaled = PageFmt<FMT>::kScaled;
     __shared__ __align__(16) uint8_t lds[L::kTotal];
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     uint8_t* vl = lds + L::kQ + wave * L::kWave;
     float* sl = reinterpret_cast<float*>(vl + L::kV);
     const int64_t plane = (int64_t)a.p.kv_heads * a.p.page;   // rows of a page's keys
-    const int64_t v_off = plane * HD * kB, head_row = (int64_t)kvh * a.p.page, head_off = head_row * HD * kB;
+    const int64_t v_off = plane * kRow, head_row = (int64_t)kvh * a.p.page, head_off = head_row * kRow;
     const int ntile = (end - begin + kDecTile - 1) / kDecTile;
 
     f4_t o[NC][kDt];
@@ -126,11 +130,13 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             s.page[h] = table[e];
         }
     };
-    u4_t k[2][kLoads], v[2][kLoads];
+    using Piece = std::conditional_t<kPiece == 16, u4_t, u2_t>;
+    Piece k[2][kLoads], v[2][kLoads];
     float ks[2], vs[2];
+    uint32_t kw[2][kWords], vw[2][kWords];
     uint32_t live = 0;   // positions of the tile in k that count
     const uint8_t* row[2];
-    const float* srow[2];
+    const uint8_t* srow[2];
     auto aim = [&](int t, const Spot& s) {   // where tile t's rows are, and which count
         uint32_t ok[2];
 #pragma unroll
@@ -139,8 +145,8 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             const bool in = begin + t * kDecTile + 16 * h + i < end;
             if (in && !have) err |= RTA_DEVERR_PAGES;
             const uint8_t* page = a.p.pool + page_offset(a.p, have ? s.page[h] : 0);
-            row[h] = page + head_off + (uint32_t)(s.off[h] * (HD * kB) + 16 * u);
-            srow[h] = reinterpret_cast<const float*>(page + 2 * v_off) + head_row + s.off[h];
+            row[h] = page + head_off + (uint32_t)(s.off[h] * kRow + kPiece * u);
+            srow[h] = page + 2 * v_off + (head_row + s.off[h]) * kScaleRow;
             ok[h] = (uint32_t)__builtin_amdgcn_ballot_w64(in && have) & 0xffffu;
         }
         live = ok[0] | ok[1] << 16;
@@ -149,10 +155,17 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int x = 0; x < kLoads; ++x) k[h][x] = *reinterpret_cast<const u4_t*>(row[h] + 64 * x);
+            for (int x = 0; x < kLoads; ++x) k[h][x] = *reinterpret_cast<const Piece*>(row[h] + 4 * kPiece * x);
             if constexpr (kScaled) {
-                ks[h] = *srow[h];
-                vs[h] = srow[h][plane];
+                ks[h] = *reinterpret_cast<const float*>(srow[h]);
+                vs[h] = *reinterpret_cast<const float*>(srow[h] + plane * kScaleRow);
+            }
+            if constexpr (kQ4) {
+#pragma unroll
+                for (int x = 0; x < kWords; ++x) {
+                    kw[h][x] = reinterpret_cast<const uint32_t*>(srow[h])[x];
+                    vw[h][x] = reinterpret_cast<const uint32_t*>(srow[h] + plane * kScaleRow)[x];
+                }
             }
         }
     };
@@ -160,7 +173,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < kLoads; ++x) v[h][x] = *reinterpret_cast<const u4_t*>(row[h] + v_off + 64 * x);
+            for (int x = 0; x < kLoads; ++x) v[h][x] = *reinterpret_cast<const Piece*>(row[h] + v_off + 4 * kPiece * x);
     };
 
     // the first tile's rows are on their way while q is prepared
@@ -237,6 +250,8 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                     codes_to_half(k[h][x][b], w[0], w[1]);
                     codes_to_half(k[h][x][b + 1], w[2], w[3]);
                     ka[h] = u4_t{w[0], w[1], w[2], w[3]};
+                } else if constexpr (kQ4) {   // dword kb of a piece: dims 32 kb + 8 u ..
+                    ka[h] = q4_to_half(k[h][kb >> 2][kb & 3], Q4Word(kw[h][kb >> 1] >> (16 * (kb & 1))));
                 } else {
                     ka[h] = k[h][kb];
                 }
@@ -280,6 +295,13 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                     hit = !(fabsf(sl[32 + 16 * h + i]) < INFINITY);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) vf[h][e] = fabsf(vf[h][e]) < INFINITY ? vf[h][e] : 0.0f;
+                } else if constexpr (kQ4) {
+#pragma unroll
+                    for (int x = 0; x < kWords; ++x)
+                        if (q4_not_finite(vw[h][x])) {   // (a scale of 0: zeros)
+                            vw[h][x] = 0;
+                            hit = true;
+                        }
                 } else {
 #pragma unroll
                     for (int x = 0; x < kLoads; ++x)
@@ -300,22 +322,32 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             if (now != 0xffffffffu) {   // uniform: the last tile, or one with a page missing
                 const bool on = (now >> (16 * h + i)) & 1u;
 #pragma unroll
-                for (int x = 0; x < kLoads; ++x) v[h][x] = on ? v[h][x] : u4_t{0, 0, 0, 0};
+                for (int x = 0; x < (kQ4 ? 0 : kLoads); ++x) v[h][x] = on ? v[h][x] : (Piece)(0u);
+                if constexpr (kQ4) {   // a scale of 0
+#pragma unroll
+                    for (int x = 0; x < kWords; ++x) vw[h][x] = on ? vw[h][x] : 0u;
+                }
                 if constexpr (kScaled) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) vf[h][e] = (now >> (16 * h + 4 * u + e)) & 1u ? vf[h][e] : 0.0f;
                 }
             }
             uint8_t* dst = vl + (16 * h + i) * L::kPitch;
+            if constexpr (kQ4) {
 #pragma unroll
-            for (int x = 0; x < kLoads; ++x) {
+                for (int x = 0; x < kKb; ++x)
+                    *reinterpret_cast<u4_t*>(dst + 64 * x + 16 * u) =
+                        q4_to_half(v[h][x >> 2][x & 3], Q4Word(vw[h][x >> 1] >> (16 * (x & 1))));
+            }
+#pragma unroll
+            for (int x = 0; x < (kQ4 ? 0 : kLoads); ++x) {
                 if constexpr (FMT == RTA_Q8_ROW) {
                     uint32_t w[8];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) codes_to_half(v[h][x][y], w[2 * y], w[2 * y + 1]);
                     *reinterpret_cast<u4_t*>(dst + 128 * x + 32 * u) = u4_t{w[0], w[1], w[2], w[3]};
                     *reinterpret_cast<u4_t*>(dst + 128 * x + 32 * u + 16) = u4_t{w[4], w[5], w[6], w[7]};
-                } else {
+                } else if constexpr (!kQ4) {
                     *reinterpret_cast<u4_t*>(dst + 64 * x + 16 * u) = v[h][x];
                 }
             }

@@ -41,7 +41,8 @@ struct PromptLds {
 template <int FMT, int HD>
 __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 1 : 2)) paged_prompt_kernel(const PagedAttnArgs a) {
     using L = PromptLds<FMT, HD>;
-    constexpr int kParts = PageFmt<FMT>::kParts, kB = PageFmt<FMT>::kBytes;
+    constexpr int kParts = PageFmt<FMT>::kParts, kRow = page_row_bytes(FMT, HD);
+    constexpr bool kQ4 = FMT == RTA_Q4_GROUP;
     // products: kDims dims of kWide positions, kH of them for 32 positions, then kWide dims of
     // 32 / kP positions; kKg and kDg of them have their operands read ahead
     constexpr int W = L::kWide, NQ = L::kNQ, kDims = 512 / W, kH = 32 / W, kP = W / 16, N = W / 8;
@@ -49,7 +50,9 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     constexpr int kDg = kDt < 4 ? kDt : 4, kDn = kP * kDt / kDg;   // V^T: kDn groups of kDg operands
     using Acc = std::conditional_t<W == 32, acc16_t, f4_t>;
     constexpr int kQuads = sizeof(Acc) / 16;
-    constexpr int kPieces = HD * kB / 16, kStep = 256 / kPieces, kPass = L::kTile / kStep;
+    // (RTA_Q4_GROUP: a dword, which becomes 16 bytes, so as many threads a row as with 2-byte elements)
+    using Piece = std::conditional_t<kQ4, uint32_t, u4_t>;
+    constexpr int kPieces = kRow / (int)sizeof(Piece), kStep = 256 / kPieces, kPass = L::kTile / kStep;
     constexpr bool kScaled = PageFmt<FMT>::kScaled;
     __shared__ __align__(16) uint8_t lds[L::kTotal];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & (W - 1), u = lane / W;
@@ -81,9 +84,10 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
     const int nt = (end - begin + L::kTile - 1) / L::kTile;
 
     // staging: thread -> piece of a row; its rows of a tile are kStep apart
-    const int64_t plane = (int64_t)hkv * a.p.page, v_off = plane * HD * kB;
-    const int64_t head_row = (int64_t)kvh * a.p.page, head_off = head_row * HD * kB;
+    const int64_t plane = (int64_t)hkv * a.p.page, v_off = plane * kRow;
+    const int64_t head_row = (int64_t)kvh * a.p.page, head_off = head_row * kRow;
     const int piece = tid % kPieces, row0 = tid / kPieces;
+    const int dim = q4_dim(HD, piece);   // RTA_Q4_GROUP: the piece's first dim
     struct Spot {
         int page[kPass], off[kPass];
     };
@@ -96,8 +100,9 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
             sp.page[k] = table[e];
         }
     };
-    u4_t kr[kPass], vr[kPass];
+    Piece kr[kPass], vr[kPass];
     float ksr[kPass], vsr[kPass];
+    uint32_t kw[kPass], vw[kPass];
     uint32_t okr = 0;
     auto load = [&](int t, const Spot& sp) {
         okr = 0;
@@ -108,9 +113,14 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
             if (in && !have) err |= RTA_DEVERR_PAGES;
             if (in && have) okr |= 1u << k;
             const uint8_t* page = a.p.pool + page_offset(a.p, have ? sp.page[k] : 0);
-            const uint8_t* src = page + head_off + (uint32_t)(sp.off[k] * (HD * kB) + 16 * piece);
-            kr[k] = *reinterpret_cast<const u4_t*>(src);
-            vr[k] = *reinterpret_cast<const u4_t*>(src + v_off);
+            const uint8_t* src = page + head_off + (uint32_t)(sp.off[k] * kRow + (int)sizeof(Piece) * piece);
+            kr[k] = *reinterpret_cast<const Piece*>(src);
+            vr[k] = *reinterpret_cast<const Piece*>(src + v_off);
+            if constexpr (kQ4) {
+                const uint16_t* w = reinterpret_cast<const uint16_t*>(page + 2 * v_off) + (head_row + sp.off[k]) * (HD / 32) + (dim >> 5);
+                kw[k] = w[0];
+                vw[k] = w[plane * (HD / 32)];
+            }
             if constexpr (kScaled) {
                 const float* f = reinterpret_cast<const float*>(page + 2 * v_off) + head_row + sp.off[k];
                 ksr[k] = f[0];
@@ -118,8 +128,10 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
             }
         }
     };
-    auto put = [&](uint8_t* dst, u4_t x) {   // one piece as 2-byte elements
-        if constexpr (FMT == RTA_Q8_ROW) {
+    auto put = [&](uint8_t* dst, Piece x, uint32_t word) {   // one piece as 2-byte elements
+        if constexpr (kQ4) {
+            *reinterpret_cast<u4_t*>(dst + 2 * dim) = q4_to_half(x, Q4Word(word));
+        } else if constexpr (FMT == RTA_Q8_ROW) {
             uint32_t w[8];
 #pragma unroll
             for (int y = 0; y < 4; ++y) codes_to_half(x[y], w[2 * y], w[2 * y + 1]);
@@ -139,7 +151,8 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
 #pragma unroll
             for (int k = 0; k < kPass; ++k)
                 if (!((okr >> k) & 1u)) {
-                    kr[k] = vr[k] = u4_t{0, 0, 0, 0};
+                    kr[k] = vr[k] = (Piece)(0u);
+                    if constexpr (kQ4) kw[k] = vw[k] = 0;   // (scales)
                     if constexpr (kScaled) ksr[k] = vsr[k] = 0.0f;
                 }
         }
@@ -155,8 +168,13 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                     }
                 } else {   // a row's threads are of one wave
                     constexpr uint64_t kRow = kPieces == 32 ? 0xffffffffull : (1ull << kPieces) - 1;
-                    const bool hit = piece_not_finite<FMT>(vr[k]);
-                    if (hit) vr[k] = u4_t{0, 0, 0, 0};
+                    bool hit;
+                    if constexpr (kQ4) hit = q4_not_finite(vw[k]);
+                    else hit = piece_not_finite<FMT>(vr[k]);
+                    if (hit) {
+                        vr[k] = (Piece)(0u);
+                        if constexpr (kQ4) vw[k] = 0;
+                    }
                     if (__builtin_amdgcn_ballot_w64(hit) & (kRow << (lane & ~(kPieces - 1)))) bad |= 1u << k;
                 }
             }
@@ -164,8 +182,8 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
 #pragma unroll
         for (int k = 0; k < kPass; ++k) {
             const int row = row0 + k * kStep;
-            put(buf + row * L::kPitch, kr[k]);
-            put(buf + L::kKeys + row * L::kPitchV, vr[k]);
+            put(buf + row * L::kPitch, kr[k], kw[k]);
+            put(buf + L::kKeys + row * L::kPitchV, vr[k], vw[k]);
             if (piece == 0) {
                 if constexpr (kScaled) {
                     float* f = reinterpret_cast<float*>(buf + L::kRows);

@@ -387,11 +387,6 @@ __global__ void __launch_bounds__(256) compact_kernel(const PageArgs a, PlanWs w
 }
 
 // ------------------------------------------------------------------ rows in, rows out ----
-template <int FMT> struct Element;
-template <> struct Element<RTA_F16> { using T = uint16_t; };
-template <> struct Element<RTA_BF16> { using T = uint16_t; };
-template <> struct Element<RTA_Q8_ROW> { using T = int8_t; };
-
 // fp32 to bfloat16, nearest even; a NaN keeps its upper bits and stays one.
 __device__ __forceinline__ uint16_t bf16_bits(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -414,6 +409,77 @@ __device__ __forceinline__ uint8_t* row_page(const PageArgs& a, const RowList& l
     return page < 0 ? nullptr : a.pool + page * a.page_bytes;
 }
 
+// RTA_Q4_GROUP's scale of a range f = (largest - smallest) / 15: six significant bits, upwards, so that the
+// range fits 15 codes, and no finer than 2^-19 (binary16 with its last five bits 0).
+__device__ __forceinline__ float q4_scale(float f) {
+    int e;
+    (void)frexpf(f, &e);
+    const int k = (e < -13 ? -13 : e) - 6;
+    return ldexpf(ceilf(ldexpf(f, -k)), k);
+}
+
+// Eight values f of head which_h (keys first) at dims d .. d + 7 into row `off` of a page; the threads of a
+// head call it together.
+template <int FMT, int HD>
+__device__ __forceinline__ void store_row8(const PageArgs& a, uint8_t* page, int which_h, int off, int d, const float f[8]) {
+    const int64_t row = (int64_t)which_h * a.page + off;
+    if constexpr (FMT == RTA_Q8_ROW) {
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fabsf(f[j]) < INFINITY ? fmaxf(m, fabsf(f[j])) : INFINITY;   // NaN too
+        m = group_max(m, HD / 8);
+        const float scale = m * (1.0f / 127.0f), den = scale > 0.0f ? scale : 1.0f;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // (a subnormal scale may be rounded down by more than the half step of code 127; an
+            // infinite one makes every value of the head 0 inf = NaN)
+            const float code = scale < INFINITY ? fminf(fmaxf(rintf(f[j] / den), -127.0f), 127.0f) : 0.0f;
+            w[j >> 2] |= ((uint32_t)(int)code & 255u) << (8 * (j & 3));
+        }
+        *reinterpret_cast<uint2*>(page + row * HD + d) = uint2{w[0], w[1]};
+        if (d == 0) reinterpret_cast<float*>(page + (int64_t)2 * a.kv_heads * a.page * HD)[row] = scale;
+    } else if constexpr (FMT == RTA_Q4_GROUP) {
+        float lo = 0.0f, hi = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool fine = fabsf(f[j]) < INFINITY;   // (NaN is not)
+            lo = fminf(lo, fine ? f[j] : 0.0f);
+            hi = fmaxf(hi, fine ? f[j] : INFINITY);
+        }
+        hi = group_max(hi, 4);   // the four threads of a group
+        lo = -group_max(-lo, 4);
+        const float range = (hi - lo) * (1.0f / 15.0f);
+        const bool fits = range <= kQ4Most;
+        const float scale = fits ? q4_scale(range) : 0.0f, den = scale > 0.0f ? scale : 1.0f, z = rintf(-lo / den);
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float code = fits ? fminf(fmaxf(rintf(f[j] / den) + z, 0.0f), 15.0f) : 0.0f;
+            w |= (uint32_t)code << (16 * (j & 1) + 4 * (j >> 1));
+        }
+        reinterpret_cast<uint32_t*>(page + row * (HD / 2))[q4_dword(HD, d)] = w;
+        if ((d & 31) == 0)
+            reinterpret_cast<uint16_t*>(page + (int64_t)a.kv_heads * a.page * HD)[row * (HD / 32) + (d >> 5)] =
+                fits ? __builtin_bit_cast(uint16_t, (_Float16)scale) | (uint16_t)z : kQ4NaN;
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint16_t lo, hi;
+            if constexpr (FMT == RTA_F16) {
+                lo = __builtin_bit_cast(uint16_t, (_Float16)f[2 * j]);
+                hi = __builtin_bit_cast(uint16_t, (_Float16)f[2 * j + 1]);
+            } else {
+                lo = bf16_bits(f[2 * j]);
+                hi = bf16_bits(f[2 * j + 1]);
+            }
+            w[j] = lo | (uint32_t)hi << 16;
+        }
+        *reinterpret_cast<uint4*>(page + (row * HD + d) * 2) = uint4{w[0], w[1], w[2], w[3]};
+    }
+}
+
 // A workgroup per row and 2048 of its 2 kv_heads hd values: 8 values a thread.
 template <int FMT, int HD>
 __device__ __forceinline__ void append_row(const PageArgs& a, const RowList& l, const float* __restrict__ k,
@@ -434,39 +500,7 @@ __device__ __forceinline__ void append_row(const PageArgs& a, const RowList& l, 
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = x[j];
-    const int64_t row = (int64_t)which_h * a.page + off;
-    if constexpr (FMT == RTA_Q8_ROW) {
-        float m = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = fabsf(f[j]) < INFINITY ? fmaxf(m, fabsf(f[j])) : INFINITY;   // NaN too
-        m = group_max(m, kPer);
-        const float scale = m * (1.0f / 127.0f), den = scale > 0.0f ? scale : 1.0f;
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            // (a subnormal scale may be rounded down by more than the half step of code 127; an
-            // infinite one makes every value of the head 0 inf = NaN)
-            const float code = scale < INFINITY ? fminf(fmaxf(rintf(f[j] / den), -127.0f), 127.0f) : 0.0f;
-            w[j >> 2] |= ((uint32_t)(int)code & 255u) << (8 * (j & 3));
-        }
-        *reinterpret_cast<uint2*>(page + row * HD + d) = uint2{w[0], w[1]};
-        if (d == 0) reinterpret_cast<float*>(page + (int64_t)2 * a.kv_heads * a.page * HD)[row] = scale;
-    } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint16_t lo, hi;
-            if constexpr (FMT == RTA_F16) {
-                lo = __builtin_bit_cast(uint16_t, (_Float16)f[2 * j]);
-                hi = __builtin_bit_cast(uint16_t, (_Float16)f[2 * j + 1]);
-            } else {
-                lo = bf16_bits(f[2 * j]);
-                hi = bf16_bits(f[2 * j + 1]);
-            }
-            w[j] = lo | (uint32_t)hi << 16;
-        }
-        *reinterpret_cast<uint4*>(page + (row * HD + d) * 2) = uint4{w[0], w[1], w[2], w[3]};
-    }
+    store_row8<FMT, HD>(a, page, which_h, off, d, f);
 }
 
 template <int FMT, int HD>
@@ -501,6 +535,14 @@ __device__ __forceinline__ void read_row(const PageArgs& a, const RowList& l, fl
             const float scale = reinterpret_cast<const float*>(page + (int64_t)2 * a.kv_heads * a.page * HD)[row];
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * scale;
+        } else if constexpr (FMT == RTA_Q4_GROUP) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(page + row * (HD / 2))[q4_dword(HD, d)];
+            const uint16_t word =
+                reinterpret_cast<const uint16_t*>(page + (int64_t)a.kv_heads * a.page * HD)[row * (HD / 32) + (d >> 5)];
+            const float scale = half_lo(word & kQ4Scale);
+            const int z = word & 15;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = (float)((int)(w >> (16 * (j & 1) + 4 * (j >> 1)) & 15u) - z) * scale;
         } else {
             const uint4 w = *reinterpret_cast<const uint4*>(page + (row * HD + d) * 2);
             const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -532,7 +574,8 @@ static void with_page_format(const rta_pages* p, F&& f) {
     };
     if (p->fmt == RTA_F16) by_hd(std::integral_constant<int, RTA_F16>{});
     else if (p->fmt == RTA_BF16) by_hd(std::integral_constant<int, RTA_BF16>{});
-    else by_hd(std::integral_constant<int, RTA_Q8_ROW>{});
+    else if (p->fmt == RTA_Q8_ROW) by_hd(std::integral_constant<int, RTA_Q8_ROW>{});
+    else by_hd(std::integral_constant<int, RTA_Q4_GROUP>{});
 }
 
 static int launched() { return hipGetLastError() == hipSuccess ? RTA_OK : RTA_ERR_LAUNCH; }

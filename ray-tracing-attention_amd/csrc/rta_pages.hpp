@@ -32,6 +32,29 @@ struct PageArgs {
     FastDiv by_page;
 };
 
+// Bytes of one position's elements of one head, and of its scales behind a page's elements.
+constexpr int page_row_bytes(int fmt, int hd) { return fmt == RTA_Q8_ROW ? hd : fmt == RTA_Q4_GROUP ? hd / 2 : 2 * hd; }
+constexpr int page_scale_bytes(int fmt, int hd) { return fmt == RTA_Q8_ROW ? 4 : fmt == RTA_Q4_GROUP ? hd / 16 : 0; }
+
+// RTA_Q4_GROUP: a group's word is a scale (binary16 of six significant bits) with the zero point in its last
+// four bits.  Scale * (code - zero) and scale * (16 + code) then have 11 bits at most and are exact in
+// binary16 up to a scale of 2112 (31 of which end at 65504).
+constexpr uint32_t kQ4Scale = 0xffe0u;
+constexpr uint16_t kQ4NaN = 0x7fe0u;
+constexpr float kQ4Most = 2112.0f;
+// Which of a row's dwords holds dims d .. d + 7 (d % 8 = 0).  Blocks of up to 128 dims; dword
+// (u, g) of a block is dims 32 g + 8 u .. of it, so that a 16-byte piece u holds, of every group, the 8 dims
+// that lane segment u feeds to the matrix cores.  Dim 2 j + b of a dword: bits 16 b + 4 j .. + 3.
+__device__ __forceinline__ int q4_dword(int hd, int d) {
+    const int groups = hd < 128 ? 2 : 4, g = (d >> 5) & (groups - 1), u = (d >> 3) & 3;
+    return (d >> 7) * 16 + u * groups + g;
+}
+// Its first dim.
+__device__ __forceinline__ int q4_dim(int hd, int dword) {
+    const int groups = hd < 128 ? 2 : 4, g = dword & (groups - 1), u = dword / groups & 3;
+    return (dword >> 4) * 128 + 32 * g + 8 * u;
+}
+
 // A row list: entry of row r, and how many rows it has.
 struct RowList {
     const int32_t* seqs;
@@ -97,21 +120,22 @@ __device__ __forceinline__ bool bad_length(const PageArgs& a, int len) {
 
 namespace host {
 
-inline int page_element(int fmt) { return fmt == RTA_F16 || fmt == RTA_BF16 ? 2 : fmt == RTA_Q8_ROW ? 1 : 0; }
+inline bool page_format(int fmt) {
+    return fmt == RTA_F16 || fmt == RTA_BF16 || fmt == RTA_Q8_ROW || fmt == RTA_Q4_GROUP;
+}
 
 inline int64_t page_bytes(int fmt, int kv_heads, int head_dim, int page) {
-    const int e = page_element(fmt);
-    if (!e || kv_heads <= 0 || kv_heads > 1024 || page <= 0 || page > 65536 ||
+    if (!page_format(fmt) || kv_heads <= 0 || kv_heads > 1024 || page <= 0 || page > 65536 ||
         (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return -1;
-    const int64_t n = 2ll * kv_heads * page * (head_dim * e + (fmt == RTA_Q8_ROW ? 4 : 0));
+    const int64_t n = 2ll * kv_heads * page * (page_row_bytes(fmt, head_dim) + page_scale_bytes(fmt, head_dim));
     return (n + 127) / 128 * 128;
 }
 
 // The descriptor's checks and its device form (layer: -1 for the calls on every layer).
 inline int pages_args(const rta_pages* p, int layer, PageArgs* a) {
     if (!p || !p->pool || !p->table || !p->lengths || !p->refs) return RTA_ERR_NULL;
-    if (!page_element(p->fmt)) return RTA_ERR_FORMAT;
+    if (!page_format(p->fmt)) return RTA_ERR_FORMAT;
     if (p->kv_heads <= 0 || p->page <= 0 || p->layers <= 0 || p->n_pages <= 0 || p->max_seqs <= 0 || p->max_pages <= 0)
         return RTA_ERR_SHAPE;
     const int64_t bytes = page_bytes(p->fmt, p->kv_heads, p->head_dim, p->page);

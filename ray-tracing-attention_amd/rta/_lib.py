@@ -14,6 +14,7 @@ LIB_PATH = PKG_ROOT / "lib" / "librta.so"
 F32, F16, Q4_K, Q6_K, BF16 = 0, 1, 12, 14, 30
 TILED = 0x100   # fmt | TILED: a K-quant matrix packed by rta_pack
 Q8_ROW = 0x200  # pages only: int8 codes, one fp32 scale per position and kv head
+Q4_GROUP = 0x400  # pages only: 4-bit codes, a scale and a zero point per 32 dims
 EPI_STORE, EPI_ACCUMULATE = 0, 1
 DEVERR_HITS, DEVERR_VOCAB, DEVERR_PAGES, DEVERR_DETECTOR = 8, 2048, 16384, 65536
 NOALLOC_SCRATCH_BYTES = 96 << 20   # RTA_NOALLOC_SCRATCH_BYTES

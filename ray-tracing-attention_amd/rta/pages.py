@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import BF16, F16, Q8_ROW, check
+from ._lib import BF16, F16, Q4_GROUP, Q8_ROW, check
 from .ops import _rows, _rs
 
 WHOLE = 2**31 - 1   # a `last` past every length
@@ -240,4 +240,4 @@ class PagedCache:
         return out, m, z
 
 
-__all__ = ["BF16", "F16", "Q8_ROW", "PagedCache", "WHOLE", "page_bytes"]
+__all__ = ["BF16", "F16", "Q4_GROUP", "Q8_ROW", "PagedCache", "WHOLE", "page_bytes"]
