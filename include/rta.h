@@ -492,6 +492,47 @@ int rta_hybrid_decode_step_capture(const rta_hybrid_shape* shape, const rta_hybr
                                    const rta_hybrid_capture* capture, void* workspace, size_t workspace_bytes,
                                    rta_stream_t stream);
 
+/* ---------------- rotary positions beyond rta_rope: pairs of neighbours or of half a head's distance, the
+ * whole head or its first values, frequencies scaled for contexts longer than the trained one.  Pair j of a
+ * head at position p turns by the angle 2 pi p turns[j] (the product and the turn in fp64, each value rounded
+ * to fp32 once):  (x, y) -> amplitude (x cos - y sin, x sin + y cos).  Values past `dims` stay as they are.
+ * The rotation at -p is its transpose: gradients go back through a call with negated positions. */
+enum rta_rotary_layout {
+    RTA_ROTARY_NEIGHBOURS = 0,   /* pair j: values 2 j and 2 j + 1 (rta_rope's) */
+    RTA_ROTARY_HALVES = 1        /* pair j: values j and j + dims / 2 */
+};
+typedef struct rta_rotary {
+    int layout;            /* rta_rotary_layout */
+    int head_dim;          /* values per head, up to 512 */
+    int dims;              /* of which the first `dims` turn: even, 2 .. head_dim */
+    double amplitude;      /* finite */
+    const double* turns;   /* device [dims / 2]: turns per position */
+} rta_rotary;
+
+/* Host only: turns[dims / 2] (host memory) and the amplitude (may be NULL) of frequencies f_j = theta^(-2j / dims),
+ * turns f / 2 pi, for a context `factor` times as long as the `original` one:
+ *   RTA_ROTARY_PLAIN   f
+ *   RTA_ROTARY_LINEAR  f / factor
+ *   RTA_ROTARY_BASE    f of theta factor^(dims / (dims - 2))
+ *   RTA_ROTARY_RAMP    g f + (1 - g) f / factor, g falling from 1 to 0 between the pairs floor(j(high)) (0 at
+ *                      least) and ceil(j(low)) (dims - 1 at most), j(r) = dims ln(original / (2 pi r)) / (2 ln
+ *                      theta) the pair that makes r turns over the original length; amplitude 0.1 ln(factor) + 1
+ *                      (factor > 1)
+ *   RTA_ROTARY_BANDS   the same with g = (r - low) / (high - low), held to 0 .. 1, r = original f / 2 pi the
+ *                      pair's own turns; amplitude 1
+ * theta > 0 (RAMP: > 1), factor > 0, original > 0 and 0 < low < high where they count, all finite. */
+enum rta_rotary_scaling {
+    RTA_ROTARY_PLAIN = 0, RTA_ROTARY_LINEAR = 1, RTA_ROTARY_BASE = 2, RTA_ROTARY_RAMP = 3, RTA_ROTARY_BANDS = 4
+};
+int rta_rotary_turns(int dims, double theta, int scaling, double factor, double original, double low, double high,
+                     double* turns, double* amplitude);
+
+/* y[r, h, :] = x[r, h, :] turned to positions[r] (device int64, any sign), x and y [rows, heads, head_dim] fp32
+ * with row strides in floats; y may be x (with the same stride), and otherwise shares no memory with it.  rows
+ * below 2^24, heads up to 65535. */
+int rta_rotate(const rta_rotary* rotary, const float* x, int64_t x_stride, int rows, int heads, const int64_t* positions,
+               float* y, int64_t y_stride, rta_stream_t stream);
+
 /* ---------------- paged history: the keys and values of many sequences in one pool of
  * pages of `page` positions, handed out, shared, copied on write and closed up on the device.
  * No counterpart in the reference, whose history is one preallocated ring per layer
@@ -585,6 +626,17 @@ int rta_pages_compact(const rta_pages* pages, int32_t* used, void* workspace, si
 int rta_paged_append(const rta_pages* pages, int layer, const float* k, int64_t k_stride, const float* v,
                      int64_t v_stride, int rows, const int32_t* seqs, const int32_t* cu_rows, int n,
                      rta_stream_t stream);
+
+/* rta_paged_append with the rotation on the way: the keys of a row are turned to the position that it is
+ * stored at (rounded to fp32, then stored as rta_paged_append stores them), and so are, with q not NULL, the
+ * queries q [rows, hq, head_dim] of the same rows into q_out (row strides in floats; q_out may be q, with the
+ * same stride).  What rta_rotate and rta_paged_append give, bit by bit, in one pass and with positions that
+ * only the book knows.  rotary->head_dim is the pages'.  A listed row without a place (a bad sequence, no
+ * page) raises RTA_DEVERR_PAGES and is left undone, its q_out as it was. */
+int rta_paged_append_rotary(const rta_pages* pages, int layer, const rta_rotary* rotary, const float* k, int64_t k_stride,
+                            const float* v, int64_t v_stride, const float* q, int64_t q_stride, int hq, float* q_out,
+                            int64_t q_out_stride, int rows, const int32_t* seqs, const int32_t* cu_rows, int n,
+                            rta_stream_t stream);
 
 /* The reverse: fp32 keys and values of those rows (either may be NULL).  A position without a
  * page reads as zeros and raises RTA_DEVERR_PAGES. */

@@ -7,6 +7,7 @@
 #include <math.h>
 
 #include "rta_pages.hpp"
+#include "rta_rotary.hpp"
 
 namespace rta {
 
@@ -394,14 +395,14 @@ __device__ __forceinline__ uint16_t bf16_bits(float v) {
     return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
 }
 
-// Where head h's row of position p lies: its element index inside the page and the page's bytes.
-__device__ __forceinline__ uint8_t* row_page(const PageArgs& a, const RowList& l, int r, int& off, bool& listed) {
+// Where row r lies: its position, its place inside the page and the page's bytes.
+__device__ __forceinline__ uint8_t* row_page(const PageArgs& a, const RowList& l, int r, int64_t& pos, int& off, bool& listed) {
     int i, first, count;
     listed = row_entry(l, r, i, first, count);
     if (!listed) return nullptr;
     const int s = list_seq(l.seqs, i);
     if ((unsigned)s >= (unsigned)a.max_seqs) return nullptr;
-    const int64_t pos = (int64_t)a.lengths[s] - count + (r - first);
+    pos = (int64_t)a.lengths[s] - count + (r - first);
     if (pos < 0 || pos >= (int64_t)a.max_pages * a.page) return nullptr;
     const int e = (int)a.by_page.div((uint32_t)pos);
     off = (int)pos - e * a.page;
@@ -487,7 +488,8 @@ __device__ __forceinline__ void append_row(const PageArgs& a, const RowList& l, 
     const int r = blockIdx.x;
     int off = 0;
     bool listed;
-    uint8_t* page = row_page(a, l, r, off, listed);
+    int64_t pos;
+    uint8_t* page = row_page(a, l, r, pos, off, listed);
     if (!page) {
         if (listed && threadIdx.x == 0 && blockIdx.y == 0) raise_error(RTA_DEVERR_PAGES);
         return;
@@ -511,13 +513,88 @@ __global__ void __launch_bounds__(256) append_kernel(const PageArgs a, const Row
     if (blockIdx.x == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
 }
 
+// The rows of append_kernel with keys turned to their positions, and with queries q of the same rows turned
+// into q_out.
+struct RotatedRows {
+    RotaryArgs r;
+    const float *k, *v, *q;
+    float* q_out;
+    int64_t k_stride, v_stride, q_stride, q_out_stride;
+    int hq;   // 0: no queries
+};
+
+// Bound by the bytes.  A workgroup takes one row, and 2048 values of [k | v | q] at a time, 8 a thread; the
+// row's angles lie in LDS (a place of padding after every four keeps the eight that each thread reads, one after
+// the other, on different banks).
+template <int FMT, int HD, int LAYOUT>
+__global__ void __launch_bounds__(256) append_rotary_kernel(const PageArgs a, const RowList l, const RotatedRows x) {
+    __shared__ double2 turn[HD / 2 + HD / 8];
+    constexpr int kPer = HD / 8;
+    const int row = blockIdx.x, half = x.r.dims / 2;
+    int off = 0;
+    bool listed;
+    int64_t pos;
+    uint8_t* page = row_page(a, l, row, pos, off, listed);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && bad_rows(l)) raise_error(RTA_DEVERR_PAGES);
+    if (!page) {
+        if (listed && threadIdx.x == 0 && blockIdx.y == 0) raise_error(RTA_DEVERR_PAGES);
+        return;
+    }
+    if (threadIdx.x < half) turn[threadIdx.x + (threadIdx.x >> 2)] = turn_of((double)pos, x.r.turns[threadIdx.x], x.r.amplitude);
+    __syncthreads();
+    const int heads = 2 * a.kv_heads + x.hq, step = gridDim.y * 256;
+    for (int base = blockIdx.y * 256; base < heads * kPer; base += step) {   // whole heads
+        const int c = base + threadIdx.x, head = c / kPer, d = 8 * (c % kPer);
+        const bool on = head < heads, query = head >= 2 * a.kv_heads;
+        float f[8];
+        if (on) {
+            const float* src = query ? x.q + row * x.q_stride + (int64_t)(head - 2 * a.kv_heads) * HD
+                               : head < a.kv_heads ? x.k + row * x.k_stride + (int64_t)head * HD
+                                                   : x.v + row * x.v_stride + (int64_t)(head - a.kv_heads) * HD;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = src[d + j];
+            if ((head < a.kv_heads || query) && d < x.r.dims) {
+                if constexpr (LAYOUT == RTA_ROTARY_NEIGHBOURS) {
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const int p = (d + j) / 2;
+                        if (p < half) turn_pair(f[j], f[j + 1], turn[p + (p >> 2)]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int dim = d + j;
+                        if (dim >= x.r.dims) break;
+                        const bool lower = dim < half;
+                        const int p = lower ? dim : dim - half;
+                        float other = src[lower ? dim + half : dim - half];
+                        const double2 t = turn[p + (p >> 2)];
+                        if (lower) turn_pair(f[j], other, t);
+                        else turn_pair(other, f[j], t);
+                    }
+                }
+            }
+        }
+        __syncthreads();   // q_out may be q: every thread of a head has read its pairs
+        if (!on) continue;
+        if (query) {
+            float* dst = x.q_out + row * x.q_out_stride + (int64_t)(head - 2 * a.kv_heads) * HD + d;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dst[j] = f[j];
+        } else {
+            store_row8<FMT, HD>(a, page, head, off, d, f);
+        }
+    }
+}
+
 template <int FMT, int HD>
 __device__ __forceinline__ void read_row(const PageArgs& a, const RowList& l, float* __restrict__ k, int64_t k_stride,
                                          float* __restrict__ v, int64_t v_stride) {
     const int r = blockIdx.x;
     int off = 0;
     bool listed;
-    const uint8_t* page = row_page(a, l, r, off, listed);
+    int64_t pos;
+    const uint8_t* page = row_page(a, l, r, pos, off, listed);
     if (!listed) return;
     if (!page && threadIdx.x == 0 && blockIdx.y == 0) raise_error(RTA_DEVERR_PAGES);
     constexpr int kPer = HD / 8;
@@ -683,6 +760,49 @@ int rta_paged_append(const rta_pages* pages, int layer, const float* k, int64_t 
         hipLaunchKernelGGL((append_kernel<decltype(fmt)::value, decltype(hd)::value>),
                            dim3(rows, (2 * width + 2047) / 2048), dim3(256), 0, (hipStream_t)stream, a, l, k, k_stride,
                            v, v_stride);
+    });
+    return launched();
+}
+
+int rta_paged_append_rotary(const rta_pages* pages, int layer, const rta_rotary* rotary, const float* k, int64_t k_stride,
+                            const float* v, int64_t v_stride, const float* q, int64_t q_stride, int hq, float* q_out,
+                            int64_t q_out_stride, int rows, const int32_t* seqs, const int32_t* cu_rows, int n,
+                            rta_stream_t stream) {
+    PageArgs a;
+    RotatedRows x{};
+    if (layer < 0) return RTA_ERR_RANGE;
+    int rc = host::pages_args(pages, layer, &a);
+    if (rc) return rc;
+    rc = host::rotary_args(rotary, &x.r);
+    if (rc) return rc;
+    if (!k || !v || !q != !q_out) return RTA_ERR_NULL;
+    RowList l;
+    rc = host::rows_args(rows, seqs, cu_rows, n, &l);
+    if (rc) return rc;
+    const int64_t width = (int64_t)pages->kv_heads * pages->head_dim, q_width = (int64_t)hq * pages->head_dim;
+    if (rotary->head_dim != pages->head_dim || k_stride < width || v_stride < width || (q && hq <= 0) ||
+        (q && (q_stride < q_width || q_out_stride < q_width)))
+        return RTA_ERR_SHAPE;
+    if (q && (hq > 65535 || (q == q_out && q_stride != q_out_stride && rows > 1))) return RTA_ERR_RANGE;
+    if (!host::aligned(k, 4) || !host::aligned(v, 4) || !host::aligned(q, 4) || !host::aligned(q_out, 4)) return RTA_ERR_ALIGN;
+    x.k = k;
+    x.v = v;
+    x.q = q;
+    x.q_out = q_out;
+    x.k_stride = k_stride;
+    x.v_stride = v_stride;
+    x.q_stride = q_stride;
+    x.q_out_stride = q_out_stride;
+    x.hq = q ? hq : 0;
+    // every workgroup computes its row's angles: a row in one where there are rows enough for the chip
+    const int64_t parts = (2 * width + (q ? q_width : 0) + 2047) / 2048;
+    const dim3 grid(rows, rows * parts <= 2048 ? parts : 1), block(256);
+    with_page_format(pages, [&](auto fmt, auto hd) {
+        constexpr int F = decltype(fmt)::value, HD = decltype(hd)::value;
+        if (rotary->layout == RTA_ROTARY_NEIGHBOURS)
+            hipLaunchKernelGGL((append_rotary_kernel<F, HD, RTA_ROTARY_NEIGHBOURS>), grid, block, 0, (hipStream_t)stream, a, l, x);
+        else
+            hipLaunchKernelGGL((append_rotary_kernel<F, HD, RTA_ROTARY_HALVES>), grid, block, 0, (hipStream_t)stream, a, l, x);
     });
     return launched();
 }

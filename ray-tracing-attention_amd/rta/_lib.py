@@ -40,7 +40,13 @@ class Pages(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("pool", "table", "lengths", "refs")]
 
 
-_remap_p, _pages_p = ctypes.POINTER(Remap), ctypes.POINTER(Pages)
+class Rotary(ctypes.Structure):
+    """struct rta_rotary: a rotation (turns: device pointer)."""
+    _fields_ = [("layout", ctypes.c_int), ("head_dim", ctypes.c_int), ("dims", ctypes.c_int),
+                ("amplitude", ctypes.c_double), ("turns", ctypes.c_void_p)]
+
+
+_remap_p, _pages_p, _rotary_p = ctypes.POINTER(Remap), ctypes.POINTER(Pages), ctypes.POINTER(Rotary)
 
 # name -> (restype, argtypes); must match include/rta.h
 SIGNATURES = {
@@ -89,6 +95,9 @@ SIGNATURES = {
     "rta_image_readout": (_i, [_i, _i, _p, _p, _i, _i, _p, _i, _p, _f, _p, _i, _p, _sz, ctypes.POINTER(_i), _p]),
     "rta_attention_receipt_records": (_i64, [_p, _i, _i, _i64, _i]),
     "rta_attention_receipts": (_i, [_p, _i, _i, _i, _i, _p, _i, _i, _p, _p, _i64, _i64, _i, _i, _p, _i64, _p]),
+    # rotary positions (rta.rotary)
+    "rta_rotary_turns": (_i, [_i, _d, _i, _d, _d, _d, _d, _p, _p]),
+    "rta_rotate": (_i, [_rotary_p, _p, _i64, _i, _i, _p, _p, _i64, _p]),
     # paged history (rta.pages)
     "rta_page_bytes": (_i64, [_i, _i, _i, _i]),
     "rta_pages_init": (_i, [_pages_p, _p]),
@@ -98,6 +107,8 @@ SIGNATURES = {
     "rta_pages_free": (_i, [_pages_p, _p, _p, _p, _i, _p]),
     "rta_pages_compact": (_i, [_pages_p, _p, _p, _sz, _p]),
     "rta_paged_append": (_i, [_pages_p, _i, _p, _i64, _p, _i64, _i, _p, _p, _i, _p]),
+    "rta_paged_append_rotary": (_i, [_pages_p, _i, _rotary_p, _p, _i64, _p, _i64, _p, _i64, _i, _p, _i64, _i, _p, _p, _i,
+                                     _p]),
     "rta_paged_read": (_i, [_pages_p, _i, _i, _p, _p, _i, _p, _i64, _p, _i64, _p]),
     "rta_paged_attention_workspace_bytes": (_sz, [_pages_p, _i, _i, _i, _i, _i, _i, _i]),
     "rta_paged_attention": (_i, [_pages_p, _i, _p, _i64, _i, _i, _p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _sz,

@@ -185,6 +185,31 @@ class PagedCache:
         self._call("rta_paged_append", layer, *self._strided(k, "k", rows), *self._strided(v, "v", rows), rows, sp, cu,
                    n)
 
+    def append_rotary(self, rotary, k, v, q=None, q_out=None, layer=0, seqs=None, cu_rows=None):
+        """append with the keys turned to their positions by `rotary` (rta.rotary.Rotary), and with them the
+        queries q [rows, hq, head_dim] fp32 of the same rows (rows may be strided) into q_out, which it
+        returns (None without q); q_out may be q."""
+        rows = _rows(k, "k").shape[0]
+        sp, cu, n = self._list(rows, seqs, cu_rows)
+        if rotary.device != self.device or rotary.head_dim != self.head_dim:
+            raise ValueError(f"rotary must be of head_dim {self.head_dim} on {self.device}")
+        qs = [None, 0, 0, None, 0]
+        if q is not None:
+            stride = rotary._check_rows(q, "q")
+            if q.shape[0] != rows:
+                raise ValueError(f"q must have {rows} rows")
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
+            out_stride = rotary._check_rows(q_out, "q_out")
+            if q_out.shape != q.shape:
+                raise ValueError(f"q_out must be of shape {tuple(q.shape)}")
+            qs = [q.data_ptr(), stride, q.shape[1], q_out.data_ptr(), out_stride]
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        self._call("rta_paged_append_rotary", layer, rotary._at, *self._strided(k, "k", rows),
+                   *self._strided(v, "v", rows), *qs, rows, sp, cu, n)
+        return q_out
+
     def read(self, rows, layer=0, seqs=None, cu_rows=None, k=None, v=None):
         """The keys and values of those rows as fp32: (k, v), each [rows, kv_heads * head_dim].
         Rows that no entry lists are left as they were in k and v, and mean nothing in tensors
