@@ -216,6 +216,28 @@ int rta_lm_head(int fmt, const void* w, int vocab, int hidden, const float* h, i
                 float margin, float* logits, uint32_t* ids,
                 void* workspace, size_t workspace_bytes, rta_stream_t stream);
 
+/* The next token of each row of logits [rows, vocab] (row stride in floats; 0: one row for all draws), by a uniform number u[r] in
+ * [0, 1) that the caller draws.  With M the row's largest logit and T its temperature, word i weighs
+ * w_i = e^((x_i - M) / T); in the order of the logits, largest first and equals by index, the row keeps
+ *   top_k   the first k words (k <= 0: all),
+ *   top_p   of these the fewest that hold p of their weight: a word stays while those before it hold less than
+ *           p of it (p >= 1 or NaN: all; p <= 0: one),
+ *   min_p   of these the words with w_i >= min_p (min_p <= 0 or NaN: all),
+ * the first word always.  ids[r] is the first word, in the order of index, up to which the kept weights add up
+ * to more than u of all of them; probs[r] (may be NULL) its share.  A temperature that is not above 0 means the
+ * largest logit's lowest index.  u below 0 or NaN counts as 0; from 1 on it means the last word.
+ * temperature, top_k, top_p and min_p are device arrays [rows], or NULL: 1, all, all, all.
+ * A logit of -inf is never drawn.  A row with a NaN or +inf, or with nothing but -inf, gets ids[r] = 2^32 - 1
+ * and probs[r] = 0 and raises RTA_DEVERR_DETECTOR.  Weights are computed in fp64 and added up as whole numbers of
+ * 2^-50 of the largest (in an order that does not matter: results repeat bit by bit); words below 2^-47 of it
+ * count as none.  vocab up to 2^24, rows ceil(vocab / 8192) below 2^22.
+ * Workspace: rta_sample_workspace_bytes() (always needed; 16-byte aligned).
+ * No reference counterpart: its word readout takes the largest (Resident::word, optical_resident.cpp:523-530). */
+size_t rta_sample_workspace_bytes(int rows, int vocab);
+int rta_sample(const float* logits, int64_t stride, int rows, int vocab, const float* temperature, const int32_t* top_k,
+               const float* top_p, const float* min_p, const float* u, uint32_t* ids, float* probs, void* workspace,
+               size_t workspace_bytes, rta_stream_t stream);
+
 /* Rotary embedding on adjacent pairs, in place: v [rows, heads, hd];
  * row r is at absolute position positions[r] (device int64).  Pairs p < rotary/2
  * of each head turn by positions[r] * theta^(-p/(rotary/2)) (phase, sin, cos in

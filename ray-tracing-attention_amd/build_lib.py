@@ -9,7 +9,7 @@ import sys
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
-SOURCES = ["csrc/rta_gemv.hip", "csrc/rta_attention.hip", "csrc/rta_step.hip", "csrc/rta_model.hip",
+SOURCES = ["csrc/rta_gemv.hip", "csrc/rta_sample.hip", "csrc/rta_attention.hip", "csrc/rta_step.hip", "csrc/rta_model.hip",
            "csrc/rta_rotary.hip", "csrc/rta_pages.hip", "csrc/rta_paged_attention.hip", "csrc/rta_asset.cpp"]
 LIB = HERE / "lib" / "librta.so"
 # the resident worker (stdin/stdout protocol of the reference's rt_optical_resident)

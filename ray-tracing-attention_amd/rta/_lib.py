@@ -81,6 +81,8 @@ SIGNATURES = {
     "rta_swiglu": (_i, [_i, _p, _p, _i, _i, _p, _i, _p, _p, _sz, _p]),
     "rta_lm_head_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "rta_lm_head": (_i, [_i, _p, _i, _i, _p, _i, _f, _p, _p, _p, _sz, _p]),
+    "rta_sample_workspace_bytes": (_sz, [_i, _i]),
+    "rta_sample": (_i, [_p, _i64, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "rta_rope": (_i, [_p, _i, _i, _i, _i, _p, _d, _p]),
     "rta_history_bytes": (_i64, [_i]),
     "rta_decode_attention_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),

@@ -245,6 +245,45 @@ def lm_head(fmt, w, vocab, hidden, h, margin=1e-4, workspace=None, logits=None, 
     return logits, ids
 
 
+def sample_workspace_bytes(rows, vocab):
+    return int(_lib.load().rta_sample_workspace_bytes(rows, vocab))
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, probs=None, workspace=None):
+    """(ids [rows] int32, probs [rows]) drawn from logits [rows, vocab] fp32 (rows may be strided or expanded) by uniform
+    numbers u [rows]; temperature, top_p, min_p [rows] fp32 and top_k [rows] int32, or None: off (the rules
+    are rta_sample's in include/rta.h).  A row without a word to draw gets id -1."""
+    lib = _lib.load()
+    _rows(logits, "logits")
+    rows, vocab = logits.shape
+    dev = logits.device
+    if logits.dtype != torch.float32:
+        raise TypeError("logits must be float32")
+    if ids is None:
+        ids = torch.empty(rows, dtype=torch.int32, device=dev)
+    if probs is None:
+        probs = torch.empty(rows, dtype=torch.float32, device=dev)
+    for t, name, dtype in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
+                           (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                           (min_p, "min_p", torch.float32), (ids, "ids", torch.int32), (probs, "probs", torch.float32)):
+        if t is None and name != "u":
+            continue
+        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dtype:
+            raise TypeError(f"{name} must be a {dtype} tensor on {dev}")
+        if tuple(t.shape) != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous of shape ({rows},)")
+    if workspace is not None and (_dev(workspace, "workspace").device != dev):
+        raise TypeError(f"workspace must be a tensor on {dev}")
+    ws = _workspace(sample_workspace_bytes(rows, vocab), dev, workspace)
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    with torch.cuda.device(dev):
+        stride = logits.stride(0) if rows > 1 else vocab
+        check(lib.rta_sample(logits.data_ptr(), stride, rows, vocab, p(temperature), p(top_k), p(top_p), p(min_p),
+                             p(u), p(ids), p(probs), p(ws), ws.numel() * ws.element_size(),
+                             torch._C._cuda_getCurrentRawStream(dev.index)), "rta_sample")
+    return ids, probs
+
+
 def rope(v, positions, rotary=None, theta=1e6):
     """In-place rotary embedding of v [rows, heads, hd] at positions [rows] (int64)."""
     lib = _lib.load()

@@ -1,0 +1,271 @@
+"""The draw from rows of logits against its 64-bit restatement: rules alone and together, ties, masks,
+sizes from one word to several hundred thousand, the ends of u, bad rows, streams and graphs.  A draw
+has to be the restatement's word unless u, or a rule, is closer to a border than the weights' own
+precision (2^-50 a word of up to 2^18, and 2^-45 of a scaled logit)."""
+import numpy as np
+import pytest
+
+import sample_reference as ref
+from rta import _lib, ops
+
+pytestmark = pytest.mark.gpu
+CLOSE = 2.0**-32
+
+
+@pytest.fixture(scope="module")
+def env():
+    import torch
+    ops.device_error(clear=True)
+    return torch, torch.device("cuda:0")
+
+
+def run(env, x, u, t=None, k=None, p=None, least=None):
+    torch, dev = env
+    up = lambda v, d: None if v is None else torch.tensor(np.asarray(v), dtype=d, device=dev)   # noqa: E731
+    f = torch.float32
+    x = x if isinstance(x, torch.Tensor) else up(x, f)
+    return ops.sample(x, up(u, f), up(t, f), up(k, torch.int32), up(p, f), up(least, f))
+
+
+def check(env, x, u, t=None, k=None, p=None, least=None, most_close=0):
+    x, u = np.asarray(x, np.float32), np.asarray(u, np.float32)
+    rows = len(x)
+    ids, probs = (v.cpu().numpy() for v in run(env, x, u, t, k, p, least))
+    pick = lambda v, r, off: off if v is None else np.asarray(v, np.float32 if off != 0 or v is not k else np.int64)[r]  # noqa: E731
+    close = 0
+    for r in range(rows):
+        i, share, near = ref.draw(x[r], u[r], pick(t, r, 1.0), pick(k, r, 0), pick(p, r, 1.0), pick(least, r, 0.0))
+        if near < CLOSE:
+            close += 1
+            continue
+        assert ids[r] == i, (r, ids[r], i, share, near)
+        # fp32's rounding, and the weights' 2^-45 of a scaled logit's bits
+        assert abs(probs[r] - share) <= share * (2.0**-24 + 2.0**-40), r
+    assert close <= most_close
+    return ids
+
+
+def logits(rng, rows, vocab, sigma=2.5, sure=6.0):
+    x = sigma * rng.standard_normal((rows, vocab)).astype(np.float32)
+    top = rng.integers(0, vocab, (rows, 20))
+    for r in range(rows):
+        x[r, top[r]] += np.float32(sure) * rng.random(20).astype(np.float32)
+    return x
+
+
+SIZES = [1, 2, 3, 5, 63, 64, 1000, 8191, 8192, 8193, 16385, 50001, 151936]
+RULES = {"none": {}, "t": dict(t=(0.2, 2.0)), "k": dict(k=(1, 3000)), "p": dict(p=(0.05, 0.999)), "least": dict(least=(1e-4, 0.5)),
+         "all": dict(t=(0.2, 2.0), k=(1, 200), p=(0.2, 0.99), least=(0.001, 0.3)),
+         "wide": dict(t=(0.7, 3.0), k=(3000, 60000), p=(0.9, 0.9999), least=(1e-6, 1e-4)), "kp": dict(k=(1, 50), p=(0.1, 1.0))}
+
+
+@pytest.mark.parametrize("vocab", SIZES)
+@pytest.mark.parametrize("rules", sorted(RULES))
+def test_rules(env, vocab, rules):
+    rng = np.random.default_rng(vocab)
+    rows = 9
+    x, u = logits(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    how = {}
+    for name, (lo, hi) in RULES[rules].items():
+        how[name] = rng.integers(lo, hi + 1, rows) if name == "k" else np.exp(rng.uniform(np.log(lo), np.log(hi), rows))
+    check(env, x, u, **how)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("vocab", [7, 900, 20000, 100003])
+@pytest.mark.parametrize("step", [0.0, 0.25, 4.0])
+def test_ties(env, vocab, step):
+    """Few distinct logits (step 0: all alike, where every sum is a whole number): bins past the list's room."""
+    rng = np.random.default_rng(vocab)
+    rows = 12
+    x = np.zeros((rows, vocab), np.float32) if step == 0 else \
+        (np.round(2.0 * rng.standard_normal((rows, vocab)) / step) * step).astype(np.float32)
+    x[3] *= -1.0   # zeros of both signs are equal
+    x[3, ::2] = np.abs(x[3, ::2])
+    u = rng.random(rows).astype(np.float32)
+    check(env, x, u)
+    check(env, x, u, k=rng.integers(1, vocab + 2, rows))
+    if step:
+        check(env, x, u, p=rng.uniform(0.05, 0.99, rows))
+        check(env, x, u, t=rng.uniform(0.3, 3, rows), k=rng.integers(1, vocab + 2, rows), p=rng.uniform(0.05, 0.99, rows),
+              least=rng.uniform(0, 0.2, rows))
+        check(env, x, u, least=np.full(rows, 1.0))
+        return
+    # halves, quarters: p of the words exactly
+    for p in (0.5, 0.25, 0.125):
+        ids, probs = (v.cpu().numpy() for v in run(env, x, u, p=np.full(rows, p)))
+        kept = int(np.ceil(vocab * p))
+        assert np.array_equal(ids, np.floor(u.astype(np.float64) * kept)) and np.allclose(probs, 1 / kept, rtol=1e-6)
+    ids = run(env, x, u, t=np.full(rows, np.inf))[0].cpu().numpy()
+    assert np.array_equal(ids, np.floor(u.astype(np.float64) * vocab))
+
+
+def test_every_word_has_its_share(env):
+    """One row many times, u over a grid: the counts are the shares, word by word."""
+    torch, dev = env
+    rng = np.random.default_rng(3)
+    x = logits(rng, 1, 9000)
+    n = 3000
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    for how in ({}, dict(k=[40]), dict(p=[0.9]), dict(least=[0.01])):
+        ids = run(env, torch.tensor(x, device=dev).expand(n, -1), u, **{a: np.repeat(v, n) for a, v in how.items()})[0].cpu().numpy()
+        assert np.all(np.diff(ids) >= 0)   # in the order of index
+        share = np.zeros(x.shape[1])
+        w = np.exp(x[0].astype(np.float64) - x.max())
+        order = np.argsort(-w, kind="stable")
+        keep = len(w)
+        if "k" in how:
+            keep = 40
+        if "p" in how:
+            keep = int((np.cumsum(w[order]) < np.float32(0.9) * w.sum()).sum()) + 1
+        if "least" in how:
+            keep = int((w >= np.float32(0.01)).sum())
+        share[order[:keep]] = w[order[:keep]] / w[order[:keep]].sum()
+        counts = np.bincount(ids, minlength=len(share))
+        assert np.all(np.abs(counts - n * share) <= 1.0 + n * 2.0**-24) and not counts[share == 0].any()
+
+
+def test_masks(env):
+    rng = np.random.default_rng(4)
+    rows, vocab = 10, 30000
+    x, u = logits(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    x[0, 1:] = -np.inf                      # one word left
+    x[1, : vocab - 1] = -np.inf
+    x[2, rng.random(vocab) < 0.999] = -np.inf
+    x[3, 8192:16384] = -np.inf              # a whole chunk
+    x[4, ::2] = np.finfo(np.float32).min    # the type's lowest value: words of no weight
+    x[5] = np.finfo(np.float32).min         # nothing else: all alike
+    x[6] = -1e30 + 0 * x[6]
+    x[6, 77] = 1e30
+    x[7] = np.finfo(np.float32).max
+    for how in ({}, dict(k=np.full(rows, 5)), dict(p=np.full(rows, 0.7)), dict(least=np.full(rows, 0.1)),
+                dict(k=np.full(rows, 20000), p=np.full(rows, 0.99)), dict(t=np.full(rows, 1e-30)), dict(t=np.full(rows, 1e30))):
+        ids = check(env, x, u, **how)
+        assert ids[0] == 0 and ids[1] == vocab - 1 and ids[4] % 2 == 1
+    assert ops.device_error() == 0
+
+
+def test_the_ends_of_u_and_of_the_rules(env):
+    rng = np.random.default_rng(5)
+    x = np.repeat(logits(rng, 1, 20000), 12, 0)
+    u = np.array([0, -1, np.nan, 1, 2, np.inf, 1 - 2.0**-24, 1e-45, 0.5, 0.5, 0.5, 0.5], np.float32)
+    ids = run(env, x, u)[0].cpu().numpy()
+    w = np.exp(x[0].astype(np.float64) - x.max())
+    first, last = np.nonzero(w)[0][[0, -1]]
+    assert (ids[:3] == first).all() and (ids[3:6] == last).all() and ids[7] == first and ids[6] <= last
+    largest = int(np.argmax(x[0]))
+    for how in (dict(t=np.array([0, -1, np.nan] * 4)), dict(k=np.ones(12)), dict(p=np.array([0, -3, 1e-30] * 4)),
+                dict(least=np.array([1, 2, np.inf] * 4)), dict(t=np.full(12, 1e-6))):
+        ids, probs = (v.cpu().numpy() for v in run(env, x, u, **how))
+        assert (ids == largest).all() and (probs == 1).all(), how
+    plain = run(env, x, u)
+    for how in (dict(k=np.array([0, -5, 20000, 2**31 - 1] * 3)), dict(p=np.array([1, 2, np.nan, np.inf] * 3)),
+                dict(least=np.array([0, -1, np.nan, -np.inf] * 3)), dict(t=np.ones(12))):
+        assert all((a == b).all() for a, b in zip(run(env, x, u, **how), plain)), how
+    assert ops.device_error() == 0
+
+
+def test_bad_rows(env):
+    torch, _ = env
+    rng = np.random.default_rng(6)
+    x = logits(rng, 8, 9001)
+    x[1, 9000], x[3, 17], x[5] = np.nan, np.inf, -np.inf
+    u = rng.random(8).astype(np.float32)
+    for how in ({}, dict(t=np.zeros(8)), dict(k=np.full(8, 3))):
+        ids, probs = (v.cpu().numpy() for v in run(env, x, u, **how))
+        assert ops.device_error() == _lib.DEVERR_DETECTOR
+        bad = np.array([1, 3, 5])
+        assert (ids[bad] == -1).all() and (probs[bad] == 0).all()
+        good = np.array([0, 2, 4, 6, 7])
+        want = [v.cpu().numpy() for v in run(env, x[good], u[good], **{a: v[good] for a, v in how.items()})]
+        assert np.array_equal(ids[good], want[0]) and np.array_equal(probs[good], want[1])
+        assert ops.device_error() == 0
+
+
+def test_greedy_rows_beside_others(env):
+    rng = np.random.default_rng(7)
+    x = np.round(logits(rng, 6, 25000))     # several words share the maximum
+    u = rng.random(6).astype(np.float32)
+    ids = check(env, x, u, t=np.array([0, 1, 0, 0.5, -2, 1]))
+    assert all(ids[r] == np.argmax(x[r]) for r in (0, 2, 4))
+
+
+def test_strides_streams_and_repeats(env):
+    torch, dev = env
+    gen = torch.Generator(device=dev).manual_seed(8)
+    rows, vocab = 5, 12345
+    wide = 3 * torch.randn(rows, vocab + 7, generator=gen, device=dev)
+    u = torch.rand(rows, generator=gen, device=dev)
+    p = torch.full((rows,), 0.9, device=dev)
+    for shift in range(4):
+        x = wide[:, shift : shift + vocab]
+        want = ops.sample(x.contiguous(), u, top_p=p)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(ops.sample(x, u, top_p=p), want))
+    one = wide[:1, 1 : 1 + vocab]
+    assert torch.equal(ops.sample(one, u[:1])[0], ops.sample(one.contiguous(), u[:1])[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.sample(wide[:, 3 : 3 + vocab] * 1.0, u, top_p=p)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graphs_with_their_own_workspaces(env):
+    torch, dev = env
+    gen = torch.Generator(device=dev).manual_seed(9)
+    rows, vocab = 4, 40000
+    x, u = torch.empty(rows, vocab, device=dev), torch.empty(rows, device=dev)
+    k = torch.tensor([0, 3, 50, 20000], dtype=torch.int32, device=dev)
+    p = torch.tensor([0.9, 1.0, 0.5, 0.99], device=dev)
+    x.normal_(generator=gen), u.uniform_(generator=gen)
+    ops.sample(x, u, top_k=k, top_p=p)
+    graphs, outs = [], []
+    for how in (dict(top_k=k, top_p=p), dict(min_p=0.1 * p)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.sample(x, u, **how))
+        graphs.append((g, how))
+    for i in range(4):
+        x.normal_(generator=gen).mul_(3), u.uniform_(generator=gen)
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (_, how), got in zip(graphs, outs):
+            assert all(torch.equal(a, b) for a, b in zip(ops.sample(x, u, **how), got)), i
+    assert ops.device_error() == 0
+
+
+def test_many_rows_and_long_vocabularies(env):
+    rng = np.random.default_rng(10)
+    x, u = logits(rng, 600, 777), rng.random(600).astype(np.float32)
+    check(env, x, u, t=rng.uniform(0.3, 2, 600), k=rng.integers(0, 60, 600), p=rng.uniform(0.3, 1.2, 600), least=rng.uniform(-0.1, 0.1, 600))
+    x, u = logits(rng, 2, 1 << 21, sigma=1.0, sure=3.0), rng.random(2).astype(np.float32)
+    for how in ({}, dict(p=[0.95, 0.5]), dict(k=[700000, 100]), dict(least=[1e-3, 0.02])):
+        check(env, x, u, **how, most_close=1)
+
+
+def test_arguments_are_checked(env):
+    torch, dev = env
+    x, u = torch.zeros(3, 100, device=dev), torch.zeros(3, device=dev)
+    with pytest.raises(TypeError):
+        ops.sample(x.half(), u)
+    with pytest.raises(TypeError):
+        ops.sample(x, u.double())
+    with pytest.raises(TypeError):
+        ops.sample(x, u.cpu())
+    with pytest.raises(TypeError):
+        ops.sample(x, None)
+    with pytest.raises(TypeError):
+        ops.sample(x, u, top_k=torch.ones(3, dtype=torch.int64, device=dev))
+    with pytest.raises(ValueError):
+        ops.sample(x, u[:2])
+    with pytest.raises(ValueError):
+        ops.sample(x[:, ::2], u)
+    with pytest.raises(ValueError):
+        ops.sample(x[0], u)
+    with pytest.raises(ValueError):
+        ops.sample(x, u, temperature=torch.ones(6, device=dev)[::2])
+    with pytest.raises(_lib.RtaError):
+        ops.sample(x, u, workspace=torch.empty(64, dtype=torch.uint8, device=dev))
