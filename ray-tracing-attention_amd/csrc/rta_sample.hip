@@ -4,9 +4,10 @@
 // The order of a row's words is by logit, largest first, equals by index; every rule keeps the first so
 // many of them, so all of them together keep the words up to one place in that order.  Two kernels:
 //   1. a workgroup per chunk of kChunk words reads the logits once and leaves the chunk's maximum and, by
-//      bins of 1/8 octave of weight below it, counts and sums of weights;
-//   2. a workgroup per row joins the bins, finds each rule's bin, ranks the words of that bin alone (read
-//      again, from the caches, into LDS) by a radix search, and draws.
+//      bins of 1/8 octave of weight below it, how many words lie in the bins up to each and their weights' sums,
+//      and which words (of the first bins, as far as the rules may ask for them);
+//   2. a workgroup per row joins the bins, finds each rule's bin, ranks the words of that bin (or of all bins up
+//      to it) in LDS by a radix search, and draws.
 // A weight is 2^(y - y of the largest), y = logit log2(e) / temperature in fp64, as a whole number of 2^-50
 // (fewer bits where more words than kChunk are summed): sums of whole numbers do not depend on the order of
 // their atomics, and those of equal logits are exact.  Words below 2^-47 of the largest count as none.
@@ -21,7 +22,7 @@ namespace rta {
 constexpr int kChunk = 8192, kChunkThreads = 512, kPerThread = kChunk / kChunkThreads;
 constexpr int kBins = 384;         // 48 octaves; the last one holds everything below, and is not kept
 constexpr int kBits = 50;          // kChunk weights of up to 2^50 stay below 2^64
-constexpr int kRowThreads = 1024, kMostChunks = 2048;
+constexpr int kRowThreads = 512, kMostChunks = 512;
 constexpr int kList = 8192;        // words ranked in LDS
 constexpr uint32_t kNoToken = 0xffffffffu;
 
@@ -31,6 +32,14 @@ struct ChunkHead {
     uint32_t arg;     // its first word
     uint32_t bad;     // a NaN or +inf
     uint32_t pad[3];
+};
+
+// What kernel 1 leaves of a chunk.
+struct Chunk {
+    ChunkHead head;
+    uint64_t mass[kBins];       // weights of all bins up to each, against the chunk's largest
+    uint16_t upto[kBins];       // and their words
+    alignas(16) uint16_t place[kChunk];   // words (from the chunk's first) by bins, in any order inside one
 };
 
 struct SampleArgs {
@@ -44,9 +53,7 @@ struct SampleArgs {
     const float* u;
     uint32_t* ids;
     float* probs;
-    ChunkHead* head;    // [rows][nchunk]
-    uint64_t* mass;     // [rows][nchunk][kBins]
-    uint32_t* count;    // [rows][nchunk][kBins]
+    Chunk* chunks;      // [rows][nchunk]
 };
 
 // log2(e) / temperature; a temperature that is not above 0 means the largest (no scale).
@@ -62,28 +69,33 @@ __device__ __forceinline__ double scaled(float v, double scale) {
     return (double)v * scale;
 }
 
-// 2^t for t <= 0, by 2^n times the series of e^(f ln 2), |f| <= 1/2, to the 11th power: 6e-15 left out.
-__device__ __forceinline__ double exp2_below(double t) {
-    const double n = rint(t), f = (t - n) * 0.6931471805599453;
-    double p = 1.0 / 39916800.0;
-    p = fma(p, f, 1.0 / 3628800.0);
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return ldexp(p, n < -1000.0 ? -1000 : (int)n);
-}
-
-// A weight of at most 1 as a whole number of 2^-bits, rounded to nearest (bits <= 51): the last bits of 2^52 + w 2^bits.
-__device__ __forceinline__ uint64_t whole(double w, int bits) {
-    return __builtin_bit_cast(uint64_t, ldexp(w, bits) + 4503599627370496.0) & 0xfffffffffffffull;
-}
+// Weights 2^t, t <= 0: 2^n times the series of e^(f ln 2), |f| <= 1/2, to the 11th power: 6e-15 left out.  The
+// coefficients are kept in scalar registers: as literals each took two moves to the vector registers a word.
+struct Exp2 {
+    double c[12];
+    __device__ __forceinline__ Exp2() {
+        double f = 1.0;
+#pragma unroll
+        for (int i = 0; i < 12; ++i) {   // ln 2^i / i!
+            c[i] = f;
+            f *= 0.6931471805599453 / (i + 1);
+        }
+#pragma unroll
+        for (int i = 2; i < 12; ++i) asm("" : "+s"(c[i]));
+    }
+    // 2^(t + bits)
+    __device__ __forceinline__ double operator()(double t, int bits = 0) const {
+        const double n = rint(t), f = t - n;
+        double p = c[11];
+#pragma unroll
+        for (int i = 10; i > 0; --i) p = fma(p, f, c[i]);
+        return ldexp(fma(p, f, 1.0), (int)n + bits);
+    }
+    // The same as a whole number, rounded to nearest (bits <= 51): the last bits of 2^52 + it.
+    __device__ __forceinline__ uint64_t whole(double t, int bits) const {
+        return __builtin_bit_cast(uint64_t, (*this)(t, bits) + 4503599627370496.0) & 0xfffffffffffffull;
+    }
+};
 
 // Words in order as ascending 64-bit numbers: logit (largest first; -0 is 0), then index.
 __device__ __forceinline__ uint64_t word_order(float x, uint32_t i) {
@@ -107,24 +119,62 @@ __device__ __forceinline__ f4_t load_words(const float* __restrict__ x, int i, i
     return v;
 }
 
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp_or_zero(T v) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    }
+}
+// The sum over the wave's lanes up to each: steps inside its rows of 16 lanes, then the rows' last lanes.
+template <class T>
+__device__ __forceinline__ T wave_prefix(T v) {
+    v += dpp_or_zero<0x111, 0xf>(v);
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);
+    v += dpp_or_zero<0x143, 0xc>(v);
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T lane_of(T v, int lane) {   // (lane: the same for all)
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+        return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    }
+}
+
 // Bound by the logits' bytes, and for many rows by some 25 fp64 instructions a word beside them.
 __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const SampleArgs a) {
-    __shared__ unsigned long long mass[kBins];
-    __shared__ uint32_t count[kBins];
-    __shared__ float wave_max[kChunkThreads / kWave];
-    __shared__ uint32_t first, bad;
-    const int row = blockIdx.x / a.nchunk, chunk = blockIdx.x - row * a.nchunk, tid = threadIdx.x;
+    constexpr int kWaves = kChunkThreads / kWave, kBinWaves = kBins / kWave;
+    __shared__ unsigned long long mass[kBins], wave_mass[kWaves];
+    __shared__ uint32_t count[kBins], wave_count[kWaves];
+    __shared__ float wave_max[kWaves];
+    __shared__ __align__(16) uint16_t place[kChunk];
+    __shared__ uint32_t first, bad, bins;
+    const int row = blockIdx.x / a.nchunk, chunk = blockIdx.x - row * a.nchunk, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* x = a.logits + row * a.stride;
     f4_t v[kPerThread / 4];
 #pragma unroll
     for (int j = 0; j < kPerThread / 4; ++j) v[j] = load_words(x, chunk * kChunk + 4 * (tid + kChunkThreads * j), a.vocab);
-    for (int b = tid; b < kBins; b += kChunkThreads) {
-        mass[b] = 0;
-        count[b] = 0;
+    const double scale = word_scale(a, row);
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f, least = a.min_p ? a.min_p[row] : 0.0f;
+    if (tid < kBins) {
+        mass[tid] = 0;
+        count[tid] = 0;
     }
     if (tid == 0) {
         first = kNoToken;
-        bad = 0;
+        bad = bins = 0;
     }
     float m = -INFINITY;
     bool odd = false;
@@ -136,299 +186,143 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
             odd |= !(v[j][e] < INFINITY);
         }
     m = wave_max_dpp(m);
-    if ((tid & 63) == 0) wave_max[tid >> 6] = m;
+    if (__builtin_amdgcn_ballot_w64(odd)) m = NAN;   // (told to all below)
+    if (lane == 0) wave_max[wave] = m;
     __syncthreads();
+    bool wrong = false;
+    m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kChunkThreads / kWave; ++w) m = fmaxf(m, wave_max[w]);
-    if (odd) bad = 1;
-    uint32_t at = kNoToken;
-#pragma unroll
-    for (int j = kPerThread / 4 - 1; j >= 0; --j)
-#pragma unroll
-        for (int e = 3; e >= 0; --e)
-            if (v[j][e] == m) at = chunk * kChunk + 4 * (tid + kChunkThreads * j) + e;
-    if (at != kNoToken && m > -INFINITY) atomicMin(&first, at);
-    const double scale = word_scale(a, row);
+    for (int w = 0; w < kWaves; ++w) {
+        wrong |= wave_max[w] != wave_max[w];
+        m = fmaxf(m, wave_max[w]);
+    }
+    Chunk& out = a.chunks[blockIdx.x];
     const double ym = m > -INFINITY ? scaled(m, scale) : 0.0, top = floor(8.0 * ym);
-    if (scale >= 0.0 && m < INFINITY) {
+    if (scale < 0.0 || wrong || !(m > -INFINITY)) {   // the largest is all that counts, if anything does
+        uint32_t at = kNoToken;
 #pragma unroll
-        for (int j = 0; j < kPerThread / 4; ++j)
+        for (int j = kPerThread / 4 - 1; j >= 0; --j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (!(v[j][e] > -INFINITY)) continue;
-                const double y = scaled(v[j][e], scale), below = top - floor(8.0 * y);
-                if (!(below < kBins - 1)) continue;
-                atomicAdd(&mass[(int)below], (unsigned long long)whole(exp2_below(y - ym), kBits));
-                atomicAdd(&count[(int)below], 1u);
-            }
+            for (int e = 3; e >= 0; --e)
+                if (v[j][e] == m) at = chunk * kChunk + 4 * (tid + kChunkThreads * j) + e;
+        if (at != kNoToken && m > -INFINITY) atomicMin(&first, at);
+        __syncthreads();
+        if (tid == 0) out.head = ChunkHead{top, m, first, wrong, {0, 0, 0}};
+        return;   // (the row's kernel reads no bins of such a chunk)
+    }
+    const Exp2 exp2;
+    uint32_t rank[kPerThread];   // bin and place inside it
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+        const float t = v[j >> 2][j & 3];
+        const double y = scaled(t, scale), below = top - floor(8.0 * y);
+        const uint64_t w = exp2.whole(y - ym, kBits);
+        rank[j] = kNoToken;
+        if (t > -INFINITY && below < kBins - 1) {
+            const int b = (int)below;
+            atomicAdd(&mass[b], (unsigned long long)w);
+            rank[j] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
+        }
     }
     __syncthreads();
-    if (tid == 0) a.head[blockIdx.x] = ChunkHead{top, m, first, bad, {0, 0, 0}};
-    if (scale < 0.0) return;
-    for (int b = tid; b < kBins; b += kChunkThreads) {
-        a.mass[(int64_t)blockIdx.x * kBins + b] = mass[b];
-        a.count[(int64_t)blockIdx.x * kBins + b] = count[b];
+    // sums over the bins up to each
+    uint64_t ms = 0;
+    uint32_t cs = 0;
+    if (wave < kBinWaves) {
+        ms = wave_prefix<uint64_t>(mass[tid]);
+        cs = wave_prefix<uint32_t>(count[tid]);
+        if (lane == kWave - 1) {
+            wave_mass[wave] = ms;
+            wave_count[wave] = cs;
+        }
     }
-}
-
-// Where the words that count end: those of the bins below `bin`, and of `bin` those up to `order`.
-struct Cut {
-    int bin;
-    uint64_t order;
-};
-__device__ __forceinline__ Cut earlier(Cut a, Cut b) {
-    return a.bin < b.bin || (a.bin == b.bin && a.order < b.order) ? a : b;
+    __syncthreads();
+    if (wave < kBinWaves) {
+        const uint32_t own = count[tid];
+#pragma unroll
+        for (int w = 0; w < kBinWaves; ++w)
+            if (w < wave) {
+                ms += wave_mass[w];
+                cs += wave_count[w];
+            }
+        out.mass[tid] = ms;
+        out.upto[tid] = (uint16_t)cs;
+        count[tid] = cs - own;   // words in front of the bin
+        // the bins whose words the rules may ask for one by one: of a chunk's words the first k, and, if top-p does
+        // not have to know what top-k keeps, those of min_p of its largest (and one bin more for the roundings)
+        const float deep = least > 0.0f && !(k > 0 && p < 1.0f) ? 2.5f - 8.0f * log2f(fminf(least, 1.0f)) : (float)kBins;
+        const bool ask = (k > 0 || p < 1.0f || least > 0.0f) && tid < kBins - 1 && tid <= deep && (k <= 0 || cs - own < (uint32_t)k);
+        const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(ask));   // (the first so many)
+        if (lane == 0 && n) atomicAdd(&bins, (uint32_t)n);
+    }
+    __syncthreads();
+    const int asked = (int)bins;
+    if (tid == 0) out.head = ChunkHead{top, m, 0, 0, {0, 0, 0}};
+    if (!asked) return;
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+        const int b = (int)(rank[j] >> 16);
+        if (b < asked) place[count[b] + (rank[j] & 0xffffu)] = (uint16_t)(4 * (tid + kChunkThreads * (j >> 2)) + (j & 3));
+    }
+    __syncthreads();
+    const int stored = (int)count[asked];   // (the last bin, which is never asked for, has words in front too)
+    for (int i = tid; i < (stored + 7) / 8; i += kChunkThreads)
+        reinterpret_cast<uint4*>(out.place)[i] = reinterpret_cast<const uint4*>(place)[i];
 }
 
 struct RowLds {
-    unsigned long long list[kList];
+    uint64_t list[kList], weight[kList];      // words in order, and their weights
     double chunk_mass[kMostChunks], chunk_scale[kMostChunks];
-    unsigned long long chunk_part[kMostChunks];   // of it, the words of the cut's own bin
+    unsigned long long chunk_part[kMostChunks];
     int chunk_shift[kMostChunks];
-    double mass[kBins], half_mass[kBins];     // of a bin, then of all up to it
-    uint32_t count[kBins], half_count[kBins];
-    unsigned long long digit_mass[256];
-    uint32_t digit_count[256];
-    unsigned long long lo, hi, sum, before_mass;
-    uint32_t n, before_count, digit, found;
-    double red[kRowThreads / kWave];
-    float fred[kRowThreads / kWave];
+    double mass[kBins];                       // of all bins up to each
+    uint32_t count[kBins];
+    // a pass fills one of them and clears the next: with three, a wave that still reads the last one is not disturbed
+    unsigned long long digit_mass[3][256];
+    uint32_t digit_count[3][256];
+    double goal, sum;
+    unsigned long long lo, hi;
+    float max[kRowThreads / kWave];
+    uint32_t n, found;
+    int least_bin;
 };
 
-// One row's search, by all threads of its workgroup.
-struct RowSearch {
-    const SampleArgs& a;
-    RowLds& l;
-    const float* x;
-    double scale, ym, top;   // y of the largest and floor(8 y)
-    int list_lo, list_hi;   // the bins whose words are in the list (none: lo > hi)
-    int list_n;
-
-    __device__ __forceinline__ double bin_of(float v) const { return top - floor(8.0 * scaled(v, scale)); }
-    __device__ __forceinline__ double weight(float v) const { return exp2_below(scaled(v, scale) - ym); }
-    __device__ __forceinline__ bool inside(uint64_t order, int bin, const Cut& c) const {
-        return bin < c.bin || (bin == c.bin && order <= c.order);
-    }
-
-    // f(order, bin) of the row's words in bins lo .. hi, each by one thread, in any order.
-    template <class F>
-    __device__ __forceinline__ void scan(int lo, int hi, F&& f) const {
-        // a range of logits that holds the bins', with room for the roundings: what is outside needs no fp64
-        const double step = 8.0 * scale;
-        const double first = (top - hi) / step, last = (top - lo + 1.0) / step;
-        const bool wide = !(step > 0.0);
-        const float from = wide ? -INFINITY : (float)(first - fabs(first) * 1e-6 - 1e-30);
-        const float to = wide ? INFINITY : (float)(last + fabs(last) * 1e-6 + 1e-30);
-        constexpr int kAtOnce = 4;
-        for (int i = 4 * threadIdx.x; i < a.vocab; i += 4 * kAtOnce * kRowThreads) {
-            f4_t v[kAtOnce];
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) v[j] = load_words(x, min(i + 4 * kRowThreads * j, a.vocab), a.vocab);
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float t = v[j][e];
-                    if (t < from || t > to || t == -INFINITY) continue;
-                    const double b = bin_of(t);
-                    if (b >= lo && b <= hi) f(word_order(t, i + 4 * kRowThreads * j + e), (int)b);
-                }
-        }
-    }
-    // The same from the list where it has them.
-    template <class F>
-    __device__ __forceinline__ void each(int lo, int hi, F&& f) const {
-        if (list_lo <= lo && hi <= list_hi) {
-            for (int i = threadIdx.x; i < list_n; i += kRowThreads) {
-                const uint64_t order = l.list[i];
-                const int b = (int)bin_of(word_logit(order));
-                if (b >= lo && b <= hi) f(order, b);
-            }
-        } else {
-            scan(lo, hi, f);
-        }
-    }
-    // Puts the words of bin b into the list, with all before it if they fit.
-    __device__ void want(int b) {
-        if (list_lo <= b && b <= list_hi) return;
-        const uint32_t upto = l.count[b], own = upto - (b ? l.count[b - 1] : 0);
-        if (own > kList) return;
-        const int lo = upto <= kList ? 0 : b;
-        __syncthreads();
-        if (threadIdx.x == 0) l.n = 0;
-        __syncthreads();
-        scan(lo, b, [&](uint64_t order, int) {
-            const uint32_t at = atomicAdd(&l.n, 1u);
-            if (at < kList) l.list[at] = order;
-        });
-        __syncthreads();
-        list_lo = lo;
-        list_hi = b;
-        list_n = min((int)l.n, kList);
-    }
-
-    // The first word, by key(order), of those of bins lo .. hi that keep(order, bin) takes at which, with the
-    // words before it, there are `words` of them (by count), or their weights reach `target` 2^-bits; the last
-    // one where none does.  before: weights of those in front.  Radix search, 8 bits a pass, over the bits in which
-    // the keys differ.
-    template <bool COUNT, class K, class P>
-    __device__ uint64_t search(int lo, int hi, K&& key, P&& keep, uint32_t words, uint64_t target, int bits, uint64_t& before) {
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            l.lo = ~0ull;
-            l.hi = 0;
-        }
-        __syncthreads();
-        uint64_t least = ~0ull, most = 0;
-        each(lo, hi, [&](uint64_t order, int b) {
-            if (!keep(order, b)) return;
-            const uint64_t k = key(order);
-            least = k < least ? k : least;
-            most = k > most ? k : most;
-        });
-        // (one atomic a wave: those of all lanes on one place would follow each other)
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t t = __shfl_xor((unsigned long long)least, o, kWave), u = __shfl_xor((unsigned long long)most, o, kWave);
-            least = t < least ? t : least;
-            most = u > most ? u : most;
-        }
-        if ((threadIdx.x & 63) == 0) {
-            atomicMin(&l.lo, (unsigned long long)least);
-            atomicMax(&l.hi, (unsigned long long)most);
-        }
-        __syncthreads();
-        uint64_t value = l.lo;   // the bits that are known, and zeros
-        const uint64_t differ = l.lo ^ l.hi;
-        before = 0;
-        uint32_t before_n = 0;
-        if (!differ) return value;
-        int end = 64 - __clzll((long long)differ);   // bits not known yet
-        value = end == 64 ? 0 : value >> end << end;
-        while (end > 0) {
-            const int shift = end > 8 ? end - 8 : 0;
-            const uint64_t known = end == 64 ? 0 : ~0ull << end;
-            const uint32_t mask = (1u << (end - shift)) - 1;
-            __syncthreads();
-            if (threadIdx.x < 256) {
-                l.digit_mass[threadIdx.x] = 0;
-                l.digit_count[threadIdx.x] = 0;
-            }
-            __syncthreads();
-            each(lo, hi, [&](uint64_t order, int b) {
-                if (!keep(order, b)) return;
-                const uint64_t k = key(order);
-                if ((k & known) != value) return;
-                const uint32_t d = (uint32_t)(k >> shift) & mask;
-                atomicAdd(&l.digit_count[d], 1u);
-                atomicAdd(&l.digit_mass[d], (unsigned long long)whole(weight(word_logit(order)), bits));
-            });
-            __syncthreads();
-            if (threadIdx.x < kWave) {   // four digits a lane
-                uint32_t c[4], cs = 0;
-                uint64_t w[4], ws = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    c[e] = l.digit_count[4 * threadIdx.x + e];
-                    w[e] = l.digit_mass[4 * threadIdx.x + e];
-                    cs += c[e];
-                    ws += w[e];
-                }
-                uint32_t ci = cs;
-                uint64_t wi = ws;
-                for (int o = 1; o < kWave; o <<= 1) {
-                    const uint32_t t = __shfl_up(ci, o, kWave);
-                    const uint64_t s = __shfl_up((unsigned long long)wi, o, kWave);
-                    if ((int)threadIdx.x >= o) {
-                        ci += t;
-                        wi += s;
-                    }
-                }
-                uint32_t cb = before_n + ci - cs;
-                uint64_t wb = before + wi - ws;
-                int hit = -1, last = -1;
-                uint32_t hit_c = 0, last_c = 0;
-                uint64_t hit_w = 0, last_w = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (c[e]) {
-                        last = e;
-                        last_c = cb;
-                        last_w = wb;
-                        if (hit < 0 && (COUNT ? cb + c[e] >= words : wb + w[e] >= target)) {
-                            hit = e;
-                            hit_c = cb;
-                            hit_w = wb;
-                        }
-                    }
-                    cb += c[e];
-                    wb += w[e];
-                }
-                const uint64_t hits = __builtin_amdgcn_ballot_w64(hit >= 0), any = __builtin_amdgcn_ballot_w64(last >= 0);
-                const int lane = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(any);
-                if ((int)threadIdx.x == lane) {
-                    const bool h = hits != 0;
-                    l.digit = 4 * lane + (h ? hit : last);
-                    l.before_count = h ? hit_c : last_c;
-                    l.before_mass = h ? hit_w : last_w;
-                    l.found = c[h ? hit : last];
-                }
-            }
-            __syncthreads();
-            before = l.before_mass;
-            before_n = l.before_count;
-            value |= (uint64_t)l.digit << shift;
-            end = shift;
-            if (l.found == 1 && end > 0) {   // the one that is left
-                const uint64_t rest = ~0ull << end;
-                each(lo, hi, [&](uint64_t order, int b) {
-                    if (!keep(order, b)) return;
-                    const uint64_t k = key(order);
-                    if ((k & rest) == value) l.lo = k;
-                });
-                __syncthreads();
-                return l.lo;
-            }
-        }
-        return value;
-    }
-};
-
-// Sums of v over the workgroup's first kBins threads up to each of them (all threads call it).
-template <class T>
-__device__ __forceinline__ void scan_bins(T* v, T* wave_sum) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    T sum = t < kBins ? v[t] : T(0);
-    for (int o = 1; o < kWave; o <<= 1) {
-        const T add = __shfl_up(sum, o, kWave);
-        if (lane >= o) sum += add;
-    }
-    if (lane == kWave - 1) wave_sum[wave] = sum;
-    __syncthreads();
-    T before = T(0);
-    for (int w = 0; w < wave; ++w) before += wave_sum[w];
-    if (t < kBins) v[t] = before + sum;
-    __syncthreads();
-}
-
+// One row.  Bound by latency: some 30 steps between barriers, and a trip to the chunks' bins, to the places of the
+// words that are ranked, and to these.
 __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArgs a) {
     __shared__ RowLds l;
+    constexpr int kWaves = kRowThreads / kWave;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const ChunkHead* head = a.head + (int64_t)row * a.nchunk;
+    const Chunk* chunks = a.chunks + (int64_t)row * a.nchunk;
+    const float* x = a.logits + row * a.stride;
     const double scale = word_scale(a, row);
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const double p = a.top_p ? (double)a.top_p[row] : 1.0, least = a.min_p ? (double)a.min_p[row] : 0.0;
+    const float given = a.u[row];
     // the row's maximum, its first word and whether all is well
     float m = -INFINITY;
-    bool bad = false;
+    bool wrong = false;
     for (int c = tid; c < a.nchunk; c += kRowThreads) {
-        m = fmaxf(m, head[c].max);
-        bad |= head[c].bad != 0;
+        m = fmaxf(m, chunks[c].head.max);
+        wrong |= chunks[c].head.bad != 0;
     }
     m = wave_max_dpp(m);
-    if (lane == 0) l.fred[wave] = m;
+    if (__builtin_amdgcn_ballot_w64(wrong)) m = NAN;
+    if (lane == 0) l.max[wave] = m;
     if (tid == 0) l.found = kNoToken;
-    const bool any_bad = __syncthreads_or(bad);
+    if (tid < 256) {
+        l.digit_mass[0][tid] = 0;
+        l.digit_count[0][tid] = 0;
+    }
+    __syncthreads();
+    wrong = false;
+    m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kRowThreads / kWave; ++w) m = fmaxf(m, l.fred[w]);
-    if (any_bad || !(m > -INFINITY)) {
+    for (int w = 0; w < kWaves; ++w) {
+        wrong |= l.max[w] != l.max[w];
+        m = fmaxf(m, l.max[w]);
+    }
+    if (wrong || !(m > -INFINITY)) {
         if (tid == 0) {
             a.ids[row] = kNoToken;
             if (a.probs) a.probs[row] = 0.0f;
@@ -438,7 +332,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
     }
     if (scale < 0.0) {   // the largest
         for (int c = tid; c < a.nchunk; c += kRowThreads)
-            if (head[c].max == m) atomicMin(&l.found, head[c].arg);
+            if (chunks[c].head.max == m) atomicMin(&l.found, chunks[c].head.arg);
         __syncthreads();
         if (tid == 0) {
             a.ids[row] = l.found;
@@ -446,161 +340,257 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         }
         return;
     }
+    const Exp2 exp2;
     const double ym = scaled(m, scale), top = floor(8.0 * ym);
-    RowSearch s{a, l, a.logits + row * a.stride, scale, ym, top, 1, 0, 0};
+    auto below = [&](float v) { return fmax(scaled(v, scale) - ym, -1000.0); };   // log2 of a weight
+    auto bin_of = [&](float v) { return top - floor(8.0 * scaled(v, scale)); };
     // how far a chunk's bins and largest weight lie below the row's
     for (int c = tid; c < a.nchunk; c += kRowThreads) {
-        const bool some = head[c].max > -INFINITY;
-        const double down = top - head[c].top;
+        const float cm = chunks[c].head.max;
+        const bool some = cm > -INFINITY;
+        const double down = top - chunks[c].head.top;
         l.chunk_shift[c] = some && down < kBins ? (int)down : kBins;
-        l.chunk_scale[c] = some ? ldexp(s.weight(head[c].max), -kBits) : 0.0;
+        l.chunk_scale[c] = some ? exp2(below(cm), -kBits) : 0.0;
     }
     __syncthreads();
-    // the row's bins: two threads each, every other chunk
-    const uint64_t* cm = a.mass + (int64_t)row * a.nchunk * kBins;
-    const uint32_t* cc = a.count + (int64_t)row * a.nchunk * kBins;
-    if (tid < 2 * kBins) {
-        const int half = tid >= kBins, b = tid - half * kBins;
+    // what the row's bins up to each hold
+    if (wave < kBins / kWave) {
         double w = 0.0;
         uint32_t n = 0;
-        if (b < kBins - 1) {
-#pragma unroll 4
-            for (int c = half; c < a.nchunk; c += 2) {
-                const int from = b - l.chunk_shift[c];
-                const int64_t at = (int64_t)c * kBins + max(from, 0);
-                const uint64_t cw = cm[at];
-                const uint32_t cn = cc[at];
-                if (from >= 0) {
-                    w += (double)cw * l.chunk_scale[c];
-                    n += cn;
+#pragma unroll 8
+        for (int c = 0; c < a.nchunk; ++c) {
+            const int at = tid - l.chunk_shift[c];
+            const double cw = (double)chunks[c].mass[max(at, 0)];
+            const uint32_t cn = chunks[c].upto[max(at, 0)];
+            w += at >= 0 ? cw * l.chunk_scale[c] : 0.0;
+            n += at >= 0 ? cn : 0;
+        }
+        l.mass[tid] = w;
+        l.count[tid] = n;
+    } else if (wave == kWaves - 1) {
+        // the bin that min-p cuts through: behind it no other rule matters (and chunks need not have kept their words)
+        const double at = least > 0.0 ? top - floor(8.0 * (ym + log2(fmin(least, 1.0)))) : (double)kBins;
+        if (lane == 0) l.least_bin = at < kBins ? (int)at : kBins;
+    }
+    __syncthreads();
+    const int least_bin = l.least_bin;
+
+    // The words that count are those up to last_order and of at least least_whole, all of bins up to last_bin
+    // (whole_bin: all of that one's).  The list holds the words of bins list_lo .. list_hi (none: list_lo > list_hi).
+    int last_bin = kBins - 2, list_lo = 1, list_hi = 0, list_n = 0;
+    uint64_t last_order = ~0ull;
+    const uint64_t least_whole = least > 0.0 ? (uint64_t)ceil(ldexp(fmin(least, 1.0), kBits)) : 0;
+    bool whole_bin = true;
+    double total = l.mass[kBins - 2];
+    int buf = 0;   // the digits that are clear
+    const double u = given > 0.0f ? fmin((double)given, 1.0) : 0.0;
+
+    // top-k, top-p, and the draw from the list (or, where many words count, the sums of the last bin's by chunk).
+    // One loop, and in it one loop of passes over the words, so that the code is there and fetched once.
+    for (int rule = 0; rule < 3; ++rule) {
+        uint32_t words = 0;   // the search: the first word up to which there are so many,
+        double goal = 0.0;    // or weights of at least (the draw: more than) goal
+        int b = last_bin;
+        if (rule == 0) {
+            if (!(k > 0) && !(least > 1.0)) continue;
+            words = least > 1.0 ? 1 : (uint32_t)k;
+        }
+        if (rule == 1) {
+            if (!(p < 1.0)) continue;
+            goal = p * total;
+        }
+        if (rule < 2) {
+            b = 0;   // the bins up to which there is not enough
+            for (int t = lane; t < kBins; t += kWave)
+                b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(t < kBins - 1 && (rule == 0 ? l.count[t] < words : l.mass[t] < goal)));
+            if (rule == 0 && (b == kBins - 1 || (b > least_bin && !(p < 1.0)))) continue;   // (not so many, or no matter)
+            if (rule == 1 && b > least_bin) continue;
+            b = min(b, last_bin);
+        } else {
+            if (least_bin <= last_bin) {
+                last_bin = b = (int)least_bin;
+                whole_bin = false;
+            }
+            if (whole_bin) break;   // no word to be looked at by itself
+        }
+        // the words of bin b, with all before it if they fit
+        const uint32_t upto = l.count[b], before_b = b ? l.count[b - 1] : 0;
+        bool listed = list_lo <= b && b <= list_hi;
+        if (!listed) {
+            const int lo = upto <= kList ? 0 : b;
+            list_n = (int)(lo ? upto - before_b : upto);
+            listed = list_n <= kList;
+            list_lo = listed ? lo : 1;
+            list_hi = listed ? b : 0;
+            if (tid == 0) l.n = 0;
+            __syncthreads();
+            for (int c = wave; listed && c < a.nchunk; c += kRowThreads / kWave) {
+                const int cb = b - l.chunk_shift[c], cl = lo - l.chunk_shift[c];
+                if (cb < 0) continue;
+                const int i0 = cl > 0 ? chunks[c].upto[cl - 1] : 0, i1 = chunks[c].upto[cb];
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&l.n, (uint32_t)(i1 - i0));
+                at = __builtin_amdgcn_readfirstlane(at);
+                for (int i = i0 + lane; i < i1; i += kWave) {
+                    const uint32_t id = min(c * kChunk + (chunks[c].place[i] & (kChunk - 1)), a.vocab - 1);
+                    const float t = x[id];
+                    l.list[at + i - i0] = word_order(t, id);
+                    l.weight[at + i - i0] = exp2.whole(below(t), kBits);
                 }
             }
-        }
-        (half ? l.half_mass : l.mass)[b] = w;
-        (half ? l.half_count : l.count)[b] = n;
-    }
-    __syncthreads();
-    if (tid < kBins) {
-        l.mass[tid] += l.half_mass[tid];
-        l.count[tid] += l.half_count[tid];
-    }
-    __syncthreads();
-    scan_bins(l.mass, l.red);
-    scan_bins(l.count, l.digit_count);
-    // the first bin up to which pred holds (kBins - 1: none)
-    auto first_bin = [&](auto pred) {
-        __syncthreads();
-        if (tid == 0) l.found = kBins - 1;
-        __syncthreads();
-        if (tid < kBins - 1 && pred(tid)) atomicMin(&l.found, (uint32_t)tid);
-        __syncthreads();
-        return (int)l.found;
-    };
-    // bits of a weight where so many are summed
-    auto bits_for = [](uint32_t n) { return min(kBits, 62 - (32 - __clz((int)(n | 1u)))); };
-    auto order_key = [](uint64_t order) { return order; };
-    Cut cut{kBins - 2, ~0ull};
-    double total = l.mass[kBins - 2];
-
-    // top-k: the first k words
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0) {
-        const int b = first_bin([&](int t) { return l.count[t] >= (uint32_t)k; });
-        if (b < kBins - 1) {
-            const uint32_t in_front = b ? l.count[b - 1] : 0;
-            s.want(b);
-            uint64_t before;
-            const int bits = bits_for(l.count[b] - in_front);
-            const uint64_t at =
-                s.search<true>(b, b, order_key, [](uint64_t, int) { return true; }, (uint32_t)k - in_front, 0, bits, before);
-            cut = Cut{b, at};
-            total = (b ? l.mass[b - 1] : 0.0) + ldexp((double)before, -bits) + s.weight(word_logit(at));
-        }
-    }
-    // top-p: the fewest of those that hold p of their weight
-    const double p = a.top_p ? (double)a.top_p[row] : 1.0;
-    if (p < 1.0) {
-        const double goal = p * total;
-        const int b = min(first_bin([&](int t) { return l.mass[t] >= goal; }), cut.bin);
-        s.want(b);
-        const double in_front = b ? l.mass[b - 1] : 0.0;
-        const int bits = bits_for(l.count[b] - (b ? l.count[b - 1] : 0));
-        const uint64_t target = goal > in_front ? (uint64_t)ceil(ldexp(goal - in_front, bits)) : 0;
-        uint64_t before;
-        const uint64_t at =
-            s.search<false>(b, b, order_key, [&](uint64_t order, int bin) { return s.inside(order, bin, cut); }, 0, target, bits, before);
-        cut = earlier(cut, Cut{b, at});
-    }
-    // min-p: those of at least min_p of the largest weight, the largest among them
-    const double least = a.min_p ? (double)a.min_p[row] : 0.0;
-    if (least > 0.0) {
-        const double down = top - floor(8.0 * (ym + log2(fmin(least, 1.0))));
-        if (down <= cut.bin) {
-            const int b = (int)down;
-            s.want(b);
             __syncthreads();
-            if (tid == 0) l.hi = 0;
-            __syncthreads();
-            s.each(b, b, [&](uint64_t order, int) {
-                if (s.weight(word_logit(order)) >= fmin(least, 1.0)) atomicMax(&l.hi, (unsigned long long)order);
-            });
-            __syncthreads();
-            cut = earlier(cut, Cut{b, l.hi});
         }
-    }
-    if (least > 1.0) {   // the first of the order alone
-        s.want(0);
-        uint64_t before;
-        cut = Cut{0, s.search<true>(0, 0, order_key, [](uint64_t, int) { return true; }, 1, 0, kBits - 11, before)};
-    }
-
-    // draw
-    const float given = a.u[row];
-    const double u = given > 0.0f ? fmin((double)given, 1.0) : 0.0;
-    if (s.list_lo == 0 && cut.bin <= s.list_hi) {
-        // every word that counts is in the list
-        auto keep = [&](uint64_t order, int bin) { return s.inside(order, bin, cut); };
-        __syncthreads();
-        if (tid == 0) l.sum = 0;
-        __syncthreads();
-        uint64_t own = 0;
-        s.each(0, cut.bin, [&](uint64_t order, int bin) {
-            if (keep(order, bin)) own += whole(s.weight(word_logit(order)), kBits);
-        });
-        for (int o = 32; o > 0; o >>= 1) own += __shfl_xor((unsigned long long)own, o, kWave);
-        if (lane == 0) atomicAdd(&l.sum, (unsigned long long)own);
-        __syncthreads();
-        const uint64_t sum = l.sum;
-        const uint64_t goal = (uint64_t)fmin(u * (double)sum, 18446744073709549568.0);
-        uint64_t before;
-        const uint64_t id = s.search<false>(0, cut.bin, [](uint64_t order) { return order & 0xffffffffull; }, keep, 0,
-                                            (goal < sum ? goal : sum - 1) + 1, kBits, before);
-        if (tid == 0) {
-            a.ids[row] = (uint32_t)id;
-            if (a.probs) a.probs[row] = (float)(s.weight(s.x[id]) / ldexp((double)sum, -kBits));
-        }
-        return;
-    }
-    // what each chunk holds: its bins below the cut's, and the words of that bin one by one
-    const bool whole_bin = cut.order == ~0ull;
-    const int bins = cut.bin + (whole_bin ? 1 : 0);
-    for (int c = wave; c < a.nchunk; c += kRowThreads / kWave) {
-        const int n = bins - l.chunk_shift[c];
-        double w = 0.0;
-        for (int b = lane; b < n; b += kWave) w += (double)cm[(int64_t)c * kBins + b];
+        const bool draw = rule == 2 && list_lo == 0 && b <= list_hi;
+        // what lies in front of the words that are searched
+        double before = list_lo == 0 || !b ? 0.0 : l.mass[b - 1];
+        uint32_t before_n = list_lo == 0 ? 0 : before_b;
+        const int bits = min(kBits, 62 - (32 - __clz((int)(upto - before_b))));
+        // a range of logits that holds bin b's, with room for the roundings
+        const double step = 8.0 * scale, e0 = (top - b) / step, e1 = (top - b + 1.0) / step;
+        const float from = step > 0.0 ? (float)fmax(e0 - fabs(e0) * 1e-6 - 1e-30, -3.4028234663852886e38) : -3.4028234663852886e38f;
+        const float to = step > 0.0 && list_lo != 0 ? fminf((float)(e1 + fabs(e1) * 1e-6 + 1e-30), m) : m;
+        // Radix search over the bits in which the keys (order, or index) may differ, 8 a pass.  kDigits counts and
+        // weighs the words of the value so far by their next 8, kOne takes the only word left, kGather puts a group
+        // that fits into the list.  kParts: the last bin's words that count, by chunk.  Where a bin is too large for
+        // the list, its words are met in the row.
+        enum { kDigits, kOne, kGather, kParts };
+        const uint64_t lowest = word_order(to, 0), highest = word_order(from, kNoToken);
+        int mode = rule < 2 || draw ? kDigits : kParts;
+        int end = draw ? 32 - __clz(a.vocab) : 64 - __clzll((long long)(lowest ^ highest));
+        uint64_t known = end == 64 ? 0 : ~0ull << end, value = draw ? 0 : lowest & known;
+        bool opened = false;   // a draw's goal is known
+        if (mode == kParts)
+            for (int c = tid; c < a.nchunk; c += kRowThreads) l.chunk_part[c] = 0;
+        if (mode == kParts) __syncthreads();
+        for (;;) {
+            const int shift = end > 8 ? end - 8 : 0, next = buf == 2 ? 0 : buf + 1;
+            const uint32_t mask = (1u << (end - shift)) - 1;
+            if (mode == kDigits && tid < 256) {
+                l.digit_mass[next][tid] = 0;
+                l.digit_count[next][tid] = 0;
+            }
+            auto visit = [&](uint64_t order, uint64_t w) {
+                if (order > last_order || (rule == 2 && w < least_whole)) return;
+                const uint64_t key = draw ? order & 0xffffffffull : order;
+                if (mode == kParts) {
+                    atomicAdd(&l.chunk_part[(uint32_t)order / kChunk], (unsigned long long)w);
+                } else if ((key & known) == value) {
+                    if (mode == kDigits) {
+                        const uint32_t d = (uint32_t)(key >> shift) & mask;
+                        atomicAdd(&l.digit_count[buf][d], 1u);
+                        atomicAdd(&l.digit_mass[buf][d], (unsigned long long)w);
+                    } else if (mode == kOne) {
+                        l.lo = key;
+                    } else {
+                        const uint32_t at = atomicAdd(&l.n, 1u);
+                        l.list[at] = order;
+                        l.weight[at] = exp2.whole(below(word_logit(order)), kBits);
+                    }
+                }
+            };
+            if (listed) {
+                for (int i = tid; i < list_n; i += kRowThreads) visit(l.list[i], l.weight[i]);
+            } else {
+                for (int i = tid; i < a.vocab; i += 4 * kRowThreads) {
+                    float t[4];
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) w += __shfl_xor(w, o, kWave);
-        if (lane == 0) l.chunk_mass[c] = w * l.chunk_scale[c];
+                    for (int j = 0; j < 4; ++j) t[j] = i + j * kRowThreads < a.vocab ? x[i + j * kRowThreads] : -INFINITY;
+#pragma unroll 1
+                    for (int j = 0; j < 4; ++j) {
+                        const float v = j == 0 ? t[0] : j == 1 ? t[1] : j == 2 ? t[2] : t[3];
+                        if (v < from || v > to || v == -INFINITY || bin_of(v) != b) continue;
+                        visit(word_order(v, i + j * kRowThreads), exp2.whole(below(v), mode == kParts ? kBits : bits));
+                    }
+                }
+            }
+            __syncthreads();
+            if (mode == kParts) break;
+            if (mode == kOne) {
+                value = l.lo;
+                break;
+            }
+            if (mode == kGather) {
+                listed = true;
+                list_n = (int)l.n;
+                mode = kDigits;
+                continue;
+            }
+            // every wave by itself: four digits a lane
+            uint32_t c[4], cs = 0;
+            uint64_t w[4], ws = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                c[e] = l.digit_count[buf][4 * lane + e];
+                w[e] = l.digit_mass[buf][4 * lane + e];
+                cs += c[e];
+                ws += w[e];
+            }
+            buf = next;
+            uint32_t cb = wave_prefix<uint32_t>(cs);
+            uint64_t wb = wave_prefix<uint64_t>(ws);
+            const int at_bits = listed ? kBits : bits;
+            if (draw && !opened) {   // all weights have been seen
+                total = ldexp((double)lane_of(wb, kWave - 1), -at_bits);
+                goal = u * total;
+                opened = true;
+            }
+            cb -= cs;
+            wb -= ws;
+            int hit = -1;
+            uint32_t hit_n = 0, hit_c = 0;
+            uint64_t hit_w = 0;
+            bool met = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double sum = before + ldexp((double)(wb + w[e]), -at_bits);
+                if (c[e] && !met) {   // (none that meets it: the last)
+                    met = rule == 0 ? before_n + cb + c[e] >= words : rule == 1 ? sum >= goal : sum > goal;
+                    hit = e;
+                    hit_n = cb;
+                    hit_c = c[e];
+                    hit_w = wb;
+                }
+                cb += c[e];
+                wb += w[e];
+            }
+            const uint64_t hits = __builtin_amdgcn_ballot_w64(met), any = __builtin_amdgcn_ballot_w64(hit >= 0);
+            const int at = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(any | 1);
+            before += ldexp((double)lane_of(hit_w, at), -at_bits);
+            before_n += lane_of(hit_n, at);
+            const uint32_t left = lane_of(hit_c, at);
+            value |= (uint64_t)(uint32_t)(4 * at + lane_of(hit, at)) << shift;
+            end = shift;
+            if (end == 0) break;
+            known = ~0ull << end;
+            if (left == 1) mode = kOne;
+            else if (!listed && left <= kList) mode = kGather;
+            if (mode == kGather) {
+                if (tid == 0) l.n = 0;
+                __syncthreads();
+            }
+        }
+        if (mode == kParts) break;
+        if (draw) {
+            const uint32_t id = (uint32_t)value;
+            if (tid == 0) {
+                a.ids[row] = id;
+                if (a.probs) a.probs[row] = (float)(exp2(below(x[id])) / total);
+            }
+            return;
+        }
+        last_bin = b;
+        last_order = value;
+        whole_bin = false;
+        total = before + exp2(below(word_logit(value)));
+        __syncthreads();   // (l.lo has been read)
     }
-    if (!whole_bin) {
-        for (int c = tid; c < a.nchunk; c += kRowThreads) l.chunk_part[c] = 0;
-        __syncthreads();
-        s.each(cut.bin, cut.bin, [&](uint64_t order, int) {
-            if (order <= cut.order)
-                atomicAdd(&l.chunk_part[(uint32_t)order / kChunk], (unsigned long long)whole(s.weight(word_logit(order)), kBits));
-        });
-        __syncthreads();
-        for (int c = tid; c < a.nchunk; c += kRowThreads) l.chunk_mass[c] += ldexp((double)l.chunk_part[c], -kBits);
+
+    // Many words: what each chunk holds, its bins before the last and of that one what has been added up.
+    const int bins = last_bin + (whole_bin ? 1 : 0);
+    for (int c = tid; c < a.nchunk; c += kRowThreads) {
+        const int n = bins - l.chunk_shift[c];
+        l.chunk_mass[c] = (n > 0 ? (double)chunks[c].mass[n - 1] * l.chunk_scale[c] : 0.0) +
+                          (whole_bin ? 0.0 : ldexp((double)l.chunk_part[c], -kBits));
     }
     __syncthreads();
     // the chunk of the word: sums in the chunks' order, 64 at a time, by one wave
@@ -609,38 +599,26 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         for (int pass = 0; pass < 2; ++pass) {
             const double goal = u * sum;   // (the second time)
             double run = 0.0, base = 0.0;
-            int at = -1, last = 0;
-            double last_base = 0.0;
+            int at = 0;
             for (int c0 = 0; c0 < a.nchunk; c0 += kWave) {
                 const double w = c0 + lane < a.nchunk ? l.chunk_mass[c0 + lane] : 0.0;
-                double upto = w;
-                for (int o = 1; o < kWave; o <<= 1) {
-                    const double t = __shfl_up(upto, o, kWave);
-                    if (lane >= o) upto += t;
+                const double upto = wave_prefix<double>(w);
+                const uint64_t any = __builtin_amdgcn_ballot_w64(w > 0.0);
+                const uint64_t hit = pass ? __builtin_amdgcn_ballot_w64(w > 0.0 && run + upto > goal) : 0;
+                if (any) {   // (none past the goal, by roundings or u = 1: the last that holds something)
+                    const int e = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);
+                    at = c0 + e;
+                    base = run + lane_of(upto - w, e);
                 }
-                if (pass == 1) {
-                    const uint64_t hit = __builtin_amdgcn_ballot_w64(w > 0.0 && run + upto > goal);
-                    const uint64_t any = __builtin_amdgcn_ballot_w64(w > 0.0);
-                    if (any) {
-                        const int e = 63 - __builtin_clzll(any);
-                        last = c0 + e;
-                        last_base = run + __shfl(upto - w, e, kWave);
-                    }
-                    if (hit) {
-                        const int e = __builtin_ctzll(hit);
-                        at = c0 + e;
-                        base = run + __shfl(upto - w, e, kWave);
-                        break;
-                    }
-                }
-                run += __shfl(upto, kWave - 1, kWave);
+                if (hit) break;
+                run += lane_of(upto, kWave - 1);
             }
             if (pass == 0) {
                 sum = run;
             } else if (lane == 0) {
-                l.found = at >= 0 ? at : last;
-                l.red[0] = goal - (at >= 0 ? base : last_base);
-                l.red[1] = sum;
+                l.found = at;
+                l.goal = goal - base;
+                l.sum = sum;
             }
         }
     }
@@ -648,35 +626,29 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
     // the word of the chunk: a thread sums kChunk / kRowThreads of them that follow each other
     constexpr int kEach = kChunk / kRowThreads;
     const int first = (int)l.found * kChunk + kEach * tid;
-    const double rest = l.red[0], sum = l.red[1];
+    const double rest = l.goal, sum = l.sum;
     uint64_t w[kEach], own = 0;
 #pragma unroll
     for (int j = 0; j < kEach; j += 4) {
-        const f4_t v = load_words(s.x, min(first + j, a.vocab), a.vocab);
+        const f4_t v = load_words(x, min(first + j, a.vocab), a.vocab);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             w[j + e] = 0;
-            if (v[e] > -INFINITY) {
-                const double b = s.bin_of(v[e]);
-                if (b < kBins - 1 && s.inside(word_order(v[e], first + j + e), (int)b, cut)) w[j + e] = whole(s.weight(v[e]), kBits);
+            if (v[e] > -INFINITY && word_order(v[e], first + j + e) <= last_order && bin_of(v[e]) < kBins - 1) {
+                const uint64_t t = exp2.whole(below(v[e]), kBits);
+                if (t >= least_whole) w[j + e] = t;
             }
             own += w[j + e];
         }
     }
-    uint64_t upto = own;
-    for (int o = 1; o < kWave; o <<= 1) {
-        const uint64_t t = __shfl_up((unsigned long long)upto, o, kWave);
-        if (lane >= o) upto += t;
-    }
-    __syncthreads();
-    unsigned long long* wave_sum = l.digit_mass;
-    if (lane == kWave - 1) wave_sum[wave] = upto;
+    uint64_t upto = wave_prefix<uint64_t>(own);
+    if (lane == kWave - 1) l.digit_mass[0][wave] = upto;
     if (tid == 0) {
         l.lo = ~0ull;   // the first word past the goal
         l.hi = 0;       // the last one with a weight, plus one
     }
     __syncthreads();
-    for (int v = 0; v < wave; ++v) upto += wave_sum[v];
+    for (int v = 0; v < wave; ++v) upto += l.digit_mass[0][v];
     const uint64_t goal = rest > 0.0 ? (uint64_t)ldexp(rest, kBits) : 0;
     uint64_t run = upto - own;
 #pragma unroll
@@ -689,12 +661,12 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
     if (tid == 0) {
         const uint32_t id = l.lo != ~0ull ? (uint32_t)l.lo : (uint32_t)l.hi - 1;
         a.ids[row] = id;
-        if (a.probs) a.probs[row] = (float)(s.weight(s.x[id]) / sum);
+        if (a.probs) a.probs[row] = (float)(exp2(below(x[id])) / sum);
     }
 }
 
 static size_t sample_bytes(int64_t rows, int64_t nchunk) {
-    return (size_t)(rows * nchunk) * (sizeof(ChunkHead) + kBins * 12);
+    return (size_t)(rows * nchunk) * sizeof(Chunk);
 }
 
 }  // namespace rta
@@ -733,9 +705,7 @@ int rta_sample(const float* logits, int64_t stride, int rows, int vocab, const f
     a.ids = ids;
     a.probs = probs;
     const int64_t chunks = (int64_t)rows * a.nchunk;
-    a.head = static_cast<ChunkHead*>(workspace);
-    a.mass = reinterpret_cast<uint64_t*>(a.head + chunks);
-    a.count = reinterpret_cast<uint32_t*>(a.mass + chunks * kBins);
+    a.chunks = static_cast<Chunk*>(workspace);
     hipStream_t s = (hipStream_t)stream;
     hipLaunchKernelGGL(sample_chunk_kernel, dim3(chunks), dim3(kChunkThreads), 0, s, a);
     hipLaunchKernelGGL(sample_row_kernel, dim3(rows), dim3(kRowThreads), 0, s, a);

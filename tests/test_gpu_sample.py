@@ -56,7 +56,9 @@ def logits(rng, rows, vocab, sigma=2.5, sure=6.0):
 SIZES = [1, 2, 3, 5, 63, 64, 1000, 8191, 8192, 8193, 16385, 50001, 151936]
 RULES = {"none": {}, "t": dict(t=(0.2, 2.0)), "k": dict(k=(1, 3000)), "p": dict(p=(0.05, 0.999)), "least": dict(least=(1e-4, 0.5)),
          "all": dict(t=(0.2, 2.0), k=(1, 200), p=(0.2, 0.99), least=(0.001, 0.3)),
-         "wide": dict(t=(0.7, 3.0), k=(3000, 60000), p=(0.9, 0.9999), least=(1e-6, 1e-4)), "kp": dict(k=(1, 50), p=(0.1, 1.0))}
+         "wide": dict(t=(0.7, 3.0), k=(3000, 60000), p=(0.9, 0.9999), least=(1e-6, 1e-4)),
+         "kp": dict(k=(1, 50), p=(0.1, 1.0)), "deep": dict(t=(0.7, 3.0), p=(0.9, 0.999), least=(0.01, 0.9)),
+         "deep k": dict(k=(100, 9000), p=(0.5, 0.99), least=(0.05, 0.9)), "k least": dict(k=(1, 9000), least=(1e-5, 0.9))}
 
 
 @pytest.mark.parametrize("vocab", SIZES)
