@@ -24,6 +24,7 @@ constexpr int kBins = 384;         // 48 octaves; the last one holds everything 
 constexpr int kBits = 50;          // kChunk weights of up to 2^50 stay below 2^64
 constexpr int kRowThreads = 512, kMostChunks = 512;
 constexpr int kList = 8192;        // words ranked in LDS
+constexpr int kFromTop = 2048;     // words of all bins up to one that are ranked rather than that bin's alone
 constexpr uint32_t kNoToken = 0xffffffffu;
 
 struct ChunkHead {
@@ -37,7 +38,7 @@ struct ChunkHead {
 // What kernel 1 leaves of a chunk.
 struct Chunk {
     ChunkHead head;
-    uint64_t mass[kBins];       // weights of all bins up to each, against the chunk's largest
+    double mass[kBins];         // weights (in 2^-kBits) of all bins up to each, against the chunk's largest
     uint16_t upto[kBins];       // and their words
     alignas(16) uint16_t place[kChunk];   // words (from the chunk's first) by bins, in any order inside one
 };
@@ -155,8 +156,9 @@ __device__ __forceinline__ T lane_of(T v, int lane) {   // (lane: the same for a
 // Bound by the logits' bytes, and for many rows by some 25 fp64 instructions a word beside them.
 __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const SampleArgs a) {
     constexpr int kWaves = kChunkThreads / kWave, kBinWaves = kBins / kWave;
-    __shared__ unsigned long long mass[kBins], wave_mass[kWaves];
-    __shared__ uint32_t count[kBins], wave_count[kWaves];
+    // (behind the bins, a place a lane for words that do not count: no branches, and no lanes on one place)
+    __shared__ unsigned long long mass[kBins + kWave], wave_mass[kWaves];
+    __shared__ uint32_t count[kBins + kWave], wave_count[kWaves];
     __shared__ float wave_max[kWaves];
     __shared__ __align__(16) uint16_t place[kChunk];
     __shared__ uint32_t first, bad, bins;
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
     const double scale = word_scale(a, row);
     const int k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f, least = a.min_p ? a.min_p[row] : 0.0f;
-    if (tid < kBins) {
+    if (tid < kBins) {   // (what lies behind is never read)
         mass[tid] = 0;
         count[tid] = 0;
     }
@@ -217,12 +219,9 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
         const float t = v[j >> 2][j & 3];
         const double y = scaled(t, scale), below = top - floor(8.0 * y);
         const uint64_t w = exp2.whole(y - ym, kBits);
-        rank[j] = kNoToken;
-        if (t > -INFINITY && below < kBins - 1) {
-            const int b = (int)below;
-            atomicAdd(&mass[b], (unsigned long long)w);
-            rank[j] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
-        }
+        const int b = t > -INFINITY && below < kBins - 1 ? (int)below : kBins + lane;
+        atomicAdd(&mass[b], (unsigned long long)w);
+        rank[j] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
     }
     __syncthreads();
     // sums over the bins up to each
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
                 ms += wave_mass[w];
                 cs += wave_count[w];
             }
-        out.mass[tid] = ms;
+        out.mass[tid] = (double)ms;
         out.upto[tid] = (uint16_t)cs;
         count[tid] = cs - own;   // words in front of the bin
         // the bins whose words the rules may ask for one by one: of a chunk's words the first k, and, if top-p does
@@ -274,6 +273,9 @@ struct RowLds {
     uint64_t list[kList], weight[kList];      // words in order, and their weights
     double chunk_mass[kMostChunks], chunk_scale[kMostChunks];
     unsigned long long chunk_part[kMostChunks];
+    uint32_t chunk_end[kMostChunks];
+    int chunk_from[kMostChunks];
+    uint32_t wave_words[kRowThreads / kWave];
     int chunk_shift[kMostChunks];
     double mass[kBins];                       // of all bins up to each
     uint32_t count[kBins];
@@ -357,13 +359,26 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
     if (wave < kBins / kWave) {
         double w = 0.0;
         uint32_t n = 0;
-#pragma unroll 8
-        for (int c = 0; c < a.nchunk; ++c) {
-            const int at = tid - l.chunk_shift[c];
-            const double cw = (double)chunks[c].mass[max(at, 0)];
-            const uint32_t cn = chunks[c].upto[max(at, 0)];
-            w += at >= 0 ? cw * l.chunk_scale[c] : 0.0;
-            n += at >= 0 ? cn : 0;
+        constexpr int kAtOnce = 24;   // on their way together: a trip takes over 1 us
+        for (int c0 = 0; c0 < a.nchunk; c0 += kAtOnce) {
+            // lane j: chunk c0 + j's (past the last one a shift that no bin reaches)
+            const int cl = min(c0 + lane, a.nchunk - 1), shifts = c0 + lane < a.nchunk ? l.chunk_shift[cl] : kBins;
+            const double scales = l.chunk_scale[cl];
+            double cw[kAtOnce];
+            uint16_t cn[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                const Chunk& c = chunks[min(c0 + j, a.nchunk - 1)];
+                const int at = max(tid - lane_of(shifts, j), 0);
+                cw[j] = c.mass[at];
+                cn[j] = c.upto[at];
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                const bool in = tid >= lane_of(shifts, j);
+                w += in ? cw[j] * lane_of(scales, j) : 0.0;
+                n += in ? cn[j] : 0;
+            }
         }
         l.mass[tid] = w;
         l.count[tid] = n;
@@ -417,25 +432,57 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         const uint32_t upto = l.count[b], before_b = b ? l.count[b - 1] : 0;
         bool listed = list_lo <= b && b <= list_hi;
         if (!listed) {
-            const int lo = upto <= kList ? 0 : b;
+            const int lo = upto <= kFromTop ? 0 : b;
             list_n = (int)(lo ? upto - before_b : upto);
             listed = list_n <= kList;
             list_lo = listed ? lo : 1;
             list_hi = listed ? b : 0;
-            if (tid == 0) l.n = 0;
-            __syncthreads();
-            for (int c = wave; listed && c < a.nchunk; c += kRowThreads / kWave) {
-                const int cb = b - l.chunk_shift[c], cl = lo - l.chunk_shift[c];
-                if (cb < 0) continue;
-                const int i0 = cl > 0 ? chunks[c].upto[cl - 1] : 0, i1 = chunks[c].upto[cb];
-                uint32_t at = 0;
-                if (lane == 0) at = atomicAdd(&l.n, (uint32_t)(i1 - i0));
-                at = __builtin_amdgcn_readfirstlane(at);
-                for (int i = i0 + lane; i < i1; i += kWave) {
-                    const uint32_t id = min(c * kChunk + (chunks[c].place[i] & (kChunk - 1)), a.vocab - 1);
-                    const float t = x[id];
-                    l.list[at + i - i0] = word_order(t, id);
-                    l.weight[at + i - i0] = exp2.whole(below(t), kBits);
+            if (listed) {
+                // where each chunk's words of these bins lie and go: thread c has chunk c
+                uint32_t i0 = 0, own = 0;
+                if (tid < a.nchunk) {
+                    const int cb = b - l.chunk_shift[tid], cl = lo - l.chunk_shift[tid];
+                    i0 = cl > 0 && cb >= 0 ? chunks[tid].upto[cl - 1] : 0;
+                    own = cb >= 0 ? chunks[tid].upto[cb] - i0 : 0;
+                }
+                uint32_t to = wave_prefix<uint32_t>(own);
+                __syncthreads();   // (their room may still be read)
+                if (lane == kWave - 1) l.wave_words[wave] = to;
+                __syncthreads();
+                for (int w = 0; w < wave; ++w) to += l.wave_words[w];
+                if (tid < a.nchunk) {
+                    l.chunk_end[tid] = to;
+                    l.chunk_from[tid] = (int)(i0 - (to - own));
+                }
+                __syncthreads();
+                constexpr int kAtOnce = 8;
+                const int first_step = 1 << (31 - __clz(a.nchunk));
+                for (int i = tid; i < list_n; i += kAtOnce * kRowThreads) {
+                    uint32_t id[kAtOnce];
+                    float t[kAtOnce];
+                    int c[kAtOnce] = {};   // the first chunk that ends behind the word
+                    for (int step = first_step; step > 0; step >>= 1)
+#pragma unroll
+                        for (int j = 0; j < kAtOnce; ++j) {
+                            const int mid = min(c[j] + step, a.nchunk);
+                            if ((int)l.chunk_end[mid - 1] <= i + j * kRowThreads) c[j] = mid;
+                        }
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        c[j] = min(c[j], a.nchunk - 1);
+                        id[j] = chunks[c[j]].place[(i + j * kRowThreads + l.chunk_from[c[j]]) & (kChunk - 1)];
+                    }
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        id[j] = min(c[j] * kChunk + (id[j] & (kChunk - 1)), (uint32_t)a.vocab - 1);
+                        t[j] = x[id[j]];
+                    }
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j)
+                        if (i + j * kRowThreads < list_n) {
+                            l.list[i + j * kRowThreads] = word_order(t[j], id[j]);
+                            l.weight[i + j * kRowThreads] = exp2.whole(below(t[j]), kBits);
+                        }
                 }
             }
             __syncthreads();
@@ -449,15 +496,15 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         const double step = 8.0 * scale, e0 = (top - b) / step, e1 = (top - b + 1.0) / step;
         const float from = step > 0.0 ? (float)fmax(e0 - fabs(e0) * 1e-6 - 1e-30, -3.4028234663852886e38) : -3.4028234663852886e38f;
         const float to = step > 0.0 && list_lo != 0 ? fminf((float)(e1 + fabs(e1) * 1e-6 + 1e-30), m) : m;
-        // Radix search over the bits in which the keys (order, or index) may differ, 8 a pass.  kDigits counts and
+        // Radix search over the keys (order, from the range's first on, or index), 8 bits a pass.  kDigits counts and
         // weighs the words of the value so far by their next 8, kOne takes the only word left, kGather puts a group
         // that fits into the list.  kParts: the last bin's words that count, by chunk.  Where a bin is too large for
         // the list, its words are met in the row.
         enum { kDigits, kOne, kGather, kParts };
         const uint64_t lowest = word_order(to, 0), highest = word_order(from, kNoToken);
         int mode = rule < 2 || draw ? kDigits : kParts;
-        int end = draw ? 32 - __clz(a.vocab) : 64 - __clzll((long long)(lowest ^ highest));
-        uint64_t known = end == 64 ? 0 : ~0ull << end, value = draw ? 0 : lowest & known;
+        int end = draw ? 32 - __clz(a.vocab) : 64 - __clzll((long long)(highest - lowest));
+        uint64_t known = end == 64 ? 0 : ~0ull << end, value = 0;
         bool opened = false;   // a draw's goal is known
         if (mode == kParts)
             for (int c = tid; c < a.nchunk; c += kRowThreads) l.chunk_part[c] = 0;
@@ -471,7 +518,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
             }
             auto visit = [&](uint64_t order, uint64_t w) {
                 if (order > last_order || (rule == 2 && w < least_whole)) return;
-                const uint64_t key = draw ? order & 0xffffffffull : order;
+                const uint64_t key = draw ? order & 0xffffffffull : order - lowest;
                 if (mode == kParts) {
                     atomicAdd(&l.chunk_part[(uint32_t)order / kChunk], (unsigned long long)w);
                 } else if ((key & known) == value) {
@@ -579,9 +626,9 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
             return;
         }
         last_bin = b;
-        last_order = value;
+        last_order = value + lowest;
         whole_bin = false;
-        total = before + exp2(below(word_logit(value)));
+        total = before + exp2(below(word_logit(last_order)));
         __syncthreads();   // (l.lo has been read)
     }
 
@@ -589,7 +636,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
     const int bins = last_bin + (whole_bin ? 1 : 0);
     for (int c = tid; c < a.nchunk; c += kRowThreads) {
         const int n = bins - l.chunk_shift[c];
-        l.chunk_mass[c] = (n > 0 ? (double)chunks[c].mass[n - 1] * l.chunk_scale[c] : 0.0) +
+        l.chunk_mass[c] = (n > 0 ? chunks[c].mass[n - 1] * l.chunk_scale[c] : 0.0) +
                           (whole_bin ? 0.0 : ldexp((double)l.chunk_part[c], -kBits));
     }
     __syncthreads();
@@ -643,23 +690,27 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
     }
     uint64_t upto = wave_prefix<uint64_t>(own);
     if (lane == kWave - 1) l.digit_mass[0][wave] = upto;
-    if (tid == 0) {
-        l.lo = ~0ull;   // the first word past the goal
-        l.hi = 0;       // the last one with a weight, plus one
-    }
+    if (tid == 0) l.lo = ~0ull;
+    if (tid < kWaves) l.wave_words[tid] = 0;
     __syncthreads();
     for (int v = 0; v < wave; ++v) upto += l.digit_mass[0][v];
     const uint64_t goal = rest > 0.0 ? (uint64_t)ldexp(rest, kBits) : 0;
     uint64_t run = upto - own;
+    uint32_t last = 0;   // the thread's last word with a weight, plus one
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         run += w[j];
-        if (w[j] && run > goal && run - w[j] <= goal) atomicMin(&l.lo, (unsigned long long)(first + j));
-        if (w[j]) atomicMax(&l.hi, (unsigned long long)(first + j + 1));
+        if (w[j]) last = first + j + 1;
+        if (w[j] && run > goal && run - w[j] <= goal) l.lo = first + j;   // (one word's)
     }
+    const uint64_t some = __builtin_amdgcn_ballot_w64(last > 0);
+    if (some && lane == 63 - __builtin_clzll(some)) l.wave_words[wave] = last;
     __syncthreads();
     if (tid == 0) {
-        const uint32_t id = l.lo != ~0ull ? (uint32_t)l.lo : (uint32_t)l.hi - 1;
+        uint32_t id = (uint32_t)l.lo;
+        if (l.lo == ~0ull)   // none past the goal: the last one
+            for (int v = 0; v < kWaves; ++v)
+                if (l.wave_words[v]) id = l.wave_words[v] - 1;
         a.ids[row] = id;
         if (a.probs) a.probs[row] = (float)(exp2(below(x[id])) / sum);
     }
