@@ -60,7 +60,7 @@ struct SampleArgs {
 // log2(e) / temperature; a temperature that is not above 0 means the largest (no scale).
 __device__ __forceinline__ double word_scale(const SampleArgs& a, int row) {
     const float t = a.temperature ? a.temperature[row] : 1.0f;
-    return t > 0.0f ? 1.4426950408889634 / (double)t : -1.0;
+    return t > 0.0f ? fmax(1.4426950408889634 / (double)t, 1e-300) : -1.0;   // (of an infinite one: never -inf times 0)
 }
 
 // y of a logit, rounded by itself: in one fma with the difference from the largest's, equal logits would
@@ -70,33 +70,45 @@ __device__ __forceinline__ double scaled(float v, double scale) {
     return (double)v * scale;
 }
 
-// Weights 2^t, t <= 0: 2^n times the series of e^(f ln 2), |f| <= 1/2, to the 11th power: 6e-15 left out.  The
+// Weights 2^t, t <= 0: 2^n times the series of e^(f ln 2), |f| <= 1/2, to the 9th power.  What is left out, 7e-12
+// of a weight at most, moves the border between two words by less than that of all weights, so the sum of
+// 2^18 borders by less than 2^-19: so often would u fall between where a border lies and where it ought to.  The
 // coefficients are kept in scalar registers: as literals each took two moves to the vector registers a word.
 struct Exp2 {
-    double c[12];
+    static constexpr int kDegree = 9;
+    double c[kDegree + 1];
     __device__ __forceinline__ Exp2() {
         double f = 1.0;
 #pragma unroll
-        for (int i = 0; i < 12; ++i) {   // ln 2^i / i!
+        for (int i = 0; i <= kDegree; ++i) {   // ln 2^i / i!
             c[i] = f;
             f *= 0.6931471805599453 / (i + 1);
         }
 #pragma unroll
-        for (int i = 2; i < 12; ++i) asm("" : "+s"(c[i]));
+        for (int i = 2; i <= kDegree; ++i) asm("" : "+s"(c[i]));
     }
     // 2^(t + bits)
     __device__ __forceinline__ double operator()(double t, int bits = 0) const {
         const double n = rint(t), f = t - n;
-        double p = c[11];
+        double p = c[kDegree];
 #pragma unroll
-        for (int i = 10; i > 0; --i) p = fma(p, f, c[i]);
+        for (int i = kDegree - 1; i > 0; --i) p = fma(p, f, c[i]);
         return ldexp(fma(p, f, 1.0), (int)n + bits);
     }
-    // The same as a whole number, rounded to nearest (bits <= 51): the last bits of 2^52 + it.
-    __device__ __forceinline__ uint64_t whole(double t, int bits) const {
-        return __builtin_bit_cast(uint64_t, (*this)(t, bits) + 4503599627370496.0) & 0xfffffffffffffull;
+    // The same as a whole number, rounded to nearest (bits <= 51): the last bits of 2^52 + it, plus kOffset.
+    static constexpr uint64_t kOffset = 0x4330000000000000ull;
+    __device__ __forceinline__ uint64_t whole_offset(double t, int bits) const {
+        return __builtin_bit_cast(uint64_t, (*this)(t, bits) + 4503599627370496.0);
     }
+    __device__ __forceinline__ uint64_t whole(double t, int bits) const { return whole_offset(t, bits) - kOffset; }
 };
+
+// A whole number, or the largest where it is none of 32 bits (a cast would not have to).
+__device__ __forceinline__ uint32_t to_int(double v) {
+    uint32_t i;
+    asm("v_cvt_i32_f64 %0, %1" : "=v"(i) : "v"(v));
+    return i;
+}
 
 // Words in order as ascending 64-bit numbers: logit (largest first; -0 is 0), then index.
 __device__ __forceinline__ uint64_t word_order(float x, uint32_t i) {
@@ -156,7 +168,7 @@ __device__ __forceinline__ T lane_of(T v, int lane) {   // (lane: the same for a
 // Bound by the logits' bytes, and for many rows by some 25 fp64 instructions a word beside them.
 __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const SampleArgs a) {
     constexpr int kWaves = kChunkThreads / kWave, kBinWaves = kBins / kWave;
-    // (behind the bins, a place a lane for words that do not count: no branches, and no lanes on one place)
+    // (from the last bin on, a place a lane for words that do not count: no branches, and no lanes on one place)
     __shared__ unsigned long long mass[kBins + kWave], wave_mass[kWaves];
     __shared__ uint32_t count[kBins + kWave], wave_count[kWaves];
     __shared__ float wave_max[kWaves];
@@ -179,16 +191,12 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
         bad = bins = 0;
     }
     float m = -INFINITY;
-    bool odd = false;
 #pragma unroll
     for (int j = 0; j < kPerThread / 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            m = fmaxf(m, v[j][e]);
-            odd |= !(v[j][e] < INFINITY);
-        }
-    m = wave_max_dpp(m);
-    if (__builtin_amdgcn_ballot_w64(odd)) m = NAN;   // (told to all below)
+        for (int e = 0; e < 4; ++e) m = __builtin_elementwise_maximum(m, v[j][e]);   // (NaN stays)
+    const uint64_t odd = __builtin_amdgcn_ballot_w64(!(m < INFINITY));
+    m = odd ? NAN : wave_max_dpp(m);
     if (lane == 0) wave_max[wave] = m;
     __syncthreads();
     bool wrong = false;
@@ -216,20 +224,19 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
     uint32_t rank[kPerThread];   // bin and place inside it
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
-        const float t = v[j >> 2][j & 3];
-        const double y = scaled(t, scale), below = top - floor(8.0 * y);
-        const uint64_t w = exp2.whole(y - ym, kBits);
-        const int b = t > -INFINITY && below < kBins - 1 ? (int)below : kBins + lane;
-        atomicAdd(&mass[b], (unsigned long long)w);
-        rank[j] = (uint32_t)b << 16 | atomicAdd(&count[b], 1u);
+        const double y = scaled(v[j >> 2][j & 3], scale);
+        const uint32_t b = min(to_int(top - floor(8.0 * y)), (uint32_t)(kBins - 1 + lane));   // (-inf: the latter)
+        atomicAdd(&mass[b], (unsigned long long)exp2.whole_offset(y - ym, kBits));
+        rank[j] = b << 16 | atomicAdd(&count[b], 1u);
     }
     __syncthreads();
     // sums over the bins up to each
     uint64_t ms = 0;
     uint32_t cs = 0;
     if (wave < kBinWaves) {
-        ms = wave_prefix<uint64_t>(mass[tid]);
-        cs = wave_prefix<uint32_t>(count[tid]);
+        cs = count[tid];
+        ms = wave_prefix<uint64_t>(mass[tid] - cs * Exp2::kOffset);
+        cs = wave_prefix<uint32_t>(cs);
         if (lane == kWave - 1) {
             wave_mass[wave] = ms;
             wave_count[wave] = cs;
@@ -494,8 +501,8 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         const int bits = min(kBits, 62 - (32 - __clz((int)(upto - before_b))));
         // a range of logits that holds bin b's, with room for the roundings
         const double step = 8.0 * scale, e0 = (top - b) / step, e1 = (top - b + 1.0) / step;
-        const float from = step > 0.0 ? (float)fmax(e0 - fabs(e0) * 1e-6 - 1e-30, -3.4028234663852886e38) : -3.4028234663852886e38f;
-        const float to = step > 0.0 && list_lo != 0 ? fminf((float)(e1 + fabs(e1) * 1e-6 + 1e-30), m) : m;
+        const float from = (float)fmax(e0 - fabs(e0) * 1e-6 - 1e-30, -3.4028234663852886e38);
+        const float to = list_lo != 0 ? fminf((float)(e1 + fabs(e1) * 1e-6 + 1e-30), m) : m;
         // Radix search over the keys (order, from the range's first on, or index), 8 bits a pass.  kDigits counts and
         // weighs the words of the value so far by their next 8, kOne takes the only word left, kGather puts a group
         // that fits into the list.  kParts: the last bin's words that count, by chunk.  Where a bin is too large for
