@@ -523,13 +523,14 @@ struct RotatedRows {
     int hq;   // 0: no queries
 };
 
-// Bound by the bytes.  A workgroup takes one row, and 2048 values of [k | v | q] at a time, 8 a thread; the
-// row's angles lie in LDS (a place of padding after every four keeps the eight that each thread reads, one after
-// the other, on different banks).
+// Bound by the bytes.  A workgroup takes one row; a thread 8 values of a head of [k | v | q] (and, with pairs of half
+// a head's distance, their partners), kAtOnce times on their way together; the row's angles lie in LDS (a place of
+// padding after every four keeps the eight that each thread reads, one after the other, on different banks).
+// q_out may be q: a head's values are all of one wave, which has read them before it writes.
 template <int FMT, int HD, int LAYOUT>
 __global__ void __launch_bounds__(256) append_rotary_kernel(const PageArgs a, const RowList l, const RotatedRows x) {
     __shared__ double2 turn[HD / 2 + HD / 8];
-    constexpr int kPer = HD / 8;
+    constexpr int kPer = HD / 8, kAtOnce = 3;
     const int row = blockIdx.x, half = x.r.dims / 2;
     int off = 0;
     bool listed;
@@ -542,47 +543,72 @@ __global__ void __launch_bounds__(256) append_rotary_kernel(const PageArgs a, co
     }
     if (threadIdx.x < half) turn[threadIdx.x + (threadIdx.x >> 2)] = turn_of((double)pos, x.r.turns[threadIdx.x], x.r.amplitude);
     __syncthreads();
-    const int heads = 2 * a.kv_heads + x.hq, step = gridDim.y * 256;
-    for (int base = blockIdx.y * 256; base < heads * kPer; base += step) {   // whole heads
-        const int c = base + threadIdx.x, head = c / kPer, d = 8 * (c % kPer);
-        const bool on = head < heads, query = head >= 2 * a.kv_heads;
-        float f[8];
-        if (on) {
-            const float* src = query ? x.q + row * x.q_stride + (int64_t)(head - 2 * a.kv_heads) * HD
-                               : head < a.kv_heads ? x.k + row * x.k_stride + (int64_t)head * HD
-                                                   : x.v + row * x.v_stride + (int64_t)(head - a.kv_heads) * HD;
+    const int all = (2 * a.kv_heads + x.hq) * kPer, step = gridDim.y * 256;   // threads of all heads
+    const int d = 8 * (threadIdx.x % kPer), dims = x.r.dims;
+    const bool whole = LAYOUT == RTA_ROTARY_HALVES && half % 8 == 0;   // partners of 8 values lie together
+    const int partner = d < half ? d + half : d - half;
+    auto source = [&](int c) {
+        const int head = c / kPer;
+        return head >= 2 * a.kv_heads ? x.q + row * x.q_stride + (int64_t)(head - 2 * a.kv_heads) * HD
+               : head < a.kv_heads    ? x.k + row * x.k_stride + (int64_t)head * HD
+                                      : x.v + row * x.v_stride + (int64_t)(head - a.kv_heads) * HD;
+    };
+    for (int c0 = blockIdx.y * 256 + threadIdx.x; c0 < all; c0 += kAtOnce * step) {
+        float f[kAtOnce][8], g[kAtOnce][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = src[d + j];
-            if ((head < a.kv_heads || query) && d < x.r.dims) {
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (c0 + i * step >= all) break;
+            const float* src = source(c0 + i * step);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[i][j] = src[d + j];
+            if (whole && d < dims) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[i][j] = src[partner + j];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int c = c0 + i * step, head = c / kPer;
+            if (c >= all) break;
+            const bool query = head >= 2 * a.kv_heads;
+            if ((query || head < a.kv_heads) && d < dims) {
                 if constexpr (LAYOUT == RTA_ROTARY_NEIGHBOURS) {
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
                         const int p = (d + j) / 2;
-                        if (p < half) turn_pair(f[j], f[j + 1], turn[p + (p >> 2)]);
+                        if (p < half) turn_pair(f[i][j], f[i][j + 1], turn[p + (p >> 2)]);
                     }
-                } else {
+                } else if (whole) {
+                    const int p = d < half ? d : partner;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int dim = d + j;
-                        if (dim >= x.r.dims) break;
-                        const bool lower = dim < half;
-                        const int p = lower ? dim : dim - half;
-                        float other = src[lower ? dim + half : dim - half];
+                        const double2 t = turn[p + j + ((p + j) >> 2)];
+                        // (x cos - y sin; the upper values: y cos + x sin)
+                        f[i][j] = turn_value(f[i][j], g[i][j], t.x, d < half ? -t.y : t.y);
+                    }
+                } else {
+                    const float* src = source(c);
+                    for (int j = 0; j < 8 && d + j < dims; ++j) {
+                        const bool lower = d + j < half;
+                        const int p = lower ? d + j : d + j - half;
                         const double2 t = turn[p + (p >> 2)];
-                        if (lower) turn_pair(f[j], other, t);
-                        else turn_pair(other, f[j], t);
+                        f[i][j] = turn_value(f[i][j], src[lower ? p + half : p], t.x, lower ? -t.y : t.y);
                     }
                 }
             }
         }
-        __syncthreads();   // q_out may be q: every thread of a head has read its pairs
-        if (!on) continue;
-        if (query) {
-            float* dst = x.q_out + row * x.q_out_stride + (int64_t)(head - 2 * a.kv_heads) * HD + d;
+        // (a loop of its own: the partners that have just been read may be stored to)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dst[j] = f[j];
-        } else {
-            store_row8<FMT, HD>(a, page, head, off, d, f);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int c = c0 + i * step, head = c / kPer;
+            if (c >= all) break;
+            if (head >= 2 * a.kv_heads) {
+                float* dst = x.q_out + row * x.q_out_stride + (int64_t)(head - 2 * a.kv_heads) * HD + d;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dst[j] = f[i][j];
+            } else {
+                store_row8<FMT, HD>(a, page, head, off, d, f[i]);
+            }
         }
     }
 }

@@ -16,42 +16,60 @@ struct RotateArgs {
 };
 
 // Bound by the bytes: a value is read and written once.  A workgroup takes one row; a thread V pairs of each of
-// its heads (V 4 where the pairs come in fours: 16-byte accesses), whose angles it computes once.
+// its heads (V 4 where the pairs come in fours: 16-byte accesses), whose angles it computes once, kAtOnce heads on
+// their way together.
 template <int V, int LAYOUT>
 __global__ void __launch_bounds__(256) rotate_kernel(const RotateArgs a) {
+    constexpr int kAtOnce = 4;
     const int row = blockIdx.x, at_once = 256 / a.units;
     const int h0 = threadIdx.x / a.units, unit = threadIdx.x - h0 * a.units;
     if (h0 >= at_once) return;
-    const int half = a.r.dims / 2, j = unit * V, first = blockIdx.y * a.per_block;
-    const int last = min(first + a.per_block, a.heads);
+    const int half = a.r.dims / 2, j = unit * V;
+    const bool turns = j < half;
+    // its values: neighbours 2 V from 2 j on; halves V from j and V from j + half on; those that stay 2 V from 2 j
+    // on (half is a multiple of V), as far as the head goes
+    const bool split = LAYOUT == RTA_ROTARY_HALVES && turns;
+    const int lo = split ? j : 2 * j, hi = split ? j + half : 2 * j + V;
+    const int part = turns ? 2 * V : min(2 * V, a.head_dim - lo);   // (below 2 V: the last values of a head)
+    const bool copies = a.x != a.y;
+    if (!turns && !copies) return;
+    const int first = blockIdx.y * a.per_block + h0, last = min((int)(blockIdx.y + 1) * a.per_block, a.heads);
     const float* x = a.x + row * a.x_stride;
     float* y = a.y + row * a.y_stride;
     typedef float vec_t __attribute__((ext_vector_type(V), aligned(4)));
-    if (j < half) {
+    double2 t[V] = {};
+    if (turns) {
         const double position = (double)a.positions[row];
-        double2 t[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) t[e] = turn_of(position, a.r.turns[j + e], a.r.amplitude);
-        // neighbours: 2 V values from 2 j on; halves: V values from j and V from j + half on
-        const int lo = LAYOUT == RTA_ROTARY_NEIGHBOURS ? 2 * j : j, hi = LAYOUT == RTA_ROTARY_NEIGHBOURS ? 2 * j + V : j + half;
-        for (int h = first + h0; h < last; h += at_once) {
-            const float* src = x + (int64_t)h * a.head_dim;
-            float v[2 * V];
-            *reinterpret_cast<vec_t*>(v) = *reinterpret_cast<const vec_t*>(src + lo);
-            *reinterpret_cast<vec_t*>(v + V) = *reinterpret_cast<const vec_t*>(src + hi);
+    }
+    if (part < 2 * V) {
+        for (int h = first; h < last; h += at_once)
+            for (int e = 0; e < part; ++e) y[(int64_t)h * a.head_dim + lo + e] = x[(int64_t)h * a.head_dim + lo + e];
+        return;
+    }
+    for (int h = first; h < last; h += kAtOnce * at_once) {
+        float v[kAtOnce][2 * V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if constexpr (LAYOUT == RTA_ROTARY_NEIGHBOURS) turn_pair(v[2 * e], v[2 * e + 1], t[e]);
-                else turn_pair(v[e], v[V + e], t[e]);
-            }
-            float* dst = y + (int64_t)h * a.head_dim;
-            *reinterpret_cast<vec_t*>(dst + lo) = *reinterpret_cast<const vec_t*>(v);
-            *reinterpret_cast<vec_t*>(dst + hi) = *reinterpret_cast<const vec_t*>(v + V);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const float* src = x + (int64_t)min(h + i * at_once, last - 1) * a.head_dim;
+            *reinterpret_cast<vec_t*>(v[i]) = *reinterpret_cast<const vec_t*>(src + lo);
+            *reinterpret_cast<vec_t*>(v[i] + V) = *reinterpret_cast<const vec_t*>(src + hi);
         }
-    } else if (x != y) {
-        const int d = 2 * j, end = min(d + 2 * V, a.head_dim);   // (half is a multiple of V)
-        for (int h = first + h0; h < last; h += at_once)
-            for (int e = d; e < end; ++e) y[(int64_t)h * a.head_dim + e] = x[(int64_t)h * a.head_dim + e];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (h + i * at_once >= last) break;
+            if (turns) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    if constexpr (LAYOUT == RTA_ROTARY_NEIGHBOURS) turn_pair(v[i][2 * e], v[i][2 * e + 1], t[e]);
+                    else turn_pair(v[i][e], v[i][V + e], t[e]);
+                }
+            }
+            float* dst = y + (int64_t)(h + i * at_once) * a.head_dim;
+            *reinterpret_cast<vec_t*>(dst + lo) = *reinterpret_cast<const vec_t*>(v[i]);
+            *reinterpret_cast<vec_t*>(dst + hi) = *reinterpret_cast<const vec_t*>(v[i] + V);
+        }
     }
 }
 

@@ -42,11 +42,16 @@ __device__ __forceinline__ double2 turn_of(double position, double turns, double
     return double2{quadrant == 1 || quadrant == 2 ? -amplitude * a : amplitude * a, quadrant & 2 ? -amplitude * b : amplitude * b};
 }
 
-// A pair (x, y) turned, each value rounded once.
+// own c + other s, rounded to fp32 once; the same operations whichever kernel and layout calls it, so that they
+// agree bit by bit.
+__device__ __forceinline__ float turn_value(float own, float other, double c, double s) {
+    return (float)fma((double)own, c, (double)other * s);
+}
+// A pair (x, y) turned.
 __device__ __forceinline__ void turn_pair(float& x, float& y, double2 t) {
-    const double a = x, b = y;
-    x = (float)fma(a, t.x, -(b * t.y));
-    y = (float)fma(a, t.y, b * t.x);
+    const float a = x;
+    x = turn_value(a, y, t.x, -t.y);
+    y = turn_value(y, a, t.x, t.y);
 }
 
 namespace host {

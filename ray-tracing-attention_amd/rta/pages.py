@@ -200,9 +200,11 @@ class PagedCache:
                 raise ValueError(f"q must have {rows} rows")
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
-            out_stride = rotary._check_rows(q_out, "q_out")
-            if q_out.shape != q.shape:
-                raise ValueError(f"q_out must be of shape {tuple(q.shape)}")
+                out_stride = q.shape[1] * self.head_dim
+            else:
+                out_stride = rotary._check_rows(q_out, "q_out")
+                if q_out.shape != q.shape:
+                    raise ValueError(f"q_out must be of shape {tuple(q.shape)}")
             qs = [q.data_ptr(), stride, q.shape[1], q_out.data_ptr(), out_stride]
         elif q_out is not None:
             raise ValueError("q_out without q")

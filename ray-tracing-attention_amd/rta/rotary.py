@@ -34,8 +34,8 @@ class Rotary:
         if layout not in LAYOUTS:
             raise ValueError(f"layout is one of {', '.join(LAYOUTS)}")
         dims = head_dim if dims is None else dims
-        if not 0 < dims <= head_dim:
-            raise ValueError(f"dims lies in 2 .. {head_dim}")
+        if not 0 < dims <= head_dim or head_dim > 512:
+            raise ValueError(f"dims lies in 2 .. head_dim, and head_dim in 2 .. 512 ({dims}, {head_dim})")
         table, own = turns(dims, theta, scaling, factor, original, low, high)
         self.head_dim, self.dims, self.layout = head_dim, dims, layout
         self.amplitude = own if amplitude is None else float(amplitude)
@@ -43,14 +43,18 @@ class Rotary:
         self.device = self.turns.device
         self._c = _lib.Rotary(LAYOUTS[layout], head_dim, dims, self.amplitude, self.turns.data_ptr())
         self._at = ctypes.byref(self._c)
+        self._rotate = _lib.load().rta_rotate
 
     def _check_rows(self, t, name, heads=None):
         if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype != torch.float32:
             raise TypeError(f"{name} must be a float32 tensor on {self.device}")
-        if t.dim() != 3 or t.shape[2] != self.head_dim or t.stride(2) != 1 or \
-                (t.shape[1] > 1 and t.stride(1) != self.head_dim):
-            raise ValueError(f"{name} must be [rows, heads, {self.head_dim}] with contiguous rows")
-        return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * self.head_dim)
+        hd = self.head_dim
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [rows, heads, {hd}]")
+        (rows, heads, width), (row, head, one) = t.shape, t.stride()
+        if width != hd or one != 1 or (heads > 1 and head != hd):
+            raise ValueError(f"{name} must be [rows, heads, {hd}] with contiguous rows")
+        return row if rows > 1 else max(row, heads * hd)
 
     def rotate(self, x, positions, out=None):
         """x [rows, heads, head_dim] fp32 (rows may be strided) turned to positions [rows] (int64, any
@@ -59,14 +63,16 @@ class Rotary:
         rows, heads, _ = x.shape
         if not isinstance(positions, torch.Tensor) or positions.device != self.device or positions.dtype != torch.int64:
             raise TypeError(f"positions must be an int64 tensor on {self.device}")
-        if tuple(positions.shape) != (rows,) or not positions.is_contiguous():
+        if positions.shape != (rows,) or not positions.is_contiguous():
             raise ValueError(f"positions must be contiguous of shape ({rows},)")
         if out is None:
-            out = torch.empty(rows, heads, self.head_dim, dtype=torch.float32, device=self.device)
-        elif out.shape != x.shape:
-            raise ValueError(f"out must be of shape {tuple(x.shape)}")
-        out_stride = self._check_rows(out, "out")
-        fn, index = _lib.load().rta_rotate, self.device.index
+            out = torch.empty(x.shape, dtype=torch.float32, device=self.device)
+            out_stride = heads * self.head_dim
+        else:
+            out_stride = self._check_rows(out, "out")
+            if out.shape != x.shape:
+                raise ValueError(f"out must be of shape {tuple(x.shape)}")
+        fn, index = self._rotate, self.device.index
         args = (self._at, x.data_ptr(), stride, rows, heads, positions.data_ptr(), out.data_ptr(), out_stride,
                 torch._C._cuda_getCurrentRawStream(index))
         if torch.cuda.current_device() == index:
