@@ -169,24 +169,29 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
     hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2v_t, __builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u)) + off);
 }
 
-// The eight values of a dword of RTA_Q4_GROUP from its group's word (in the lower half), as binary16 in
-// order of their dims: the codes as the upper bits of a fraction under 16's exponent are 16 + c, and
+// The eight values of a dword of RTA_Q4_GROUP from its group's word, as binary16 in order of their dims: the codes as the upper bits of a fraction under 16's exponent are 16 + c, and
 // scale (16 + c) - scale (16 + zero), one fma, is exact.
-struct Q4Word {
+struct Q4Bits {    // kept in registers: one v_and_or_b32 where two literals would take two instructions
+    uint32_t fraction = 0x03c003c0u, sixteen = 0x4c004c00u;
+    __device__ __forceinline__ Q4Bits() { asm("" : "+s"(fraction), "+v"(sixteen)); }
+};
+struct Q4Words {   // of two groups
     h2v_t scale, off;
-    __device__ __forceinline__ explicit Q4Word(uint32_t word) {
-        const uint32_t s = word & kQ4Scale, z = (word & 15u) << 6 | 0x4c00u;
-        scale = __builtin_bit_cast(h2v_t, s | s << 16);
-        off = -scale * __builtin_bit_cast(h2v_t, z | z << 16);
+    __device__ __forceinline__ explicit Q4Words(uint32_t words) {
+        const uint32_t z = (words & 0x000f000fu) << 6 | 0x4c004c00u;
+        scale = __builtin_bit_cast(h2v_t, words & (kQ4Scale << 16 | kQ4Scale));
+        off = -scale * __builtin_bit_cast(h2v_t, z);
     }
 };
-__device__ __forceinline__ u4_t q4_to_half(uint32_t w, const Q4Word& g) {
+template <int G>   // of which group G's dword
+__device__ __forceinline__ u4_t q4_to_half(uint32_t w, const Q4Words& g, const Q4Bits& b) {
+    const h2v_t scale = {g.scale[G], g.scale[G]}, off = {g.off[G], g.off[G]};   // (selected by the instruction)
     u4_t r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const uint32_t x = j == 0 ? w << 6 : j == 1 ? w << 2 : j == 2 ? w >> 2 : w >> 6;
-        r[j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(h2v_t, (x & 0x03c003c0u) | 0x4c004c00u),
-                                                                      g.scale, g.off));
+        r[j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(h2v_t, (x & b.fraction) | b.sixteen),
+                                                                      scale, off));
     }
     return r;
 }

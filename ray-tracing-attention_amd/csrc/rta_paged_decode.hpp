@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
     const int64_t v_off = plane * kRow, head_row = (int64_t)kvh * a.p.page, head_off = head_row * kRow;
     const int ntile = (end - begin + kDecTile - 1) / kDecTile;
 
+    const Q4Bits q4;
     f4_t o[NC][kDt];
     Softmax<NC, 2, FMT> sm;
     sm.start();
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
         f4_t s[NC][2];
 #pragma unroll
         for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        Q4Words kg[2] = {Q4Words(0), Q4Words(0)};   // of the products' pair of groups
 #pragma unroll
         for (int kb = 0; kb < kKb; ++kb) {
             u4_t ka[2];
@@ -251,7 +253,12 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
                     codes_to_half(k[h][x][b + 1], w[2], w[3]);
                     ka[h] = u4_t{w[0], w[1], w[2], w[3]};
                 } else if constexpr (kQ4) {   // dword kb of a piece: dims 32 kb + 8 u ..
-                    ka[h] = q4_to_half(k[h][kb >> 2][kb & 3], Q4Word(kw[h][kb >> 1] >> (16 * (kb & 1))));
+                    if (kb & 1) {
+                        ka[h] = q4_to_half<1>(k[h][kb >> 2][kb & 3], kg[h], q4);
+                    } else {
+                        kg[h] = Q4Words(kw[h][kb >> 1]);
+                        ka[h] = q4_to_half<0>(k[h][kb >> 2][kb & 3], kg[h], q4);
+                    }
                 } else {
                     ka[h] = k[h][kb];
                 }
@@ -335,9 +342,11 @@ __global__ void __launch_bounds__(64 * kDecWaves, (DecLds<FMT, HD, NC, MULTI>::k
             uint8_t* dst = vl + (16 * h + i) * L::kPitch;
             if constexpr (kQ4) {
 #pragma unroll
-                for (int x = 0; x < kKb; ++x)
-                    *reinterpret_cast<u4_t*>(dst + 64 * x + 16 * u) =
-                        q4_to_half(v[h][x >> 2][x & 3], Q4Word(vw[h][x >> 1] >> (16 * (x & 1))));
+                for (int x = 0; x < kKb; x += 2) {
+                    const Q4Words g(vw[h][x >> 1]);
+                    *reinterpret_cast<u4_t*>(dst + 64 * x + 16 * u) = q4_to_half<0>(v[h][x >> 2][x & 3], g, q4);
+                    *reinterpret_cast<u4_t*>(dst + 64 * x + 64 + 16 * u) = q4_to_half<1>(v[h][x >> 2][(x & 3) + 1], g, q4);
+                }
             }
 #pragma unroll
             for (int x = 0; x < (kQ4 ? 0 : kLoads); ++x) {

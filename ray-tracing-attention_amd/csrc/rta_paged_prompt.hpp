@@ -128,9 +128,10 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
             }
         }
     };
+    const Q4Bits q4;
     auto put = [&](uint8_t* dst, Piece x, uint32_t word) {   // one piece as 2-byte elements
         if constexpr (kQ4) {
-            *reinterpret_cast<u4_t*>(dst + 2 * dim) = q4_to_half(x, Q4Word(word));
+            *reinterpret_cast<u4_t*>(dst + 2 * dim) = q4_to_half<0>(x, Q4Words(word), q4);
         } else if constexpr (FMT == RTA_Q8_ROW) {
             uint32_t w[8];
 #pragma unroll
