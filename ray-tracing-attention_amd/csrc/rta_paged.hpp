@@ -373,7 +373,7 @@ __device__ __forceinline__ void mask_columns(f4_t (*x)[N], uint32_t ok, const Vi
         }
 }
 
-// The online softmax of NC column tiles, a lane holding 4N positions of its column of each, N = 2
+// The online softmax of NC column tiles, a lane holding 4N positions of its column of each, N = 1 or 2
 // (16 columns) or 4 (32 columns) (products x; score = x fac in log2 units, fac a power of two: so a
 // score is its product exactly, and its distance from low is rounded once, however large both are).
 // Weights are 2^(score - low), 2^kTop for the largest score when low was set; low follows the
@@ -403,11 +403,11 @@ struct Softmax {
     }
     // Over the lanes that hold a column.
     static __device__ __forceinline__ float column_max(float v) {
-        if constexpr (N == 2) v = max_xor16(v);
+        if constexpr (N <= 2) v = max_xor16(v);
         return max_xor32(v);
     }
     static __device__ __forceinline__ float column_sum(float v) {
-        if constexpr (N == 2) v = add_xor16(v);
+        if constexpr (N <= 2) v = add_xor16(v);
         return add_xor32(v);
     }
     __device__ __forceinline__ void watch(const f4_t (*x)[N], bool whole) {
@@ -471,9 +471,9 @@ struct Softmax {
         const float base = low[c] == -INFINITY ? 0.0f : low[c];   // (nothing seen yet: weights 0)
         return __builtin_amdgcn_exp2f(fmaf(x, fac, -base));
     }
-    __device__ __forceinline__ void weights(int c, const f4_t* x, float fac, float w[8]) {
+    __device__ __forceinline__ void weights(int c, const f4_t* x, float fac, float w[N == 1 ? 4 : 8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < (N == 1 ? 4 : 8); ++j) {
             w[j] = weight(c, x[j >> 2][j & 3], fac);
             z[c] += w[j];
         }

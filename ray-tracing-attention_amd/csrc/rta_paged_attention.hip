@@ -1,5 +1,6 @@
 // rta_paged_attention.hip -- causal attention of new rows over the paged history, with a sliding
 // window and first positions that stay visible (gfx950).
+#include "rta_paged_decode4.hpp"
 #include "rta_paged_prompt.hpp"
 
 namespace rta {
@@ -155,7 +156,9 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
                                    dim3(256), 0, s, a);
             } else {
                 const dim3 grid(rows * decode_heads(pages->kv_heads, a.group, HD), 1, cut.nchunk), block(64 * kDecWaves);
-                if (decode_nc(a.group, HD) == 1)
+                if (F == RTA_Q4_GROUP && a.group <= 4)
+                    hipLaunchKernelGGL((paged_decode4_kernel<HD>), grid, block, 0, s, a);
+                else if (decode_nc(a.group, HD) == 1)
                     hipLaunchKernelGGL((paged_decode_kernel<F, HD, 1, false>), grid, block, 0, s, a);
                 else if constexpr (HD < 256) hipLaunchKernelGGL((paged_decode_kernel<F, HD, 2, false>), grid, block, 0, s, a);
             }
