@@ -16,7 +16,11 @@ constexpr int kDecGroups = 4096;
 struct Cut {
     int chunk, nchunk;
 };
-static Cut decode_cut(int64_t rows, int heads, int hd, int64_t most) {
+// Over 4-bit pages calls of up to 512 positions are not cut at all: a chunk's bytes are a quarter, so the merge and
+// its launch weigh more (us in one chunk / in several: 32 rows of 300 8.0 / 11.1, of 500 9.2 / 12.5, 128 of 300 15.3 / 25,
+// one of 300 7.7 / 8.5, of 500 8.9 / 8.4, and 4 more of the host's for the second launch).
+static Cut decode_cut(int64_t rows, int heads, int hd, int64_t most, bool q4 = false) {
+    if (q4 && most <= 512) return Cut{512, 1};
     const int64_t want = (rows * heads * most / kDecGroups + 127) / 128 * 128;
     const int64_t least = rows * heads * ((most + 127) / 128) <= (hd == 256 ? 256 : 512) ? 128 : 256;
     const int64_t chunk = want < least ? least : want < 1 << 30 ? want : 1 << 30;
@@ -62,7 +66,7 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
     *ntile = 0;
     if (!several)
         return decode_cut(rows, decode_heads(p->kv_heads, group, p->head_dim), p->head_dim,
-                          most_visible(len, window, sinks));
+                          most_visible(len, window, sinks), p->fmt == RTA_Q4_GROUP);
     const bool few = few_rows(max_rows, group, p->head_dim);
     const int cols = few ? few_cols(max_rows * group) : prompt_cols(p->head_dim);
     *ntile = (int)(((int64_t)max_rows * group + cols - 1) / cols);
@@ -156,6 +160,7 @@ int rta_paged_attention(const rta_pages* pages, int layer, const float* q, int64
                                    dim3(256), 0, s, a);
             } else {
                 const dim3 grid(rows * decode_heads(pages->kv_heads, a.group, HD), 1, cut.nchunk), block(64 * kDecWaves);
+                // (us, this / the other kernel: 8 sequences of 60000 to 131072 178 / 205, 32 of 256 to 8192 32.6 / 37)
                 if (F == RTA_Q4_GROUP && a.group <= 4)
                     hipLaunchKernelGGL((paged_decode4_kernel<HD>), grid, block, 0, s, a);
                 else if (decode_nc(a.group, HD) == 1)

@@ -423,8 +423,11 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         }
         if (rule < 2) {
             b = 0;   // the bins up to which there is not enough
-            for (int t = lane; t < kBins; t += kWave)
+#pragma unroll
+            for (int j = 0; j < kBins / kWave; ++j) {
+                const int t = lane + j * kWave;
                 b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(t < kBins - 1 && (rule == 0 ? l.count[t] < words : l.mass[t] < goal)));
+            }
             if (rule == 0 && (b == kBins - 1 || (b > least_bin && !(p < 1.0)))) continue;   // (not so many, or no matter)
             if (rule == 1 && b > least_bin) continue;
             b = min(b, last_bin);

@@ -255,3 +255,40 @@ def test_a_captured_step_replays(env):
         for layer in range(2):
             assert torch.equal(eager.out[layer], graph.out[layer]), (i, layer)
     assert ops.device_error() == 0
+
+
+def test_pools_past_four_gigabytes(env):
+    torch, pages, dev = env
+    page = 1024
+    pb = pages.page_bytes(Q4, 4, 128, page)
+    n_pages = (5 << 30) // pb
+    pool = torch.empty(1, n_pages, pb, dtype=torch.uint8, device=dev)
+    refs = torch.zeros(n_pages, dtype=torch.int32, device=dev)
+    table = torch.full((1, 4), -1, dtype=torch.int32, device=dev)
+    names = [n_pages - 1, n_pages - 3, 0]
+    table[0, :3] = ints(torch, names, dev)
+    refs[names] = 1
+    lens = [2 * page + 77]
+    c = pages.PagedCache(Q4, 4, 128, page, pool=pool, table=table, lengths=ints(torch, lens, dev), refs=refs)
+    base.fill(env, c, lens, 21)
+    for hq, rows in ((8, 1), (24, 1), (8, 3), (8, 40)):   # each of the kernels
+        q = base.rows_of(torch, dev, rows, hq, 128, 22)
+        got = c.attention(q, cu_rows=ints(torch, [0, rows], dev), max_rows=rows)
+        ref.check_rows(got, base.want_rows(c, q, [(0, 0, rows)]))
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (3, 1), (10, 2)])
+def test_lengths_around_the_cut(env, hd, hq, hkv):
+    """Calls of up to 512 positions in one piece, longer ones in chunks; tiles and chunks that end early."""
+    torch, _, dev = env
+    lens = [511, 512, 513, 31, 33, 127, 640, 1025]
+    c = filled(env, Q4, hkv, hd, 24, lens)
+    base.fill(env, c, lens, 41)
+    q = base.rows_of(torch, dev, len(lens), hq, hd, 42)
+    want = base.want_rows(c, q, [(s, s, 1) for s in range(len(lens))])
+    ref.check_rows(c.attention(q, max_len=1025), want)
+    few = [1, 3, 4, 5]
+    ref.check_rows(c.attention(q[few].contiguous(), seqs=ints(torch, few, dev), max_len=512), [want[s] for s in few])
+    assert ops.device_error() == 0

@@ -182,6 +182,18 @@ def test_many_rows(env, fmt):
     assert ops.device_error() == 0
 
 
+def test_rows_past_two_to_the_31(env):
+    torch, _, dev = env
+    r, p = rotary.Rotary(64, 32, "halves"), torch.tensor([7, 123456], device=dev)
+    x = rows_of(torch, dev, 2, 3, 64, 16).contiguous()
+    far = torch.zeros((1 << 31) + 1000, device=dev)
+    view = far.as_strided((2, 3, 64), (1 << 31, 64, 1), 3)
+    view.copy_(x)
+    assert torch.equal(r.rotate(view, p), r.rotate(x, p))
+    r.rotate(x, p, out=view)
+    assert torch.equal(view, r.rotate(x, p))
+
+
 def test_bad_rows_are_left_undone(env):
     torch, _, dev = env
     c = filled(env, _lib.F16, 2, 64, 4, [10, 6], extra=4)

@@ -167,6 +167,35 @@ def test_the_ends_of_u_and_of_the_rules(env):
     assert ops.device_error() == 0
 
 
+def test_an_infinite_temperature_makes_all_words_alike(env):
+    rng = np.random.default_rng(11)
+    rows, vocab = 6, 70001
+    x, u = logits(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    x[1, ::3] = -np.inf
+    t = np.full(rows, np.inf)
+    for how in ({}, dict(k=rng.integers(1, vocab, rows)), dict(p=np.full(rows, 0.5)), dict(least=np.full(rows, 0.5)),
+                dict(k=rng.integers(1, 100, rows), p=np.full(rows, 0.25))):
+        ids, probs = (v.cpu().numpy() for v in run(env, x, u, t=t, **how))
+        for r in range(rows):
+            order = np.lexsort((np.arange(vocab), -x[r]))
+            n = int((x[r] > -np.inf).sum())
+            n = min(n, int(how["k"][r])) if "k" in how else n
+            n = int(np.ceil(n * how["p"][r])) if "p" in how else n
+            assert ids[r] == np.sort(order[:n])[int(np.floor(float(u[r]) * n))] and abs(probs[r] * n - 1) < 1e-6, (how, r)
+    assert ops.device_error() == 0
+
+
+def test_rows_past_two_to_the_31(env):
+    torch, dev = env
+    rng = np.random.default_rng(12)
+    x, u = logits(rng, 2, 20000), rng.random(2).astype(np.float32)
+    far = torch.empty((1 << 31) + 30000, device=dev)
+    view = far.as_strided((2, 20000), (1 << 31, 1), 5)
+    view.copy_(torch.tensor(x, device=dev))
+    for how in ({}, dict(k=[40, 3000], p=[0.9, 0.5])):
+        assert all(torch.equal(a, b) for a, b in zip(run(env, view, u, **how), run(env, x, u, **how)))
+
+
 def test_bad_rows(env):
     torch, _ = env
     rng = np.random.default_rng(6)
