@@ -16,13 +16,17 @@ constexpr int kDecGroups = 4096;
 struct Cut {
     int chunk, nchunk;
 };
-// Over 4-bit pages calls of up to 512 positions are not cut at all: a chunk's bytes are a quarter, so the merge and
-// its launch weigh more (us in one chunk / in several: 32 rows of 300 8.0 / 11.1, of 500 9.2 / 12.5, 128 of 300 15.3 / 25,
-// one of 300 7.7 / 8.5, of 500 8.9 / 8.4, and 4 more of the host's for the second launch).
-static Cut decode_cut(int64_t rows, int heads, int hd, int64_t most, bool q4 = false) {
-    if (q4 && most <= 512) return Cut{512, 1};
-    const int64_t want = (rows * heads * most / kDecGroups + 127) / 128 * 128;
-    const int64_t least = rows * heads * ((most + 127) / 128) <= (hd == 256 ? 256 : 512) ? 128 : 256;
+// Over 4-bit pages a chunk's bytes are a quarter, so its start, the merge and the second launch weigh more.  Up to 512
+// positions, and up to 1024 where the rows alone fill the chip's four workgroups per compute unit, are not cut at all (us in
+// one chunk / in several: 32 rows of 300 8.0 / 11.1, of 500 9.2 / 12.5, 128 of 300 15.3 / 25, of 600 21.6 / 31.3, one of
+// 300 7.7 / 8.5, of 500 8.9 / 8.4, and 4 less of the host's); calls that do not run in one go have chunks of 512 at least
+// (512 / 256: one of 16000 13.5 / 15.8, 32 of 1000 16.7 / 17.5), and a single sequence, which no other can be longer than,
+// one round of them (one of 100000 37, so 44; 32 of 256 to 8192 would take 34.9, so 32.4).
+static Cut decode_cut(int64_t rows, int heads, int hd, int64_t most, bool q4 = false, int at_least = 128) {
+    if (q4 && (most <= 512 || (most <= 1024 && rows * heads >= 1024))) return Cut{1024, 1};
+    const int64_t want = (rows * heads * most / (q4 && rows == 1 ? 1024 : kDecGroups) + 127) / 128 * 128;
+    const int64_t some = rows * heads * ((most + 127) / 128) <= (hd == 256 ? 256 : 512) ? 128 : q4 ? 512 : 256;
+    const int64_t least = some < at_least ? at_least : some;
     const int64_t chunk = want < least ? least : want < 1 << 30 ? want : 1 << 30;
     return Cut{(int)chunk, (int)((most + chunk - 1) / chunk)};
 }
@@ -76,6 +80,9 @@ static Cut cut_of(const rta_pages* p, int hq, int rows, int n, bool several, int
         const int64_t span = (int64_t)window + cols / group + 1;
         most = most_visible(len, (int)(span < INT_MAX ? span : INT_MAX), sinks);
     }
+    // (4-bit pages, us so / as the others: 16 sequences of 5 rows over 500 to 16384 positions 58 / 84, 4 of 8 over 4000
+    // 23 / 27, one of 4 over 30000 25 / 32, 32 of 4 over 300 8 / 11; 24 of 5 through a window of 4096 25.5 / 25.4)
+    if (few && p->fmt == RTA_Q4_GROUP) return decode_cut(2 * (int64_t)n, p->kv_heads, p->head_dim, most, true, 512);
     if (few) return decode_cut(4 * (int64_t)n, p->kv_heads, p->head_dim, most);
     return prompt_cut((int64_t)*ntile * n * p->kv_heads, most);
 }
