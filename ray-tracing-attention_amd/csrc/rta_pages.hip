@@ -527,6 +527,8 @@ struct RotatedRows {
 // a head's distance, their partners), kAtOnce times on their way together; the row's angles lie in LDS (a place of
 // padding after every four keeps the eight that each thread reads, one after the other, on different banks).
 // q_out may be q: a head's values are all of one wave, which has read them before it writes.
+// (9.9 thousand rows of 8 + 8 + 32 heads into 4 bits: 87 us, 4.7 TB/s; partners one by one and a barrier for every 2048
+// values: 155.)
 template <int FMT, int HD, int LAYOUT>
 __global__ void __launch_bounds__(256) append_rotary_kernel(const PageArgs a, const RowList l, const RotatedRows x) {
     __shared__ double2 turn[HD / 2 + HD / 8];

@@ -24,7 +24,10 @@ constexpr int kBins = 384;         // 48 octaves; the last one holds everything 
 constexpr int kBits = 50;          // kChunk weights of up to 2^50 stay below 2^64
 constexpr int kRowThreads = 512, kMostChunks = 512;
 constexpr int kList = 8192;        // words ranked in LDS
-constexpr int kFromTop = 2048;     // words of all bins up to one that are ranked rather than that bin's alone
+// Words of all bins up to one that are ranked rather than that bin's alone: then the draw needs no sums over chunks,
+// but more words are gathered and searched (256 flat rows, the slowest's time: with 8192 for it 60 us, so, and with the
+// places looked up together, 43).
+constexpr int kFromTop = 2048;
 constexpr uint32_t kNoToken = 0xffffffffu;
 
 struct ChunkHead {
@@ -165,7 +168,8 @@ __device__ __forceinline__ T lane_of(T v, int lane) {   // (lane: the same for a
     }
 }
 
-// Bound by the logits' bytes, and for many rows by some 25 fp64 instructions a word beside them.
+// Bound by latency for a few rows (one: 6 us), for many by vector instructions, 25 a word and as many again for its place
+// (256 rows of 151936 words by top-p: 62 us, on 73% of the cycles; 155 MB read and 78 of places written).
 __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const SampleArgs a) {
     constexpr int kWaves = kChunkThreads / kWave, kBinWaves = kBins / kWave;
     // (from the last bin on, a place a lane for words that do not count: no branches, and no lanes on one place)
@@ -296,8 +300,9 @@ struct RowLds {
     int least_bin;
 };
 
-// One row.  Bound by latency: some 30 steps between barriers, and a trip to the chunks' bins, to the places of the
-// words that are ranked, and to these.
+// One row.  Bound by latency: some 20 steps between barriers, and a trip to the chunks' heads, to their bins, to the
+// places of the words that are ranked, and to these (one row of 151936 words, every rule: 14.5 us; 256 by top-p, whose
+// bins hold some 3000 words: 39).
 __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArgs a) {
     __shared__ RowLds l;
     constexpr int kWaves = kRowThreads / kWave;
