@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
     __shared__ uint32_t count[kBins + kWave], wave_count[kWaves];
     __shared__ float wave_max[kWaves];
     __shared__ __align__(16) uint16_t place[kChunk];
-    __shared__ uint32_t first, bad, bins;
+    __shared__ uint32_t first, bins;
     const int row = blockIdx.x / a.nchunk, chunk = blockIdx.x - row * a.nchunk, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* x = a.logits + row * a.stride;
     f4_t v[kPerThread / 4];
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
     }
     if (tid == 0) {
         first = kNoToken;
-        bad = bins = 0;
+        bins = 0;
     }
     float m = -INFINITY;
 #pragma unroll
@@ -294,7 +294,7 @@ struct RowLds {
     unsigned long long digit_mass[3][256];
     uint32_t digit_count[3][256];
     double goal, sum;
-    unsigned long long lo, hi;
+    unsigned long long lo;
     float max[kRowThreads / kWave];
     uint32_t n, found;
     int least_bin;
