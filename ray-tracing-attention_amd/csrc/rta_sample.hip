@@ -298,6 +298,7 @@ struct RowLds {
     float max[kRowThreads / kWave];
     uint32_t n, found;
     int least_bin;
+    double least_log;
 };
 
 // One row.  Bound by latency: some 20 steps between barriers, and a trip to the chunks' heads, to their bins, to the
@@ -396,17 +397,21 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         l.count[tid] = n;
     } else if (wave == kWaves - 1) {
         // the bin that min-p cuts through: behind it no other rule matters (and chunks need not have kept their words)
-        const double at = least > 0.0 ? top - floor(8.0 * (ym + log2(fmin(least, 1.0)))) : (double)kBins;
-        if (lane == 0) l.least_bin = at < kBins ? (int)at : kBins;
+        const double log = least > 0.0 ? log2(fmin(least, 1.0)) : -INFINITY, at = top - floor(8.0 * (ym + log));
+        if (lane == 0) {
+            l.least_log = log;
+            l.least_bin = at < kBins ? (int)at : kBins;
+        }
     }
     __syncthreads();
     const int least_bin = l.least_bin;
+    // (by logarithms: of a min-p of 2^-37 the whole numbers would leave 13 bits)
+    auto weighs_enough = [&](float v) { return below(v) >= l.least_log; };
 
-    // The words that count are those up to last_order and of at least least_whole, all of bins up to last_bin
+    // The words that count are those up to last_order, all of bins up to last_bin, of it those that weigh enough
     // (whole_bin: all of that one's).  The list holds the words of bins list_lo .. list_hi (none: list_lo > list_hi).
     int last_bin = kBins - 2, list_lo = 1, list_hi = 0, list_n = 0;
     uint64_t last_order = ~0ull;
-    const uint64_t least_whole = least > 0.0 ? (uint64_t)ceil(ldexp(fmin(least, 1.0), kBits)) : 0;
     bool whole_bin = true;
     double total = l.mass[kBins - 2];
     int buf = 0;   // the digits that are clear
@@ -532,7 +537,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
                 l.digit_count[next][tid] = 0;
             }
             auto visit = [&](uint64_t order, uint64_t w) {
-                if (order > last_order || (rule == 2 && w < least_whole)) return;
+                if (order > last_order || (rule == 2 && !weighs_enough(word_logit(order)))) return;
                 const uint64_t key = draw ? order & 0xffffffffull : order - lowest;
                 if (mode == kParts) {
                     atomicAdd(&l.chunk_part[(uint32_t)order / kChunk], (unsigned long long)w);
@@ -696,9 +701,11 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             w[j + e] = 0;
-            if (v[e] > -INFINITY && word_order(v[e], first + j + e) <= last_order && bin_of(v[e]) < kBins - 1) {
-                const uint64_t t = exp2.whole(below(v[e]), kBits);
-                if (t >= least_whole) w[j + e] = t;
+            const double b = bin_of(v[e]);   // (-inf: none)
+            if (b < kBins - 1 && word_order(v[e], first + j + e) <= last_order) {
+                // as in the sums: bins before the last one count whole (they lie above min-p but for roundings), so
+                // the chunk that is drawn has a word
+                if (b < bins || (b == last_bin && weighs_enough(v[e]))) w[j + e] = exp2.whole(below(v[e]), kBits);
             }
             own += w[j + e];
         }

@@ -167,6 +167,27 @@ def test_the_ends_of_u_and_of_the_rules(env):
     assert ops.device_error() == 0
 
 
+def test_a_word_on_min_ps_border_alone_in_its_chunk(env):
+    """One word that min-p just keeps or drops, in a chunk of its own behind more words than are ranked at
+    once: with u = 1 it is the draw if it is kept, and the last of the largest words if it is not."""
+    rng = np.random.default_rng(23)
+    rows = 256
+    x = np.full((rows, 20000), -np.inf, np.float32)
+    t = rng.uniform(1e-3, 3, rows).astype(np.float32)
+    least = (2.0 ** -(rng.integers(1, 300, rows) / 8)).astype(np.float32)   # (borders of the bins of eighths too)
+    top = rng.uniform(-30, 30, rows).astype(np.float32)
+    top[::3] = 0
+    x[:, :8192] = top[:, None]
+    word = (top + t.astype(np.float64) * np.log(least.astype(np.float64))).astype(np.float32)
+    for r in range(rows):
+        for _ in range(abs(r % 5 - 2)):
+            word[r] = np.nextafter(word[r], np.float32(np.inf if r % 5 > 2 else -np.inf))
+    x[np.arange(rows), 9000] = word
+    ids = check(env, x, np.ones(rows), t=t, least=least, most_close=2)
+    assert set(ids.tolist()) == {8191, 9000}
+    assert ops.device_error() == 0
+
+
 def test_an_infinite_temperature_makes_all_words_alike(env):
     rng = np.random.default_rng(11)
     rows, vocab = 6, 70001
