@@ -151,16 +151,21 @@ __global__ void __launch_bounds__(64 * kDecWaves, (Decode4Lds<HD>::kPerSimd)) pa
     for (int t = wave; t < ntile; t += kDecWaves) {
         const uint32_t now = live;
         const bool more = t + kDecWaves < ntile, whole = now == 0xffffffffu;
+        // A position that does not count: zeros (scales of 0), keys too.  Its scores are masked, but a row of the product
+        // holds a second position, which meets its values times zeros: NaN from what lies there without a page.
+        if (!whole) {
+            const bool on = (now >> (16 * set + i)) & 1u;
+#pragma unroll
+            for (int x = 0; x < kGroups / 2; ++x) {
+                kw[x] = on ? kw[x] : 0u;
+                vw[x] = on ? vw[x] : 0u;
+            }
+        }
         f4_t s[2] = {f4_t{0.0f, 0.0f, 0.0f, 0.0f}, f4_t{0.0f, 0.0f, 0.0f, 0.0f}};   // (neighbours go into different sums)
         each(k, kw, [&](int g, int y, u4_t ka) {
             s[y] = page_mfma<FMT>(ka, *reinterpret_cast<const u4_t*>(ql + (2 * g + y) * 256), s[y]);
         });
-        // V into LDS (rows that do not count as zeros: a scale of 0), then the next tile's rows
-        if (!whole) {
-            const bool on = (now >> (16 * set + i)) & 1u;
-#pragma unroll
-            for (int x = 0; x < kGroups / 2; ++x) vw[x] = on ? vw[x] : 0u;
-        }
+        // V into LDS, then the next tile's rows
         uint8_t* dst = vl + (16 * set + i) * L::kPitch + 32 * half;
         each(v, vw, [&](int g, int y, u4_t x) { *reinterpret_cast<u4_t*>(dst + 64 * g + 16 * y) = x; });
         if (more) {

@@ -292,3 +292,38 @@ def test_lengths_around_the_cut(env, hd, hq, hkv):
     few = [1, 3, 4, 5]
     ref.check_rows(c.attention(q[few].contiguous(), seqs=ints(torch, few, dev), max_len=512), [want[s] for s in few])
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("fmt", [ref.F16, ref.BF16, ref.Q8_ROW, Q4])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv", [(4, 1), (6, 2), (12, 1)])
+def test_what_lies_in_other_pages_does_not_matter_where_one_is_missing(env, fmt, hd, hq, hkv):
+    """Positions without a page beside positions with one, page 0 free and full of NaN: the rows, and the score
+    of every other position, are those of the positions that have a page."""
+    torch, pages, dev = env
+    page, lens = 16, [100, 33, 700]
+    c = pages.PagedCache(fmt, hkv, hd, page, n_pages=60, max_seqs=3, max_pages=50)
+    c.pool.fill_(255)   # NaN in every format's elements or scales
+    at = 1
+    for s, n in enumerate(lens):
+        held = -(-n // page)
+        c.table[s, :held] = torch.arange(at, at + held, dtype=torch.int32, device=dev)
+        c.refs[at : at + held] = 1
+        at += held
+    c.lengths[:] = ints(torch, lens, dev)
+    base.fill(env, c, lens, 43)
+    # pages behind a window given back (of either half of a tile of 32, and whole tiles), an entry past the pool
+    c.free(ints(torch, [0, 2], dev), ints(torch, [16, 64], dev), ints(torch, [48, 144], dev))
+    assert ops.device_error() == 0
+    c.table[0, 4], c.table[1, 1], c.table[2, 20] = 10**8, -1, -(2**31)
+    assert int(c.refs[0]) == 0
+    q = base.rows_of(torch, dev, 3, hq, hd, 44)
+    got = c.attention(q, max_len=700)
+    assert ops.device_error() == _lib.DEVERR_PAGES
+    ref.check_rows(got, base.want_rows(c, q, [(s, s, 1) for s in range(3)], missing_ok=True))
+    for rows in (2, 90):   # few rows and many
+        q = base.rows_of(torch, dev, rows, hq, hd, 45)
+        for s in (0, 2):
+            got = c.attention(q, seqs=ints(torch, [s], dev), cu_rows=ints(torch, [0, rows], dev), max_rows=rows)
+            assert ops.device_error() == _lib.DEVERR_PAGES
+            ref.check_rows(got, base.want_rows(c, q, [(s, 0, rows)], missing_ok=True), (rows, s))
