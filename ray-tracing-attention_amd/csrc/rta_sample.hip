@@ -60,10 +60,13 @@ struct SampleArgs {
     Chunk* chunks;      // [rows][nchunk]
 };
 
-// log2(e) / temperature; a temperature that is not above 0 means the largest (no scale).
+// log2(e) / temperature; a temperature that is not above 0 means the largest (no scale).  An infinite one: kAlike, by
+// which every finite logit's weight is 1 (the largest difference times it is 7e-212), bins keep two signs apart (the
+// smallest logit times it, 1e-295, is no zero), and -inf stays -inf.
+constexpr double kAlike = 1e-250;
 __device__ __forceinline__ double word_scale(const SampleArgs& a, int row) {
     const float t = a.temperature ? a.temperature[row] : 1.0f;
-    return t > 0.0f ? fmax(1.4426950408889634 / (double)t, 1e-300) : -1.0;   // (of an infinite one: never -inf times 0)
+    return t > 0.0f ? fmax(1.4426950408889634 / (double)t, kAlike) : -1.0;
 }
 
 // y of a logit, rounded by itself: in one fma with the difference from the largest's, equal logits would
@@ -397,7 +400,9 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         l.count[tid] = n;
     } else if (wave == kWaves - 1) {
         // the bin that min-p cuts through: behind it no other rule matters (and chunks need not have kept their words)
-        const double log = least > 0.0 ? log2(fmin(least, 1.0)) : -INFINITY, at = top - floor(8.0 * (ym + log));
+        double log = least > 0.0 ? log2(fmin(least, 1.0)) : -INFINITY;
+        if (scale == kAlike) log = fmin(log, -1e-200);   // (below 0: a min-p of 1 keeps all finite logits too)
+        const double at = top - floor(8.0 * (ym + log));
         if (lane == 0) {
             l.least_log = log;
             l.least_bin = at < kBins ? (int)at : kBins;

@@ -321,3 +321,36 @@ def test_arguments_are_checked(env):
         ops.sample(x, u, temperature=torch.ones(6, device=dev)[::2])
     with pytest.raises(_lib.RtaError):
         ops.sample(x, u, workspace=torch.empty(64, dtype=torch.uint8, device=dev))
+
+
+@pytest.mark.parametrize("vocab", [5, 900, 70001])
+def test_an_infinite_temperature_with_every_min_p_and_logits_near_zero(env, vocab):
+    """Every finite logit weighs 1, whatever its size or sign, and 1 is not below a min-p of 1."""
+    rng = np.random.default_rng(vocab)
+    tiny = (rng.standard_normal(vocab) * np.exp2(rng.uniform(-149, -60, vocab))).astype(np.float32)
+    rows = [logits(rng, 1, vocab)[0], -np.abs(tiny), np.abs(tiny), tiny, -np.abs(tiny), -np.abs(tiny), tiny, tiny]
+    x = np.stack(rows).astype(np.float32)
+    x[4, vocab // 2] = 3.0
+    x[5, rng.random(vocab) < 0.3] = 0.0
+    x[5, ::2] *= np.float32(-1.0)                                   # zeros of both signs
+    x[6, rng.random(vocab) < 0.5] = -np.inf
+    x[6, 1] = -np.finfo(np.float32).max
+    x[7, rng.random(vocab) < 0.4] *= np.float32(1e38)
+    x[7, 2], x[7, 3] = np.finfo(np.float32).max, np.finfo(np.float32).min
+    n_rows = len(x)
+    full = lambda v: np.full(n_rows, v)   # noqa: E731
+    for how in (dict(), dict(least=full(1.0)), dict(least=full(0.5)), dict(least=full(2.0)), dict(k=rng.integers(1, vocab + 1, n_rows)),
+                dict(p=full(0.5)), dict(k=rng.integers(1, vocab + 1, n_rows), least=full(1.0)), dict(p=full(0.25), least=full(1.0)),
+                dict(k=rng.integers(1, vocab + 1, n_rows), p=full(0.5), least=full(1.0))):
+        for u in (rng.random(n_rows).astype(np.float32), np.zeros(n_rows, np.float32), np.ones(n_rows, np.float32)):
+            ids, probs = (v.cpu().numpy() for v in run(env, x, u, t=full(np.inf), **how))
+            for r in range(n_rows):
+                order = np.lexsort((np.arange(vocab), -x[r].astype(np.float64)))
+                n = int((x[r] > -np.inf).sum())
+                n = min(n, int(how["k"][r])) if "k" in how else n
+                n = int(np.ceil(n * how["p"][r])) if "p" in how else n
+                n = 1 if "least" in how and how["least"][r] > 1 else n
+                want = np.sort(order[:n])[min(int(np.floor(float(u[r]) * n)), n - 1)]   # (whole sums: exact)
+                assert ids[r] == want, (how, r, ids[r], want)
+                assert abs(probs[r] * n - 1) <= 2.0**-24 + 2.0**-40, (how, r)
+    assert ops.device_error() == 0
