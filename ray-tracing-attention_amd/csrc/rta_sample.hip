@@ -8,7 +8,7 @@
 //      and which words (of the first bins, as far as the rules may ask for them);
 //   2. a workgroup per row joins the bins, finds each rule's bin, ranks the words of that bin (or of all bins up
 //      to it) in LDS by a radix search, and draws.
-// A weight is 2^(y - y of the largest), y = logit log2(e) / temperature in fp64, as a whole number of 2^-50
+// A weight is 2^t, t = (logit - the largest) log2(e) / temperature in fp64, as a whole number of 2^-50
 // (fewer bits where more words than kChunk are summed): sums of whole numbers do not depend on the order of
 // their atomics, and those of equal logits are exact.  Words below 2^-47 of the largest count as none.
 #include <limits.h>
@@ -31,7 +31,7 @@ constexpr int kFromTop = 2048;
 constexpr uint32_t kNoToken = 0xffffffffu;
 
 struct ChunkHead {
-    double top;       // floor(8 y) of the largest
+    double top;       // the largest's eighth
     float max;
     uint32_t arg;     // its first word
     uint32_t bad;     // a NaN or +inf
@@ -69,12 +69,15 @@ __device__ __forceinline__ double word_scale(const SampleArgs& a, int row) {
     return t > 0.0f ? fmax(1.4426950408889634 / (double)t, kAlike) : -1.0;
 }
 
-// y of a logit, rounded by itself: in one fma with the difference from the largest's, equal logits would
-// differ by the product's rounding.
-__device__ __forceinline__ double scaled(float v, double scale) {
+// t, the log2 of v's weight against the largest m's.  The difference is exact but for logits 2^29 apart in size, so t is
+// off by 2^-52 of itself, however large logits and scale are (of two products the difference would be off by 2^-53 of
+// these).  The product is rounded by itself: in one fma with what is subtracted from it, it would differ from place to place.
+__device__ __forceinline__ double distance(float v, float m, double scale) {
 #pragma clang fp contract(off)
-    return (double)v * scale;
+    return ((double)v - (double)m) * scale;
 }
+// Which eighth of an octave a logit lies in: bins are these, counted from the largest's, the same ones in every chunk.
+__device__ __forceinline__ double eighth(float v, double scale) { return floor((double)v * (8.0 * scale)); }
 
 // Weights 2^t, t <= 0: 2^n times the series of e^(f ln 2), |f| <= 1/2, to the 9th power.  What is left out, 7e-12
 // of a weight at most, moves the border between two words by less than that of all weights, so the sum of
@@ -116,16 +119,17 @@ __device__ __forceinline__ uint32_t to_int(double v) {
     return i;
 }
 
-// Words in order as ascending 64-bit numbers: logit (largest first; -0 is 0), then index.
-__device__ __forceinline__ uint64_t word_order(float x, uint32_t i) {
+// Floats in order as ascending numbers (-0 is 0), and back.
+__device__ __forceinline__ uint32_t order_bits(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
-    const uint32_t up = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (uint64_t)~up << 32 | i;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float word_logit(uint64_t order) {
-    const uint32_t up = ~(uint32_t)(order >> 32);
+__device__ __forceinline__ float bits_order(uint32_t up) {
     return __builtin_bit_cast(float, up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
+// Words in order as ascending 64-bit numbers: logit, largest first, then index.
+__device__ __forceinline__ uint64_t word_order(float x, uint32_t i) { return (uint64_t)~order_bits(x) << 32 | i; }
+__device__ __forceinline__ float word_logit(uint64_t order) { return bits_order(~(uint32_t)(order >> 32)); }
 
 typedef f4_t f4w_t __attribute__((aligned(4)));
 
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
         m = fmaxf(m, wave_max[w]);
     }
     Chunk& out = a.chunks[blockIdx.x];
-    const double ym = m > -INFINITY ? scaled(m, scale) : 0.0, top = floor(8.0 * ym);
+    const double top = m > -INFINITY ? eighth(m, scale) : 0.0;
     if (scale < 0.0 || wrong || !(m > -INFINITY)) {   // the largest is all that counts, if anything does
         uint32_t at = kNoToken;
 #pragma unroll
@@ -231,9 +235,9 @@ __global__ void __launch_bounds__(kChunkThreads) sample_chunk_kernel(const Sampl
     uint32_t rank[kPerThread];   // bin and place inside it
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j) {
-        const double y = scaled(v[j >> 2][j & 3], scale);
-        const uint32_t b = min(to_int(top - floor(8.0 * y)), (uint32_t)(kBins - 1 + lane));   // (-inf: the latter)
-        atomicAdd(&mass[b], (unsigned long long)exp2.whole_offset(y - ym, kBits));
+        const float x = v[j >> 2][j & 3];
+        const uint32_t b = min(to_int(top - eighth(x, scale)), (uint32_t)(kBins - 1 + lane));   // (-inf: the latter)
+        atomicAdd(&mass[b], (unsigned long long)exp2.whole_offset(distance(x, m, scale), kBits));
         rank[j] = b << 16 | atomicAdd(&count[b], 1u);
     }
     __syncthreads();
@@ -301,7 +305,7 @@ struct RowLds {
     float max[kRowThreads / kWave];
     uint32_t n, found;
     int least_bin;
-    double least_log;
+    float edge;
 };
 
 // One row.  Bound by latency: some 20 steps between barriers, and a trip to the chunks' heads, to their bins, to the
@@ -359,9 +363,9 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         return;
     }
     const Exp2 exp2;
-    const double ym = scaled(m, scale), top = floor(8.0 * ym);
-    auto below = [&](float v) { return fmax(scaled(v, scale) - ym, -1000.0); };   // log2 of a weight
-    auto bin_of = [&](float v) { return top - floor(8.0 * scaled(v, scale)); };
+    const double top = eighth(m, scale);
+    auto below = [&](float v) { return fmax(distance(v, m, scale), -1000.0); };   // log2 of a weight
+    auto bin_of = [&](float v) { return top - eighth(v, scale); };
     // how far a chunk's bins and largest weight lie below the row's
     for (int c = tid; c < a.nchunk; c += kRowThreads) {
         const float cm = chunks[c].head.max;
@@ -399,19 +403,31 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         l.mass[tid] = w;
         l.count[tid] = n;
     } else if (wave == kWaves - 1) {
-        // the bin that min-p cuts through: behind it no other rule matters (and chunks need not have kept their words)
+        // The smallest logit that weighs enough, by the weights' logarithms (of a min-p of 2^-37 the whole numbers would
+        // leave 13 bits): of all floats from the lowest up to the largest, by their order, 64 of them tried at once.  What
+        // it divides is then the same wherever it is asked, and the bin that it lies in is the last that matters (behind
+        // it chunks need not have kept their words).
         double log = least > 0.0 ? log2(fmin(least, 1.0)) : -INFINITY;
         if (scale == kAlike) log = fmin(log, -1e-200);   // (below 0: a min-p of 1 keeps all finite logits too)
-        const double at = top - floor(8.0 * (ym + log));
+        const uint32_t lowest = order_bits(-3.4028234663852886e38f), span = order_bits(m) - lowest;
+        uint32_t at = 0;                                 // those below it do not weigh enough
+#pragma unroll 1
+        for (int shift = 26; shift >= 0; shift = shift > 6 ? shift - 6 : shift ? 0 : -1) {
+            const uint64_t tried = at + ((uint64_t)lane << shift);
+            const bool enough = tried >= span || distance(bits_order(lowest + (uint32_t)tried), m, scale) >= log;
+            const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(!enough));   // (the first so many)
+            if (n) at += ((uint32_t)(n - 1) << shift) + 1;
+        }
         if (lane == 0) {
-            l.least_log = log;
-            l.least_bin = at < kBins ? (int)at : kBins;
+            const double bin = bin_of(bits_order(lowest + at));
+            l.edge = bits_order(lowest + at);
+            l.least_bin = at && bin < kBins ? (int)bin : kBins;   // (all of them: no matter)
         }
     }
     __syncthreads();
     const int least_bin = l.least_bin;
-    // (by logarithms: of a min-p of 2^-37 the whole numbers would leave 13 bits)
-    auto weighs_enough = [&](float v) { return below(v) >= l.least_log; };
+    const float edge = l.edge;
+    auto weighs_enough = [&](float v) { return v >= edge; };
 
     // The words that count are those up to last_order, all of bins up to last_bin, of it those that weigh enough
     // (whole_bin: all of that one's).  The list holds the words of bins list_lo .. list_hi (none: list_lo > list_hi).
@@ -708,8 +724,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
             w[j + e] = 0;
             const double b = bin_of(v[e]);   // (-inf: none)
             if (b < kBins - 1 && word_order(v[e], first + j + e) <= last_order) {
-                // as in the sums: bins before the last one count whole (they lie above min-p but for roundings), so
-                // the chunk that is drawn has a word
+                // (as in the sums, so the chunk that is drawn has a word)
                 if (b < bins || (b == last_bin && weighs_enough(v[e]))) w[j + e] = exp2.whole(below(v[e]), kBits);
             }
             own += w[j + e];

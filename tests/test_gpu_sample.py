@@ -354,3 +354,47 @@ def test_an_infinite_temperature_with_every_min_p_and_logits_near_zero(env, voca
                 assert ids[r] == want, (how, r, ids[r], want)
                 assert abs(probs[r] * n - 1) <= 2.0**-24 + 2.0**-40, (how, r)
     assert ops.device_error() == 0
+
+
+def pairs(seed, rows=16384):
+    """Rows (small word, large word) of logits up to 10^6 and temperatures down to 10^-4, a tenth of a temperature to three of
+    them apart, and the smaller one's weight in 64 bits of fraction."""
+    rng = np.random.default_rng(seed)
+    big = (rng.choice([-1.0, 1.0], rows) * np.exp(rng.uniform(np.log(0.1), np.log(1e6), rows))).astype(np.float32)
+    t = np.maximum(np.exp(rng.uniform(np.log(1e-4), np.log(3.0), rows)), np.abs(big) * 2.0**-22).astype(np.float32)
+    small = (big.astype(np.float64) - t.astype(np.float64) * rng.uniform(0.1, 3.0, rows)).astype(np.float32)
+    apart = big.astype(np.longdouble) - small.astype(np.longdouble)
+    use = (apart > 0) & (apart < 4 * t)
+    w = np.exp(-apart / t.astype(np.longdouble))
+    return big[use], small[use], t[use], w[use]
+
+
+def check_pairs(env, seed, off):
+    """Draws and min-p at borders that lie between two floats: right wherever u, or min-p, is further from it than `off` of it."""
+    big, small, t, w = pairs(seed)
+    x = np.stack((small, big), 1)
+    share = w / (1 + w)
+    u = share.astype(np.float32)
+    far = np.abs(u.astype(np.longdouble) - share) > off * share
+    assert far.mean() > 0.98
+    for how in ({}, dict(k=np.full(len(u), 2))):
+        ids, probs = (v.cpu().numpy() for v in run(env, x, u, t=t, **how))
+        want = np.where(u < share, 0, 1)
+        wrong = far & (ids != want)
+        assert not wrong.any(), (int(wrong.sum()), np.nonzero(wrong)[0][:5])
+        p = np.where(want, 1 - share, share)
+        assert (np.abs(probs - p) <= p * (2.0**-24 + 2 * off))[far].all()
+    least = w.astype(np.float32)
+    far = np.abs(least.astype(np.longdouble) - w) > 2.0**-45 * w   # (no weight is computed: roundings of logarithms)
+    assert far.mean() > 0.98
+    ids = run(env, x[:, ::-1].copy(), np.ones(len(u)), t=t, least=least)[0].cpu().numpy()   # u = 1: the last word that stays
+    wrong = far & (ids != np.where(w >= least, 1, 0))
+    assert not wrong.any(), (int(wrong.sum()), np.nonzero(wrong)[0][:5])
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("seed", [31, 32, 33, 34])
+def test_weights_of_large_logits_and_low_temperatures(env, seed):
+    """A weight is its series' 9.7e-12 (2^-36.6) off at most, wherever on the scale the logits lie: 2^-36 with the roundings (the
+    difference's and two of its scale's, 2^-51 of up to 6 octaves; 2^-51 of a weight of 0.05 as a whole number: 2^-46)."""
+    check_pairs(env, seed, 2.0**-36)
