@@ -356,22 +356,24 @@ def test_an_infinite_temperature_with_every_min_p_and_logits_near_zero(env, voca
     assert ops.device_error() == 0
 
 
-def pairs(seed, rows=16384):
+def pairs(seed, rows=16384, halves=False):
     """Rows (small word, large word) of logits up to 10^6 and temperatures down to 10^-4, a tenth of a temperature to three of
-    them apart, and the smaller one's weight in 64 bits of fraction."""
+    them apart (halves: about one half, three halves, .. of an octave of weight), and the smaller one's weight in 64 bits of
+    fraction."""
     rng = np.random.default_rng(seed)
     big = (rng.choice([-1.0, 1.0], rows) * np.exp(rng.uniform(np.log(0.1), np.log(1e6), rows))).astype(np.float32)
     t = np.maximum(np.exp(rng.uniform(np.log(1e-4), np.log(3.0), rows)), np.abs(big) * 2.0**-22).astype(np.float32)
-    small = (big.astype(np.float64) - t.astype(np.float64) * rng.uniform(0.1, 3.0, rows)).astype(np.float32)
+    far = np.log(2) * (rng.integers(0, 4, rows) + rng.uniform(0.47, 0.53, rows)) if halves else rng.uniform(0.1, 3.0, rows)
+    small = (big.astype(np.float64) - t.astype(np.float64) * far).astype(np.float32)
     apart = big.astype(np.longdouble) - small.astype(np.longdouble)
     use = (apart > 0) & (apart < 4 * t)
     w = np.exp(-apart / t.astype(np.longdouble))
     return big[use], small[use], t[use], w[use]
 
 
-def check_pairs(env, seed, off):
+def check_pairs(env, seed, off, **how):
     """Draws and min-p at borders that lie between two floats: right wherever u, or min-p, is further from it than `off` of it."""
-    big, small, t, w = pairs(seed)
+    big, small, t, w = pairs(seed, **how)
     x = np.stack((small, big), 1)
     share = w / (1 + w)
     u = share.astype(np.float32)
@@ -398,3 +400,11 @@ def test_weights_of_large_logits_and_low_temperatures(env, seed):
     """A weight is its series' 9.7e-12 (2^-36.6) off at most, wherever on the scale the logits lie: 2^-36 with the roundings (the
     difference's and two of its scale's, 2^-51 of up to 6 octaves; 2^-51 of a weight of 0.05 as a whole number: 2^-46)."""
     check_pairs(env, seed, 2.0**-36)
+
+
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("seed", [41, 42, 43])
+def test_weights_hold_what_the_shares_are_held_to(env, seed, halves):
+    """check() allows a share 2^-40 besides its rounding, so a weight and its sum 2^-41 each.  The series is 2^-44.2 off at most (its
+    ends: half an octave from a power of two), the roundings together 2^-46 as above: 2^-43."""
+    check_pairs(env, seed, 2.0**-43, halves=halves)
