@@ -230,8 +230,9 @@ int rta_lm_head(int fmt, const void* w, int vocab, int hidden, const float* h, i
  * A logit of -inf is never drawn.  A row with a NaN or +inf, or with nothing but -inf, gets ids[r] = 2^32 - 1
  * and probs[r] = 0 and raises RTA_DEVERR_DETECTOR.  Weights are computed in fp64 (to 2^-43 of
  * themselves, however large logits and 1 / T are) and added up as whole numbers of 2^-50 of the largest, or of its 8192
- * words' largest (in an order that does not matter: results repeat bit by bit; those of equal logits are exactly
- * alike); words below 2^-47 of it count as none.  vocab up to 2^22, rows ceil(vocab / 8192) below 2^22.
+ * words' largest (in an order that does not matter: results repeat bit by bit; those of equal logits by
+ * the same largest are exactly alike).  Words below a bound count as none: it lies between 2^-47.875 and 2^-47.75 of
+ * the row's largest, at a whole eighth of x log2(e) / T.  vocab up to 2^22, rows ceil(vocab / 8192) below 2^22.
  * Workspace: rta_sample_workspace_bytes() (always needed; 16-byte aligned).
  * No reference counterpart: its word readout takes the largest (Resident::word, optical_resident.cpp:523-530). */
 size_t rta_sample_workspace_bytes(int rows, int vocab);

@@ -10,7 +10,8 @@
 //      to it) in LDS by a radix search, and draws.
 // A weight is 2^t, t = (logit - the largest) log2(e) / temperature in fp64, as a whole number of 2^-50
 // (fewer bits where more words than kChunk are summed): sums of whole numbers do not depend on the order of
-// their atomics, and those of equal logits are exact.  Words below 2^-47 of the largest count as none.
+// their atomics, and those of equal logits are exact.  Words below the last bin that is
+// kept, 2^-47.875 to 2^-47.75 of the largest by where in its eighth of an octave that one lies, count as none.
 #include <limits.h>
 #include <math.h>
 

@@ -408,3 +408,21 @@ def test_weights_hold_what_the_shares_are_held_to(env, seed, halves):
     """check() allows a share 2^-40 besides its rounding, so a weight and its sum 2^-41 each.  The series is 2^-44.2 off at most (its
     ends: half an octave from a power of two), the roundings together 2^-46 as above: 2^-43."""
     check_pairs(env, seed, 2.0**-43, halves=halves)
+
+
+@pytest.mark.parametrize("vocab", [3, 9000, 40000])
+def test_the_least_weight_that_counts(env, vocab):
+    """Words of 2^-47.74 of the largest are drawn where nothing lies in front of them (u = 0), words of 2^-47.88 never, wherever
+    in its eighth of an octave the largest lies; in the largest's chunk and in one of their own."""
+    rng = np.random.default_rng(vocab)
+    rows = 64
+    t = rng.uniform(0.1, 3.0, rows).astype(np.float32)
+    top = rng.uniform(-40, 40, rows).astype(np.float32)
+    for octaves, counts in ((47.74, True), (47.88, False)):
+        x = np.full((rows, vocab), -np.inf, np.float32)
+        x[:, vocab - 1] = top
+        x[:, 0] = top.astype(np.float64) - octaves * np.log(2) * t.astype(np.float64)   # (fp32: 6e-5 of an octave off at most)
+        for how in ({}, dict(k=np.full(rows, 2)), dict(least=np.full(rows, 1e-30))):
+            ids = run(env, x, np.zeros(rows), t=t, **how)[0].cpu().numpy()
+            assert (ids == (0 if counts else vocab - 1)).all(), (octaves, how)
+    assert ops.device_error() == 0
