@@ -29,6 +29,14 @@ __device__ __forceinline__ float half_hi(uint32_t w) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
 }
 
+// A whole number as 32 bits with sign, the nearest of these where it is none of them, 0 for NaN (all of which a
+// cast leaves undefined).
+__device__ __forceinline__ uint32_t to_int(double v) {
+    uint32_t i;
+    asm("v_cvt_i32_f64 %0, %1" : "=v"(i) : "v"(v));
+    return i;
+}
+
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 // Reinterprets a dword whose halves hold small integer codes c (bits 0..9) as two

@@ -37,7 +37,7 @@ __device__ __forceinline__ double2 turn_of(double position, double turns, double
     c = fma(c, z, -0.5);
     s = fma(s * z, x, x);
     c = fma(c, z, 1.0);
-    const int quadrant = (int)n & 3;
+    const uint32_t quadrant = to_int(n) & 3;
     const double a = quadrant & 1 ? s : c, b = quadrant & 1 ? c : s;
     return double2{quadrant == 1 || quadrant == 2 ? -amplitude * a : amplitude * a, quadrant & 2 ? -amplitude * b : amplitude * b};
 }

@@ -114,13 +114,13 @@ struct Exp2 {
 #pragma unroll
         for (int i = 2; i <= kDegree; ++i) asm("" : "+s"(c[i]));
     }
-    // 2^(t + bits)
+    // 2^(t + bits); 0 for t however low (of -inf NaN, which the chunks' kernel adds where nothing is read)
     __device__ __forceinline__ double operator()(double t, int bits = 0) const {
         const double n = rint(t), f = t - n;
         double p = c[kDegree];
 #pragma unroll
         for (int i = kDegree - 1; i > 0; --i) p = fma(p, f, c[i]);
-        return ldexp(fma(p, f, 1.0), (int)n + bits);
+        return ldexp(fma(p, f, 1.0), (int)(to_int(n) + (uint32_t)bits));
     }
     // The same as a whole number, rounded to nearest (bits <= 51): the last bits of 2^52 + it, plus kOffset.
     static constexpr uint64_t kOffset = 0x4330000000000000ull;
@@ -129,13 +129,6 @@ struct Exp2 {
     }
     __device__ __forceinline__ uint64_t whole(double t, int bits) const { return whole_offset(t, bits) - kOffset; }
 };
-
-// A whole number, or the largest where it is none of 32 bits (a cast would not have to).
-__device__ __forceinline__ uint32_t to_int(double v) {
-    uint32_t i;
-    asm("v_cvt_i32_f64 %0, %1" : "=v"(i) : "v"(v));
-    return i;
-}
 
 // Floats in order as ascending numbers (-0 is 0), and back.
 __device__ __forceinline__ uint32_t order_bits(float x) {

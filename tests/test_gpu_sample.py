@@ -426,3 +426,21 @@ def test_the_least_weight_that_counts(env, vocab):
             ids = run(env, x, np.zeros(rows), t=t, **how)[0].cpu().numpy()
             assert (ids == (0 if counts else vocab - 1)).all(), (octaves, how)
     assert ops.device_error() == 0
+
+
+def test_the_lowest_temperatures(env):
+    """Exponents far past 32 bits: the largest word alone, by every rule, masked words beside it."""
+    rng = np.random.default_rng(51)
+    rows, vocab = 6, 20011
+    x, u = logits(rng, rows, vocab), rng.random(rows).astype(np.float32)
+    x[1, ::3] = -np.inf
+    x[2] *= np.float32(1e37)
+    x[3] *= np.float32(1e-37)
+    x[4, 5:9000] = np.finfo(np.float32).min
+    for t in (2.0**-149, 2.0**-126, 1e-30, 1e-20):   # (the fourth row's largest are 2e-38 apart)
+        for how in ({}, dict(k=np.full(rows, 40)), dict(p=np.full(rows, 0.9)), dict(least=np.full(rows, 1e-9)),
+                    dict(k=np.full(rows, 9000), p=np.full(rows, 0.99), least=np.full(rows, 0.1))):
+            keep = np.array([0, 1, 2, 4, 5]) if t > 2.0**-149 else np.arange(rows)
+            ids, probs = (v.cpu().numpy() for v in run(env, x, u, t=np.full(rows, t), **how))
+            assert np.array_equal(ids[keep], np.argmax(x, 1)[keep]) and (probs[keep] == 1).all(), (t, how)
+    assert ops.device_error() == 0
