@@ -518,8 +518,8 @@ int rta_hybrid_decode_step_capture(const rta_hybrid_shape* shape, const rta_hybr
 
 /* ---------------- rotary positions beyond rta_rope: pairs of neighbours or of half a head's distance, the
  * whole head or its first values, frequencies scaled for contexts longer than the trained one.  Pair j of a
- * head at position p turns by the angle 2 pi p turns[j] (the product and the turn in fp64, each value rounded
- * to fp32 once):  (x, y) -> amplitude (x cos - y sin, x sin + y cos).  Values past `dims` stay as they are.
+ * head at position p turns by the angle 2 pi p turns[j] (the product's fraction of a turn exact to 2^-53, however
+ * far the position, up to 2^53; the turn in fp64, each value rounded to fp32 once):  (x, y) -> amplitude (x cos - y sin, x sin + y cos).  Values past `dims` stay as they are.
  * The rotation at -p is its transpose: gradients go back through a call with negated positions. */
 enum rta_rotary_layout {
     RTA_ROTARY_NEIGHBOURS = 0,   /* pair j: values 2 j and 2 j + 1 (rta_rope's) */

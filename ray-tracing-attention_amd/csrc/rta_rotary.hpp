@@ -13,13 +13,12 @@ struct RotaryArgs {
     int dims;
 };
 
-// amplitude (cos, sin) of 2 pi position turns.  The product is rounded to 64 bits; only its distance from a
-// whole number of quarter turns counts, and that is exact (so far positions lose what the product's own
-// rounding loses: 2^-53 of the turns made).  Within half a quarter turn the power series, to theta^16
-// and theta^15: the first terms left out are 2e-18 and 5e-17.
+// amplitude (cos, sin) of 2 pi position turns.  Only the product's distance from a whole number of turns counts: the
+// rounded product says which one, and one fma takes it off the exact product, so far positions lose nothing (but for
+// the conversion to fp64 past 2^53; the rounded product would be off by 2^-53 of the turns made).  Within half a quarter
+// turn the power series, to theta^16 and theta^15: the first terms left out are 2e-18 and 5e-17.
 __device__ __forceinline__ double2 turn_of(double position, double turns, double amplitude) {
-    const double t = position * turns;
-    const double quarters = 4.0 * (t - rint(t)), n = rint(quarters);
+    const double quarters = 4.0 * fma(position, turns, -rint(position * turns)), n = rint(quarters);
     const double x = (quarters - n) * 1.5707963267948966, z = x * x;   // pi / 2
     double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;     // 15!, 16!
     s = fma(s, z, 1.0 / 6227020800.0);

@@ -277,3 +277,34 @@ def test_streams_and_graphs(env):
         c.append(r.rotate(k.unflatten(1, (2, 128)), pos).flatten(1), v, cu_rows=cu)
         assert all(torch.equal(a, b) for a, b in zip(stored, c.read(rows, cu_rows=cu))), i
     assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("layout", ["neighbours", "halves"])
+def test_far_positions_lose_nothing(env, layout):
+    """Positions up to 2^53 against the exact product of position and turns: its fraction of a turn, however many were made, is held
+    to 2^-53 and the result to one rounding (the rounded product would be off by up to an eighth of a turn)."""
+    from fractions import Fraction
+    torch, _, dev = env
+    rows, heads, hd, dims = 64, 3, 64, 48
+    r = rotary.Rotary(hd, dims, layout, theta=1e4, scaling="bands", factor=8.0, original=8192, low=1.0, high=4.0)
+    rng = np.random.default_rng(17)
+    p = np.round(np.exp2(rng.uniform(20, 53, rows))).astype(np.int64) * rng.choice([-1, 1], rows)
+    p[:4] = [1 << 53, -(1 << 53), (1 << 53) - 1, 1 << 52]
+    x = rows_of(torch, dev, rows, heads, hd, 18)
+    y = r.rotate(x, torch.tensor(p, device=dev)).cpu().double().numpy()
+    table = r.turns.cpu().numpy()
+    part = np.empty((rows, dims // 2))
+    for i in range(rows):
+        for j in range(dims // 2):
+            made = int(p[i]) * Fraction(float(table[j]))
+            part[i, j] = float(made - round(made))
+    angle = 2 * np.pi * part[:, None]
+    c, s = np.cos(angle), np.sin(angle)
+    lo, hi = (np.arange(0, dims, 2), np.arange(1, dims, 2)) if layout == "neighbours" else (np.arange(dims // 2), np.arange(dims // 2, dims))
+    x = x.cpu().double().numpy()
+    a, b = x[..., lo], x[..., hi]
+    # one rounding; the fraction's, the series' and the products' in fp64, here and in numpy, below 2^-48 together
+    bound = (np.abs(a) + np.abs(b)) * (2.0**-24 + 2.0**-48)
+    assert np.all(np.abs(y[..., lo] - (a * c - b * s)) <= bound)
+    assert np.all(np.abs(y[..., hi] - (a * s + b * c)) <= bound)
+    assert np.array_equal(y[..., dims:], x[..., dims:])
