@@ -654,7 +654,7 @@ int rta_paged_append(const rta_pages* pages, int layer, const float* k, int64_t 
 /* rta_paged_append with the rotation on the way: the keys of a row are turned to the position that it is
  * stored at (rounded to fp32, then stored as rta_paged_append stores them), and so are, with q not NULL, the
  * queries q [rows, hq, head_dim] of the same rows into q_out (row strides in floats; q_out may be q, with the
- * same stride).  What rta_rotate and rta_paged_append give, bit by bit, in one pass and with positions that
+ * same stride, and otherwise shares no memory with q, k or v).  What rta_rotate and rta_paged_append give, bit by bit, in one pass and with positions that
  * only the book knows.  rotary->head_dim is the pages'.  A listed row without a place (a bad sequence, no
  * page) raises RTA_DEVERR_PAGES and is left undone, its q_out as it was. */
 int rta_paged_append_rotary(const rta_pages* pages, int layer, const rta_rotary* rotary, const float* k, int64_t k_stride,

@@ -599,7 +599,10 @@ __global__ void __launch_bounds__(256) append_rotary_kernel(const PageArgs a, co
                 }
             }
         }
-        // (a loop of its own: the partners that have just been read may be stored to)
+        // A loop of its own: in place, a value is the partner of another lane of its head, which is one of this wave's.
+        // All have been read before any is stored.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
             const int c = c0 + i * step, head = c / kPer;

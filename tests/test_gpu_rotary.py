@@ -308,3 +308,20 @@ def test_far_positions_lose_nothing(env, layout):
     assert np.all(np.abs(y[..., lo] - (a * c - b * s)) <= bound)
     assert np.all(np.abs(y[..., hi] - (a * s + b * c)) <= bound)
     assert np.array_equal(y[..., dims:], x[..., dims:])
+
+
+@pytest.mark.parametrize("hd,dims", [(64, 20), (64, 62), (128, 94), (128, 12), (256, 250), (256, 130)])
+@pytest.mark.parametrize("rows,hq", [(3, 40), (700, 24), (2100, 7)])
+def test_queries_in_place_with_partners_one_by_one(env, hd, dims, rows, hq):
+    """Halves that are no multiple of eight values: partners that other lanes of the wave store to, in rows of one workgroup and
+    of several, heads of one wave and of many."""
+    torch, _, dev = env
+    c, cu, rows, k, v, pos = append_case(env, _lib.Q8_ROW, 2, hd, 32, [rows + 5], [rows])
+    r = rotary.Rotary(hd, dims, "halves", theta=1e4)
+    q = rows_of(torch, dev, rows, hq, hd, 19).contiguous()
+    want = r.rotate(q, pos)
+    for _ in range(3):
+        y = q.clone()
+        assert torch.equal(c.append_rotary(r, k, v, y, y, cu_rows=cu), want)
+    assert torch.equal(c.append_rotary(r, k, v, q, cu_rows=cu), want)
+    assert ops.device_error() == 0
