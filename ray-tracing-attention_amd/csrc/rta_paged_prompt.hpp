@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                         bad |= 1u << k;
                     }
                 } else {   // a row's threads are of one wave
-                    constexpr uint64_t kRow = kPieces == 32 ? 0xffffffffull : (1ull << kPieces) - 1;
+                    constexpr uint64_t kLanes = kPieces == 32 ? 0xffffffffull : (1ull << kPieces) - 1;
                     bool hit;
                     if constexpr (kQ4) hit = q4_not_finite(vw[k]);
                     else hit = piece_not_finite<FMT>(vr[k]);
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(256, (PromptLds<FMT, HD>::kTotal > 80 << 10 ? 
                         vr[k] = (Piece)(0u);
                         if constexpr (kQ4) vw[k] = 0;
                     }
-                    if (__builtin_amdgcn_ballot_w64(hit) & (kRow << (lane & ~(kPieces - 1)))) bad |= 1u << k;
+                    if (__builtin_amdgcn_ballot_w64(hit) & (kLanes << (lane & ~(kPieces - 1)))) bad |= 1u << k;
                 }
             }
         }
