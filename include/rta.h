@@ -233,7 +233,7 @@ int rta_lm_head(int fmt, const void* w, int vocab, int hidden, const float* h, i
  * words' largest (in an order that does not matter: results repeat bit by bit; those of equal logits by
  * the same largest are exactly alike).  Words below a bound count as none: it lies between 2^-47.875 and 2^-47.75 of
  * the row's largest, at a whole eighth of x log2(e) / T.  vocab up to 2^22, rows ceil(vocab / 8192) below 2^22.
- * Workspace: rta_sample_workspace_bytes() (always needed; 16-byte aligned).
+ * Workspace: rta_sample_workspace_bytes() (always needed; 16-byte aligned), some 20 KB per row and 8192 words.
  * No reference counterpart: its word readout takes the largest (Resident::word, optical_resident.cpp:523-530). */
 size_t rta_sample_workspace_bytes(int rows, int vocab);
 int rta_sample(const float* logits, int64_t stride, int rows, int vocab, const float* temperature, const int32_t* top_k,

@@ -8,8 +8,9 @@
 //   (slots 16 .. 31: the same dims); columns 0 .. 7 hold the queries in the first slots and zeros in the others,
 //   columns 8 .. 15 the reverse.  So a lane has 4 scores, none twice, and one row's address and words to deal with.
 //   O^T: the weights of columns 0 .. 7 lie in the slots of the first half's positions, zeros in the others.
-// The two halves of the columns are summed as if they were rows of their own, and joined with the waves'.  374
-// instructions a tile, on 70% of the cycles: 845 MB of 8 sequences in 164 us (5.2 TB/s; so 196), 88 MB of 32 in 28.5.
+// The two halves of the columns are summed as if they were rows of their own, and joined with the waves'.  368
+// instructions a tile, on 70% of the cycles.  845 MB of 8 sequences: 164 us at least in a kernel trace (5.2 TB/s;
+// paged_decode_kernel 196), where the median of 20 is 210; 180 untraced, with the merge (205).  88 MB of 32: 28.4, median 30.5.
 #pragma once
 #include "rta_paged_decode.hpp"
 
