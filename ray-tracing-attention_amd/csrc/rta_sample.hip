@@ -9,7 +9,7 @@
 //   2. a workgroup per row joins the bins, finds each rule's bin, ranks the words of that bin (or of all bins up
 //      to it) in LDS by a radix search, and draws.
 // A weight is 2^t, t = (logit - the largest) log2(e) / temperature in fp64, as a whole number of 2^-50
-// (fewer bits where more words than kChunk are summed): sums of whole numbers do not depend on the order of
+// (of one bin's words, of its own weights: as many bits as their sum has room for): sums of whole numbers do not depend on the order of
 // their atomics, and those of equal logits are exact.  Words below the last bin that is
 // kept, 2^-47.875 to 2^-47.75 of the largest by where in its eighth of an octave that one lies, count as none.
 #include <limits.h>
@@ -71,7 +71,7 @@ __device__ __forceinline__ double word_scale(const SampleArgs& a, int row) {
 }
 
 // t, the log2 of v's weight against the largest m's.  The difference is exact but for logits 2^29 apart in size, so t is
-// off by 2^-52 of itself, however large logits and scale are (of two products the difference would be off by 2^-53 of
+// off by 2^-51 of itself, however large logits and scale are (of two products the difference would be off by 2^-53 of
 // these).  The product is rounded by itself: in one fma with what is subtracted from it, it would differ from place to place.
 __device__ __forceinline__ double distance(float v, float m, double scale) {
 #pragma clang fp contract(off)
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
 
     // The words that count are those up to last_order, all of bins up to last_bin, of it those that weigh enough
     // (whole_bin: all of that one's).  The list holds the words of bins list_lo .. list_hi (none: list_lo > list_hi).
-    int last_bin = kBins - 2, list_lo = 1, list_hi = 0, list_n = 0;
+    int last_bin = kBins - 2, list_lo = 1, list_hi = 0, list_n = 0, list_bits = kBits, part_bits = kBits;
     uint64_t last_order = ~0ull;
     bool whole_bin = true;
     double total = l.mass[kBins - 2];
@@ -482,6 +482,9 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         }
         // the words of bin b, with all before it if they fit
         const uint32_t upto = l.count[b], before_b = b ? l.count[b - 1] : 0;
+        // Whole numbers of words of this bin alone keep as many bits as fit of the bin's own weights, which are at most
+        // 2^-((b - 1) / 8) of the largest: 2^17 equal words at 2^-36 of it would have 8 bits of 2^-44.
+        const int below_one = b > 0 ? (b - 1) / 8 : 0;
         bool listed = list_lo <= b && b <= list_hi;
         if (!listed) {
             const int lo = upto <= kFromTop ? 0 : b;
@@ -489,6 +492,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
             listed = list_n <= kList;
             list_lo = listed ? lo : 1;
             list_hi = listed ? b : 0;
+            list_bits = lo ? kBits + below_one : kBits;
             if (listed) {
                 // where each chunk's words of these bins lie and go: thread c has chunk c
                 uint32_t i0 = 0, own = 0;
@@ -533,7 +537,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
                     for (int j = 0; j < kAtOnce; ++j)
                         if (i + j * kRowThreads < list_n) {
                             l.list[i + j * kRowThreads] = word_order(t[j], id[j]);
-                            l.weight[i + j * kRowThreads] = exp2.whole(below(t[j]), kBits);
+                            l.weight[i + j * kRowThreads] = exp2.whole(below(t[j]), list_bits);
                         }
                 }
             }
@@ -543,7 +547,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         // what lies in front of the words that are searched
         double before = list_lo == 0 || !b ? 0.0 : l.mass[b - 1];
         uint32_t before_n = list_lo == 0 ? 0 : before_b;
-        const int bits = min(kBits, 62 - (32 - __clz((int)(upto - before_b))));
+        const int bits = min(kBits, 62 - (32 - __clz((int)(upto - before_b)))) + below_one;
         // a range of logits that holds bin b's, with room for the roundings
         const double step = 8.0 * scale, e0 = (top - b) / step, e1 = (top - b + 1.0) / step;
         const float from = (float)fmax(e0 - fabs(e0) * 1e-6 - 1e-30, -3.4028234663852886e38);
@@ -558,6 +562,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
         int end = draw ? 32 - __clz(a.vocab) : 64 - __clzll((long long)(highest - lowest));
         uint64_t known = end == 64 ? 0 : ~0ull << end, value = 0;
         bool opened = false;   // a draw's goal is known
+        part_bits = kBits + below_one;   // (kParts' words are of this bin, and kChunk of a chunk at most)
         if (mode == kParts)
             for (int c = tid; c < a.nchunk; c += kRowThreads) l.chunk_part[c] = 0;
         if (mode == kParts) __syncthreads();
@@ -583,7 +588,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
                     } else {
                         const uint32_t at = atomicAdd(&l.n, 1u);
                         l.list[at] = order;
-                        l.weight[at] = exp2.whole(below(word_logit(order)), kBits);
+                        l.weight[at] = exp2.whole(below(word_logit(order)), kBits + below_one);
                     }
                 }
             };
@@ -598,7 +603,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
                     for (int j = 0; j < 4; ++j) {
                         const float v = j == 0 ? t[0] : j == 1 ? t[1] : j == 2 ? t[2] : t[3];
                         if (v < from || v > to || v == -INFINITY || bin_of(v) != b) continue;
-                        visit(word_order(v, i + j * kRowThreads), exp2.whole(below(v), mode == kParts ? kBits : bits));
+                        visit(word_order(v, i + j * kRowThreads), exp2.whole(below(v), mode == kParts ? part_bits : bits));
                     }
                 }
             }
@@ -611,6 +616,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
             if (mode == kGather) {
                 listed = true;
                 list_n = (int)l.n;
+                list_bits = kBits + below_one;
                 mode = kDigits;
                 continue;
             }
@@ -627,7 +633,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
             buf = next;
             uint32_t cb = wave_prefix<uint32_t>(cs);
             uint64_t wb = wave_prefix<uint64_t>(ws);
-            const int at_bits = listed ? kBits : bits;
+            const int at_bits = listed ? list_bits : bits;
             if (draw && !opened) {   // all weights have been seen
                 total = ldexp((double)lane_of(wb, kWave - 1), -at_bits);
                 goal = u * total;
@@ -689,7 +695,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(const SampleArg
     for (int c = tid; c < a.nchunk; c += kRowThreads) {
         const int n = bins - l.chunk_shift[c];
         l.chunk_mass[c] = (n > 0 ? chunks[c].mass[n - 1] * l.chunk_scale[c] : 0.0) +
-                          (whole_bin ? 0.0 : ldexp((double)l.chunk_part[c], -kBits));
+                          (whole_bin ? 0.0 : ldexp((double)l.chunk_part[c], -part_bits));
     }
     __syncthreads();
     // the chunk of the word: sums in the chunks' order, 64 at a time, by one wave

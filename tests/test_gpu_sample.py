@@ -397,8 +397,9 @@ def check_pairs(env, seed, off, **how):
 
 @pytest.mark.parametrize("seed", [31, 32, 33, 34])
 def test_weights_of_large_logits_and_low_temperatures(env, seed):
-    """A weight is its series' 9.7e-12 (2^-36.6) off at most, wherever on the scale the logits lie: 2^-36 with the roundings (the
-    difference's and two of its scale's, 2^-51 of up to 6 octaves; 2^-51 of a weight of 0.05 as a whole number: 2^-46)."""
+    """A series to the 9th power as it stands is 9.5e-12 (2^-36.6) off at most, wherever on the scale the logits lie: 2^-36 with
+    the roundings (the difference's and two of its scale's, 2^-51 of up to 6 octaves; 2^-51 of a weight of 0.05 as a whole
+    number: 2^-46)."""
     check_pairs(env, seed, 2.0**-36)
 
 
@@ -443,4 +444,30 @@ def test_the_lowest_temperatures(env):
             keep = np.array([0, 1, 2, 4, 5]) if t > 2.0**-149 else np.arange(rows)
             ids, probs = (v.cpu().numpy() for v in run(env, x, u, t=np.full(rows, t), **how))
             assert np.array_equal(ids[keep], np.argmax(x, 1)[keep]) and (probs[keep] == 1).all(), (t, how)
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("words", [9000, 131072, 600000])
+@pytest.mark.parametrize("far", [3.0, 17.0, 22.0, 25.0])
+def test_top_p_among_many_equal_words_of_little_weight(env, words, far):
+    """One word of all but a little of the weight and many equal ones of little: top-p's border among these lies where it ought to
+    but for the whole numbers of 2^-50 (2^-51 a word), the weights' 2^-43 of what they are, and one word.  u = 1 is the last
+    word that stays."""
+    rows = 24
+    w = np.exp(-np.longdouble(np.float32(far)))
+    rest = words * w
+    # p from 1 down to the first word's share, as floats
+    first = float(1 / (1 + rest))
+    p = np.unique(np.linspace(first, 1.0, rows + 2).astype(np.float32)[1:-1])
+    p = p[(p < 1) & (p > np.float32(first))]
+    assert len(p)
+    x = np.full((len(p), words + 1), -far, np.float32)
+    x[:, 5] = 0.0
+    goal = p.astype(np.longdouble) * (1 + rest)
+    want = np.ceil((goal - 1) / w)                  # of the equal words
+    off = (words * 2.0**-51 + rest * 2.0**-43 + goal * 2.0**-52) / w + 1
+    for how in ({}, dict(least=np.full(len(p), 1e-14)), dict(k=np.full(len(p), words + 1))):
+        ids = run(env, x, np.ones(len(p)), p=p, **how)[0].cpu().numpy()
+        stay = ids.astype(np.int64) + 1 - (ids > 5)     # the words up to the last one, without the large one
+        assert (np.abs(stay - want) <= off).all(), (how, stay - want, off)
     assert ops.device_error() == 0
